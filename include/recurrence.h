@@ -366,6 +366,73 @@ int rr_gdn_bwd(const float* dy, const float* dfinal, const void* q, const void* 
                int64_t seg, const float* h0, const float* ckpt, void* dq, void* dk, void* dv, void* dalpha,
                void* dbeta, float* dh0, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------ output head --
+ * What a model of these layers ends in: the norm in front of the head and the
+ * losses over the vocabulary.  No reference counterpart (the reference has the
+ * scans alone).
+ */
+
+/* Layer norm over the last axis: y = (x - mean) * rstd * w + b with the mean and
+ * rstd = 1 / sqrt(var + eps) of each row of x [rows, D], D <= 32768.  w and b [D]
+ * of type w_dtype; null: 1 and 0.  y_dtype is x_dtype, or any type where x is
+ * fp32.  mean and rstd [rows] fp32 are what the backward needs (both null: not
+ * wanted). */
+int rr_layer_norm_fwd(const void* x, int x_dtype, const void* w, const void* b, int w_dtype, int64_t rows,
+                      int64_t D, float eps, void* y, int y_dtype, float* mean, float* rstd, void* stream);
+
+/* Workspace of rr_layer_norm_bwd where dw or db is wanted. */
+size_t rr_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t D);
+
+/* Gradients of rr_layer_norm_fwd from dy [rows, D] (y_dtype): dx (x_dtype), dw and
+ * db [D] (w_dtype), each null where not wanted.  Sums over rows are made in a fixed
+ * order; rows = 0 gives dw = db = 0. */
+int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, const void* w, int w_dtype,
+                      const float* mean, const float* rstd, int64_t rows, int64_t D, void* dx, void* dw, void* db,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Losses on the logits hidden [rows, D] x weight [V, D]^T, which are never stored:
+ * `reduction` 0 leaves a loss a row (loss [rows] fp32), 1 their mean over the rows
+ * that count, 2 their sum (loss [1]; both 0 where no row counts).  The forward
+ * leaves in `state` (16-byte aligned, rr_linear_loss_state_bytes) what
+ * rr_linear_loss_bwd reads; its contents are the library's own.  K: teacher
+ * entries a row, 1 to 1024; 1 for labels.  V <= 2^24, D <= 65536. */
+size_t rr_linear_loss_state_bytes(int64_t rows, int64_t K);
+
+/* Workspace of the forward (pass = 0) or backward (pass = 1); 0 for invalid
+ * arguments.  The backward's holds a piece of the logits' gradient: about
+ * 512 MiB at most, and 2048 columns of the vocabulary at least. */
+size_t rr_linear_loss_workspace_bytes(int64_t rows, int64_t D, int64_t V, int dtype, int pass);
+
+/* Cross entropy: with z = hidden weight^T and lse = log sum exp z of a row,
+ *   loss = lse - z[label] + z_loss * lse^2,
+ * 0 for a row whose label is ignore_index (such a row counts for nothing, whatever
+ * its hidden state holds).  Any other label outside [0, V) makes the row's loss,
+ * and every gradient, NaN. */
+int rr_linear_ce_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                     const int64_t* labels, int64_t ignore_index, float z_loss, int reduction, float* loss,
+                     void* state, size_t state_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits (teacher_logits and teacher_ids
+ * [rows, K]): with p the softmax of a row's teacher logits / temperature over its
+ * entries and q that of z / temperature over the vocabulary,
+ *   loss = temperature^2 * sum_k p_k (log p_k - log q[id_k]).
+ * An entry with a negative id or a logit of -inf is absent; a row without entries
+ * counts for nothing.  An id >= V makes the row's loss, and every gradient, NaN.
+ * The teacher gets no gradient. */
+int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                     const void* teacher_logits, int teacher_dtype, const int64_t* teacher_ids, int64_t K,
+                     float temperature, int reduction, float* loss, void* state, size_t state_bytes,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of either loss: dloss fp32 ([rows] for reduction 0, else [1]), the
+ * forward's inputs and state, K = 1 and temperature = 1 for the cross entropy,
+ * z_loss = 0 for the distillation.  dhidden [rows, D] and dweight [V, D] in
+ * `dtype`, each null where not wanted; rows that do not count get dhidden 0. */
+int rr_linear_loss_bwd(const float* dloss, const void* hidden, const void* weight, int dtype, int64_t rows,
+                       int64_t D, int64_t V, int64_t K, float z_loss, float temperature, int reduction,
+                       const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

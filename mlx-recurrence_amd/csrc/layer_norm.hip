@@ -1,0 +1,368 @@
+// layer_norm.hip — layer norm over the last axis on gfx950, forward and backward.
+//
+//   forward   mu = mean(x);  r = 1 / sqrt(mean((x - mu)^2) + eps);  xh = (x - mu) r
+//             y = xh w + b
+//   backward  g = dy w;  dx = r (g - mean(g) - xh mean(g xh))
+//             dw = sum over rows of dy xh;  db = sum over rows of dy
+//
+// The rows are streamed once: a row stays in the registers of its threads
+// between the statistics and the output, so the variance is that of the
+// differences (two passes over registers, no cancellation) and HBM sees x (and
+// dy) once and y (dx) once.  The kernels are bound by those bytes, a single
+// token by its launch.
+//
+// A row belongs to TPR threads, eight consecutive elements per thread and step.
+// Up to kWaveRow channels that is one wave, whose sums need no barrier; wider
+// rows take a workgroup.
+// Rows start at any element (odd D): the 16-byte accesses are made at the
+// element type's alignment, which global memory allows, and only a row's last
+// piece is element by element.
+//
+// The weight's and bias's gradients: each thread of the backward owns fixed
+// columns and adds them up over its rows in fp32, a workgroup leaves one partial
+// row, and ln_param_kernel adds the partial rows in a fixed order (no atomics:
+// the same inputs give the same bits).
+#include "rr_common.h"
+
+#include <algorithm>
+#include <string>
+
+namespace {
+
+using rr::bf16;
+using rr::f16;
+
+constexpr int64_t kMaxChannels = 32768;   // 1024 threads, 4 steps of 8 elements
+constexpr int kPartRows = 512;            // partial rows of dw and db at most
+
+// Eight elements from p (any alignment of T), widened.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+  } else {
+    typedef uint16_t u8 __attribute__((ext_vector_type(8), aligned(2)));
+    const u8 a = *reinterpret_cast<const u8*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = rr::to_f32(__builtin_bit_cast(T, (uint16_t)a[e]));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    *reinterpret_cast<f4*>(p) = f4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f4*>(p + 4) = f4{v[4], v[5], v[6], v[7]};
+  } else {
+    typedef uint16_t u8 __attribute__((ext_vector_type(8), aligned(2)));
+    u8 a;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = __builtin_bit_cast(uint16_t, rr::from_f32<T>(v[e]));
+    *reinterpret_cast<u8*>(p) = a;
+  }
+}
+// The elements of columns c .. c + 7 of a row of D (0 past its end).
+template <typename T>
+__device__ __forceinline__ void load_cols(const T* row, int c, int D, float (&v)[8]) {
+  if (c + 8 <= D) {
+    load8(row + c, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < D ? rr::to_f32(row[c + e]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&v)[8]) {
+  if (c + 8 <= D) {
+    store8(row + c, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < D) row[c + e] = rr::from_f32<T>(v[e]);
+  }
+}
+// The weight or bias, of any of the three types (one uniform branch a piece), or `fill` where there is none.
+__device__ __forceinline__ void load_param(const void* p, int dtype, int c, int D, float fill, float (&v)[8]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fill;
+  } else if (dtype == RR_F32) {
+    load_cols(static_cast<const float*>(p), c, D, v);
+  } else if (dtype == RR_BF16) {
+    load_cols(static_cast<const bf16*>(p), c, D, v);
+  } else {
+    load_cols(static_cast<const f16*>(p), c, D, v);
+  }
+}
+
+// Sums of a and b over the TPR threads of a row, in every thread (the same bits
+// in each).  TPR > 64: a workgroup, through `buf` (2 floats a wave).
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* buf) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o, 64), b += __shfl_xor(b, o, 64);
+  if constexpr (TPR > 64) {
+    const int w = threadIdx.x >> 6;
+    __syncthreads();   // the last sum's reads of buf are done
+    if ((threadIdx.x & 63) == 0) buf[2 * w] = a, buf[2 * w + 1] = b;
+    __syncthreads();
+    a = 0.f, b = 0.f;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) a += buf[2 * i], b += buf[2 * i + 1];
+  }
+}
+
+template <int TPR> constexpr int block_threads() { return TPR == 64 ? 256 : TPR; }
+
+// One row per TPR threads; NV pieces of 8 elements per thread.
+template <typename X, typename Y, int TPR, int NV>
+__global__ void __launch_bounds__(block_threads<TPR>())
+ln_fwd_kernel(const X* __restrict__ x, const void* w, const void* b, int wdt, int64_t rows, int D, float eps,
+              Y* __restrict__ y, float* mean, float* rstd) {
+  __shared__ float buf[2 * (TPR / 64)];
+  constexpr int RPB = block_threads<TPR>() / TPR;
+  const int lane = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  if (row >= rows) return;   // a whole wave (TPR 64), or no row at all
+  const X* xr = x + row * D;
+  float v[NV][8];
+  float s = 0.f, zero = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) load_cols(xr, (j * TPR + lane) * 8, D, v[j]);
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[j][e];
+  row_sum2<TPR>(s, zero, buf);
+  const float inv = 1.f / (float)D;
+  const float mu = s * inv;
+  float q = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = (j * TPR + lane) * 8 + e < D ? v[j][e] - mu : 0.f;
+      v[j][e] = d;
+      q += d * d;
+    }
+  zero = 0.f;
+  row_sum2<TPR>(q, zero, buf);
+  const float r = 1.f / sqrtf(q * inv + eps);
+  if (mean != nullptr && lane == 0) mean[row] = mu, rstd[row] = r;
+  Y* yr = y + row * D;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * TPR + lane) * 8;
+    if (c >= D) break;
+    float wv[8], bv[8], o[8];
+    load_param(w, wdt, c, D, 1.f, wv);
+    load_param(b, wdt, c, D, 0.f, bv);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = v[j][e] * r * wv[e] + bv[e];
+    store_cols(yr, c, D, o);
+  }
+}
+
+// Rows strided over the grid; dw and db partials of the workgroup's rows in
+// part[block][2][D] (null: not wanted).
+template <typename X, typename Y, int TPR, int NV>
+__global__ void __launch_bounds__(block_threads<TPR>())
+ln_bwd_kernel(const Y* __restrict__ dy, const X* __restrict__ x, const void* w, int wdt, const float* mean,
+              const float* rstd, int64_t rows, int D, X* __restrict__ dx, float* __restrict__ part) {
+  __shared__ float buf[2 * (TPR / 64)];
+  constexpr int RPB = block_threads<TPR>() / TPR;
+  __shared__ float cols[RPB > 1 ? (RPB - 1) * 64 * 8 : 1];
+  const int lane = threadIdx.x % TPR;
+  const int slot = threadIdx.x / TPR;
+  float wv[NV][8], dw[NV][8], db[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * TPR + lane) * 8;
+    if (c < D) load_param(w, wdt, c, D, 1.f, wv[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (c >= D) wv[j][e] = 0.f;
+      dw[j][e] = 0.f, db[j][e] = 0.f;
+    }
+  }
+  const float inv = 1.f / (float)D;
+  for (int64_t row = (int64_t)blockIdx.x * RPB + slot; row < rows; row += (int64_t)gridDim.x * RPB) {
+    const float mu = mean[row], r = rstd[row];
+    float xh[NV][8], g[NV][8];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TPR + lane) * 8;
+      load_cols(x + row * D, c, D, xh[j]);
+      load_cols(dy + row * D, c, D, g[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = g[j][e];          // 0 past the row's end
+        const float h = (j * TPR + lane) * 8 + e < D ? (xh[j][e] - mu) * r : 0.f;
+        dw[j][e] += d * h, db[j][e] += d;
+        xh[j][e] = h;
+        g[j][e] = d * wv[j][e];
+        s1 += g[j][e], s2 += g[j][e] * h;
+      }
+    if (dx != nullptr) {
+      row_sum2<TPR>(s1, s2, buf);
+      s1 *= inv, s2 *= inv;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * TPR + lane) * 8;
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = r * (g[j][e] - s1 - xh[j][e] * s2);
+        if (c < D) store_cols(dx + row * D, c, D, o);
+      }
+    }
+  }
+  if (part == nullptr) return;
+  float* pw = part + (int64_t)blockIdx.x * 2 * D;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float(&acc)[8] = h == 0 ? dw[j] : db[j];
+      if constexpr (RPB > 1) {   // the waves of the workgroup, in order
+        __syncthreads();
+        if (slot > 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) cols[((slot - 1) * 8 + e) * 64 + lane] = acc[e];
+        }
+        __syncthreads();
+        if (slot == 0) {
+          for (int q = 0; q < RPB - 1; ++q)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += cols[(q * 8 + e) * 64 + lane];
+        }
+      }
+      const int c = (j * TPR + lane) * 8;
+      if (slot == 0 && c < D) store_cols(pw + h * D, c, D, acc);
+    }
+}
+
+// dw and db from the partial rows: a workgroup takes 64 columns of one of them,
+// its four waves every fourth partial row, added up in order.
+__global__ void __launch_bounds__(256)
+ln_param_kernel(const float* __restrict__ part, int n, int D, void* dw, void* db, int wdt) {
+  __shared__ float buf[4][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int c = blockIdx.x * 64 + lane, h = blockIdx.y;
+  void* out = h == 0 ? dw : db;
+  if (out == nullptr) return;
+  float s = 0.f;
+  if (c < D)
+    for (int i = wave; i < n; i += 4) s += part[((int64_t)i * 2 + h) * D + c];
+  buf[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || c >= D) return;
+  s = buf[0][lane] + buf[1][lane] + buf[2][lane] + buf[3][lane];
+  if (wdt == RR_F32) static_cast<float*>(out)[c] = s;
+  else if (wdt == RR_BF16) static_cast<bf16*>(out)[c] = rr::from_f32<bf16>(s);
+  else static_cast<f16*>(out)[c] = rr::from_f32<f16>(s);
+}
+
+// Threads a row and pieces a thread for D channels.
+struct Shape { int tpr, nv; };
+Shape shape_of(int64_t D, bool bwd) {
+  const int64_t v = (D + 7) / 8;   // pieces of a row
+  const int tpr = v <= 64 * (bwd ? 2 : 4) ? 64 : v <= 256 * 4 ? 256 : 1024;
+  return {tpr, (int)((v + tpr - 1) / tpr)};
+}
+int64_t bwd_blocks(int64_t rows, int64_t D) {
+  const Shape s = shape_of(D, true);
+  const int64_t rpb = s.tpr == 64 ? 4 : 1;
+  return std::max<int64_t>(1, std::min<int64_t>(kPartRows, (rows + rpb - 1) / rpb));
+}
+
+int check_args(const char* who, int64_t rows, int64_t D, int xdt, int ydt, int wdt) {
+  const std::string w(who);
+  if (rows < 0 || D <= 0) return rr::fail(RR_EINVAL, w + ": rows must be >= 0 and D > 0");
+  if (D > kMaxChannels) return rr::fail(RR_EUNSUPPORTED, w + ": at most " + std::to_string(kMaxChannels) +
+                                                             " channels, got " + std::to_string(D));
+  if (!rr::valid_dtype(xdt) || !rr::valid_dtype(ydt) || !rr::valid_dtype(wdt)) {
+    return rr::fail(RR_EINVAL, w + ": unsupported dtype");
+  }
+  if (ydt != xdt && xdt != RR_F32) return rr::fail(RR_EINVAL, w + ": y has x's dtype, or any where x is fp32");
+  if (rows >= ((int64_t)1 << 31)) return rr::fail(RR_EUNSUPPORTED, w + ": too many rows");
+  return RR_OK;
+}
+
+}  // namespace
+
+#define LN_NV(TPR, KERNEL, NB, ...)                                                                              \
+  switch (sh.nv) {                                                                                               \
+    case 1: KERNEL<X, Y, TPR, 1><<<NB, block_threads<TPR>(), 0, s>>>(__VA_ARGS__); break;                        \
+    case 2: KERNEL<X, Y, TPR, 2><<<NB, block_threads<TPR>(), 0, s>>>(__VA_ARGS__); break;                        \
+    case 3: KERNEL<X, Y, TPR, 3><<<NB, block_threads<TPR>(), 0, s>>>(__VA_ARGS__); break;                        \
+    default: KERNEL<X, Y, TPR, 4><<<NB, block_threads<TPR>(), 0, s>>>(__VA_ARGS__); break;                       \
+  }
+#define LN_SHAPE(KERNEL, NB, ...)                                                                                \
+  if (sh.tpr == 64) { LN_NV(64, KERNEL, NB, __VA_ARGS__) }                                                       \
+  else if (sh.tpr == 256) { LN_NV(256, KERNEL, NB, __VA_ARGS__) }                                                \
+  else { LN_NV(1024, KERNEL, NB, __VA_ARGS__) }
+// x and y types: the same, or fp32 x with any y.
+#define LN_TYPES(...)                                                                                            \
+  if (x_dtype == RR_BF16) { using X = bf16; using Y = bf16; __VA_ARGS__ }                                        \
+  else if (x_dtype == RR_F16) { using X = f16; using Y = f16; __VA_ARGS__ }                                      \
+  else if (y_dtype == RR_F32) { using X = float; using Y = float; __VA_ARGS__ }                                  \
+  else if (y_dtype == RR_BF16) { using X = float; using Y = bf16; __VA_ARGS__ }                                  \
+  else { using X = float; using Y = f16; __VA_ARGS__ }
+
+extern "C" int rr_layer_norm_fwd(const void* x, int x_dtype, const void* w, const void* b, int w_dtype, int64_t rows,
+                                 int64_t D, float eps, void* y, int y_dtype, float* mean, float* rstd, void* stream) {
+  if (int rc = check_args("rr_layer_norm_fwd", rows, D, x_dtype, y_dtype, w_dtype)) return rc;
+  if (!(eps >= 0.f)) return rr::fail(RR_EINVAL, "rr_layer_norm_fwd: eps must not be negative");
+  if (rows == 0) return RR_OK;
+  if (x == nullptr || y == nullptr || (mean == nullptr) != (rstd == nullptr)) {
+    return rr::fail(RR_EINVAL, "rr_layer_norm_fwd: null pointer");
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const Shape sh = shape_of(D, false);
+  const int nb = (int)(sh.tpr == 64 ? (rows + 3) / 4 : rows);
+  LN_TYPES(LN_SHAPE(ln_fwd_kernel, nb, static_cast<const X*>(x), w, b, w_dtype, rows, (int)D, eps, static_cast<Y*>(y), mean,
+                    rstd))
+  return rr::check_launch("rr_layer_norm_fwd");
+}
+
+extern "C" size_t rr_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t D) {
+  if (rows <= 0 || D <= 0 || D > kMaxChannels) return 0;
+  return (size_t)bwd_blocks(rows, D) * 2 * (size_t)D * sizeof(float);
+}
+
+extern "C" int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, const void* w, int w_dtype,
+                                 const float* mean, const float* rstd, int64_t rows, int64_t D, void* dx, void* dw,
+                                 void* db, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_args("rr_layer_norm_bwd", rows, D, x_dtype, y_dtype, w_dtype)) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool params = dw != nullptr || db != nullptr;
+  const int64_t nb = rows == 0 ? 0 : bwd_blocks(rows, D);
+  if (rows > 0) {
+    if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr) {
+      return rr::fail(RR_EINVAL, "rr_layer_norm_bwd: null pointer");
+    }
+    if (params && (workspace == nullptr || workspace_bytes < rr_layer_norm_bwd_workspace_bytes(rows, D))) {
+      return rr::fail(RR_EWORKSPACE, "rr_layer_norm_bwd: workspace too small");
+    }
+    if (params && reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+      return rr::fail(RR_EWORKSPACE, "rr_layer_norm_bwd: workspace misaligned");
+    }
+    if (!params && dx == nullptr) return RR_OK;
+    float* part = params ? static_cast<float*>(workspace) : nullptr;
+    const Shape sh = shape_of(D, true);
+    LN_TYPES(LN_SHAPE(ln_bwd_kernel, (int)nb, static_cast<const Y*>(dy), static_cast<const X*>(x), w, w_dtype, mean, rstd,
+                      rows, (int)D, static_cast<X*>(dx), part))
+  }
+  if (params) {
+    const dim3 grid((unsigned)((D + 63) / 64), 2);
+    ln_param_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(workspace), (int)nb, (int)D, dw, db, w_dtype);
+  }
+  return rr::check_launch("rr_layer_norm_bwd");
+}

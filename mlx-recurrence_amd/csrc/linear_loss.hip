@@ -1,0 +1,949 @@
+// linear_loss.hip — losses over a large vocabulary straight from hidden states, on
+// gfx950: cross entropy on labels and distillation from a teacher's top logits.
+//
+//   z = h w^T  [rows, V];  s = z / tau;  lse = log sum_v exp(s_v);  q = exp(s - lse)
+//   cross entropy (tau = 1)  loss = lse - z_label + zl lse^2
+//                            dz = c ((1 + 2 zl lse) q - 1[v = label])
+//   distillation             p = softmax over the row's teacher entries of t / tau
+//                            loss = tau^2 sum_k p_k (log p_k - log q_{id_k})
+//                            dz = c tau (q - sum_{k: id_k = v} p_k)
+//   dh = dz w,  dw = dz^T h,  c the row's upstream gradient
+//
+// A label is a teacher with one entry of weight 1, so both run on the same
+// kernels.  The logits [rows, V] are never stored.  The forward forms them a tile
+// at a time and keeps each row's running maximum and sum per tile and the logits
+// of the row's entries.  The backward forms them again, a piece of the vocabulary
+// at a time, rounds that piece of dz to the operands' 16 bits (for fp32 inputs and
+// for few rows to two planes of them, below), and uses it for dw (complete for the
+// piece) and dh (added up over the pieces in fp32).
+//
+// Rows that count for nothing (an ignored label, no teacher entry) are left out
+// before the products: the rows that remain are gathered, in order, and their
+// number stays on the device.  What such a row's hidden state holds is not read.
+//
+// fp32 inputs are split into two fp16 planes, x s = hi + lo (s a power of two that
+// brings the largest finite value of the tensor just below 2^15; the pair holds 22
+// bits), and a product is the three of the planes that are not below the last bit:
+// about fp32's own accuracy at a third of the fp16 rate, above the fp32 MFMA's.
+// fp16 dz, and the planes of fp32's, carry a power of two that brings the largest
+// |dz| just below 2^14, so that small probabilities keep their bits; bf16 needs
+// none.
+//
+// Everything is added up in a fixed order: no atomics but integer maxima.
+#include "rr_common.h"
+#include "rr_gemm.h"
+#include "rr_mfma.h"
+
+#include <algorithm>
+#include <string>
+
+namespace {
+
+using rr::bf16;
+using rr::f16;
+using namespace rr::gemm;
+
+constexpr int kAbsent = 0x7fffffff;
+constexpr int64_t kMaxEntries = 1024;      // teacher entries of a row
+constexpr int64_t kMaxVocab = 1 << 24;
+constexpr int64_t kMaxChannels = 1 << 16;
+constexpr int64_t kPieceBytes = (int64_t)512 << 20;   // of dz, where the rows leave room for a piece of kMinPiece
+constexpr int64_t kMinPiece = 2048;
+constexpr int64_t kFewRows = 64;           // rows whose dz keeps a second plane
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+constexpr int BM = 128, BN = 128;
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// ------------------------------------------------------------------ state
+// What the forward leaves for the backward, in one buffer of the caller's.
+struct Header {
+  int n;                 // rows that count
+  uint32_t amax_h, amax_w;   // largest finite |hidden| (rows that count) and |weight|, as bits (fp32 inputs)
+  uint32_t pad[61];
+};
+struct State {
+  Header* hdr;
+  int* rows;     // [rows] the i-th row that counts
+  int* pos;      // [rows] its place there, -1 for a row that does not count
+  float* lse2;   // [rows] log2 of the row's sum of exponentials (in the order of `rows`)
+  float* loss;   // [rows]
+  int* ids;      // [rows][K] the entries' columns, ascending; kAbsent past the last
+  float* p;      // [rows][K] their weights
+  float* z2;     // [rows][K] their logits, times log2(e) / tau
+};
+size_t state_layout(int64_t T, int64_t K, char* base, State* s) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* at = base + off;
+    off += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  State t;
+  t.hdr = reinterpret_cast<Header*>(take(sizeof(Header)));
+  t.rows = reinterpret_cast<int*>(take((size_t)T * 4));
+  t.pos = reinterpret_cast<int*>(take((size_t)T * 4));
+  t.lse2 = reinterpret_cast<float*>(take((size_t)T * 4));
+  t.loss = reinterpret_cast<float*>(take((size_t)T * 4));
+  t.ids = reinterpret_cast<int*>(take((size_t)T * K * 4));
+  t.p = reinterpret_cast<float*>(take((size_t)T * K * 4));
+  t.z2 = reinterpret_cast<float*>(take((size_t)T * K * 4));
+  if (s != nullptr) *s = t;
+  return off;
+}
+
+// ------------------------------------------------------------------ plan
+struct Plan {
+  int64_t T, D, V;
+  int dtype;
+  int planes;          // of the inputs: 2 for fp32
+  int planes_z;        // of dz
+  bool copy_w;         // the weight is copied (planes, or rows that are not whole 16-byte chunks)
+  int64_t Tp, Dp;      // rows to whole tiles, channels to whole k steps
+  int64_t nvt, ntt, ndt;   // tiles of V, T, D
+  // backward
+  int64_t Vp;          // columns of a piece (whole tiles)
+  int64_t splits;      // parts of a piece's columns that dh is added up in
+};
+Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
+  Plan p{};
+  p.T = T, p.D = D, p.V = V, p.dtype = dtype;
+  p.planes = dtype == RR_F32 ? 2 : 1;
+  // The rounding of dz to 16 bits averages out over the rows of dw; few rows get a
+  // second plane, which costs nothing there (the weight's bytes bound the products).
+  p.planes_z = p.planes == 2 || T <= kFewRows ? 2 : 1;
+  p.copy_w = p.planes == 2 || D % 8 != 0;
+  p.Tp = up(T, BN), p.Dp = up(D, BK);
+  p.nvt = up(V, BM) / BM, p.ntt = p.Tp / BN, p.ndt = up(D, BM) / BM;
+  const int64_t most = std::max(kMinPiece, kPieceBytes / (p.Tp * 2 * p.planes_z) / BM * BM);
+  const int64_t pieces = (p.nvt * BM + most - 1) / most;
+  p.Vp = up((p.nvt * BM + pieces - 1) / pieces, BM);
+  // enough workgroups for the GPU, of at least 8 k steps each
+  const int64_t tiles = p.ntt * p.ndt;
+  p.splits = std::max<int64_t>(1, std::min<int64_t>({1024 / std::max<int64_t>(1, tiles), p.Vp / (8 * BK), 64}));
+  return p;
+}
+
+struct FwdWs {
+  uint16_t* h;     // [planes][T][Dp]
+  uint16_t* w;     // [planes][V][Dp] where the weight is copied
+  float2* part;    // [nvt][Tp] maximum and sum of a tile's row
+};
+size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* at = base + off;
+    off += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  const size_t planes = p.planes;
+  FwdWs t;
+  t.h = reinterpret_cast<uint16_t*>(take(planes * p.T * p.Dp * 2));
+  t.w = reinterpret_cast<uint16_t*>(take(p.copy_w ? planes * p.V * p.Dp * 2 : 0));
+  t.part = reinterpret_cast<float2*>(take((size_t)p.nvt * p.Tp * sizeof(float2)));
+  if (s != nullptr) *s = t;
+  return off;
+}
+struct BwdWs {
+  uint16_t* h;
+  uint16_t* w;
+  float* scale;    // [0] the factor on both gradients
+  float2* coef;    // [Tp] a row's factors (coef_kernel)
+  uint16_t* dz;    // [planes_z][Tp][Vp]
+  float* dh;       // [splits][Tp][ndt * BM]
+};
+size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* at = base + off;
+    off += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  const size_t planes = p.planes;
+  BwdWs t;
+  t.h = reinterpret_cast<uint16_t*>(take(planes * p.T * p.Dp * 2));
+  t.w = reinterpret_cast<uint16_t*>(take(p.copy_w ? planes * p.V * p.Dp * 2 : 0));
+  t.scale = reinterpret_cast<float*>(take(256));
+  t.coef = reinterpret_cast<float2*>(take((size_t)p.Tp * sizeof(float2)));
+  t.dz = reinterpret_cast<uint16_t*>(take((size_t)p.planes_z * p.Tp * p.Vp * 2));
+  t.dh = reinterpret_cast<float*>(take((size_t)p.splits * p.Tp * p.ndt * BM * 4));
+  if (s != nullptr) *s = t;
+  return off;
+}
+
+// ------------------------------------------------------------------ rows and entries
+// A power of two that brings a largest value of these bits into [2^(e - 1), 2^e)
+// (1 where there is none); kept within 2^+-60 so that products of two stay finite.
+__device__ __forceinline__ float pow2_to(uint32_t amax_bits, int e) {
+  if (amax_bits == 0) return 1.f;
+  const int x = (int)(amax_bits >> 23) - 127;   // floor(log2) of a normal value
+  return ldexpf(1.f, max(-60, min(60, e - 1 - x)));
+}
+__device__ __forceinline__ float scale_h(const Header* h) { return pow2_to(h->amax_h, 15); }
+__device__ __forceinline__ float scale_w(const Header* h) { return pow2_to(h->amax_w, 15); }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// A row's teacher entries by column (a wave per row): ids ascending, absent ones
+// (id < 0 or a logit of -inf) last, and their softmax weights.  An id past the
+// vocabulary makes the row's weights, and with them its loss and gradients, NaN.
+// pos[row] = 1 where the row has an entry.
+template <typename E>
+__global__ void __launch_bounds__(64)
+entries_kernel(const E* __restrict__ logits, const int64_t* __restrict__ ids_in, int K, int KP, int V, float inv_tau,
+               int* __restrict__ ids, float* __restrict__ p, int* __restrict__ pos) {
+  extern __shared__ char sm[];
+  int* id = reinterpret_cast<int*>(sm);
+  float* t = reinterpret_cast<float*>(sm) + KP;
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  float worst = 0.f;   // NaN: an id past the vocabulary
+  for (int k = lane; k < KP; k += 64) {
+    int i = kAbsent;
+    float v = -INFINITY;
+    if (k < K) {
+      const int64_t raw = ids_in[row * K + k];
+      const float x = rr::to_f32(logits[row * K + k]) * inv_tau;
+      if (raw >= V) worst = NAN;
+      if (raw >= 0 && raw < V && x != -INFINITY) i = (int)raw, v = x;
+    }
+    id[k] = i, t[k] = v;
+  }
+  __syncthreads();
+  for (int size = 2; size <= KP; size *= 2)
+    for (int step = size / 2; step > 0; step /= 2) {
+      for (int k = lane; k < KP / 2; k += 64) {
+        const int a = 2 * k - (k & (step - 1)), b = a + step;
+        const bool asc = (a & size) == 0;
+        const int ia = id[a], ib = id[b];
+        if ((ia > ib) == asc && ia != ib) {
+          const float ta = t[a], tb = t[b];
+          id[a] = ib, id[b] = ia, t[a] = tb, t[b] = ta;
+        }
+      }
+      __syncthreads();
+    }
+  float m = -INFINITY;
+  for (int k = lane; k < K; k += 64) m = fmaxf(m, t[k]);
+  m = wave_max(m);
+  const bool any = id[0] != kAbsent;
+  float s = 0.f;
+  for (int k = lane; k < K; k += 64)
+    if (id[k] != kAbsent) s += expf(t[k] - m);
+  s = wave_add(s) + wave_add(worst);
+  for (int k = lane; k < K; k += 64) {
+    ids[row * K + k] = id[k];
+    p[row * K + k] = id[k] != kAbsent ? expf(t[k] - m) / s : s != s ? NAN : 0.f;
+  }
+  if (lane == 0) pos[row] = any || s != s ? 1 : 0;
+}
+
+// The rows that count, in order (one workgroup).  Labels: `labels` decides, and
+// their entries are written here; an invalid label is an absent entry of weight
+// NaN.  Teacher: pos holds what entries_kernel found.
+template <bool LABELS>
+__global__ void __launch_bounds__(1024)
+rows_kernel(const int64_t* __restrict__ labels, int64_t ignore, int64_t T, int V, State st) {
+  __shared__ int sums[16];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  int base = 0;
+  for (int64_t i0 = 0; i0 < T; i0 += 1024) {
+    const int64_t i = i0 + tid;
+    bool in = false;
+    if (i < T) {
+      if constexpr (LABELS) {
+        const int64_t l = labels[i];
+        in = l != ignore;
+        const bool ok = l >= 0 && l < V;
+        st.ids[i] = ok ? (int)l : kAbsent;
+        st.p[i] = ok || !in ? 1.f : NAN;
+      } else {
+        in = st.pos[i] != 0;
+      }
+    }
+    const uint64_t b = __ballot(in);
+    const int before = __popcll(b & ((1ull << lane) - 1));
+    __syncthreads();   // the last turn's reads of sums are done
+    if (lane == 0) sums[wave] = __popcll(b);
+    __syncthreads();
+    int at = base, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) at += sums[w];
+      all += sums[w];
+    }
+    at += before;
+    if (i < T) {
+      st.pos[i] = in ? at : -1;
+      if (in) st.rows[at] = (int)i;
+      if (!in) st.loss[i] = 0.f;
+    }
+    base += all;
+  }
+  if (tid == 0) st.hdr->n = base, st.hdr->amax_h = 0, st.hdr->amax_w = 0;
+}
+
+// Largest finite |x| of the rows (through `rows`, the first hdr->n of them, where given).
+__global__ void __launch_bounds__(256)
+amax_kernel(const float* __restrict__ x, int64_t n_rows, int D, const int* rows, const Header* hdr, uint32_t* out) {
+  const int64_t n = rows != nullptr ? hdr->n : n_rows;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float m = 0.f;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < n; r += (int64_t)gridDim.x * 4) {
+    const float* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
+    for (int c = lane; c < D; c += 64) {
+      const float a = fabsf(xr[c]);
+      if (a < INFINITY) m = fmaxf(m, a);   // neither infinite nor NaN
+    }
+  }
+  m = wave_max(m);
+  if (lane == 0 && m > 0.f) atomicMax(out, __float_as_uint(m));
+}
+
+// Rows as operands: copied (16-bit inputs) or split into two planes (fp32), padded
+// with zeros to Dp channels; through `rows` (the first hdr->n of them) where given.
+template <typename X>
+__global__ void __launch_bounds__(256)
+pack_kernel(const X* __restrict__ x, int64_t n_rows, int D, int Dp, const int* rows, const Header* hdr, int which,
+            uint16_t* __restrict__ out, int64_t plane) {
+  const int64_t n = rows != nullptr ? hdr->n : n_rows;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float sc = 1.f;
+  if constexpr (sizeof(X) == 4) sc = which == 0 ? scale_h(hdr) : scale_w(hdr);
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < n; r += (int64_t)gridDim.x * 4) {
+    const X* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
+    uint16_t* o = out + r * Dp;
+    for (int c = lane * 2; c < Dp; c += 128) {
+      if constexpr (sizeof(X) == 4) {
+        uint32_t hi = 0, lo = 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float v = c + e < D ? xr[c + e] * sc : 0.f;
+          const uint16_t hb = op_bits<OpF16>(v);
+          hi |= (uint32_t)hb << (16 * e);
+          lo |= (uint32_t)op_bits<OpF16>(v - op_val<OpF16>(hb)) << (16 * e);
+        }
+        *reinterpret_cast<uint32_t*>(o + c) = hi;
+        *reinterpret_cast<uint32_t*>(o + plane + c) = lo;
+      } else {
+        uint32_t v = 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (c + e < D) v |= (uint32_t)__builtin_bit_cast(uint16_t, xr[c + e]) << (16 * e);
+        *reinterpret_cast<uint32_t*>(o + c) = v;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ logits
+struct LogitArgs {
+  const uint16_t* w;      // [V][ldw]
+  const uint16_t* h;      // [n][Dp]
+  int64_t ldw, ldh, plane_w, plane_h;
+  int V, D, Dp, K, Tp;
+  float c;                // log2(e) / tau
+  State st;
+  float2* part;           // forward
+  const float2* coef;     // backward
+  uint16_t* dz;
+  int64_t ldz, plane_z;
+  int v_first;            // the piece's first column
+};
+
+// A logit in units of log2 is rounded before the maximum or lse is taken off: fused into
+// one operation, a logit would not be 0 off itself, and a sure word's probability not 1.
+__device__ __forceinline__ float rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Walks the entries of row `orig` whose column lies in this wave's v0 .. v0 + 32 MI
+// and in this lane's half of the accumulator rows: f(k, element) with the element's
+// index mi * 16 + e.
+template <int MI, typename F>
+__device__ __forceinline__ void each_entry(const int* ids, int K, int v0, int half, bool on, F f) {
+  int lo = 0;
+  if (on) {
+    int hi = K;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (ids[mid] < v0) lo = mid + 1;
+      else hi = mid;
+    }
+  }
+  for (int k = lo; on && k < K; ++k) {
+    const int rel = ids[k] - v0;
+    if (rel >= 32 * MI) break;
+    if (((rel >> 2) & 1) == half) f(k, (rel >> 5) * 16 + ((rel & 31) >> 3) * 4 + (rel & 3));
+  }
+}
+
+// z^T tiles: m = vocabulary, n = rows, so that a lane holds 16 MI logits of one row.
+template <typename Op, bool GRAD, int PX, int PZ>
+__global__ void __launch_bounds__(256)
+logits_kernel(LogitArgs a) {
+  using P = Product<Op, BM, BN, 2, 2, false, false>;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
+  const int n = a.st.hdr->n;
+  const int ntt = a.Tp / BN;
+  const int tt = blockIdx.x % ntt, vt = blockIdx.x / ntt;
+  const int t0 = tt * BN, v0 = a.v_first + vt * BM;
+  if (t0 >= n) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / P::WN, wn = wave % P::WN;
+  const int half = lane >> 5;
+
+  typename P::Acc acc;
+  const Operand A{a.w + (int64_t)v0 * a.ldw, a.ldw, a.plane_w, a.V - v0, (int)a.ldw};
+  const Operand B{a.h + (int64_t)t0 * a.ldh, a.ldh, a.plane_h, n - t0, a.Dp};
+  P::template run<PX, PX>(acc, A, B, 0, a.Dp, lds);
+
+  float c = a.c;
+  if constexpr (PX == 2) c /= scale_h(a.st.hdr) * scale_w(a.st.hdr);
+  const int vw = v0 + wm * (BM / P::WM);
+  float* red = reinterpret_cast<float*>(lds);   // forward: [WM][BN][2]
+#pragma unroll
+  for (int j = 0; j < P::NI; ++j) {
+    const int tl = wn * (BN / P::WN) + 32 * j + (lane & 31);
+    const int t = t0 + tl;
+    const bool on = t < n;
+    const int64_t orig = on ? a.st.rows[t] : 0;
+    const int* ids = a.st.ids + orig * a.K;
+    if constexpr (!GRAD) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int v = vw + 32 * i + 8 * (e / 4) + 4 * half + e % 4;
+          acc[i][j][e] = v < a.V ? rounded(acc[i][j][e] * c) : -INFINITY;
+          m = fmaxf(m, acc[i][j][e]);
+        }
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s += m == -INFINITY ? acc[i][j][e] - m : exp2_fast(acc[i][j][e] - m);
+      if (m == -INFINITY && s != s) {   // no column of the vocabulary, or NaN among the logits
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) bad |= acc[i][j][e] != acc[i][j][e];
+        s = bad ? NAN : 0.f;
+      }
+      each_entry<P::MI>(ids, a.K, vw, half, on, [&](int k, int el) {
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z = el == i * 16 + e ? acc[i][j][e] : z;
+        a.st.z2[orig * a.K + k] = z;
+      });
+      // the other half's rows of the same column, then the waves along m
+      const float m2 = __shfl_xor(m, 32, 64), s2 = __shfl_xor(s, 32, 64);
+      const float mm = fmaxf(m, m2);
+      s = (m == mm ? s : s * exp2_fast(m - mm)) + (m2 == mm ? s2 : s2 * exp2_fast(m2 - mm));
+      if (half == 0) {
+        red[(wm * BN + tl) * 2] = mm;
+        red[(wm * BN + tl) * 2 + 1] = s;
+      }
+    } else {
+      const float2 co = on ? a.coef[t] : make_float2(0.f, 0.f);
+      const float l2 = on ? a.st.lse2[t] : 0.f;
+#pragma unroll
+      for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int v = vw + 32 * i + 8 * (e / 4) + 4 * half + e % 4;
+          acc[i][j][e] = on && v < a.V ? exp2_fast(rounded(acc[i][j][e] * c) - l2) : 0.f;
+        }
+      // q - p first, so that what is left of a sure label keeps its bits
+      each_entry<P::MI>(ids, a.K, vw, half, on, [&](int k, int el) {
+        const float p = a.st.p[orig * a.K + k], r = p * co.y;
+#pragma unroll
+        for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = el == i * 16 + e ? acc[i][j][e] - p + r : acc[i][j][e];
+      });
+      uint16_t* o = a.dz + (int64_t)t * a.ldz + (vw - a.v_first) + 4 * half;
+#pragma unroll
+      for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          rr::u16x4_t hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = on ? co.x * acc[i][j][4 * q + e] : 0.f;
+            hi[e] = op_bits<Op>(v);
+            if constexpr (PZ == 2) lo[e] = op_bits<Op>(v - op_val<Op>(hi[e]));
+          }
+          *reinterpret_cast<rr::u16x4_t*>(o + 32 * i + 8 * q) = hi;
+          if constexpr (PZ == 2) *reinterpret_cast<rr::u16x4_t*>(o + a.plane_z + 32 * i + 8 * q) = lo;
+        }
+    }
+  }
+  if constexpr (!GRAD) {
+    __syncthreads();
+    for (int tl = threadIdx.x; tl < BN; tl += P::THREADS) {
+      float m = -INFINITY, s = 0.f;
+      for (int w = 0; w < P::WM; ++w) m = fmaxf(m, red[(w * BN + tl) * 2]);
+      for (int w = 0; w < P::WM; ++w) {
+        const float mw = red[(w * BN + tl) * 2], sw = red[(w * BN + tl) * 2 + 1];
+        s += mw == m ? sw : sw * exp2_fast(mw - m);
+      }
+      a.part[(int64_t)vt * a.Tp + t0 + tl] = make_float2(m, s);
+    }
+  }
+}
+
+// Per row: the tiles' maxima and sums to the row's lse, and its loss.  A wave per row.
+__global__ void __launch_bounds__(256)
+row_loss_kernel(State st, const float2* __restrict__ part, int64_t T, int nvt, int64_t Tp, int K, bool labels, float zl,
+                float tau, float* __restrict__ out) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+  if (t >= st.hdr->n) return;
+  const int64_t row = st.rows[t];
+  float m = -INFINITY, s = 0.f;
+  for (int v = lane; v < nvt; v += 64) {
+    const float2 x = part[(int64_t)v * Tp + t];
+    const float mm = fmaxf(m, x.x);
+    s = (m == mm ? s : s * exp2f(m - mm)) + (x.x == mm ? x.y : x.y * exp2f(x.x - mm));
+    m = mm;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+    const float mm = fmaxf(m, m2);
+    s = (m == mm ? s : s * exp2f(m - mm)) + (m2 == mm ? s2 : s2 * exp2f(m2 - mm));
+    m = mm;
+  }
+  float l2 = m + log2f(s);
+  float loss = 0.f;
+  for (int k = lane; k < K; k += 64) {
+    const float p = st.p[row * K + k];
+    if (p == 0.f) continue;
+    if (st.ids[row * K + k] == kAbsent) {   // an id outside the vocabulary
+      loss = NAN;
+      continue;
+    }
+    const float logq = (st.z2[row * K + k] - l2) * kLn2;
+    loss += labels ? -logq : p * (logf(p) - logq);
+  }
+  loss = wave_add(loss);
+  if (labels) {
+    const float lse = l2 * kLn2;
+    loss += zl * lse * lse;
+  } else {
+    loss *= tau * tau;
+  }
+  if (lane == 0) {
+    out[row] = loss;
+    st.lse2[t] = loss != loss ? NAN : l2;   // the backward's row is NaN where the loss is
+  }
+}
+
+// The sum of the rows' losses, over the number that count where `mean` (0 without any).
+__global__ void __launch_bounds__(1024)
+sum_loss_kernel(const float* __restrict__ loss, int64_t T, const Header* hdr, bool mean, float* out) {
+  __shared__ float buf[16];
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < T; i += 1024) s += loss[i];
+  s = wave_add(s);
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  s = 0.f;
+  for (int w = 0; w < 16; ++w) s += buf[w];
+  out[0] = mean ? s / (float)max(1, hdr->n) : s;
+}
+
+// ------------------------------------------------------------------ gradients
+// coef[t] = (c f, 1 - 1 / f) with f = 1 + 2 zl lse, so that a row of dz is
+// c f (q - p + p (1 - 1 / f)), and the factor on both gradients, scale[0].  One upstream
+// gradient for all rows goes into that factor and c = 1: -1 at a label is exact in 16
+// bits, where -c would be off by the same rounding in every row.  Otherwise c is the
+// row's.  `scaled`: c carries the power of two that brings the largest of them below
+// 2^14, and the factor its inverse.  One workgroup.
+__global__ void __launch_bounds__(1024)
+coef_kernel(State st, const float* __restrict__ dloss, bool per_row, bool mean, float factor, float zl, bool scaled,
+            float2* __restrict__ coef, float* scale) {
+  __shared__ float buf[16];
+  const int n = st.hdr->n;
+  float m = 0.f;
+  for (int t = threadIdx.x; t < n; t += 1024) {
+    const float c = per_row ? dloss[st.rows[t]] * factor : 1.f;
+    const float x = 2.f * zl * st.lse2[t] * kLn2;
+    float f = 1.f + x;
+    if (f == 0.f) f = 1e-30f;
+    coef[t] = make_float2(c * f, x / f);
+    const float a = fmaxf(fabsf(c * f), fabsf(c));   // |dz| <= 2 a
+    if (a < INFINITY) m = fmaxf(m, a);
+  }
+  float sc = 1.f;
+  if (scaled) {   // the same for the whole workgroup
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = 0.f;
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, buf[w]);
+    sc = pow2_to(__float_as_uint(m), 14);
+    for (int t = threadIdx.x; t < n; t += 1024) coef[t].x *= sc;   // this thread's own
+  }
+  if (threadIdx.x == 0) scale[0] = (per_row ? 1.f : dloss[0] * factor * (mean ? 1.f / (float)max(1, n) : 1.f)) / sc;
+}
+
+// dh^T tiles of one part of the piece: m = channels, n = rows, k = the piece's columns.
+struct DhArgs {
+  const uint16_t* w;     // at the piece's first row
+  const uint16_t* dz;
+  int64_t ldw, ldz, plane_w, plane_z;
+  int V, D, Dp, Tp, ndt, splits, cols;   // V: rows of w from the piece on; cols: the piece's columns to whole k steps
+  float* out;            // [splits][Tp][ndt * BM]
+  bool first;
+  State st;
+};
+template <typename Op, int PX, int PZ>
+__global__ void __launch_bounds__(256)
+dh_kernel(DhArgs a) {
+  using P = Product<Op, BM, BN, 2, 2, true, false>;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
+  const int n = a.st.hdr->n;
+  int b = blockIdx.x;
+  const int dt = b % a.ndt;
+  b /= a.ndt;
+  const int tt = b % (a.Tp / BN), sp = b / (a.Tp / BN);
+  const int t0 = tt * BN, d0 = dt * BM;
+  if (t0 >= n) return;
+  const int steps = a.cols / BK;
+  const int k0 = (int)((int64_t)steps * sp / a.splits) * BK, k1 = (int)((int64_t)steps * (sp + 1) / a.splits) * BK;
+  typename P::Acc acc;
+  const Operand A{a.w + d0, a.ldw, a.plane_w, a.V, (int)a.ldw - d0};
+  const Operand B{a.dz + (int64_t)t0 * a.ldz, a.ldz, a.plane_z, a.Tp - t0, a.cols};
+  P::template run<PX, PZ>(acc, A, B, k0, k1, lds);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / P::WN, wn = wave % P::WN;
+#pragma unroll
+  for (int j = 0; j < P::NI; ++j) {
+    const int t = t0 + wn * (BN / P::WN) + 32 * j + (lane & 31);
+    float* o = a.out + ((int64_t)sp * a.Tp + t) * a.ndt * BM + d0 + wm * (BM / P::WM) + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float4* at = reinterpret_cast<float4*>(o + 32 * i + 8 * q);
+        float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+        if (!a.first) {
+          const float4 u = *at;
+          v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        *at = v;
+      }
+  }
+}
+
+// dh of every row from its parts, in the inputs' type; 0 for rows that do not count.
+template <typename X>
+__global__ void __launch_bounds__(256)
+dh_out_kernel(State st, const float* __restrict__ part, int64_t T, int D, int64_t ldp, int64_t stride, int splits,
+              const float* scale, X* __restrict__ dh) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  if (row >= T) return;
+  const int t = st.pos[row];
+  float f = scale[0];
+  if constexpr (sizeof(X) == 4) f /= scale_w(st.hdr);
+  for (int c = lane; c < D; c += 64) {
+    float s = 0.f;
+    if (t >= 0)
+      for (int i = 0; i < splits; ++i) s += part[(int64_t)i * stride + (int64_t)t * ldp + c];
+    dh[row * D + c] = rr::from_f32<X>(s * f);
+  }
+}
+
+// dw^T tiles of the piece: m = channels, n = the piece's columns, k = rows.
+struct DwArgs {
+  const uint16_t* h;
+  const uint16_t* dz;
+  int64_t ldh, ldz, plane_h, plane_z;
+  int V, D, Dp, ndt;     // V: rows of dw from the piece on
+  const float* scale;
+  void* out;             // dw at the piece's first row
+  State st;
+};
+template <typename Op, typename X, int PX, int PZ>
+__global__ void __launch_bounds__(256)
+dw_kernel(DwArgs a) {
+  using P = Product<Op, BM, BN, 2, 2, true, true>;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
+  const int n = a.st.hdr->n;
+  const int dt = blockIdx.x % a.ndt, vt = blockIdx.x / a.ndt;
+  const int d0 = dt * BM, v0 = vt * BN;
+  typename P::Acc acc;
+  const Operand A{a.h + d0, a.ldh, a.plane_h, n, a.Dp - d0};
+  const Operand B{a.dz + v0, a.ldz, a.plane_z, n, BN};
+  P::template run<PX, PZ>(acc, A, B, 0, (n + BK - 1) / BK * BK, lds);
+  float f = a.scale[0];
+  if constexpr (PX == 2) f /= scale_h(a.st.hdr);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / P::WN, wn = wave % P::WN;
+#pragma unroll
+  for (int j = 0; j < P::NI; ++j) {
+    const int v = v0 + wn * (BN / P::WN) + 32 * j + (lane & 31);
+    if (v >= a.V) continue;
+    X* o = static_cast<X*>(a.out) + (int64_t)v * a.D;
+#pragma unroll
+    for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int d = d0 + wm * (BM / P::WM) + 32 * i + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+        if (d < a.D) o[d] = rr::from_f32<X>(acc[i][j][e] * f);
+      }
+  }
+}
+
+// ------------------------------------------------------------------ host
+int check_dims(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int dtype, int reduction) {
+  const std::string w(who);
+  if (T < 0 || D <= 0 || V <= 0) return rr::fail(RR_EINVAL, w + ": rows must be >= 0, channels and vocabulary > 0");
+  if (!rr::valid_dtype(dtype)) return rr::fail(RR_EINVAL, w + ": unsupported dtype");
+  if (reduction < 0 || reduction > 2) return rr::fail(RR_EINVAL, w + ": reduction must be 0 (none), 1 (mean) or 2 (sum)");
+  if (K < 1 || K > kMaxEntries) {
+    return rr::fail(RR_EUNSUPPORTED, w + ": 1 to " + std::to_string(kMaxEntries) + " teacher entries a row, got " +
+                                         std::to_string(K));
+  }
+  if (V > kMaxVocab || D > kMaxChannels) {
+    return rr::fail(RR_EUNSUPPORTED, w + ": at most " + std::to_string(kMaxVocab) + " words and " +
+                                         std::to_string(kMaxChannels) + " channels");
+  }
+  if (T >= ((int64_t)1 << 24) || up(V, BM) / BM * (up(T, BN) / BN) >= (1 << 23)) {   // grids below 2^32 threads
+    return rr::fail(RR_EUNSUPPORTED, w + ": too many rows");
+  }
+  return RR_OK;
+}
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <typename X>
+void pack_rows(const Plan& p, const void* hidden, const void* weight, const State& st, uint16_t* h, uint16_t* w, bool amax,
+               hipStream_t s) {
+  if constexpr (sizeof(X) == 4) {
+    if (amax) {
+      amax_kernel<<<512, 256, 0, s>>>(static_cast<const float*>(hidden), p.T, (int)p.D, st.rows, st.hdr, &st.hdr->amax_h);
+      amax_kernel<<<1024, 256, 0, s>>>(static_cast<const float*>(weight), p.V, (int)p.D, nullptr, st.hdr, &st.hdr->amax_w);
+    }
+  }
+  pack_kernel<X><<<(unsigned)std::min<int64_t>(2048, (p.T + 3) / 4), 256, 0, s>>>(
+      static_cast<const X*>(hidden), p.T, (int)p.D, (int)p.Dp, st.rows, st.hdr, 0, h, p.T * p.Dp);
+  if (p.copy_w) {
+    pack_kernel<X><<<(unsigned)std::min<int64_t>(8192, (p.V + 3) / 4), 256, 0, s>>>(
+        static_cast<const X*>(weight), p.V, (int)p.D, (int)p.Dp, nullptr, st.hdr, 1, w, p.V * p.Dp);
+  }
+}
+
+// What both products read of the weight.
+LogitArgs logit_args(const Plan& p, const State& st, const void* weight, uint16_t* h, uint16_t* w, int K, float tau) {
+  LogitArgs a{};
+  a.w = p.copy_w ? w : static_cast<const uint16_t*>(weight);
+  a.h = h;
+  a.ldw = p.copy_w ? p.Dp : p.D, a.ldh = p.Dp;
+  a.plane_w = p.V * p.Dp, a.plane_h = p.T * p.Dp;
+  a.V = (int)p.V, a.D = (int)p.D, a.Dp = (int)p.Dp, a.K = K, a.Tp = (int)p.Tp;
+  a.c = kLog2e / tau;
+  a.st = st;
+  return a;
+}
+
+template <typename X, typename Op, int PX>
+int forward(const Plan& p, const void* hidden, const void* weight, const State& st, const FwdWs& ws, int K, bool labels,
+            float zl, float tau, int reduction, float* loss, hipStream_t s) {
+  pack_rows<X>(p, hidden, weight, st, ws.h, ws.w, true, s);
+  LogitArgs a = logit_args(p, st, weight, ws.h, ws.w, K, tau);
+  a.part = ws.part;
+  logits_kernel<Op, false, PX, PX><<<(unsigned)(p.nvt * p.ntt), 256, 0, s>>>(a);
+  float* rows = reduction == 0 ? loss : st.loss;
+  row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, p.T, (int)p.nvt, p.Tp, K, labels, zl, tau, rows);
+  if (reduction != 0) sum_loss_kernel<<<1, 1024, 0, s>>>(st.loss, p.T, st.hdr, reduction == 1, loss);
+  return rr::check_launch("rr_linear_loss");
+}
+
+template <typename X, typename Op, int PX, int PZ>
+int backward(const Plan& p, const float* dloss, const void* hidden, const void* weight, const State& st, const BwdWs& ws,
+             int K, float zl, float tau, int reduction, void* dh, void* dw, hipStream_t s) {
+  pack_rows<X>(p, hidden, weight, st, ws.h, ws.w, false, s);
+  coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, reduction == 1, tau, zl, !__is_same(Op, OpBf16), ws.coef,
+                                 ws.scale);
+  for (int64_t v = 0; v < p.nvt * BM; v += p.Vp) {
+    const int64_t cols = std::min(p.Vp, p.nvt * BM - v);   // whole tiles
+    LogitArgs a = logit_args(p, st, weight, ws.h, ws.w, K, tau);
+    a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp, a.plane_z = p.Tp * p.Vp, a.v_first = (int)v;
+    logits_kernel<Op, true, PX, PZ><<<(unsigned)(cols / BM * p.ntt), 256, 0, s>>>(a);
+    if (dh != nullptr) {
+      DhArgs b{};
+      b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = p.Vp, b.plane_w = a.plane_w, b.plane_z = a.plane_z;
+      b.V = (int)(p.V - v), b.D = a.D, b.Dp = a.Dp, b.Tp = a.Tp, b.ndt = (int)p.ndt, b.splits = (int)p.splits;
+      b.cols = (int)cols, b.out = ws.dh, b.first = v == 0, b.st = st;
+      dh_kernel<Op, PX, PZ><<<(unsigned)(p.ndt * p.ntt * p.splits), 256, 0, s>>>(b);
+    }
+    if (dw != nullptr) {
+      DwArgs c{};
+      c.h = ws.h, c.dz = ws.dz, c.ldh = p.Dp, c.ldz = p.Vp, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
+      c.V = (int)(p.V - v), c.D = a.D, c.Dp = a.Dp, c.ndt = (int)p.ndt, c.scale = ws.scale;
+      c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
+      dw_kernel<Op, X, PX, PZ><<<(unsigned)(cols / BN * p.ndt), 256, 0, s>>>(c);
+    }
+  }
+  if (dh != nullptr) {
+    dh_out_kernel<X><<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.dh, p.T, (int)p.D, p.ndt * BM, p.Tp * p.ndt * BM,
+                                                              (int)p.splits, ws.scale, static_cast<X*>(dh));
+  }
+  return rr::check_launch("rr_linear_loss_bwd");
+}
+
+// One more kernel for what has no rows: the loss is 0, the gradients are 0.
+__global__ void zero_kernel(uint32_t* p, int64_t words, uint16_t* tail) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) p[i] = 0;
+  if (tail != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *tail = 0;
+}
+void zero(void* p, int64_t bytes, hipStream_t s) {
+  if (p == nullptr || bytes == 0) return;
+  zero_kernel<<<1024, 256, 0, s>>>(static_cast<uint32_t*>(p), bytes / 4,
+                                   bytes % 4 ? static_cast<uint16_t*>(p) + bytes / 2 - 1 : nullptr);
+}
+
+int run_forward(const char* who, const void* hidden, const void* weight, int dtype, int64_t T, int64_t D, int64_t V,
+                int64_t K, bool labels, float zl, float tau, int reduction, float* loss, const State& st, void* workspace,
+                size_t workspace_bytes, hipStream_t s) {
+  const Plan p = plan_of(T, D, V, dtype);
+  FwdWs ws;
+  fwd_layout(p, static_cast<char*>(workspace), &ws);
+  if (dtype == RR_BF16) return forward<bf16, OpBf16, 1>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
+  if (dtype == RR_F16) return forward<f16, OpF16, 1>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
+  return forward<float, OpF16, 2>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
+}
+
+int check_buffers(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int dtype, int pass, const void* hidden,
+                  const void* weight, const void* state, size_t state_bytes, const void* ws, size_t ws_bytes) {
+  const std::string w(who);
+  if (hidden == nullptr || weight == nullptr || state == nullptr || ws == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
+  if (!aligned16(hidden) || !aligned16(weight)) return rr::fail(RR_EINVAL, w + ": buffers must be 16-byte aligned");
+  if (state_bytes < rr_linear_loss_state_bytes(T, K)) return rr::fail(RR_EWORKSPACE, w + ": state buffer too small");
+  if (ws_bytes < rr_linear_loss_workspace_bytes(T, D, V, dtype, pass)) return rr::fail(RR_EWORKSPACE, w + ": workspace too small");
+  if (!aligned16(state) || !aligned16(ws)) return rr::fail(RR_EWORKSPACE, w + ": state buffer or workspace misaligned");
+  return RR_OK;
+}
+
+}  // namespace
+
+extern "C" size_t rr_linear_loss_state_bytes(int64_t rows, int64_t K) {
+  if (rows <= 0 || K < 1 || K > kMaxEntries) return 0;
+  return state_layout(rows, K, nullptr, nullptr);
+}
+
+extern "C" size_t rr_linear_loss_workspace_bytes(int64_t rows, int64_t D, int64_t V, int dtype, int pass) {
+  if (rows <= 0 || check_dims("rr_linear_loss_workspace_bytes", rows, D, V, 1, dtype, 0) != RR_OK) return 0;
+  const Plan p = plan_of(rows, D, V, dtype);
+  return pass == 0 ? fwd_layout(p, nullptr, nullptr) : bwd_layout(p, nullptr, nullptr);
+}
+
+extern "C" int rr_linear_ce_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                                const int64_t* labels, int64_t ignore_index, float z_loss, int reduction, float* loss,
+                                void* state, size_t state_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "rr_linear_ce_fwd";
+  if (int rc = check_dims(who, rows, D, V, 1, dtype, reduction)) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows > 0 || reduction != 0) {
+    if (loss == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
+  }
+  if (rows == 0) {
+    if (reduction != 0) zero(loss, 4, s);
+    return rr::check_launch(who);
+  }
+  if (labels == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
+  if (int rc = check_buffers(who, rows, D, V, 1, dtype, 0, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
+  State st;
+  state_layout(rows, 1, static_cast<char*>(state), &st);
+  State in = st;
+  if (reduction == 0) in.loss = loss;   // where rows that do not count leave their 0
+  rows_kernel<true><<<1, 1024, 0, s>>>(labels, ignore_index, rows, (int)V, in);
+  return run_forward(who, hidden, weight, dtype, rows, D, V, 1, true, z_loss, 1.f, reduction, loss, st, workspace,
+                     workspace_bytes, s);
+}
+
+extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                                const void* teacher_logits, int teacher_dtype, const int64_t* teacher_ids, int64_t K,
+                                float temperature, int reduction, float* loss, void* state, size_t state_bytes,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "rr_linear_kd_fwd";
+  if (int rc = check_dims(who, rows, D, V, K, dtype, reduction)) return rc;
+  if (!rr::valid_dtype(teacher_dtype)) return rr::fail(RR_EINVAL, std::string(who) + ": unsupported teacher dtype");
+  if (!(temperature > 0.f) || !(temperature < 1e30f)) {
+    return rr::fail(RR_EINVAL, std::string(who) + ": temperature must be positive and finite");
+  }
+  if (rows * K >= ((int64_t)1 << 31)) return rr::fail(RR_EUNSUPPORTED, std::string(who) + ": too many teacher entries");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows > 0 || reduction != 0) {
+    if (loss == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
+  }
+  if (rows == 0) {
+    if (reduction != 0) zero(loss, 4, s);
+    return rr::check_launch(who);
+  }
+  if (teacher_logits == nullptr || teacher_ids == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
+  if (int rc = check_buffers(who, rows, D, V, K, dtype, 0, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
+  State st;
+  state_layout(rows, K, static_cast<char*>(state), &st);
+  int KP = 1;
+  while (KP < K) KP *= 2;
+  RR_DISPATCH_DTYPE(teacher_dtype, {
+    entries_kernel<InT><<<(unsigned)rows, 64, (size_t)KP * 8, s>>>(static_cast<const InT*>(teacher_logits), teacher_ids, (int)K,
+                                                                  KP, (int)V, 1.f / temperature, st.ids, st.p, st.pos);
+  });
+  State in = st;
+  if (reduction == 0) in.loss = loss;
+  rows_kernel<false><<<1, 1024, 0, s>>>(nullptr, 0, rows, (int)V, in);
+  return run_forward(who, hidden, weight, dtype, rows, D, V, K, false, 0.f, temperature, reduction, loss, st, workspace,
+                     workspace_bytes, s);
+}
+
+extern "C" int rr_linear_loss_bwd(const float* dloss, const void* hidden, const void* weight, int dtype, int64_t rows,
+                                  int64_t D, int64_t V, int64_t K, float z_loss, float temperature, int reduction,
+                                  const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  const char* who = "rr_linear_loss_bwd";
+  if (int rc = check_dims(who, rows, D, V, K, dtype, reduction)) return rc;
+  if (!(temperature > 0.f) || !(temperature < 1e30f)) {
+    return rr::fail(RR_EINVAL, std::string(who) + ": temperature must be positive and finite");
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t es = dtype == RR_F32 ? 4 : 2;
+  if (rows == 0) {
+    zero(dweight, V * D * es, s);
+    return rr::check_launch(who);
+  }
+  if (dloss == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
+  if (int rc = check_buffers(who, rows, D, V, K, dtype, 1, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
+  if (dhidden == nullptr && dweight == nullptr) return RR_OK;
+  const Plan p = plan_of(rows, D, V, dtype);
+  State st;
+  state_layout(rows, K, static_cast<char*>(const_cast<void*>(state)), &st);
+  BwdWs ws;
+  bwd_layout(p, static_cast<char*>(workspace), &ws);
+#define LL_BACKWARD(X, OP, PX, PZ) \
+  backward<X, OP, PX, PZ>(p, dloss, hidden, weight, st, ws, (int)K, z_loss, temperature, reduction, dhidden, dweight, s)
+  if (dtype == RR_BF16) return p.planes_z == 2 ? LL_BACKWARD(bf16, OpBf16, 1, 2) : LL_BACKWARD(bf16, OpBf16, 1, 1);
+  if (dtype == RR_F16) return p.planes_z == 2 ? LL_BACKWARD(f16, OpF16, 1, 2) : LL_BACKWARD(f16, OpF16, 1, 1);
+  return LL_BACKWARD(float, OpF16, 2, 2);
+#undef LL_BACKWARD
+}

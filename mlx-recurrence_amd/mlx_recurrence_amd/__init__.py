@@ -8,6 +8,13 @@ Drop-in counterpart of the v2 scan API of D-CSIL/mlx-recurrence 0.3.0
     rglru   — RG-LRU diagonal recurrence
     rotlru  — rotational LRU (complex-diagonal scan over (u, w) pairs)
 
+and, next to the scans, what a model of these layers ends in (no counterpart in
+the reference):
+
+    norm         — layer norm
+    linear_loss  — cross entropy and distillation over a large vocabulary, from
+                   hidden states, without storing the logits
+
 Each scan keeps the reference's signature, shape rules and fp32 state /
 accumulation, and is differentiable through ``torch.autograd``.  The compute
 runs in hand-written HIP kernels for gfx950 (librecurrence_gfx950.so, C ABI in
@@ -28,6 +35,9 @@ from ._chassis import DEFAULT_SEG, SIMD_WIDTH, get_or_build_kernel, check_segmen
 from ._lib import async_status
 from .step import ssd_step, gla_step, rglru_step, rotlru_step
 from .gdn import gated_deltanet_scan, gated_deltanet_scan_with_state, gated_deltanet_reference
+from .norm import layer_norm, layer_norm_reference
+from .linear_loss import (linear_cross_entropy, linear_cross_entropy_reference, linear_distillation,
+                          linear_distillation_reference)
 
 __all__ = [
     "ssd_scan",
@@ -60,6 +70,10 @@ __all__ = [
     "gated_deltanet_scan",
     "gated_deltanet_scan_with_state",
     "gated_deltanet_reference",
+    "layer_norm",
+    "layer_norm_reference",
+    "linear_cross_entropy",
+    "linear_cross_entropy_reference",
+    "linear_distillation",
+    "linear_distillation_reference",
 ]
-
-__version__ = "0.3.0+gfx950"

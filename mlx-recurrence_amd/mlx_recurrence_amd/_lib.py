@@ -34,6 +34,7 @@ _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
 _c_ptr = ctypes.c_void_p
 _c_size = ctypes.c_size_t
+_c_f32 = ctypes.c_float
 
 # name -> (restype, argtypes)
 _SIGS = {
@@ -79,6 +80,18 @@ _SIGS = {
     "rr_gdn_fwd_workspace_bytes": (_c_size, [_c_i64] * 5 + [_c_int]),
     "rr_gdn_workspace_bytes": (_c_size, [_c_i64] * 5 + [_c_int]),
     "rr_gdn_bwd": (_c_int, [_c_ptr] * 7 + [_c_int] + [_c_i64] * 5 + [_c_ptr] * 9 + [_c_size, _c_ptr]),
+    "rr_layer_norm_fwd": (_c_int, [_c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_i64, _c_i64, _c_f32, _c_ptr, _c_int]
+                          + [_c_ptr] * 3),
+    "rr_layer_norm_bwd_workspace_bytes": (_c_size, [_c_i64] * 2),
+    "rr_layer_norm_bwd": (_c_int, [_c_ptr, _c_int] * 3 + [_c_ptr] * 2 + [_c_i64] * 2 + [_c_ptr] * 4 + [_c_size, _c_ptr]),
+    "rr_linear_loss_state_bytes": (_c_size, [_c_i64] * 2),
+    "rr_linear_loss_workspace_bytes": (_c_size, [_c_i64] * 3 + [_c_int] * 2),
+    "rr_linear_ce_fwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 3 + [_c_ptr, _c_i64, _c_f32, _c_int]
+                         + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
+    "rr_linear_kd_fwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 3 + [_c_ptr, _c_int, _c_ptr, _c_i64, _c_f32, _c_int]
+                         + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
+    "rr_linear_loss_bwd": (_c_int, [_c_ptr] * 3 + [_c_int] + [_c_i64] * 4 + [_c_f32] * 2 + [_c_int, _c_ptr, _c_size]
+                           + [_c_ptr] * 3 + [_c_size, _c_ptr]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGS)
@@ -501,3 +514,47 @@ def gdn_bwd(dy, dfinal, q, k, v, alpha, beta, h0, ckpt, seg, dq, dk, dv, dalpha,
                              DTYPE_CODE[q.dtype], B, L, H, Dh, seg, ptr(h0), ptr(ckpt), ptr(dq), ptr(dk), ptr(dv),
                              ptr(dalpha), ptr(dbeta), ptr(dh0), ptr(ws), 0 if ws is None else ws.numel(),
                              stream_of(q)), "rr_gdn_bwd")
+
+
+# ---------------------------------------------------------------- output head
+def layer_norm_fwd(x, w, b, w_dtype, rows, D, eps, y, mean, rstd):
+    _check(load().rr_layer_norm_fwd(ptr(x), DTYPE_CODE[x.dtype], ptr(w), ptr(b), DTYPE_CODE[w_dtype], rows, D, eps, ptr(y),
+                                    DTYPE_CODE[y.dtype], ptr(mean), ptr(rstd), stream_of(x)), "rr_layer_norm_fwd")
+
+
+def layer_norm_bwd(dy, x, w, w_dtype, mean, rstd, rows, D, dx, dw, db):
+    params = dw is not None or db is not None
+    ws = _alloc_ws(_ws_bytes("rr_layer_norm_bwd_workspace_bytes", (rows, D)), x.device) if params else None
+    _check(load().rr_layer_norm_bwd(ptr(dy), DTYPE_CODE[dy.dtype], ptr(x), DTYPE_CODE[x.dtype], ptr(w), DTYPE_CODE[w_dtype],
+                                    ptr(mean), ptr(rstd), rows, D, ptr(dx), ptr(dw), ptr(db), ptr(ws),
+                                    0 if ws is None else ws.numel(), stream_of(x)), "rr_layer_norm_bwd")
+
+
+def linear_loss_buffers(rows, D, V, K, dtype, device):
+    """State (kept for the backward) and workspace of a forward."""
+    state = _alloc_ws(_ws_bytes("rr_linear_loss_state_bytes", (rows, K)), device)
+    return state, _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[dtype], 0)), device)
+
+
+def linear_ce_fwd(hidden, weight, labels, ignore_index, z_loss, reduction, loss, state, ws):
+    (rows, D), V = hidden.shape, weight.shape[0]
+    _check(load().rr_linear_ce_fwd(ptr(hidden), ptr(weight), DTYPE_CODE[hidden.dtype], rows, D, V, ptr(labels), ignore_index,
+                                   z_loss, reduction, ptr(loss), ptr(state), 0 if state is None else state.numel(), ptr(ws),
+                                   0 if ws is None else ws.numel(), stream_of(hidden)), "rr_linear_ce_fwd")
+
+
+def linear_kd_fwd(hidden, weight, teacher_logits, teacher_ids, temperature, reduction, loss, state, ws):
+    (rows, D), V = hidden.shape, weight.shape[0]
+    _check(load().rr_linear_kd_fwd(ptr(hidden), ptr(weight), DTYPE_CODE[hidden.dtype], rows, D, V, ptr(teacher_logits),
+                                   DTYPE_CODE[teacher_logits.dtype], ptr(teacher_ids), teacher_ids.shape[1], temperature,
+                                   reduction, ptr(loss), ptr(state), 0 if state is None else state.numel(), ptr(ws),
+                                   0 if ws is None else ws.numel(), stream_of(hidden)), "rr_linear_kd_fwd")
+
+
+def linear_loss_bwd(dloss, hidden, weight, K, z_loss, temperature, reduction, state, dhidden, dweight):
+    (rows, D), V = hidden.shape, weight.shape[0]
+    ws = _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[hidden.dtype], 1)), hidden.device)
+    _check(load().rr_linear_loss_bwd(ptr(dloss), ptr(hidden), ptr(weight), DTYPE_CODE[hidden.dtype], rows, D, V, K, z_loss,
+                                     temperature, reduction, ptr(state), 0 if state is None else state.numel(),
+                                     ptr(dhidden), ptr(dweight), ptr(ws), 0 if ws is None else ws.numel(),
+                                     stream_of(hidden)), "rr_linear_loss_bwd")
