@@ -49,10 +49,12 @@ constexpr int64_t kMaxVocab = 1 << 24;
 constexpr int64_t kMaxChannels = 1 << 16;
 constexpr int64_t kPieceBytes = (int64_t)512 << 20;   // of dz, where the rows leave room for a piece of kMinPiece
 constexpr int64_t kMinPiece = 2048;
+constexpr int64_t kMaxPiece = 1 << 20;       // a row of a tile's operand is at most so long
 constexpr int64_t kFewRows = 64;           // rows whose dz keeps a second plane
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-constexpr int BM = 128, BN = 128;
+constexpr int BM = 256, BN = 256;   // a tile of each product
+constexpr int kThreads = 512;
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
@@ -116,7 +118,7 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   p.copy_w = p.planes == 2 || D % 8 != 0;
   p.Tp = up(T, BN), p.Dp = up(D, BK);
   p.nvt = up(V, BM) / BM, p.ntt = p.Tp / BN, p.ndt = up(D, BM) / BM;
-  const int64_t most = std::max(kMinPiece, kPieceBytes / (p.Tp * 2 * p.planes_z) / BM * BM);
+  const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * 2 * p.planes_z) / BM * BM));
   const int64_t pieces = (p.nvt * BM + most - 1) / most;
   p.Vp = up((p.nvt * BM + pieces - 1) / pieces, BM);
   // enough workgroups for the GPU, of at least 8 k steps each
@@ -391,9 +393,9 @@ __device__ __forceinline__ void each_entry(const int* ids, int K, int v0, int ha
 
 // z^T tiles: m = vocabulary, n = rows, so that a lane holds 16 MI logits of one row.
 template <typename Op, bool GRAD, int PX, int PZ>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
 logits_kernel(LogitArgs a) {
-  using P = Product<Op, BM, BN, 2, 2, false, false>;
+  using P = Product<Op, BM, BN, 2, 4, false, false>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
   const int ntt = a.Tp / BN;
@@ -616,9 +618,9 @@ struct DhArgs {
   State st;
 };
 template <typename Op, int PX, int PZ>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
 dh_kernel(DhArgs a) {
-  using P = Product<Op, BM, BN, 2, 2, true, false>;
+  using P = Product<Op, BM, BN, 2, 4, true, false>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
   int b = blockIdx.x;
@@ -684,9 +686,9 @@ struct DwArgs {
   State st;
 };
 template <typename Op, typename X, int PX, int PZ>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads)
 dw_kernel(DwArgs a) {
-  using P = Product<Op, BM, BN, 2, 2, true, true>;
+  using P = Product<Op, BM, BN, 2, 4, true, true>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
   const int dt = blockIdx.x % a.ndt, vt = blockIdx.x / a.ndt;
@@ -771,7 +773,7 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
   pack_rows<X>(p, hidden, weight, st, ws.h, ws.w, true, s);
   LogitArgs a = logit_args(p, st, weight, ws.h, ws.w, K, tau);
   a.part = ws.part;
-  logits_kernel<Op, false, PX, PX><<<(unsigned)(p.nvt * p.ntt), 256, 0, s>>>(a);
+  logits_kernel<Op, false, PX, PX><<<(unsigned)(p.nvt * p.ntt), kThreads, 0, s>>>(a);
   float* rows = reduction == 0 ? loss : st.loss;
   row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, p.T, (int)p.nvt, p.Tp, K, labels, zl, tau, rows);
   if (reduction != 0) sum_loss_kernel<<<1, 1024, 0, s>>>(st.loss, p.T, st.hdr, reduction == 1, loss);
@@ -788,20 +790,20 @@ int backward(const Plan& p, const float* dloss, const void* hidden, const void* 
     const int64_t cols = std::min(p.Vp, p.nvt * BM - v);   // whole tiles
     LogitArgs a = logit_args(p, st, weight, ws.h, ws.w, K, tau);
     a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp, a.plane_z = p.Tp * p.Vp, a.v_first = (int)v;
-    logits_kernel<Op, true, PX, PZ><<<(unsigned)(cols / BM * p.ntt), 256, 0, s>>>(a);
+    logits_kernel<Op, true, PX, PZ><<<(unsigned)(cols / BM * p.ntt), kThreads, 0, s>>>(a);
     if (dh != nullptr) {
       DhArgs b{};
       b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = p.Vp, b.plane_w = a.plane_w, b.plane_z = a.plane_z;
       b.V = (int)(p.V - v), b.D = a.D, b.Dp = a.Dp, b.Tp = a.Tp, b.ndt = (int)p.ndt, b.splits = (int)p.splits;
       b.cols = (int)cols, b.out = ws.dh, b.first = v == 0, b.st = st;
-      dh_kernel<Op, PX, PZ><<<(unsigned)(p.ndt * p.ntt * p.splits), 256, 0, s>>>(b);
+      dh_kernel<Op, PX, PZ><<<(unsigned)(p.ndt * p.ntt * p.splits), kThreads, 0, s>>>(b);
     }
     if (dw != nullptr) {
       DwArgs c{};
       c.h = ws.h, c.dz = ws.dz, c.ldh = p.Dp, c.ldz = p.Vp, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
       c.V = (int)(p.V - v), c.D = a.D, c.Dp = a.Dp, c.ndt = (int)p.ndt, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
-      dw_kernel<Op, X, PX, PZ><<<(unsigned)(cols / BN * p.ndt), 256, 0, s>>>(c);
+      dw_kernel<Op, X, PX, PZ><<<(unsigned)(cols / BN * p.ndt), kThreads, 0, s>>>(c);
     }
   }
   if (dh != nullptr) {

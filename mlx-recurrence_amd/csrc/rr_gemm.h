@@ -11,6 +11,13 @@
 // are permuted by row (an XOR) to spread them over the banks:
 //   k contiguous  row r, 8 chunks of 8 k:      chunk c at c ^ ((r & 7) ^ ((r >> 3) & 1))
 //   k-major       row k, pieces of 16 columns: piece q at q ^ (2 (k & 3) ^ ((k >> 1) & 1))
+//
+// A step of 64 k is loaded by buffer loads that write LDS themselves (16 bytes a lane,
+// the permutation made by the lanes' addresses), into one of two LDS buffers, while the
+// other is multiplied.  The loads of a step are issued as soon as every wave has read
+// its last fragments of the buffer, a whole step before they are waited for, so one
+// barrier a step does: it says both that the buffer is free and that the next is full.
+// Fragments are read one k group (16) ahead of their products.
 #pragma once
 
 #include "rr_common.h"
@@ -51,13 +58,31 @@ __device__ __forceinline__ float op_val(uint16_t b) {
 // o < outer, i < inner it reads as 0.  k contiguous: o = the tile's row, i = k;
 // k-major: o = k, i = the tile's column.  ld and inner are multiples of 8, p
 // 16-byte aligned.  `plane`: elements from the high to the low plane of an
-// operand that is split in two.
+// operand that is split in two.  ld <= 2^20, so that a tile spans less than 2^30 bytes.
 struct Operand {
   const uint16_t* p;
   int64_t ld;
   int64_t plane;
   int outer, inner;
 };
+
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+// 16 bytes a lane from buffer `rsrc` at byte `voff` (0 where that is past its end) to
+// LDS byte `lds` + 16 lane.  Not known to the compiler: the reader waits for vmcnt.
+__device__ __forceinline__ void load_to_lds(i32x4_t rsrc, int voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+// What is written before stays before (the compiler would sink the reads to their uses).
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
+// A barrier behind this wave's LDS reads and its loads to LDS.
+__device__ __forceinline__ void loads_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lds_byte(const uint16_t* p) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane(
+      (int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t*)p);
+}
 
 template <int ROWS, bool KMAJOR>
 struct Tile {
@@ -94,41 +119,86 @@ struct Tile {
   }
 };
 
+// The loads of one operand's tile by the WAVES waves of a workgroup.
+template <int ROWS, bool KMAJOR, int WAVES>
+struct Loader {
+  using T = Tile<ROWS, KMAJOR>;
+  static constexpr int N = T::CHUNKS / (64 * WAVES);   // loads a thread and step
+  static_assert(T::CHUNKS % (64 * WAVES) == 0, "every thread stages the same number of chunks");
+  static constexpr int kPast = 0x40000000;   // beyond any buffer here
+  int voff[N];
+  int col;          // first element of this thread's chunks along the inner axis
+  int ldb, outer, inner;
+  const char* at;   // the next step
+
+  __device__ __forceinline__ void init(const Operand& o, int wave, int lane) {
+    ldb = (int)o.ld * 2, outer = o.outer, inner = o.inner;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      int row, c;
+      T::at((j * WAVES + wave) * 64 + lane, row, c);   // c is the same for every j
+      voff[j] = row * ldb + c * 16;
+      col = c * 8;
+    }
+    if constexpr (KMAJOR) {
+      if (col >= inner)
+#pragma unroll
+        for (int j = 0; j < N; ++j) voff[j] = kPast;
+    }
+  }
+  __device__ __forceinline__ void seek(const uint16_t* p, int k) {
+    at = reinterpret_cast<const char*>(p) + (KMAJOR ? (int64_t)k * ldb : (int64_t)k * 2);
+  }
+  // The step that starts at k, to LDS byte `lds`.
+  __device__ __forceinline__ void issue(int k, uint32_t lds, int wave) {
+    const int rows = KMAJOR ? min(outer - k, BK) : min(outer, ROWS);
+    const int bytes = rows <= 0 ? 0 : (rows - 1) * ldb + (KMAJOR ? inner : inner - k) * 2;
+    const uint64_t b = reinterpret_cast<uint64_t>(at);
+    i32x4_t r;
+    r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff);
+    r[2] = __builtin_amdgcn_readfirstlane(bytes);
+    r[3] = 0x00020000;   // raw 32-bit buffer
+    const int past = !KMAJOR && k + col >= inner ? kPast : 0;   // the rest of a last step's row
+#pragma unroll
+    for (int j = 0; j < N; ++j) load_to_lds(r, voff[j] | past, lds + (uint32_t)(j * WAVES + wave) * 1024);
+    at += KMAJOR ? (int64_t)BK * ldb : BK * 2;
+  }
+};
+
 // WM x WN waves, each with MI x NI blocks of 32 x 32.
 template <typename OpT, int BM_, int BN_, int WM_, int WN_, bool AK_, bool BK_MAJOR_>
 struct Product {
   using Op = OpT;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
-  static constexpr int THREADS = 64 * WM * WN;
+  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
   using TA = Tile<BM, AK_>;
   using TB = Tile<BN, BK_MAJOR_>;
-  static constexpr int LDS_ELEMS = TA::ELEMS + TB::ELEMS;
+  static constexpr int STEP = TA::ELEMS + TB::ELEMS;
+  static constexpr int LDS_ELEMS = 2 * STEP;
   typedef f32x16_t Acc[MI][NI];
 
-  template <typename T>
-  static __device__ __forceinline__ void stage(const Operand& o, const uint16_t* base, int k0, uint16_t* lds, bool kmajor) {
-    constexpr int N = T::CHUNKS / THREADS;
-    static_assert(T::CHUNKS % THREADS == 0, "every thread stages the same number of chunks");
-    u16x8_t v[N];
+  struct Frags { u16x8_t a[MI], b[NI]; };
+  static __device__ __forceinline__ void read(Frags& f, const uint16_t* buf, int wm, int wn, int ks, int lane) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      int row, col;
-      T::at(j * THREADS + (int)threadIdx.x, row, col);
-      const int ou = kmajor ? k0 + row : row, in = kmajor ? col * 8 : k0 + col * 8;
-      v[j] = u16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
-      if (ou < o.outer && in < o.inner) v[j] = *reinterpret_cast<const u16x8_t*>(base + (int64_t)ou * o.ld + in);
-    }
+    for (int i = 0; i < MI; ++i) f.a[i] = TA::frag32(buf, wm * (BM / WM) + 32 * i, ks, lane);
 #pragma unroll
-    for (int j = 0; j < N; ++j) *reinterpret_cast<u16x8_t*>(lds + (j * THREADS + (int)threadIdx.x) * 8) = v[j];
+    for (int j = 0; j < NI; ++j) f.b[j] = TB::frag32(buf + TA::ELEMS, wn * (BN / WN) + 32 * j, ks, lane);
+  }
+  static __device__ __forceinline__ void multiply(Acc& acc, const Frags& f) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = mma<Op>(f.a[i], f.b[j], acc[i][j]);
   }
 
   // k from k0 to k1 (multiples of BK).  PA, PB: the operands' planes; of two times
-  // two, the three products that are not below the last bit.
+  // two, the three products that are not below the last bit: hi hi, hi lo, lo hi.
   template <int PA, int PB>
   static __device__ __forceinline__ void run(Acc& acc, const Operand& a, const Operand& b, int k0, int k1,
                                              uint16_t* lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -136,31 +206,52 @@ struct Product {
       for (int j = 0; j < NI; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    uint16_t* la = lds;
-    uint16_t* lb = lds + TA::ELEMS;
-    for (int seg = 0; seg < PA + PB - 1; ++seg) {   // hi hi, then hi lo, then lo hi
-      const uint16_t* pa = a.p + (seg >= PB ? a.plane : 0);
-      const uint16_t* pb = b.p + (PB == 2 && seg == 1 ? b.plane : 0);
-      for (int k = k0; k < k1; k += BK) {
-        __syncthreads();
-        stage<TA>(a, pa, k, la, AK_);
-        stage<TB>(b, pb, k, lb, BK_MAJOR_);
-        __syncthreads();
-#pragma unroll
-        for (int ks = 0; ks < BK / 16; ++ks) {
-          u16x8_t fa[MI], fb[NI];
-#pragma unroll
-          for (int i = 0; i < MI; ++i) fa[i] = TA::frag32(la, wm * (BM / WM) + 32 * i, ks, lane);
-#pragma unroll
-          for (int j = 0; j < NI; ++j) fb[j] = TB::frag32(lb, wn * (BN / WN) + 32 * j, ks, lane);
-#pragma unroll
-          for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = mma<Op>(fa[i], fb[j], acc[i][j]);
-        }
+    const int per = (k1 - k0) / BK, steps = per * (PA + PB - 1);
+    if (steps <= 0) return;
+    Loader<BM, AK_, WAVES> la;
+    Loader<BN, BK_MAJOR_, WAVES> lb;
+    la.init(a, wave, lane);
+    lb.init(b, wave, lane);
+    const uint32_t base = lds_byte(lds);
+    int seg = 0, k = k1;   // the step that is loaded next
+    auto issue = [&](int buf) {
+      if (k == k1) {
+        la.seek(a.p + (PA == 2 && seg >= PB ? a.plane : 0), k0);
+        lb.seek(b.p + (PB == 2 && seg == 1 ? b.plane : 0), k0);
+        ++seg, k = k0;
       }
+      const uint32_t at = base + (uint32_t)buf * (STEP * 2);
+      la.issue(k, at, wave);
+      lb.issue(k, at + TA::ELEMS * 2, wave);
+      k += BK;
+    };
+    Frags f0, f1;
+    issue(0);
+    loads_barrier();
+    if (steps > 1) issue(1);
+    read(f0, lds, wm, wn, 0, lane);
+    for (int s = 0; s < steps; ++s) {
+      const uint16_t* buf = lds + (s & 1) * STEP;
+      read(f1, buf, wm, wn, 1, lane);
+      keep_order();
+      multiply(acc, f0);
+      keep_order();
+      read(f0, buf, wm, wn, 2, lane);
+      keep_order();
+      multiply(acc, f1);
+      keep_order();
+      read(f1, buf, wm, wn, 3, lane);
+      keep_order();
+      multiply(acc, f0);
+      keep_order();
+      loads_barrier();   // the buffer is read, the other full
+      if (s + 2 < steps) issue(s & 1);
+      read(f0, lds + ((s + 1) & 1) * STEP, wm, wn, 0, lane);   // of no step behind the last: not used
+      keep_order();
+      multiply(acc, f1);
+      keep_order();
     }
-    __syncthreads();   // the tile's LDS is free
+    __syncthreads();   // the LDS is free
   }
 };
 
