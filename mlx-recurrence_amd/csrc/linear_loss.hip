@@ -352,7 +352,7 @@ struct LogitArgs {
   const uint16_t* w;      // [V][ldw]
   const uint16_t* h;      // [n][Dp]
   int64_t ldw, ldh, plane_w, plane_h;
-  int V, D, Dp, K, Tp;
+  int V, D, Dp, K, Tp, nvt;   // nvt: tiles of this launch
   float c;                // log2(e) / tau
   State st;
   float2* part;           // forward
@@ -398,8 +398,8 @@ logits_kernel(LogitArgs a) {
   using P = Product<Op, BM, BN, 2, 4, false, false>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
-  const int ntt = a.Tp / BN;
-  const int tt = blockIdx.x % ntt, vt = blockIdx.x / ntt;
+  int vt, tt;
+  tile_of(blockIdx.x, a.nvt, a.Tp / BN, vt, tt);
   const int t0 = tt * BN, v0 = a.v_first + vt * BM;
   if (t0 >= n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -623,10 +623,9 @@ dh_kernel(DhArgs a) {
   using P = Product<Op, BM, BN, 2, 4, true, false>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
-  int b = blockIdx.x;
-  const int dt = b % a.ndt;
-  b /= a.ndt;
-  const int tt = b % (a.Tp / BN), sp = b / (a.Tp / BN);
+  int dt, tt;
+  const int ntt = a.Tp / BN, sp = blockIdx.x / (a.ndt * ntt);
+  tile_of(blockIdx.x - sp * a.ndt * ntt, a.ndt, ntt, dt, tt);
   const int t0 = tt * BN, d0 = dt * BM;
   if (t0 >= n) return;
   const int steps = a.cols / BK;
@@ -691,7 +690,8 @@ dw_kernel(DwArgs a) {
   using P = Product<Op, BM, BN, 2, 4, true, true>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
-  const int dt = blockIdx.x % a.ndt, vt = blockIdx.x / a.ndt;
+  int dt, vt;
+  tile_of(blockIdx.x, a.ndt, gridDim.x / a.ndt, dt, vt);
   const int d0 = dt * BM, v0 = vt * BN;
   typename P::Acc acc;
   const Operand A{a.h + d0, a.ldh, a.plane_h, n, a.Dp - d0};
@@ -772,7 +772,7 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
             float zl, float tau, int reduction, float* loss, hipStream_t s) {
   pack_rows<X>(p, hidden, weight, st, ws.h, ws.w, true, s);
   LogitArgs a = logit_args(p, st, weight, ws.h, ws.w, K, tau);
-  a.part = ws.part;
+  a.part = ws.part, a.nvt = (int)p.nvt;
   logits_kernel<Op, false, PX, PX><<<(unsigned)(p.nvt * p.ntt), kThreads, 0, s>>>(a);
   float* rows = reduction == 0 ? loss : st.loss;
   row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, p.T, (int)p.nvt, p.Tp, K, labels, zl, tau, rows);
@@ -789,7 +789,7 @@ int backward(const Plan& p, const float* dloss, const void* hidden, const void* 
   for (int64_t v = 0; v < p.nvt * BM; v += p.Vp) {
     const int64_t cols = std::min(p.Vp, p.nvt * BM - v);   // whole tiles
     LogitArgs a = logit_args(p, st, weight, ws.h, ws.w, K, tau);
-    a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp, a.plane_z = p.Tp * p.Vp, a.v_first = (int)v;
+    a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp, a.plane_z = p.Tp * p.Vp, a.v_first = (int)v, a.nvt = (int)(cols / BM);
     logits_kernel<Op, true, PX, PZ><<<(unsigned)(cols / BM * p.ntt), kThreads, 0, s>>>(a);
     if (dh != nullptr) {
       DhArgs b{};

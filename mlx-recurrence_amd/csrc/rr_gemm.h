@@ -166,6 +166,21 @@ struct Loader {
   }
 };
 
+// Tile of workgroup `b` of nm x nn.  Workgroups go to the 8 XCDs in turn, each with an
+// L2 of its own: an XCD takes a contiguous part of the tiles, in bands of kBand tiles
+// along m walked along n, so that the tiles it multiplies at one time share rows of
+// both operands.
+constexpr int kXcds = 8, kBand = 8;
+__device__ __forceinline__ void tile_of(int b, int nm, int nn, int& m, int& n) {
+  const int all = nm * nn, each = all / kXcds, more = all % kXcds;
+  const int x = b % kXcds;
+  const int id = x * each + min(x, more) + b / kXcds;
+  const int band = id / (kBand * nn), in = id - band * kBand * nn;
+  const int wide = min(kBand, nm - band * kBand);
+  m = band * kBand + in % wide;
+  n = in / wide;
+}
+
 // WM x WN waves, each with MI x NI blocks of 32 x 32.
 template <typename OpT, int BM_, int BN_, int WM_, int WN_, bool AK_, bool BK_MAJOR_>
 struct Product {
