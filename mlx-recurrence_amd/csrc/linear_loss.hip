@@ -54,7 +54,8 @@ constexpr int64_t kFewRows = 64;           // rows whose dz keeps a second plane
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 constexpr int BM = 256, BN = 256;   // a tile of each product
-constexpr int kThreads = 512;
+constexpr int WM = 2, WN = 4;             // its waves
+constexpr int kThreads = 64 * WM * WN;
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
@@ -370,11 +371,11 @@ __device__ __forceinline__ float rounded(float x) {
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Walks the entries of row `orig` whose column lies in this wave's v0 .. v0 + 32 MI
-// and in this lane's half of the accumulator rows: f(k, element) with the element's
-// index mi * 16 + e.
+// Walks the entries of row `orig` whose column lies in this wave's v0 .. v0 + 16 MI
+// and in this lane's quarter of the accumulator rows: f(k, element) with the element's
+// index 4 i + e.
 template <int MI, typename F>
-__device__ __forceinline__ void each_entry(const int* ids, int K, int v0, int half, bool on, F f) {
+__device__ __forceinline__ void each_entry(const int* ids, int K, int v0, int quarter, bool on, F f) {
   int lo = 0;
   if (on) {
     int hi = K;
@@ -386,16 +387,16 @@ __device__ __forceinline__ void each_entry(const int* ids, int K, int v0, int ha
   }
   for (int k = lo; on && k < K; ++k) {
     const int rel = ids[k] - v0;
-    if (rel >= 32 * MI) break;
-    if (((rel >> 2) & 1) == half) f(k, (rel >> 5) * 16 + ((rel & 31) >> 3) * 4 + (rel & 3));
+    if (rel >= 16 * MI) break;
+    if (((rel >> 2) & 3) == quarter) f(k, (rel >> 4) * 4 + (rel & 3));
   }
 }
 
-// z^T tiles: m = vocabulary, n = rows, so that a lane holds 16 MI logits of one row.
+// z^T tiles: m = vocabulary, n = rows, so that a lane holds 4 MI logits of a row.
 template <typename Op, bool GRAD, int PX, int PZ>
 __global__ void __launch_bounds__(kThreads)
 logits_kernel(LogitArgs a) {
-  using P = Product<Op, BM, BN, 2, 4, false, false>;
+  using P = Product<Op, BM, BN, WM, WN, false, false>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
   int vt, tt;
@@ -404,7 +405,7 @@ logits_kernel(LogitArgs a) {
   if (t0 >= n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN, wn = wave % P::WN;
-  const int half = lane >> 5;
+  const int quarter = lane >> 4;
 
   typename P::Acc acc;
   const Operand A{a.w + (int64_t)v0 * a.ldw, a.ldw, a.plane_w, a.V - v0, (int)a.ldw};
@@ -413,11 +414,11 @@ logits_kernel(LogitArgs a) {
 
   float c = a.c;
   if constexpr (PX == 2) c /= scale_h(a.st.hdr) * scale_w(a.st.hdr);
-  const int vw = v0 + wm * (BM / P::WM);
+  const int vw = v0 + wm * P::MW;
   float* red = reinterpret_cast<float*>(lds);   // forward: [WM][BN][2]
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
-    const int tl = wn * (BN / P::WN) + 32 * j + (lane & 31);
+    const int tl = wn * P::NW + 16 * j + (lane & 15);
     const int t = t0 + tl;
     const bool on = t < n;
     const int64_t orig = on ? a.st.rows[t] : 0;
@@ -427,8 +428,8 @@ logits_kernel(LogitArgs a) {
 #pragma unroll
       for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int v = vw + 32 * i + 8 * (e / 4) + 4 * half + e % 4;
+        for (int e = 0; e < 4; ++e) {
+          const int v = vw + 16 * i + 4 * quarter + e;
           acc[i][j][e] = v < a.V ? rounded(acc[i][j][e] * c) : -INFINITY;
           m = fmaxf(m, acc[i][j][e]);
         }
@@ -436,29 +437,33 @@ logits_kernel(LogitArgs a) {
 #pragma unroll
       for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s += m == -INFINITY ? acc[i][j][e] - m : exp2_fast(acc[i][j][e] - m);
+        for (int e = 0; e < 4; ++e) s += m == -INFINITY ? acc[i][j][e] - m : exp2_fast(acc[i][j][e] - m);
       if (m == -INFINITY && s != s) {   // no column of the vocabulary, or NaN among the logits
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) bad |= acc[i][j][e] != acc[i][j][e];
+          for (int e = 0; e < 4; ++e) bad |= acc[i][j][e] != acc[i][j][e];
         s = bad ? NAN : 0.f;
       }
-      each_entry<P::MI>(ids, a.K, vw, half, on, [&](int k, int el) {
+      each_entry<P::MI>(ids, a.K, vw, quarter, on, [&](int k, int el) {
         float z = 0.f;
 #pragma unroll
         for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) z = el == i * 16 + e ? acc[i][j][e] : z;
+          for (int e = 0; e < 4; ++e) z = el == i * 4 + e ? acc[i][j][e] : z;
         a.st.z2[orig * a.K + k] = z;
       });
-      // the other half's rows of the same column, then the waves along m
-      const float m2 = __shfl_xor(m, 32, 64), s2 = __shfl_xor(s, 32, 64);
-      const float mm = fmaxf(m, m2);
-      s = (m == mm ? s : s * exp2_fast(m - mm)) + (m2 == mm ? s2 : s2 * exp2_fast(m2 - mm));
-      if (half == 0) {
-        red[(wm * BN + tl) * 2] = mm;
+      // the other quarters' words of the same row, then the waves along m
+#pragma unroll
+      for (int o = 16; o < 64; o *= 2) {
+        const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+        const float mm = fmaxf(m, m2);
+        s = (m == mm ? s : s * exp2_fast(m - mm)) + (m2 == mm ? s2 : s2 * exp2_fast(m2 - mm));
+        m = mm;
+      }
+      if (quarter == 0) {
+        red[(wm * BN + tl) * 2] = m;
         red[(wm * BN + tl) * 2 + 1] = s;
       }
     } else {
@@ -467,33 +472,31 @@ logits_kernel(LogitArgs a) {
 #pragma unroll
       for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int v = vw + 32 * i + 8 * (e / 4) + 4 * half + e % 4;
+        for (int e = 0; e < 4; ++e) {
+          const int v = vw + 16 * i + 4 * quarter + e;
           acc[i][j][e] = on && v < a.V ? exp2_fast(rounded(acc[i][j][e] * c) - l2) : 0.f;
         }
       // q - p first, so that what is left of a sure label keeps its bits
-      each_entry<P::MI>(ids, a.K, vw, half, on, [&](int k, int el) {
+      each_entry<P::MI>(ids, a.K, vw, quarter, on, [&](int k, int el) {
         const float p = a.st.p[orig * a.K + k], r = p * co.y;
 #pragma unroll
         for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][j][e] = el == i * 16 + e ? acc[i][j][e] - p + r : acc[i][j][e];
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = el == i * 4 + e ? acc[i][j][e] - p + r : acc[i][j][e];
       });
-      uint16_t* o = a.dz + (int64_t)t * a.ldz + (vw - a.v_first) + 4 * half;
+      uint16_t* o = a.dz + (int64_t)t * a.ldz + (vw - a.v_first) + 4 * quarter;
 #pragma unroll
-      for (int i = 0; i < P::MI; ++i)
+      for (int i = 0; i < P::MI; ++i) {
+        rr::u16x4_t hi, lo;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          rr::u16x4_t hi, lo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float v = on ? co.x * acc[i][j][4 * q + e] : 0.f;
-            hi[e] = op_bits<Op>(v);
-            if constexpr (PZ == 2) lo[e] = op_bits<Op>(v - op_val<Op>(hi[e]));
-          }
-          *reinterpret_cast<rr::u16x4_t*>(o + 32 * i + 8 * q) = hi;
-          if constexpr (PZ == 2) *reinterpret_cast<rr::u16x4_t*>(o + a.plane_z + 32 * i + 8 * q) = lo;
+        for (int e = 0; e < 4; ++e) {
+          const float v = on ? co.x * acc[i][j][e] : 0.f;
+          hi[e] = op_bits<Op>(v);
+          if constexpr (PZ == 2) lo[e] = op_bits<Op>(v - op_val<Op>(hi[e]));
         }
+        *reinterpret_cast<rr::u16x4_t*>(o + 16 * i) = hi;
+        if constexpr (PZ == 2) *reinterpret_cast<rr::u16x4_t*>(o + a.plane_z + 16 * i) = lo;
+      }
     }
   }
   if constexpr (!GRAD) {
@@ -620,7 +623,7 @@ struct DhArgs {
 template <typename Op, int PX, int PZ>
 __global__ void __launch_bounds__(kThreads)
 dh_kernel(DhArgs a) {
-  using P = Product<Op, BM, BN, 2, 4, true, false>;
+  using P = Product<Op, BM, BN, WM, WN, true, false>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
   int dt, tt;
@@ -638,20 +641,18 @@ dh_kernel(DhArgs a) {
   const int wm = wave / P::WN, wn = wave % P::WN;
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
-    const int t = t0 + wn * (BN / P::WN) + 32 * j + (lane & 31);
-    float* o = a.out + ((int64_t)sp * a.Tp + t) * a.ndt * BM + d0 + wm * (BM / P::WM) + 4 * (lane >> 5);
+    const int t = t0 + wn * P::NW + 16 * j + (lane & 15);
+    float* o = a.out + ((int64_t)sp * a.Tp + t) * a.ndt * BM + d0 + wm * P::MW + 4 * (lane >> 4);
 #pragma unroll
-    for (int i = 0; i < P::MI; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float4* at = reinterpret_cast<float4*>(o + 32 * i + 8 * q);
-        float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-        if (!a.first) {
-          const float4 u = *at;
-          v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-        }
-        *at = v;
+    for (int i = 0; i < P::MI; ++i) {
+      float4* at = reinterpret_cast<float4*>(o + 16 * i);
+      float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+      if (!a.first) {
+        const float4 u = *at;
+        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
       }
+      *at = v;
+    }
   }
 }
 
@@ -687,7 +688,7 @@ struct DwArgs {
 template <typename Op, typename X, int PX, int PZ>
 __global__ void __launch_bounds__(kThreads)
 dw_kernel(DwArgs a) {
-  using P = Product<Op, BM, BN, 2, 4, true, true>;
+  using P = Product<Op, BM, BN, WM, WN, true, true>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
   int dt, vt;
@@ -703,14 +704,14 @@ dw_kernel(DwArgs a) {
   const int wm = wave / P::WN, wn = wave % P::WN;
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
-    const int v = v0 + wn * (BN / P::WN) + 32 * j + (lane & 31);
+    const int v = v0 + wn * P::NW + 16 * j + (lane & 15);
     if (v >= a.V) continue;
     X* o = static_cast<X*>(a.out) + (int64_t)v * a.D;
 #pragma unroll
     for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int d = d0 + wm * (BM / P::WM) + 32 * i + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+      for (int e = 0; e < 4; ++e) {
+        const int d = d0 + wm * P::MW + 16 * i + 4 * (lane >> 4) + e;
         if (d < a.D) o[d] = rr::from_f32<X>(acc[i][j][e] * f);
       }
   }

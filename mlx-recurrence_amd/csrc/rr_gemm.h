@@ -1,7 +1,7 @@
 // rr_gemm.h — the tiled matrix product of the output-head losses on gfx950.
 //
 // acc[m][n] = sum_k A(m, k) B(n, k) for a BM x BN tile, 16-bit operands, fp32
-// accumulation on the 32x32x16 MFMA.  An operand lies in memory either with k
+// accumulation on the 16x16x32 MFMA.  An operand lies in memory either with k
 // contiguous (its rows are m or n) or k-major (its rows are k); in LDS the tile
 // keeps the orientation it has in memory, and k-major tiles are read with the
 // transposing LDS read, so no operand is ever transposed in memory.
@@ -9,15 +9,23 @@
 // LDS holds 16-byte chunks.  A fragment read takes the same chunk column of many
 // rows, whose addresses differ by a multiple of the row length, so chunk columns
 // are permuted by row (an XOR) to spread them over the banks:
-//   k contiguous  row r, 8 chunks of 8 k:      chunk c at c ^ ((r & 7) ^ ((r >> 3) & 1))
-//   k-major       row k, pieces of 16 columns: piece q at q ^ (2 (k & 3) ^ ((k >> 1) & 1))
+//   k contiguous  row r, 8 chunks of 8 k:      chunk c at c ^ ((r >> 1) & 7)
+//   k-major       row k, pieces of 16 columns: piece q at q ^ ((k & 3) + 4 ((k >> 3) & 1))
 //
 // A step of 64 k is loaded by buffer loads that write LDS themselves (16 bytes a lane,
 // the permutation made by the lanes' addresses), into one of two LDS buffers, while the
-// other is multiplied.  The loads of a step are issued as soon as every wave has read
-// its last fragments of the buffer, a whole step before they are waited for, so one
-// barrier a step does: it says both that the buffer is free and that the next is full.
-// Fragments are read one k group (16) ahead of their products.
+// other is multiplied.  One barrier a step, behind the first two rows of blocks of its
+// second half, says both that the buffer has been read and that the other is full; the
+// loads of the step after next follow it, a whole step before they are waited for.
+// A fragment of A is read again, for the next half, one row of blocks behind its last
+// use, so that reads, loads and products alternate without a pause.
+//
+// What bounds it: the power limit.  At 8192 x 65536 x 2560 the matrix units are busy
+// 65 % of the cycles, at 1.8 of 2.4 GHz; variants with fewer idle cycles ran at a lower
+// clock in the same time.  What counts is energy: 16x16x32 products in place of
+// 32x32x16 (whose accumulators move twice the bytes a flop) took 2.10 ms in place of
+// 2.39, with 4 waves of 128 x 128 in place of 8 of 128 x 64 nothing was won.  LDS reads
+// without bank conflicts (half of the LDS cycles before) took 1 % off.
 #pragma once
 
 #include "rr_common.h"
@@ -32,12 +40,12 @@ struct OpBf16 {};
 struct OpF16 {};
 
 template <typename Op>
-__device__ __forceinline__ f32x16_t mma(const u16x8_t& a, const u16x8_t& b, f32x16_t c) {
+__device__ __forceinline__ f32x4_t mma(const u16x8_t& a, const u16x8_t& b, f32x4_t c) {
   if constexpr (__is_same(Op, OpBf16)) {
-    return mfma32(a, b, c);
+    return mfma16(a, b, c);
   } else {
     typedef _Float16 f16x8_t __attribute__((__vector_size__(16)));
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
                                                   0, 0);
   }
 }
@@ -91,8 +99,8 @@ struct Tile {
   static constexpr int PER_ROW = KMAJOR ? ROWS / 8 : BK / 8;
   static constexpr int PIECES = ROWS / 16;   // of a k-major row
   static __device__ __forceinline__ int swz(int row) {
-    if constexpr (KMAJOR) return ((2 * (row & 3)) ^ ((row >> 1) & 1)) & (PIECES - 1);
-    else return (row & 7) ^ ((row >> 3) & 1);
+    if constexpr (KMAJOR) return ((row & 3) | ((row >> 1) & 4)) & (PIECES - 1);
+    else return (row >> 1) & 7;
   }
   // Row and chunk column of the chunk that lies at 16-byte position P.
   static __device__ __forceinline__ void at(int P, int& row, int& col) {
@@ -101,19 +109,17 @@ struct Tile {
     if constexpr (KMAJOR) col = ((c >> 1) ^ swz(row)) * 2 + (c & 1);
     else col = c ^ swz(row);
   }
-  // Fragment of rows (k contiguous) or columns (k-major) r0 .. r0 + 31, k = 16 ks ..:
-  // lane l holds row l % 32, k = 8 (l / 32) + e.
-  static __device__ __forceinline__ u16x8_t frag32(const uint16_t* t, int r0, int ks, int lane) {
+  // Fragment of rows (k contiguous) or columns (k-major) r0 .. r0 + 15, k = 32 ks ..:
+  // lane l holds row l % 16, k = 8 (l / 16) + e.
+  static __device__ __forceinline__ u16x8_t frag16(const uint16_t* t, int r0, int ks, int lane) {
+    const int g = lane >> 4, i = lane & 15;
     if constexpr (KMAJOR) {
-      const int g = lane >> 4, i = lane & 15;
-      const int k = 16 * ks + 8 * (g >> 1) + (i >> 2);
-      const int q = (r0 >> 4) + (g & 1);
-      const uint16_t* a = t + k * ROWS + (q ^ swz(k)) * 16 + 4 * (i & 3);   // swz(k + 4) = swz(k)
+      const int k = 32 * ks + 8 * g + (i >> 2);
+      const uint16_t* a = t + k * ROWS + ((r0 >> 4) ^ swz(k)) * 16 + 4 * (i & 3);   // swz(k + 4) = swz(k)
       const u16x4_t lo = tr_read4(a), hi = tr_read4(a + 4 * ROWS);
       return u16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     } else {
-      const int r = r0 + (lane & 31);
-      const int c = 2 * ks + (lane >> 5);
+      const int r = r0 + i, c = 4 * ks + g;
       return frag(t + r * BK + (c ^ swz(r)) * 8);
     }
   }
@@ -124,10 +130,10 @@ template <int ROWS, bool KMAJOR, int WAVES>
 struct Loader {
   using T = Tile<ROWS, KMAJOR>;
   static constexpr int N = T::CHUNKS / (64 * WAVES);   // loads a thread and step
-  static_assert(T::CHUNKS % (64 * WAVES) == 0, "every thread stages the same number of chunks");
+  static_assert(T::CHUNKS % (64 * WAVES) == 0 && WAVES % 2 == 0, "every thread loads the same number of chunks");
   static constexpr int kPast = 0x40000000;   // beyond any buffer here
   int voff[N];
-  int col;          // first element of this thread's chunks along the inner axis
+  int col;          // k contiguous: first k of this thread's chunks
   int ldb, outer, inner;
   const char* at;   // the next step
 
@@ -136,33 +142,28 @@ struct Loader {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       int row, c;
-      T::at((j * WAVES + wave) * 64 + lane, row, c);   // c is the same for every j
-      voff[j] = row * ldb + c * 16;
-      col = c * 8;
-    }
-    if constexpr (KMAJOR) {
-      if (col >= inner)
-#pragma unroll
-        for (int j = 0; j < N; ++j) voff[j] = kPast;
+      T::at((j * WAVES + wave) * 64 + lane, row, c);
+      voff[j] = KMAJOR && c * 8 >= inner ? kPast : row * ldb + c * 16;
+      col = c * 8;   // k contiguous: the same for every j, WAVES being even
     }
   }
   __device__ __forceinline__ void seek(const uint16_t* p, int k) {
     at = reinterpret_cast<const char*>(p) + (KMAJOR ? (int64_t)k * ldb : (int64_t)k * 2);
   }
-  // The step that starts at k, to LDS byte `lds`.
-  __device__ __forceinline__ void issue(int k, uint32_t lds, int wave) {
+  // The buffer of the step that starts at k, and this thread's offset past its end.
+  __device__ __forceinline__ void step(int k, i32x4_t& r, int& past) {
     const int rows = KMAJOR ? min(outer - k, BK) : min(outer, ROWS);
     const int bytes = rows <= 0 ? 0 : (rows - 1) * ldb + (KMAJOR ? inner : inner - k) * 2;
     const uint64_t b = reinterpret_cast<uint64_t>(at);
-    i32x4_t r;
     r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
     r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff);
     r[2] = __builtin_amdgcn_readfirstlane(bytes);
     r[3] = 0x00020000;   // raw 32-bit buffer
-    const int past = !KMAJOR && k + col >= inner ? kPast : 0;   // the rest of a last step's row
-#pragma unroll
-    for (int j = 0; j < N; ++j) load_to_lds(r, voff[j] | past, lds + (uint32_t)(j * WAVES + wave) * 1024);
+    past = !KMAJOR && k + col >= inner ? kPast : 0;   // the rest of a last step's row
     at += KMAJOR ? (int64_t)BK * ldb : BK * 2;
+  }
+  __device__ __forceinline__ void load(int j, i32x4_t r, int past, uint32_t lds, int wave) const {
+    load_to_lds(r, voff[j] | past, lds + (uint32_t)(j * WAVES + wave) * 1024);
   }
 };
 
@@ -181,32 +182,35 @@ __device__ __forceinline__ void tile_of(int b, int nm, int nn, int& m, int& n) {
   n = in / wide;
 }
 
-// WM x WN waves, each with MI x NI blocks of 32 x 32.
+// WM x WN waves, each with MI x NI blocks of 16 x 16: element e of a lane's block (i, j)
+// is row 16 i + 4 (lane / 16) + e and column 16 j + lane % 16 of the wave's part.
 template <typename OpT, int BM_, int BN_, int WM_, int WN_, bool AK_, bool BK_MAJOR_>
 struct Product {
   using Op = OpT;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
-  static constexpr int MI = BM / WM / 32, NI = BN / WN / 32;
+  static constexpr int MW = BM / WM, NW = BN / WN;   // a wave's part
+  static constexpr int MI = MW / 16, NI = NW / 16;
   using TA = Tile<BM, AK_>;
   using TB = Tile<BN, BK_MAJOR_>;
   static constexpr int STEP = TA::ELEMS + TB::ELEMS;
   static constexpr int LDS_ELEMS = 2 * STEP;
-  typedef f32x16_t Acc[MI][NI];
+  static_assert(MI >= 2, "the barrier of a step lies behind the second row of blocks");
+  typedef f32x4_t Acc[MI][NI];
 
-  struct Frags { u16x8_t a[MI], b[NI]; };
-  static __device__ __forceinline__ void read(Frags& f, const uint16_t* buf, int wm, int wn, int ks, int lane) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i) f.a[i] = TA::frag32(buf, wm * (BM / WM) + 32 * i, ks, lane);
-#pragma unroll
-    for (int j = 0; j < NI; ++j) f.b[j] = TB::frag32(buf + TA::ELEMS, wn * (BN / WN) + 32 * j, ks, lane);
-  }
-  static __device__ __forceinline__ void multiply(Acc& acc, const Frags& f) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = mma<Op>(f.a[i], f.b[j], acc[i][j]);
-  }
+  // The step whose loads are under way.
+  struct Steps {
+    Loader<BM, AK_, WAVES> a;
+    Loader<BN, BK_MAJOR_, WAVES> b;
+    i32x4_t ra, rb;
+    int pa, pb;
+    uint32_t lds;
+    static constexpr int N = decltype(a)::N + decltype(b)::N;
+    __device__ __forceinline__ void load(int j, int wave) const {
+      if (j < decltype(a)::N) a.load(j, ra, pa, lds, wave);
+      else b.load(j - decltype(a)::N, rb, pb, lds + TA::ELEMS * 2, wave);
+    }
+  };
 
   // k from k0 to k1 (multiples of BK).  PA, PB: the operands' planes; of two times
   // two, the three products that are not below the last bit: hi hi, hi lo, lo hi.
@@ -218,55 +222,81 @@ struct Product {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+      for (int j = 0; j < NI; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     const int per = (k1 - k0) / BK, steps = per * (PA + PB - 1);
     if (steps <= 0) return;
-    Loader<BM, AK_, WAVES> la;
-    Loader<BN, BK_MAJOR_, WAVES> lb;
-    la.init(a, wave, lane);
-    lb.init(b, wave, lane);
+    Steps st;
+    st.a.init(a, wave, lane);
+    st.b.init(b, wave, lane);
     const uint32_t base = lds_byte(lds);
-    int seg = 0, k = k1;   // the step that is loaded next
-    auto issue = [&](int buf) {
+    int seg = 0, k = k1, loaded = 0;   // the step that is loaded next
+    auto next_step = [&] {
       if (k == k1) {
-        la.seek(a.p + (PA == 2 && seg >= PB ? a.plane : 0), k0);
-        lb.seek(b.p + (PB == 2 && seg == 1 ? b.plane : 0), k0);
+        st.a.seek(a.p + (PA == 2 && seg >= PB ? a.plane : 0), k0);
+        st.b.seek(b.p + (PB == 2 && seg == 1 ? b.plane : 0), k0);
         ++seg, k = k0;
       }
-      const uint32_t at = base + (uint32_t)buf * (STEP * 2);
-      la.issue(k, at, wave);
-      lb.issue(k, at + TA::ELEMS * 2, wave);
-      k += BK;
+      st.lds = base + (uint32_t)(loaded & 1) * (STEP * 2);
+      st.a.step(k, st.ra, st.pa);
+      st.b.step(k, st.rb, st.pb);
+      if (loaded >= steps) st.ra[2] = st.rb[2] = 0;   // behind the last step: loads of nothing (zeros)
+      k += BK, ++loaded;
     };
-    Frags f0, f1;
-    issue(0);
+    u16x8_t fa[MI], fb[2][NI];
+    auto read_a = [&](int i, const uint16_t* buf, int ks) { fa[i] = TA::frag16(buf, wm * MW + 16 * i, ks, lane); };
+    auto read_b = [&](int j, const uint16_t* buf, int ks) { fb[ks][j] = TB::frag16(buf + TA::ELEMS, wn * NW + 16 * j, ks, lane); };
+    // Row i of the products of k group ks.
+    auto row = [&](int i, int ks) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = mma<Op>(fa[i], fb[ks][j], acc[i][j]);
+      keep_order();
+    };
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      next_step();
+#pragma unroll
+      for (int j = 0; j < Steps::N; ++j) st.load(j, wave);
+    }
     loads_barrier();
-    if (steps > 1) issue(1);
-    read(f0, lds, wm, wn, 0, lane);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) read_a(i, lds, 0);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) read_b(j, lds, 0);
+    keep_order();
+    // A row's fragment of A is read again, for the next k group, one row behind its last
+    // use; the fragments of B have a set for each group.
     for (int s = 0; s < steps; ++s) {
       const uint16_t* buf = lds + (s & 1) * STEP;
-      read(f1, buf, wm, wn, 1, lane);
-      keep_order();
-      multiply(acc, f0);
-      keep_order();
-      read(f0, buf, wm, wn, 2, lane);
-      keep_order();
-      multiply(acc, f1);
-      keep_order();
-      read(f1, buf, wm, wn, 3, lane);
-      keep_order();
-      multiply(acc, f0);
-      keep_order();
-      loads_barrier();   // the buffer is read, the other full
-      if (s + 2 < steps) issue(s & 1);
-      read(f0, lds + ((s + 1) & 1) * STEP, wm, wn, 0, lane);   // of no step behind the last: not used
-      keep_order();
-      multiply(acc, f1);
-      keep_order();
+      const uint16_t* other = lds + ((s + 1) & 1) * STEP;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        row(i, 0);
+        if (i == 0) read_a(MI - 1, buf, 0);
+        else read_a(i - 1, buf, 1);
+#pragma unroll
+        for (int j = i * NI / MI; j < (i + 1) * NI / MI; ++j) read_b(j, buf, 1);
+        keep_order();
+      }
+      next_step();
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        row(i, 1);
+        if (i == 0) {
+          read_a(MI - 1, buf, 1);
+          keep_order();
+          continue;
+        }
+        if (i == 1) loads_barrier();   // the buffer is read, the other full
+        read_a(i - 1, other, 0);
+        constexpr int R = MI - 1;      // behind the last step the fragments are of no step and not used
+#pragma unroll
+        for (int j = (i - 1) * NI / R; j < i * NI / R; ++j) read_b(j, other, 0);
+#pragma unroll
+        for (int l = (i - 1) * Steps::N / R; l < i * Steps::N / R; ++l) st.load(l, wave);
+        keep_order();
+      }
     }
-    __syncthreads();   // the LDS is free
+    loads_barrier();   // the LDS is free
   }
 };
 
