@@ -1,8 +1,8 @@
-// autograd.cpp — C++ autograd bindings of the SSD and GLA scans for PyTorch
-// (module mlx_recurrence_amd._autograd).
+// autograd.cpp — C++ autograd bindings of the SSD and GLA scans and of the output head
+// (layer norm, losses from hidden states) for PyTorch (module mlx_recurrence_amd._autograd).
 //
 // The same forward / backward as the Python torch.autograd.Functions of
-// ssd.py and gla.py (the counterparts of the reference's mx.custom_function
+// norm.py, linear_loss.py, ssd.py and gla.py (the counterparts of the reference's mx.custom_function
 // VJPs, reference ssd.py:314-341 and gla.py:277-300), written against the
 // C ABI of librecurrence_gfx950.so: input preparation, output / workspace
 // allocation, the kernel calls and the saved state live in one
@@ -298,12 +298,143 @@ std::tuple<Tensor, Tensor> gla_scan(const Tensor& q, const Tensor& k, const Tens
   return {out[0], out[1]};
 }
 
+// ------------------------------------------------------------------ layer norm
+at::ScalarType dtype_of(int64_t code) {
+  return code == RR_F32 ? at::kFloat : code == RR_BF16 ? at::kBFloat16 : at::kHalf;
+}
+Tensor opt(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+
+// x of one of the three input types; weight and bias, where given, of one type.
+Tensor layer_norm_fwd(const Tensor& x_, const Tensor& w_, const Tensor& b_, double eps, int64_t out, Tensor* stats) {
+  const int64_t D = x_.size(-1), rows = x_.numel() / D;
+  const Tensor& p = w_.defined() ? w_ : b_;
+  Tensor y = at::empty(x_.sizes(), x_.options().dtype(dtype_of(out)));
+  if (stats != nullptr) *stats = at::empty({2, rows}, x_.options().dtype(at::kFloat));
+  float* mean = stats != nullptr ? stats->data_ptr<float>() : nullptr;
+  check(rr_layer_norm_fwd(P(x_), dtype_code(x_.scalar_type()), P(w_), P(b_), p.defined() ? dtype_code(p.scalar_type()) : RR_F32,
+                          rows, D, (float)eps, P(y), (int)out, mean, mean == nullptr ? nullptr : mean + rows, stream_of(x_)),
+        "rr_layer_norm_fwd");
+  return y;
+}
+
+struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& w,
+                        const c10::optional<Tensor>& b, double eps, int64_t out) {
+    const at::DeviceGuard guard(x.device());
+    const Tensor x_ = prep(x, x.scalar_type());
+    const Tensor w_ = w.has_value() ? prep(*w, w->scalar_type()) : Tensor();
+    const Tensor b_ = b.has_value() ? prep(*b, b->scalar_type()) : Tensor();
+    Tensor stats;
+    Tensor y = layer_norm_fwd(x_, w_, b_, eps, out, &stats);
+    ctx->save_for_backward({x_, w_, stats});
+    ctx->saved_data["w"] = w.has_value();
+    ctx->saved_data["b"] = b.has_value();
+    const Tensor& p = w_.defined() ? w_ : b_;
+    ctx->saved_data["wd"] = (int64_t)(p.defined() ? dtype_code(p.scalar_type()) : RR_F32);
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x_ = s[0], &w_ = s[1], &stats = s[2];
+    const at::DeviceGuard guard(x_.device());
+    const bool has_w = ctx->saved_data["w"].toBool(), has_b = ctx->saved_data["b"].toBool();
+    const int64_t wd = ctx->saved_data["wd"].toInt();
+    const int64_t D = x_.size(-1), rows = x_.numel() / D;
+    // (autograd edges exist only for the tensors passed: x, then the weight, then the bias)
+    const bool need_w = has_w && ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(has_w ? 2 : 1);
+    const Tensor dy = prep(grads[0], grads[0].scalar_type());
+    Tensor dx = ctx->needs_input_grad(0) ? at::empty_like(x_) : Tensor();
+    const auto params = x_.options().dtype(dtype_of(wd));
+    Tensor dw = need_w ? at::empty({D}, params) : Tensor(), db = need_b ? at::empty({D}, params) : Tensor();
+    const size_t wsb = need_w || need_b ? rr_layer_norm_bwd_workspace_bytes(rows, D) : 0;
+    const Tensor ws = workspace(wsb, x_.options());
+    const float* mean = stats.data_ptr<float>();
+    check(rr_layer_norm_bwd(P(dy), dtype_code(dy.scalar_type()), P(x_), dtype_code(x_.scalar_type()), P(w_), (int)wd, mean,
+                            mean + rows, rows, D, P(dx), P(dw), P(db), P(ws), wsb, stream_of(x_)),
+          "rr_layer_norm_bwd");
+    return {dx, dw, db, Tensor(), Tensor()};
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& w, const c10::optional<Tensor>& b, double eps, int64_t out) {
+  const Tensor wt = opt(w), bt = opt(b);
+  require_device({&x, &wt, &bt});
+  if (records({&x, &wt, &bt})) return LayerNormFn::apply(x, w, b, eps, out);
+  const at::DeviceGuard guard(x.device());
+  return layer_norm_fwd(prep(x, x.scalar_type()), wt.defined() ? prep(wt, wt.scalar_type()) : wt,
+                        bt.defined() ? prep(bt, bt.scalar_type()) : bt, eps, out, nullptr);
+}
+
+// ------------------------------------------------------------------ losses from hidden states
+// hidden [rows, D] and weight [V, D] of one type; labels [rows], or teacher logits and ids [rows, K].
+struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
+                        const c10::optional<Tensor>& labels, const c10::optional<Tensor>& t_logits,
+                        const c10::optional<Tensor>& t_ids, int64_t ignore, double zl, double tau, int64_t reduction) {
+    const at::DeviceGuard guard(hidden.device());
+    const at::ScalarType dt = hidden.scalar_type();
+    const Tensor h_ = prep(hidden, dt), w_ = prep(weight, dt);
+    const int64_t rows = h_.size(0), D = h_.size(1), V = w_.size(0), K = t_ids.has_value() ? t_ids->size(1) : 1;
+    const int dtc = dtype_code(dt);
+    Tensor loss = reduction == 0 ? at::empty({rows}, h_.options().dtype(at::kFloat)) : at::empty({}, h_.options().dtype(at::kFloat));
+    const size_t sb = rr_linear_loss_state_bytes(rows, K), wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 0);
+    const Tensor state = workspace(sb, h_.options()), ws = workspace(wsb, h_.options());
+    if (t_ids.has_value()) {
+      const at::ScalarType tdt = common_dtype({&*t_logits});
+      const Tensor tl = prep(*t_logits, tdt), ti = prep(*t_ids, at::kLong);
+      check(rr_linear_kd_fwd(P(h_), P(w_), dtc, rows, D, V, P(tl), dtype_code(tdt), ti.data_ptr<int64_t>(), K, (float)tau,
+                             (int)reduction, loss.data_ptr<float>(), P(state), sb, P(ws), wsb, stream_of(h_)),
+            "rr_linear_kd_fwd");
+    } else {
+      const Tensor l = prep(*labels, at::kLong);
+      check(rr_linear_ce_fwd(P(h_), P(w_), dtc, rows, D, V, l.data_ptr<int64_t>(), ignore, (float)zl, (int)reduction,
+                             loss.data_ptr<float>(), P(state), sb, P(ws), wsb, stream_of(h_)),
+            "rr_linear_ce_fwd");
+    }
+    ctx->save_for_backward({h_, w_, state});
+    ctx->saved_data["K"] = K;
+    ctx->saved_data["zl"] = zl;
+    ctx->saved_data["tau"] = tau;
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &h_ = s[0], &w_ = s[1], &state = s[2];
+    const at::DeviceGuard guard(h_.device());
+    const int64_t rows = h_.size(0), D = h_.size(1), V = w_.size(0), K = ctx->saved_data["K"].toInt();
+    const int dtc = dtype_code(h_.scalar_type());
+    const Tensor dloss = prep(grads[0], at::kFloat);
+    Tensor dh = ctx->needs_input_grad(0) ? at::empty_like(h_) : Tensor();
+    Tensor dw = ctx->needs_input_grad(1) ? at::empty_like(w_) : Tensor();
+    const size_t wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 1);
+    const Tensor ws = workspace(wsb, h_.options());
+    check(rr_linear_loss_bwd(dloss.data_ptr<float>(), P(h_), P(w_), dtc, rows, D, V, K, (float)ctx->saved_data["zl"].toDouble(),
+                             (float)ctx->saved_data["tau"].toDouble(), (int)ctx->saved_data["reduction"].toInt(), P(state),
+                             state.defined() ? (size_t)state.numel() : 0, P(dh), P(dw), P(ws), wsb, stream_of(h_)),
+          "rr_linear_loss_bwd");
+    return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor linear_loss(const Tensor& hidden, const Tensor& weight, const c10::optional<Tensor>& labels,
+                   const c10::optional<Tensor>& t_logits, const c10::optional<Tensor>& t_ids, int64_t ignore, double zl,
+                   double tau, int64_t reduction) {
+  const Tensor a = opt(labels), b = opt(t_logits), c = opt(t_ids);
+  require_device({&hidden, &weight, &a, &b, &c});
+  return LinearLossFn::apply(hidden, weight, labels, t_logits, t_ids, ignore, zl, tau, reduction);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
-  m.doc() = "C++ autograd bindings of the gfx950 SSD and GLA scans";
+  m.doc() = "C++ autograd bindings of the gfx950 SSD and GLA scans and of the output head";
   m.def("ssd_scan", &ssd_scan, "SSD scan (y, final state) as one C++ autograd node");
   m.def("gla_scan", &gla_scan, "GLA scan (y, final state) as one C++ autograd node");
+  m.def("layer_norm", &layer_norm, "layer norm as one C++ autograd node");
+  m.def("linear_loss", &linear_loss, "cross entropy or distillation from hidden states as one C++ autograd node");
   // the header revision this module was compiled against (not the loaded
   // library's, which the Python loader compares it with)
   m.def("abi_version", [] { return RR_ABI_VERSION; });

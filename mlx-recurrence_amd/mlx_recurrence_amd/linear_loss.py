@@ -72,13 +72,16 @@ def _check_ids(name, t):
         raise TypeError(f"{name} must be integers, got {t.dtype}")
 
 
-def _apply(hidden, weight, labels, t_logits, t_ids, ignore_index, z_loss, temperature, reduction):
+def _apply(hidden, weight, *args):
+    """args: what _LinearLoss takes behind the weight."""
     lead, D = hidden.shape[:-1], hidden.shape[-1]
     dt = _lib.common_dtype(hidden, weight)
-    h = hidden.reshape(-1, D)
-    loss = _LinearLoss.apply(h if h.dtype == dt else h.to(dt), weight if weight.dtype == dt else weight.to(dt), labels,
-                             t_logits, t_ids, ignore_index, z_loss, temperature, _REDUCTIONS[reduction])
-    return loss.reshape(lead) if reduction == "none" else loss
+    h = hidden if len(lead) == 1 else hidden.reshape(-1, D)
+    h, w = h if h.dtype == dt else h.to(dt), weight if weight.dtype == dt else weight.to(dt)
+    ext = _lib.autograd_ext()
+    # the same forward / backward as one C++ autograd node where it is built
+    loss = _LinearLoss.apply(h, w, *args) if ext is None else ext.linear_loss(h, w, *args)
+    return loss.reshape(lead) if len(lead) != 1 and loss.ndim == 1 else loss
 
 
 def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, z_loss=0.0, reduction="mean"):
@@ -110,7 +113,8 @@ def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, z_loss=0.
     _check_ids("labels", labels)
     if not math.isfinite(float(z_loss)):
         raise ValueError(f"z_loss must be finite, got {z_loss}")
-    return _apply(hidden, weight, labels.reshape(-1), None, None, int(ignore_index), float(z_loss), 1.0, reduction)
+    return _apply(hidden, weight, labels.reshape(-1), None, None, int(ignore_index), float(z_loss), 1.0,
+                  _REDUCTIONS[reduction])
 
 
 def linear_distillation(hidden, weight, teacher_logits, teacher_ids, *, temperature=1.0, reduction="mean"):
@@ -149,7 +153,7 @@ def linear_distillation(hidden, weight, teacher_logits, teacher_ids, *, temperat
         raise ValueError(f"temperature must be positive and finite, got {temperature}")
     K = teacher_ids.shape[-1]
     return _apply(hidden, weight, None, teacher_logits.detach().reshape(-1, K), teacher_ids.reshape(-1, K), 0, 0.0,
-                  float(temperature), reduction)
+                  float(temperature), _REDUCTIONS[reduction])
 
 
 def _reduce(loss, valid, reduction):

@@ -72,23 +72,27 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, out_dtype=None):
     """
     if x.ndim < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must be [..., D] with D > 0, got shape {tuple(x.shape)}")
-    D = x.shape[-1]
+    shape = x.shape[-1:]
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and tuple(t.shape) != (D,):
-            raise ValueError(f"{name} must be [D] = [{D}], got {tuple(t.shape)}")
-    if not (float(eps) >= 0 and math.isfinite(float(eps))):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"{name} must be [D] = [{shape[0]}], got {tuple(t.shape)}")
+    eps = float(eps)
+    if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     dt = _lib.common_dtype(x)
     out = dt if out_dtype is None else out_dtype
-    if out not in _lib.DTYPE_CODE or (out != dt and dt != torch.float32):
+    if out != dt and (out not in _lib.DTYPE_CODE or dt != torch.float32):
         raise ValueError(f"out_dtype must be {dt} (or any input type for a float32 x), got {out_dtype}")
-    params = [t for t in (weight, bias) if t is not None]
-    if params:
-        wdt = _lib.common_dtype(*params)
+    if weight is not None or bias is not None:
+        wdt = _lib.common_dtype(*(t for t in (weight, bias) if t is not None))
         weight = weight if weight is None or weight.dtype == wdt else weight.to(wdt)
         bias = bias if bias is None or bias.dtype == wdt else bias.to(wdt)
-    return _LayerNorm.apply(x if x.dtype == dt else x.to(dt), weight, bias, float(eps), out,
-                            _lib.records(x, weight, bias))
+    if x.dtype != dt:
+        x = x.to(dt)
+    ext = _lib.autograd_ext()
+    if ext is not None:   # the same forward / backward as one C++ autograd node
+        return ext.layer_norm(x, weight, bias, eps, _lib.DTYPE_CODE[out])
+    return _LayerNorm.apply(x, weight, bias, eps, out, _lib.records(x, weight, bias))
 
 
 def layer_norm_reference(x, weight=None, bias=None, eps=1e-5, *, out_dtype=None):

@@ -440,3 +440,28 @@ def test_weight_past_2_31_elements():
 
 def test_async_status_is_clean():
     _lib.async_status()
+
+
+def test_python_and_cpp_bindings_agree(monkeypatch):
+    """The C++ autograd nodes and the Python Functions make the same calls: the same bits."""
+    assert _lib.autograd_ext() is not None
+
+    def everything():
+        g = gen(21)
+        x, w, b = (t.requires_grad_(True) for t in (randn(g, 30, 100), randn(g, 100), randn(g, 100)))
+        y = mr.layer_norm(x, w, b, out_dtype=BF16)
+        out = [y, *torch.autograd.grad(y, (x, w, b), torch.ones_like(y))]
+        y = mr.layer_norm(x, None, b.detach())
+        out += [y, *torch.autograd.grad(y, (x,), torch.ones_like(y))]
+        g, h, w, labels = head_inputs(50, 64, 700, BF16, 22)
+        t, ids = teacher(g, 50, 7, 700, labels)
+        one = torch.ones((), device="cuda")
+        out += run_ce(h, w, labels, one, z_loss=1e-3) + run_kd(h, w, t, ids, one, temperature=2.0, reduction="sum")
+        with torch.no_grad():
+            out += [mr.layer_norm(x), mr.linear_cross_entropy(h, w, labels, reduction="none")]
+        return out
+
+    cpp = everything()
+    monkeypatch.setattr(_lib, "autograd_ext", lambda: None)
+    for a, b in zip(cpp, everything()):
+        assert a.dtype == b.dtype and torch.equal(a, b)
