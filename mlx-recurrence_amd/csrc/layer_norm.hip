@@ -11,9 +11,11 @@
 // dy) once and y (dx) once.  The kernels are bound by those bytes, a single
 // token by its launch.
 //
-// A row belongs to TPR threads, eight consecutive elements per thread and step.
-// Up to kWaveRow channels that is one wave, whose sums need no barrier; wider
-// rows take a workgroup.
+// A row belongs to TPR threads, eight consecutive elements per thread and step: a wave,
+// whose sums need no barrier, while its registers hold the row, else a workgroup.
+// Reached on an MI355X (a 2 GiB copy: 4.9 TB/s): 32768 x 2560 bf16 forward 4.5 TB/s,
+// backward 4.6 TB/s, the reduction of the parameters' gradients included; 1536 x 768
+// 5 and 11 us, one token 5 us, launches mostly.
 // Rows start at any element (odd D): the 16-byte accesses are made at the
 // element type's alignment, which global memory allows, and only a row's last
 // piece is element by element.
@@ -23,6 +25,7 @@
 // row, and ln_param_kernel adds the partial rows in a fixed order (no atomics:
 // the same inputs give the same bits).
 #include "rr_common.h"
+#include "rr_mfma.h"
 
 #include <algorithm>
 #include <string>
@@ -35,49 +38,53 @@ using rr::f16;
 constexpr int64_t kMaxChannels = 32768;   // 1024 threads, 4 steps of 8 elements
 constexpr int kPartRows = 512;            // partial rows of dw and db at most
 
-// Eight elements from p (any alignment of T), widened.
+// Eight consecutive elements as they lie in memory (any alignment of T).
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-    const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
-  } else {
-    typedef uint16_t u8 __attribute__((ext_vector_type(8), aligned(2)));
-    const u8 a = *reinterpret_cast<const u8*>(p);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = rr::to_f32(__builtin_bit_cast(T, (uint16_t)a[e]));
+struct Raw {
+  typedef uint32_t Words __attribute__((ext_vector_type(2 * sizeof(T))));
+  Words w;
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+    else return rr::to_f32(__builtin_bit_cast(T, (uint16_t)(w[e / 2] >> (16 * (e % 2)))));
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-    *reinterpret_cast<f4*>(p) = f4{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f4*>(p + 4) = f4{v[4], v[5], v[6], v[7]};
-  } else {
-    typedef uint16_t u8 __attribute__((ext_vector_type(8), aligned(2)));
-    u8 a;
+  // Columns c .. c + 7 of a row of D (0 past its end).
+  __device__ __forceinline__ void load(const T* row, int c, int D) {
+    if (c + 8 <= D) {
+      typedef Words Any __attribute__((aligned(sizeof(T))));
+      w = *reinterpret_cast<const Any*>(row + c);
+      return;
+    }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = __builtin_bit_cast(uint16_t, rr::from_f32<T>(v[e]));
-    *reinterpret_cast<u8*>(p) = a;
+    for (int i = 0; i < (int)(2 * sizeof(T)); ++i) w[i] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (c + e >= D) continue;
+      if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(row[c + e]);
+      else w[e / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, row[c + e]) << (16 * (e % 2));
+    }
   }
-}
-// The elements of columns c .. c + 7 of a row of D (0 past its end).
+};
 template <typename T>
 __device__ __forceinline__ void load_cols(const T* row, int c, int D, float (&v)[8]) {
-  if (c + 8 <= D) {
-    load8(row + c, v);
-  } else {
+  Raw<T> r;
+  r.load(row, c, D);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < D ? rr::to_f32(row[c + e]) : 0.f;
-  }
+  for (int e = 0; e < 8; ++e) v[e] = r.get(e);
 }
 template <typename T>
 __device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&v)[8]) {
   if (c + 8 <= D) {
-    store8(row + c, v);
+    typedef typename Raw<T>::Words Words;
+    typedef Words Any __attribute__((aligned(sizeof(T))));
+    Words w;
+#pragma unroll
+    for (int i = 0; i < (int)(2 * sizeof(T)); ++i) {
+      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+      else if constexpr (__is_same(T, bf16)) w[i] = rr::bf_pack2(v[2 * i], v[2 * i + 1]);
+      else w[i] = __builtin_bit_cast(uint16_t, rr::from_f32<T>(v[2 * i])) |
+                  (uint32_t)__builtin_bit_cast(uint16_t, rr::from_f32<T>(v[2 * i + 1])) << 16;
+    }
+    *reinterpret_cast<Any*>(row + c) = w;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -166,8 +173,8 @@ ln_fwd_kernel(const X* __restrict__ x, const void* w, const void* b, int wdt, in
   }
 }
 
-// Rows strided over the grid; dw and db partials of the workgroup's rows in
-// part[block][2][D] (null: not wanted).
+// Rows strided over the grid, the next row's loads issued ahead of this row's sums; dw
+// and db partials of the workgroup's rows in part[block][2][D] (null: not wanted).
 template <typename X, typename Y, int TPR, int NV>
 __global__ void __launch_bounds__(block_threads<TPR>())
 ln_bwd_kernel(const Y* __restrict__ dy, const X* __restrict__ x, const void* w, int wdt, const float* mean,
@@ -189,26 +196,37 @@ ln_bwd_kernel(const Y* __restrict__ dy, const X* __restrict__ x, const void* w, 
     }
   }
   const float inv = 1.f / (float)D;
-  for (int64_t row = (int64_t)blockIdx.x * RPB + slot; row < rows; row += (int64_t)gridDim.x * RPB) {
-    const float mu = mean[row], r = rstd[row];
-    float xh[NV][8], g[NV][8];
-    float s1 = 0.f, s2 = 0.f;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + slot;
+  Raw<X> xn[NV];
+  Raw<Y> gn[NV];
+  float mn = 0.f, rn = 0.f;
+  auto fetch = [&](int64_t r) {
+    mn = mean[r], rn = rstd[r];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * TPR + lane) * 8;
-      load_cols(x + row * D, c, D, xh[j]);
-      load_cols(dy + row * D, c, D, g[j]);
+      xn[j].load(x + r * D, (j * TPR + lane) * 8, D);
+      gn[j].load(dy + r * D, (j * TPR + lane) * 8, D);
     }
+  };
+  if (row < rows) fetch(row);
+  for (; row < rows; row += step) {
+    Raw<X> xc[NV];
+    Raw<Y> gc[NV];
+    const float mu = mn, r = rn;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) xc[j] = xn[j], gc[j] = gn[j];
+    if (row + step < rows) fetch(row + step);
+    float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float d = g[j][e];          // 0 past the row's end
-        const float h = (j * TPR + lane) * 8 + e < D ? (xh[j][e] - mu) * r : 0.f;
-        dw[j][e] += d * h, db[j][e] += d;
-        xh[j][e] = h;
-        g[j][e] = d * wv[j][e];
-        s1 += g[j][e], s2 += g[j][e] * h;
+        const float d = gc[j].get(e);     // 0 past the row's end
+        const float h = (xc[j].get(e) - mu) * r;
+        const float g = d * wv[j][e];
+        db[j][e] += d, s1 += g;
+        dw[j][e] += d * h, s2 += g * h;
       }
     if (dx != nullptr) {
       row_sum2<TPR>(s1, s2, buf);
@@ -218,7 +236,7 @@ ln_bwd_kernel(const Y* __restrict__ dy, const X* __restrict__ x, const void* w, 
         const int c = (j * TPR + lane) * 8;
         float o[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = r * (g[j][e] - s1 - xh[j][e] * s2);
+        for (int e = 0; e < 8; ++e) o[e] = r * (gc[j].get(e) * wv[j][e] - s1 - (xc[j].get(e) - mu) * r * s2);
         if (c < D) store_cols(dx + row * D, c, D, o);
       }
     }
@@ -248,37 +266,49 @@ ln_bwd_kernel(const Y* __restrict__ dy, const X* __restrict__ x, const void* w, 
     }
 }
 
-// dw and db from the partial rows: a workgroup takes 64 columns of one of them,
-// its four waves every fourth partial row, added up in order.
-__global__ void __launch_bounds__(256)
+// dw and db from the partial rows: a workgroup takes 64 columns of one of them, its
+// sixteen waves every sixteenth partial row, added up in order.
+__global__ void __launch_bounds__(1024)
 ln_param_kernel(const float* __restrict__ part, int n, int D, void* dw, void* db, int wdt) {
-  __shared__ float buf[4][64];
+  __shared__ float buf[16][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int c = blockIdx.x * 64 + lane, h = blockIdx.y;
   void* out = h == 0 ? dw : db;
   if (out == nullptr) return;
   float s = 0.f;
-  if (c < D)
-    for (int i = wave; i < n; i += 4) s += part[((int64_t)i * 2 + h) * D + c];
+  if (c < D) {
+#pragma unroll 8
+    for (int i = wave; i < n; i += 16) s += part[((int64_t)i * 2 + h) * D + c];
+  }
   buf[wave][lane] = s;
   __syncthreads();
   if (wave != 0 || c >= D) return;
-  s = buf[0][lane] + buf[1][lane] + buf[2][lane] + buf[3][lane];
+  for (int i = 1; i < 16; ++i) s += buf[i][lane];
   if (wdt == RR_F32) static_cast<float*>(out)[c] = s;
   else if (wdt == RR_BF16) static_cast<bf16*>(out)[c] = rr::from_f32<bf16>(s);
   else static_cast<f16*>(out)[c] = rr::from_f32<f16>(s);
 }
 
-// Threads a row and pieces a thread for D channels.
+// Threads a row and pieces a thread for D channels.  A wave a row (no barrier) while its
+// registers hold the row: 8 pieces forward, 5 backward (3 of fp32), where the next row and
+// the parameters' sums are held too.  32768 x 2560 bf16: 74 and 111 us; with a workgroup a
+// row 87 and 146 us.
+constexpr int wave_pieces(bool bwd, bool fp32) { return !bwd ? 8 : fp32 ? 3 : 5; }
 struct Shape { int tpr, nv; };
-Shape shape_of(int64_t D, bool bwd) {
+Shape shape_of(int64_t D, bool bwd, bool fp32) {
   const int64_t v = (D + 7) / 8;   // pieces of a row
-  const int tpr = v <= 64 * (bwd ? 2 : 4) ? 64 : v <= 256 * 4 ? 256 : 1024;
+  const int tpr = v <= 64 * wave_pieces(bwd, fp32) ? 64 : v <= 256 * 4 ? 256 : 1024;
   return {tpr, (int)((v + tpr - 1) / tpr)};
 }
+// Whether shape_of gives this one.
+constexpr bool reached(bool bwd, bool fp32, int tpr, int nv) {
+  const int w = wave_pieces(bwd, fp32);
+  return tpr == 64 ? nv <= w : tpr == 256 ? nv <= 4 && nv * 256 > w * 64 : nv <= 4 && nv * 1024 > 1024;
+}
+// Workgroups of the backward: two rows a wave (or workgroup) where that leaves fewer than
+// kPartRows partial rows.
 int64_t bwd_blocks(int64_t rows, int64_t D) {
-  const Shape s = shape_of(D, true);
-  const int64_t rpb = s.tpr == 64 ? 4 : 1;
+  const int64_t rpb = D <= 64 * 8 * wave_pieces(true, false) ? 8 : 2;
   return std::max<int64_t>(1, std::min<int64_t>(kPartRows, (rows + rpb - 1) / rpb));
 }
 
@@ -297,17 +327,20 @@ int check_args(const char* who, int64_t rows, int64_t D, int xdt, int ydt, int w
 
 }  // namespace
 
-#define LN_NV(TPR, KERNEL, NB, ...)                                                                              \
+#define LN_CASE(BWD, TPR, NV, KERNEL, NB, ...)                                                                   \
+  case NV:                                                                                                       \
+    if constexpr (reached(BWD, sizeof(X) == 4, TPR, NV)) KERNEL<X, Y, TPR, NV><<<NB, block_threads<TPR>(), 0, s>>>(__VA_ARGS__); \
+    break;
+#define LN_NV(BWD, TPR, ...)                                                                                     \
   switch (sh.nv) {                                                                                               \
-    case 1: KERNEL<X, Y, TPR, 1><<<NB, block_threads<TPR>(), 0, s>>>(__VA_ARGS__); break;                        \
-    case 2: KERNEL<X, Y, TPR, 2><<<NB, block_threads<TPR>(), 0, s>>>(__VA_ARGS__); break;                        \
-    case 3: KERNEL<X, Y, TPR, 3><<<NB, block_threads<TPR>(), 0, s>>>(__VA_ARGS__); break;                        \
-    default: KERNEL<X, Y, TPR, 4><<<NB, block_threads<TPR>(), 0, s>>>(__VA_ARGS__); break;                       \
+    LN_CASE(BWD, TPR, 1, __VA_ARGS__) LN_CASE(BWD, TPR, 2, __VA_ARGS__) LN_CASE(BWD, TPR, 3, __VA_ARGS__)        \
+    LN_CASE(BWD, TPR, 4, __VA_ARGS__) LN_CASE(BWD, TPR, 5, __VA_ARGS__) LN_CASE(BWD, TPR, 6, __VA_ARGS__)        \
+    LN_CASE(BWD, TPR, 7, __VA_ARGS__) LN_CASE(BWD, TPR, 8, __VA_ARGS__)                                          \
   }
-#define LN_SHAPE(KERNEL, NB, ...)                                                                                \
-  if (sh.tpr == 64) { LN_NV(64, KERNEL, NB, __VA_ARGS__) }                                                       \
-  else if (sh.tpr == 256) { LN_NV(256, KERNEL, NB, __VA_ARGS__) }                                                \
-  else { LN_NV(1024, KERNEL, NB, __VA_ARGS__) }
+#define LN_SHAPE(BWD, ...)                                                                                       \
+  if (sh.tpr == 64) { LN_NV(BWD, 64, __VA_ARGS__) }                                                              \
+  else if (sh.tpr == 256) { LN_NV(BWD, 256, __VA_ARGS__) }                                                       \
+  else { LN_NV(BWD, 1024, __VA_ARGS__) }
 // x and y types: the same, or fp32 x with any y.
 #define LN_TYPES(...)                                                                                            \
   if (x_dtype == RR_BF16) { using X = bf16; using Y = bf16; __VA_ARGS__ }                                        \
@@ -325,9 +358,9 @@ extern "C" int rr_layer_norm_fwd(const void* x, int x_dtype, const void* w, cons
     return rr::fail(RR_EINVAL, "rr_layer_norm_fwd: null pointer");
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const Shape sh = shape_of(D, false);
+  const Shape sh = shape_of(D, false, x_dtype == RR_F32);
   const int nb = (int)(sh.tpr == 64 ? (rows + 3) / 4 : rows);
-  LN_TYPES(LN_SHAPE(ln_fwd_kernel, nb, static_cast<const X*>(x), w, b, w_dtype, rows, (int)D, eps, static_cast<Y*>(y), mean,
+  LN_TYPES(LN_SHAPE(false, ln_fwd_kernel, nb, static_cast<const X*>(x), w, b, w_dtype, rows, (int)D, eps, static_cast<Y*>(y), mean,
                     rstd))
   return rr::check_launch("rr_layer_norm_fwd");
 }
@@ -356,13 +389,13 @@ extern "C" int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int
     }
     if (!params && dx == nullptr) return RR_OK;
     float* part = params ? static_cast<float*>(workspace) : nullptr;
-    const Shape sh = shape_of(D, true);
-    LN_TYPES(LN_SHAPE(ln_bwd_kernel, (int)nb, static_cast<const Y*>(dy), static_cast<const X*>(x), w, w_dtype, mean, rstd,
+    const Shape sh = shape_of(D, true, x_dtype == RR_F32);
+    LN_TYPES(LN_SHAPE(true, ln_bwd_kernel, (int)nb, static_cast<const Y*>(dy), static_cast<const X*>(x), w, w_dtype, mean, rstd,
                       rows, (int)D, static_cast<X*>(dx), part))
   }
   if (params) {
     const dim3 grid((unsigned)((D + 63) / 64), 2);
-    ln_param_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(workspace), (int)nb, (int)D, dw, db, w_dtype);
+    ln_param_kernel<<<grid, 1024, 0, s>>>(static_cast<const float*>(workspace), (int)nb, (int)D, dw, db, w_dtype);
   }
   return rr::check_launch("rr_layer_norm_bwd");
 }
