@@ -394,9 +394,10 @@ int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, c
  * `reduction` 0 leaves a loss a row (loss [rows] fp32), 1 their mean over the rows
  * that count, 2 their sum (loss [1]; both 0 where no row counts).  The forward
  * leaves in `state` (16-byte aligned, rr_linear_loss_state_bytes) what
- * rr_linear_loss_bwd reads; its contents are the library's own.  K: teacher
+ * rr_linear_loss_bwd reads, the hidden states that count among it (the backward
+ * needs `hidden` no more); its contents are the library's own.  K: teacher
  * entries a row, 1 to 1024; 1 for labels.  V <= 2^24, D <= 65536. */
-size_t rr_linear_loss_state_bytes(int64_t rows, int64_t K);
+size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t K, int dtype);
 
 /* Workspace of the forward (pass = 0) or backward (pass = 1); 0 for invalid
  * arguments.  The backward's holds a piece of the logits' gradient: about
@@ -425,11 +426,10 @@ int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtype, int64_t 
                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients of either loss: dloss fp32 ([rows] for reduction 0, else [1]), the
- * forward's inputs and state, K = 1 and temperature = 1 for the cross entropy,
+ * forward's weight and state, K = 1 and temperature = 1 for the cross entropy,
  * z_loss = 0 for the distillation.  dhidden [rows, D] and dweight [V, D] in
  * `dtype`, each null where not wanted; rows that do not count get dhidden 0. */
-int rr_linear_loss_bwd(const float* dloss, const void* hidden, const void* weight, int dtype, int64_t rows,
-                       int64_t D, int64_t V, int64_t K, float z_loss, float temperature, int reduction,
+int rr_linear_loss_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V, int64_t K, float z_loss, float temperature, int reduction,
                        const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
                        size_t workspace_bytes, void* stream);
 

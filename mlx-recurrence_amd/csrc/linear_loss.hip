@@ -36,6 +36,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 namespace {
 
@@ -53,9 +54,14 @@ constexpr int64_t kMaxPiece = 1 << 20;       // a row of a tile's operand is at 
 constexpr int64_t kFewRows = 64;           // rows whose dz keeps a second plane
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-constexpr int BM = 256, BN = 256;   // a tile of each product
-constexpr int WM = 2, WN = 4;             // its waves
-constexpr int kThreads = 64 * WM * WN;
+// Tiles: BM (words, or channels) x BN (rows, or words), WM x WN waves.  Tile256 moves the
+// fewest bytes a flop; two Tile128 share a CU, for products whose Tile256 would leave CUs
+// without work; Tile32 is for a few rows, whose products are bound by the weight's bytes.
+struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, THREADS = 512; };
+struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, THREADS = 256; };
+struct Tile32 { static constexpr int BM = 256, BN = 32, WM = 4, WN = 1, THREADS = 256; };
+enum Tiles { kTile256, kTile128, kTile32 };
+constexpr int kEdge = 256;       // buffers hold whole tiles of any kind
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
@@ -75,8 +81,9 @@ struct State {
   int* ids;      // [rows][K] the entries' columns, ascending; kAbsent past the last
   float* p;      // [rows][K] their weights
   float* z2;     // [rows][K] their logits, times log2(e) / tau
+  uint16_t* h;   // [planes][rows][Dp] the hidden states that count, as an operand
 };
-size_t state_layout(int64_t T, int64_t K, char* base, State* s) {
+size_t state_layout(int64_t T, int64_t D, int64_t K, int dtype, char* base, State* s) {
   size_t off = 0;
   auto take = [&](size_t bytes) {
     char* at = base + off;
@@ -92,6 +99,7 @@ size_t state_layout(int64_t T, int64_t K, char* base, State* s) {
   t.ids = reinterpret_cast<int*>(take((size_t)T * K * 4));
   t.p = reinterpret_cast<float*>(take((size_t)T * K * 4));
   t.z2 = reinterpret_cast<float*>(take((size_t)T * K * 4));
+  t.h = reinterpret_cast<uint16_t*>(take((size_t)T * up(D, BK) * (dtype == RR_F32 ? 4 : 2)));
   if (s != nullptr) *s = t;
   return off;
 }
@@ -104,11 +112,27 @@ struct Plan {
   int planes_z;        // of dz
   bool copy_w;         // the weight is copied (planes, or rows that are not whole 16-byte chunks)
   int64_t Tp, Dp;      // rows to whole tiles, channels to whole k steps
-  int64_t nvt, ntt, ndt;   // tiles of V, T, D
+  int64_t Vt, Dt;      // words and channels to whole tiles
+  Tiles logits, dh, dw;
   // backward
   int64_t Vp;          // columns of a piece (whole tiles)
   int64_t splits;      // parts of a piece's columns that dh is added up in
 };
+constexpr int64_t kCus = 256;
+// Time of a product of `tiles` tiles of `steps` k steps each: full rounds of workgroups, in
+// steps of a Tile256.  A Tile128 has a quarter of its products; a pair of them that share a
+// CU takes 0.6 of its time where two quarters would be half.
+double rounds(Tiles t, int64_t tiles, double steps) {
+  const int64_t slots = t == kTile256 ? kCus : 2 * kCus;
+  return (double)((tiles + slots - 1) / slots) * steps * (t == kTile256 ? 1.0 : 0.6);
+}
+int64_t tiles_of(Tiles t, int64_t m, int64_t n) {
+  const int64_t e = t == kTile256 ? 256 : 128;
+  return up(m, e) / e * (up(n, e) / e);
+}
+Tiles choose(int64_t m, int64_t n) {
+  return rounds(kTile128, tiles_of(kTile128, m, n), 1.0) < rounds(kTile256, tiles_of(kTile256, m, n), 1.0) ? kTile128 : kTile256;
+}
 Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   Plan p{};
   p.T = T, p.D = D, p.V = V, p.dtype = dtype;
@@ -117,21 +141,32 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   // second plane, which costs nothing there (the weight's bytes bound the products).
   p.planes_z = p.planes == 2 || T <= kFewRows ? 2 : 1;
   p.copy_w = p.planes == 2 || D % 8 != 0;
-  p.Tp = up(T, BN), p.Dp = up(D, BK);
-  p.nvt = up(V, BM) / BM, p.ntt = p.Tp / BN, p.ndt = up(D, BM) / BM;
-  const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * 2 * p.planes_z) / BM * BM));
-  const int64_t pieces = (p.nvt * BM + most - 1) / most;
-  p.Vp = up((p.nvt * BM + pieces - 1) / pieces, BM);
-  // enough workgroups for the GPU, of at least 8 k steps each
-  const int64_t tiles = p.ntt * p.ndt;
-  p.splits = std::max<int64_t>(1, std::min<int64_t>({1024 / std::max<int64_t>(1, tiles), p.Vp / (8 * BK), 64}));
+  const bool few = T <= Tile32::BN;
+  p.Tp = few ? Tile32::BN : up(T, kEdge), p.Dp = up(D, BK);
+  p.Vt = up(V, kEdge), p.Dt = up(D, kEdge);
+  const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * 2 * p.planes_z) / kEdge * kEdge));
+  const int64_t pieces = (p.Vt + most - 1) / most;
+  p.Vp = up((p.Vt + pieces - 1) / pieces, kEdge);
+  p.logits = few ? kTile32 : choose(p.Vp, T);
+  p.dw = choose(D, p.Vp);
+  // dh has few tiles: its sum over the piece's columns is cut in parts, each at the cost of
+  // writing and reading its part of dh (in steps of a Tile256, which take 1.5 us, at 4 TB/s).
+  const int64_t steps = p.Vp / BK * (p.planes + p.planes_z - 1);
+  const double part = (double)(std::min(p.Tp, up(T, 32)) * D * 8) / 4e12 / 1.5e-6;
+  double best = 0;
+  for (int t = few ? kTile32 : kTile256; t <= (few ? kTile32 : kTile128); ++t) {
+    const int64_t tiles = t == kTile32 ? p.Dt / Tile32::BM : tiles_of((Tiles)t, D, T);
+    for (int64_t n = 1; n <= 64 && n * 4 <= std::max<int64_t>(4, p.Vp / BK); ++n) {
+      const double cost = rounds((Tiles)t, tiles * n, (double)steps / (double)n) + (double)n * part;
+      if (best == 0 || cost < best) best = cost, p.dh = (Tiles)t, p.splits = n;
+    }
+  }
   return p;
 }
 
 struct FwdWs {
-  uint16_t* h;     // [planes][T][Dp]
   uint16_t* w;     // [planes][V][Dp] where the weight is copied
-  float2* part;    // [nvt][Tp] maximum and sum of a tile's row
+  float2* part;    // [word tiles][Tp] maximum and sum of a tile's row
 };
 size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
   size_t off = 0;
@@ -140,21 +175,18 @@ size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
     off += (bytes + 255) / 256 * 256;
     return at;
   };
-  const size_t planes = p.planes;
   FwdWs t;
-  t.h = reinterpret_cast<uint16_t*>(take(planes * p.T * p.Dp * 2));
-  t.w = reinterpret_cast<uint16_t*>(take(p.copy_w ? planes * p.V * p.Dp * 2 : 0));
-  t.part = reinterpret_cast<float2*>(take((size_t)p.nvt * p.Tp * sizeof(float2)));
+  t.w = reinterpret_cast<uint16_t*>(take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * 2 : 0));
+  t.part = reinterpret_cast<float2*>(take((size_t)(p.Vt / 128) * p.Tp * sizeof(float2)));
   if (s != nullptr) *s = t;
   return off;
 }
 struct BwdWs {
-  uint16_t* h;
-  uint16_t* w;
+  uint16_t* w;     // as forward
   float* scale;    // [0] the factor on both gradients
   float2* coef;    // [Tp] a row's factors (coef_kernel)
   uint16_t* dz;    // [planes_z][Tp][Vp]
-  float* dh;       // [splits][Tp][ndt * BM]
+  float* dh;       // [splits][Tp][Dt]
 };
 size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
   size_t off = 0;
@@ -163,14 +195,12 @@ size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
     off += (bytes + 255) / 256 * 256;
     return at;
   };
-  const size_t planes = p.planes;
   BwdWs t;
-  t.h = reinterpret_cast<uint16_t*>(take(planes * p.T * p.Dp * 2));
-  t.w = reinterpret_cast<uint16_t*>(take(p.copy_w ? planes * p.V * p.Dp * 2 : 0));
+  t.w = reinterpret_cast<uint16_t*>(take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * 2 : 0));
   t.scale = reinterpret_cast<float*>(take(256));
   t.coef = reinterpret_cast<float2*>(take((size_t)p.Tp * sizeof(float2)));
   t.dz = reinterpret_cast<uint16_t*>(take((size_t)p.planes_z * p.Tp * p.Vp * 2));
-  t.dh = reinterpret_cast<float*>(take((size_t)p.splits * p.Tp * p.ndt * BM * 4));
+  t.dh = reinterpret_cast<float*>(take((size_t)p.splits * p.Tp * p.Dt * 4));
   if (s != nullptr) *s = t;
   return off;
 }
@@ -295,21 +325,40 @@ rows_kernel(const int64_t* __restrict__ labels, int64_t ignore, int64_t T, int V
   if (tid == 0) st.hdr->n = base, st.hdr->amax_h = 0, st.hdr->amax_w = 0;
 }
 
+// Eight elements from column c of a row of D as they lie in memory, 0 past its end (a row
+// may start at any element).
+template <typename X>
+__device__ __forceinline__ void load8(const X* row, int c, int D, X (&v)[8]) {
+  if (c + 8 <= D) {
+    typedef uint32_t Words __attribute__((ext_vector_type(2 * sizeof(X))));
+    typedef Words Any __attribute__((aligned(sizeof(X))));
+    const Words w = *reinterpret_cast<const Any*>(row + c);
+    __builtin_memcpy(v, &w, sizeof(w));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < D ? row[c + e] : X{};
+  }
+}
+
 // Largest finite |x| of the rows (through `rows`, the first hdr->n of them, where given).
 __global__ void __launch_bounds__(256)
 amax_kernel(const float* __restrict__ x, int64_t n_rows, int D, const int* rows, const Header* hdr, uint32_t* out) {
   const int64_t n = rows != nullptr ? hdr->n : n_rows;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   float m = 0.f;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < n; r += (int64_t)gridDim.x * 4) {
+  for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const float* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
-    for (int c = lane; c < D; c += 64) {
-      const float a = fabsf(xr[c]);
-      if (a < INFINITY) m = fmaxf(m, a);   // neither infinite nor NaN
+    for (int c = threadIdx.x * 8; c < D; c += 2048) {
+      float v[8];
+      load8(xr, c, D, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = fabsf(v[e]);
+        if (a < INFINITY) m = fmaxf(m, a);   // neither infinite nor NaN
+      }
     }
   }
   m = wave_max(m);
-  if (lane == 0 && m > 0.f) atomicMax(out, __float_as_uint(m));
+  if ((threadIdx.x & 63) == 0 && m > 0.f) atomicMax(out, __float_as_uint(m));
 }
 
 // Rows as operands: copied (16-bit inputs) or split into two planes (fp32), padded
@@ -319,31 +368,26 @@ __global__ void __launch_bounds__(256)
 pack_kernel(const X* __restrict__ x, int64_t n_rows, int D, int Dp, const int* rows, const Header* hdr, int which,
             uint16_t* __restrict__ out, int64_t plane) {
   const int64_t n = rows != nullptr ? hdr->n : n_rows;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   float sc = 1.f;
   if constexpr (sizeof(X) == 4) sc = which == 0 ? scale_h(hdr) : scale_w(hdr);
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < n; r += (int64_t)gridDim.x * 4) {
+  for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const X* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
     uint16_t* o = out + r * Dp;
-    for (int c = lane * 2; c < Dp; c += 128) {
-      if constexpr (sizeof(X) == 4) {
-        uint32_t hi = 0, lo = 0;
+    for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
+      X v[8];
+      load8(xr, c, D, v);
+      rr::u16x8_t hi, lo;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float v = c + e < D ? xr[c + e] * sc : 0.f;
-          const uint16_t hb = op_bits<OpF16>(v);
-          hi |= (uint32_t)hb << (16 * e);
-          lo |= (uint32_t)op_bits<OpF16>(v - op_val<OpF16>(hb)) << (16 * e);
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (sizeof(X) == 4) {
+          hi[e] = op_bits<OpF16>(v[e] * sc);
+          lo[e] = op_bits<OpF16>(v[e] * sc - op_val<OpF16>(hi[e]));
+        } else {
+          hi[e] = __builtin_bit_cast(uint16_t, v[e]);
         }
-        *reinterpret_cast<uint32_t*>(o + c) = hi;
-        *reinterpret_cast<uint32_t*>(o + plane + c) = lo;
-      } else {
-        uint32_t v = 0;
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (c + e < D) v |= (uint32_t)__builtin_bit_cast(uint16_t, xr[c + e]) << (16 * e);
-        *reinterpret_cast<uint32_t*>(o + c) = v;
       }
+      *reinterpret_cast<rr::u16x8_t*>(o + c) = hi;
+      if constexpr (sizeof(X) == 4) *reinterpret_cast<rr::u16x8_t*>(o + plane + c) = lo;
     }
   }
 }
@@ -392,15 +436,36 @@ __device__ __forceinline__ void each_entry(const int* ids, int K, int v0, int qu
   }
 }
 
+// One of a wave's column blocks (16 rows of the output, MW consecutive values of each) to
+// memory through LDS, so that a row leaves in whole lines: value(i) is the lane's four of
+// block i (its row lane % 16, from 16 i + 4 (lane / 16)), store(r, c, v) takes 16 bytes of
+// row r from value c on.  `lds`: 16 (MW + 16 / sizeof(T)) values of the wave's own.
+template <int MI, typename T, typename F, typename S>
+__device__ __forceinline__ void store_block(T* lds, int lane, F value, S store) {
+  constexpr int MW = 16 * MI, VEC = 16 / sizeof(T), PITCH = MW + VEC, PER_ROW = MW / VEC;
+  typedef T Four __attribute__((ext_vector_type(4)));
+  typedef T Vec __attribute__((ext_vector_type(VEC)));
+#pragma unroll
+  for (int i = 0; i < MI; ++i) *reinterpret_cast<Four*>(lds + (lane & 15) * PITCH + 16 * i + 4 * (lane >> 4)) = value(i);
+  rr::wave_lds_sync();
+#pragma unroll
+  for (int q = 0; q < 16 * PER_ROW / 64; ++q) {
+    const int r = q * (64 / PER_ROW) + lane / PER_ROW, c = lane % PER_ROW * VEC;
+    store(r, c, *reinterpret_cast<const Vec*>(lds + r * PITCH + c));
+  }
+  rr::wave_lds_sync();
+}
+
 // z^T tiles: m = vocabulary, n = rows, so that a lane holds 4 MI logits of a row.
-template <typename Op, bool GRAD, int PX, int PZ>
-__global__ void __launch_bounds__(kThreads)
+template <typename C, typename Op, bool GRAD, int PX, int PZ>
+__global__ void __launch_bounds__(C::THREADS, 2)
 logits_kernel(LogitArgs a) {
-  using P = Product<Op, BM, BN, WM, WN, false, false>;
+  constexpr int BM = C::BM, BN = C::BN;
+  using P = Product<Op, BM, BN, C::WM, C::WN, false, false>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
   int vt, tt;
-  tile_of(blockIdx.x, a.nvt, a.Tp / BN, vt, tt);
+  tile_of(blockIdx.x, a.nvt, gridDim.x / a.nvt, vt, tt);
   const int t0 = tt * BN, v0 = a.v_first + vt * BM;
   if (t0 >= n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -484,18 +549,26 @@ logits_kernel(LogitArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = el == i * 4 + e ? acc[i][j][e] - p + r : acc[i][j][e];
       });
-      uint16_t* o = a.dz + (int64_t)t * a.ldz + (vw - a.v_first) + 4 * quarter;
+      typedef uint16_t u16x4_e __attribute__((ext_vector_type(4)));
+      typedef uint16_t u16x8_e __attribute__((ext_vector_type(8)));
+      uint16_t* stage = lds + wave * 16 * (P::MW + 8);
+      uint16_t* o = a.dz + (int64_t)(t0 + wn * P::NW + 16 * j) * a.ldz + (vw - a.v_first);
+      auto store = [&](int r, int v, u16x8_e x) { *reinterpret_cast<u16x8_e*>(o + (int64_t)r * a.ldz + v) = x; };
 #pragma unroll
-      for (int i = 0; i < P::MI; ++i) {
-        rr::u16x4_t hi, lo;
+      for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = on ? co.x * acc[i][j][e] : 0.f;
-          hi[e] = op_bits<Op>(v);
-          if constexpr (PZ == 2) lo[e] = op_bits<Op>(v - op_val<Op>(hi[e]));
-        }
-        *reinterpret_cast<rr::u16x4_t*>(o + 16 * i) = hi;
-        if constexpr (PZ == 2) *reinterpret_cast<rr::u16x4_t*>(o + a.plane_z + 16 * i) = lo;
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = on ? co.x * acc[i][j][e] : 0.f;
+      store_block<P::MI>(stage, lane, [&](int i) {
+        return u16x4_e{op_bits<Op>(acc[i][j][0]), op_bits<Op>(acc[i][j][1]), op_bits<Op>(acc[i][j][2]), op_bits<Op>(acc[i][j][3])};
+      }, store);
+      if constexpr (PZ == 2) {
+        o += a.plane_z;
+        store_block<P::MI>(stage, lane, [&](int i) {
+          u16x4_e lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) lo[e] = op_bits<Op>(acc[i][j][e] - op_val<Op>(op_bits<Op>(acc[i][j][e])));
+          return lo;
+        }, store);
       }
     }
   }
@@ -513,10 +586,10 @@ logits_kernel(LogitArgs a) {
   }
 }
 
-// Per row: the tiles' maxima and sums to the row's lse, and its loss.  A wave per row.
+// Per row (a wave each): the tiles' maxima and sums to the row's lse, and its loss.
 __global__ void __launch_bounds__(256)
-row_loss_kernel(State st, const float2* __restrict__ part, int64_t T, int nvt, int64_t Tp, int K, bool labels, float zl,
-                float tau, float* __restrict__ out) {
+row_loss_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, int K, bool labels, float zl, float tau,
+                float* __restrict__ out) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t t = (int64_t)blockIdx.x * 4 + wave;
   if (t >= st.hdr->n) return;
@@ -535,7 +608,7 @@ row_loss_kernel(State st, const float2* __restrict__ part, int64_t T, int nvt, i
     s = (m == mm ? s : s * exp2f(m - mm)) + (m2 == mm ? s2 : s2 * exp2f(m2 - mm));
     m = mm;
   }
-  float l2 = m + log2f(s);
+  const float l2 = m + log2f(s);
   float loss = 0.f;
   for (int k = lane; k < K; k += 64) {
     const float p = st.p[row * K + k];
@@ -560,11 +633,14 @@ row_loss_kernel(State st, const float2* __restrict__ part, int64_t T, int nvt, i
   }
 }
 
-// The sum of the rows' losses, over the number that count where `mean` (0 without any).
+// The sum of the rows' losses, over the number that count where `mean` (0 without any).  A
+// launch of its own: the fences by which row_loss_kernel's last workgroup could do it
+// took 160 us at 8192 rows.
 __global__ void __launch_bounds__(1024)
 sum_loss_kernel(const float* __restrict__ loss, int64_t T, const Header* hdr, bool mean, float* out) {
   __shared__ float buf[16];
   float s = 0.f;
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < T; i += 1024) s += loss[i];
   s = wave_add(s);
   if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = s;
@@ -616,19 +692,21 @@ struct DhArgs {
   const uint16_t* dz;
   int64_t ldw, ldz, plane_w, plane_z;
   int V, D, Dp, Tp, ndt, splits, cols;   // V: rows of w from the piece on; cols: the piece's columns to whole k steps
-  float* out;            // [splits][Tp][ndt * BM]
+  float* out;            // [splits][Tp][Dt]
+  int Dt;
   bool first;
   State st;
 };
-template <typename Op, int PX, int PZ>
-__global__ void __launch_bounds__(kThreads)
+template <typename C, typename Op, int PX, int PZ>
+__global__ void __launch_bounds__(C::THREADS, 2)
 dh_kernel(DhArgs a) {
-  using P = Product<Op, BM, BN, WM, WN, true, false>;
+  constexpr int BM = C::BM, BN = C::BN;
+  using P = Product<Op, BM, BN, C::WM, C::WN, true, false>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
   int dt, tt;
-  const int ntt = a.Tp / BN, sp = blockIdx.x / (a.ndt * ntt);
-  tile_of(blockIdx.x - sp * a.ndt * ntt, a.ndt, ntt, dt, tt);
+  const int tiles = gridDim.x / a.splits, sp = blockIdx.x / tiles;
+  tile_of(blockIdx.x - sp * tiles, a.ndt, tiles / a.ndt, dt, tt);
   const int t0 = tt * BN, d0 = dt * BM;
   if (t0 >= n) return;
   const int steps = a.cols / BK;
@@ -642,7 +720,7 @@ dh_kernel(DhArgs a) {
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
     const int t = t0 + wn * P::NW + 16 * j + (lane & 15);
-    float* o = a.out + ((int64_t)sp * a.Tp + t) * a.ndt * BM + d0 + wm * P::MW + 4 * (lane >> 4);
+    float* o = a.out + ((int64_t)sp * a.Tp + t) * a.Dt + d0 + wm * P::MW + 4 * (lane >> 4);
 #pragma unroll
     for (int i = 0; i < P::MI; ++i) {
       float4* at = reinterpret_cast<float4*>(o + 16 * i);
@@ -656,23 +734,33 @@ dh_kernel(DhArgs a) {
   }
 }
 
-// dh of every row from its parts, in the inputs' type; 0 for rows that do not count.
+// dh of every row from its parts, in the inputs' type; 0 for rows that do not count.  A
+// workgroup per row and 1024 channels, four a thread.
 template <typename X>
 __global__ void __launch_bounds__(256)
-dh_out_kernel(State st, const float* __restrict__ part, int64_t T, int D, int64_t ldp, int64_t stride, int splits,
+dh_out_kernel(State st, const float* __restrict__ part, int D, int64_t ldp, int64_t stride, int splits,
               const float* scale, X* __restrict__ dh) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-  if (row >= T) return;
+  const int64_t row = blockIdx.x;
+  const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (c >= D) return;
   const int t = st.pos[row];
   float f = scale[0];
   if constexpr (sizeof(X) == 4) f /= scale_w(st.hdr);
-  for (int c = lane; c < D; c += 64) {
-    float s = 0.f;
-    if (t >= 0)
-      for (int i = 0; i < splits; ++i) s += part[(int64_t)i * stride + (int64_t)t * ldp + c];
-    dh[row * D + c] = rr::from_f32<X>(s * f);
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (t >= 0) {
+    const float* at = part + (int64_t)t * ldp + c;   // ldp is whole tiles
+#pragma unroll 4
+    for (int i = 0; i < splits; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(at + (int64_t)i * stride);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    s.x *= f, s.y *= f, s.z *= f, s.w *= f;
   }
+  X* o = dh + row * D + c;
+  const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < D) o[e] = rr::from_f32<X>(v[e]);
 }
 
 // dw^T tiles of the piece: m = channels, n = the piece's columns, k = rows.
@@ -685,10 +773,11 @@ struct DwArgs {
   void* out;             // dw at the piece's first row
   State st;
 };
-template <typename Op, typename X, int PX, int PZ>
-__global__ void __launch_bounds__(kThreads)
+template <typename C, typename Op, typename X, int PX, int PZ>
+__global__ void __launch_bounds__(C::THREADS, 2)
 dw_kernel(DwArgs a) {
-  using P = Product<Op, BM, BN, WM, WN, true, true>;
+  constexpr int BM = C::BM, BN = C::BN;
+  using P = Product<Op, BM, BN, C::WM, C::WN, true, true>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
   const int n = a.st.hdr->n;
   int dt, vt;
@@ -704,16 +793,28 @@ dw_kernel(DwArgs a) {
   const int wm = wave / P::WN, wn = wave % P::WN;
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
-    const int v = v0 + wn * P::NW + 16 * j + (lane & 15);
-    if (v >= a.V) continue;
-    X* o = static_cast<X*>(a.out) + (int64_t)v * a.D;
+    using Bits = typename std::conditional<sizeof(X) == 4, float, uint16_t>::type;   // of X
+    typedef Bits Four __attribute__((ext_vector_type(4)));
+    typedef Bits Vec __attribute__((ext_vector_type(16 / sizeof(X))));
+    typedef Vec Any __attribute__((aligned(sizeof(X))));   // rows of dw start at any element
+    const int v = v0 + wn * P::NW + 16 * j, d = d0 + wm * P::MW;
+    Bits* o = static_cast<Bits*>(a.out) + (int64_t)v * a.D + d;
+    store_block<P::MI>(reinterpret_cast<Bits*>(lds) + wave * 16 * (P::MW + 16 / (int)sizeof(X)), lane, [&](int i) {
+      Four x;
 #pragma unroll
-    for (int i = 0; i < P::MI; ++i)
+      for (int e = 0; e < 4; ++e) x[e] = __builtin_bit_cast(Bits, rr::from_f32<X>(acc[i][j][e] * f));
+      return x;
+    }, [&](int r, int c, Vec x) {
+      if (v + r >= a.V) return;
+      Bits* at = o + (int64_t)r * a.D + c;
+      if (d + c + (int)(16 / sizeof(X)) <= a.D) {
+        *reinterpret_cast<Any*>(at) = x;
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = d0 + wm * P::MW + 16 * i + 4 * (lane >> 4) + e;
-        if (d < a.D) o[d] = rr::from_f32<X>(acc[i][j][e] * f);
+        for (int e = 0; e < (int)(16 / sizeof(X)); ++e)
+          if (d + c + e < a.D) at[e] = x[e];
       }
+    });
   }
 }
 
@@ -731,35 +832,25 @@ int check_dims(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int 
     return rr::fail(RR_EUNSUPPORTED, w + ": at most " + std::to_string(kMaxVocab) + " words and " +
                                          std::to_string(kMaxChannels) + " channels");
   }
-  if (T >= ((int64_t)1 << 24) || up(V, BM) / BM * (up(T, BN) / BN) >= (1 << 23)) {   // grids below 2^32 threads
+  if (T >= ((int64_t)1 << 24) || up(V, 128) / 128 * (up(T, 128) / 128) >= (1 << 23)) {   // grids below 2^32 threads
     return rr::fail(RR_EUNSUPPORTED, w + ": too many rows");
   }
   return RR_OK;
 }
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// The weight as an operand, where it is not one itself.
 template <typename X>
-void pack_rows(const Plan& p, const void* hidden, const void* weight, const State& st, uint16_t* h, uint16_t* w, bool amax,
-               hipStream_t s) {
-  if constexpr (sizeof(X) == 4) {
-    if (amax) {
-      amax_kernel<<<512, 256, 0, s>>>(static_cast<const float*>(hidden), p.T, (int)p.D, st.rows, st.hdr, &st.hdr->amax_h);
-      amax_kernel<<<1024, 256, 0, s>>>(static_cast<const float*>(weight), p.V, (int)p.D, nullptr, st.hdr, &st.hdr->amax_w);
-    }
-  }
-  pack_kernel<X><<<(unsigned)std::min<int64_t>(2048, (p.T + 3) / 4), 256, 0, s>>>(
-      static_cast<const X*>(hidden), p.T, (int)p.D, (int)p.Dp, st.rows, st.hdr, 0, h, p.T * p.Dp);
-  if (p.copy_w) {
-    pack_kernel<X><<<(unsigned)std::min<int64_t>(8192, (p.V + 3) / 4), 256, 0, s>>>(
-        static_cast<const X*>(weight), p.V, (int)p.D, (int)p.Dp, nullptr, st.hdr, 1, w, p.V * p.Dp);
-  }
+void pack_weight(const Plan& p, const void* weight, const State& st, uint16_t* w, hipStream_t s) {
+  if (!p.copy_w) return;
+  pack_kernel<X><<<(unsigned)std::min<int64_t>(8192, p.V), 256, 0, s>>>(
+      static_cast<const X*>(weight), p.V, (int)p.D, (int)p.Dp, nullptr, st.hdr, 1, w, p.V * p.Dp);
 }
 
-// What both products read of the weight.
-LogitArgs logit_args(const Plan& p, const State& st, const void* weight, uint16_t* h, uint16_t* w, int K, float tau) {
+LogitArgs logit_args(const Plan& p, const State& st, const void* weight, uint16_t* w, int K, float tau) {
   LogitArgs a{};
   a.w = p.copy_w ? w : static_cast<const uint16_t*>(weight);
-  a.h = h;
+  a.h = st.h;
   a.ldw = p.copy_w ? p.Dp : p.D, a.ldh = p.Dp;
   a.plane_w = p.V * p.Dp, a.plane_h = p.T * p.Dp;
   a.V = (int)p.V, a.D = (int)p.D, a.Dp = (int)p.Dp, a.K = K, a.Tp = (int)p.Tp;
@@ -767,49 +858,84 @@ LogitArgs logit_args(const Plan& p, const State& st, const void* weight, uint16_
   a.st = st;
   return a;
 }
+// The logits of `cols` columns (whole tiles).
+template <typename C, typename Op, bool GRAD, int PX, int PZ>
+void launch_logits(LogitArgs a, int64_t T, int64_t cols, hipStream_t s) {
+  a.nvt = (int)(cols / C::BM);
+  logits_kernel<C, Op, GRAD, PX, PZ><<<(unsigned)(a.nvt * (up(T, C::BN) / C::BN)), C::THREADS, 0, s>>>(a);
+}
+template <typename C, typename Op, int PX, int PZ>
+void launch_dh(DhArgs a, const Plan& p, hipStream_t s) {
+  a.ndt = (int)(up(p.D, C::BM) / C::BM);
+  dh_kernel<C, Op, PX, PZ><<<(unsigned)(a.ndt * (up(p.T, C::BN) / C::BN) * p.splits), C::THREADS, 0, s>>>(a);
+}
+template <typename C, typename Op, typename X, int PX, int PZ>
+void launch_dw(DwArgs a, const Plan& p, int64_t cols, hipStream_t s) {
+  a.ndt = (int)(up(p.D, C::BM) / C::BM);
+  dw_kernel<C, Op, X, PX, PZ><<<(unsigned)(a.ndt * (cols / C::BN)), C::THREADS, 0, s>>>(a);
+}
 
 template <typename X, typename Op, int PX>
 int forward(const Plan& p, const void* hidden, const void* weight, const State& st, const FwdWs& ws, int K, bool labels,
             float zl, float tau, int reduction, float* loss, hipStream_t s) {
-  pack_rows<X>(p, hidden, weight, st, ws.h, ws.w, true, s);
-  LogitArgs a = logit_args(p, st, weight, ws.h, ws.w, K, tau);
-  a.part = ws.part, a.nvt = (int)p.nvt;
-  logits_kernel<Op, false, PX, PX><<<(unsigned)(p.nvt * p.ntt), kThreads, 0, s>>>(a);
+  if constexpr (PX == 2) {
+    amax_kernel<<<1024, 256, 0, s>>>(static_cast<const float*>(hidden), p.T, (int)p.D, st.rows, st.hdr, &st.hdr->amax_h);
+    amax_kernel<<<2048, 256, 0, s>>>(static_cast<const float*>(weight), p.V, (int)p.D, nullptr, st.hdr, &st.hdr->amax_w);
+  }
+  pack_kernel<X><<<(unsigned)std::min<int64_t>(8192, p.T), 256, 0, s>>>(
+      static_cast<const X*>(hidden), p.T, (int)p.D, (int)p.Dp, st.rows, st.hdr, 0, st.h, p.T * p.Dp);
+  pack_weight<X>(p, weight, st, ws.w, s);
+  LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
+  a.part = ws.part;
+  int edge = 256;
+  if (p.logits == kTile256) {
+    launch_logits<Tile256, Op, false, PX, PX>(a, p.T, p.Vt, s);
+  } else if (p.logits == kTile128) {
+    launch_logits<Tile128, Op, false, PX, PX>(a, p.T, p.Vt, s);
+    edge = 128;
+  } else {
+    launch_logits<Tile32, Op, false, PX, PX>(a, p.T, p.Vt, s);
+  }
   float* rows = reduction == 0 ? loss : st.loss;
-  row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, p.T, (int)p.nvt, p.Tp, K, labels, zl, tau, rows);
+  row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, (int)(p.Vt / edge), p.Tp, K, labels, zl, tau, rows);
   if (reduction != 0) sum_loss_kernel<<<1, 1024, 0, s>>>(st.loss, p.T, st.hdr, reduction == 1, loss);
   return rr::check_launch("rr_linear_loss");
 }
 
 template <typename X, typename Op, int PX, int PZ>
-int backward(const Plan& p, const float* dloss, const void* hidden, const void* weight, const State& st, const BwdWs& ws,
-             int K, float zl, float tau, int reduction, void* dh, void* dw, hipStream_t s) {
-  pack_rows<X>(p, hidden, weight, st, ws.h, ws.w, false, s);
+int backward(const Plan& p, const float* dloss, const void* weight, const State& st, const BwdWs& ws, int K, float zl,
+             float tau, int reduction, void* dh, void* dw, hipStream_t s) {
+  pack_weight<X>(p, weight, st, ws.w, s);
   coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, reduction == 1, tau, zl, !__is_same(Op, OpBf16), ws.coef,
                                  ws.scale);
-  for (int64_t v = 0; v < p.nvt * BM; v += p.Vp) {
-    const int64_t cols = std::min(p.Vp, p.nvt * BM - v);   // whole tiles
-    LogitArgs a = logit_args(p, st, weight, ws.h, ws.w, K, tau);
-    a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp, a.plane_z = p.Tp * p.Vp, a.v_first = (int)v, a.nvt = (int)(cols / BM);
-    logits_kernel<Op, true, PX, PZ><<<(unsigned)(cols / BM * p.ntt), kThreads, 0, s>>>(a);
+  for (int64_t v = 0; v < p.Vt; v += p.Vp) {
+    const int64_t cols = std::min(p.Vp, p.Vt - v);   // whole tiles
+    LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
+    a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp, a.plane_z = p.Tp * p.Vp, a.v_first = (int)v;
+    if (p.logits == kTile256) launch_logits<Tile256, Op, true, PX, PZ>(a, p.T, cols, s);
+    else if (p.logits == kTile128) launch_logits<Tile128, Op, true, PX, PZ>(a, p.T, cols, s);
+    else if constexpr (PZ == 2) launch_logits<Tile32, Op, true, PX, PZ>(a, p.T, cols, s);
     if (dh != nullptr) {
       DhArgs b{};
       b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = p.Vp, b.plane_w = a.plane_w, b.plane_z = a.plane_z;
-      b.V = (int)(p.V - v), b.D = a.D, b.Dp = a.Dp, b.Tp = a.Tp, b.ndt = (int)p.ndt, b.splits = (int)p.splits;
-      b.cols = (int)cols, b.out = ws.dh, b.first = v == 0, b.st = st;
-      dh_kernel<Op, PX, PZ><<<(unsigned)(p.ndt * p.ntt * p.splits), kThreads, 0, s>>>(b);
+      b.V = (int)(p.V - v), b.D = a.D, b.Dp = a.Dp, b.Tp = a.Tp, b.splits = (int)p.splits, b.cols = (int)cols;
+      b.out = ws.dh, b.Dt = (int)p.Dt, b.first = v == 0, b.st = st;
+      if (p.dh == kTile256) launch_dh<Tile256, Op, PX, PZ>(b, p, s);
+      else if (p.dh == kTile128) launch_dh<Tile128, Op, PX, PZ>(b, p, s);
+      else if constexpr (PZ == 2) launch_dh<Tile32, Op, PX, PZ>(b, p, s);
     }
     if (dw != nullptr) {
       DwArgs c{};
-      c.h = ws.h, c.dz = ws.dz, c.ldh = p.Dp, c.ldz = p.Vp, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
-      c.V = (int)(p.V - v), c.D = a.D, c.Dp = a.Dp, c.ndt = (int)p.ndt, c.scale = ws.scale;
+      c.h = st.h, c.dz = ws.dz, c.ldh = p.Dp, c.ldz = p.Vp, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
+      c.V = (int)(p.V - v), c.D = a.D, c.Dp = a.Dp, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
-      dw_kernel<Op, X, PX, PZ><<<(unsigned)(cols / BN * p.ndt), kThreads, 0, s>>>(c);
+      if (p.dw == kTile256) launch_dw<Tile256, Op, X, PX, PZ>(c, p, cols, s);
+      else launch_dw<Tile128, Op, X, PX, PZ>(c, p, cols, s);
     }
   }
   if (dh != nullptr) {
-    dh_out_kernel<X><<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.dh, p.T, (int)p.D, p.ndt * BM, p.Tp * p.ndt * BM,
-                                                              (int)p.splits, ws.scale, static_cast<X*>(dh));
+    dh_out_kernel<X><<<dim3((unsigned)p.T, (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
+        st, ws.dh, (int)p.D, p.Dt, p.Tp * p.Dt, (int)p.splits, ws.scale, static_cast<X*>(dh));
   }
   return rr::check_launch("rr_linear_loss_bwd");
 }
@@ -839,9 +965,9 @@ int run_forward(const char* who, const void* hidden, const void* weight, int dty
 int check_buffers(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int dtype, int pass, const void* hidden,
                   const void* weight, const void* state, size_t state_bytes, const void* ws, size_t ws_bytes) {
   const std::string w(who);
-  if (hidden == nullptr || weight == nullptr || state == nullptr || ws == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
+  if ((pass == 0 && hidden == nullptr) || weight == nullptr || state == nullptr || ws == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
   if (!aligned16(hidden) || !aligned16(weight)) return rr::fail(RR_EINVAL, w + ": buffers must be 16-byte aligned");
-  if (state_bytes < rr_linear_loss_state_bytes(T, K)) return rr::fail(RR_EWORKSPACE, w + ": state buffer too small");
+  if (state_bytes < rr_linear_loss_state_bytes(T, D, K, dtype)) return rr::fail(RR_EWORKSPACE, w + ": state buffer too small");
   if (ws_bytes < rr_linear_loss_workspace_bytes(T, D, V, dtype, pass)) return rr::fail(RR_EWORKSPACE, w + ": workspace too small");
   if (!aligned16(state) || !aligned16(ws)) return rr::fail(RR_EWORKSPACE, w + ": state buffer or workspace misaligned");
   return RR_OK;
@@ -849,9 +975,9 @@ int check_buffers(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, i
 
 }  // namespace
 
-extern "C" size_t rr_linear_loss_state_bytes(int64_t rows, int64_t K) {
-  if (rows <= 0 || K < 1 || K > kMaxEntries) return 0;
-  return state_layout(rows, K, nullptr, nullptr);
+extern "C" size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t K, int dtype) {
+  if (rows <= 0 || check_dims("rr_linear_loss_state_bytes", rows, D, 1, K, dtype, 0) != RR_OK) return 0;
+  return state_layout(rows, D, K, dtype, nullptr, nullptr);
 }
 
 extern "C" size_t rr_linear_loss_workspace_bytes(int64_t rows, int64_t D, int64_t V, int dtype, int pass) {
@@ -876,7 +1002,7 @@ extern "C" int rr_linear_ce_fwd(const void* hidden, const void* weight, int dtyp
   if (labels == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
   if (int rc = check_buffers(who, rows, D, V, 1, dtype, 0, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
   State st;
-  state_layout(rows, 1, static_cast<char*>(state), &st);
+  state_layout(rows, D, 1, dtype, static_cast<char*>(state), &st);
   State in = st;
   if (reduction == 0) in.loss = loss;   // where rows that do not count leave their 0
   rows_kernel<true><<<1, 1024, 0, s>>>(labels, ignore_index, rows, (int)V, in);
@@ -906,7 +1032,7 @@ extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtyp
   if (teacher_logits == nullptr || teacher_ids == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
   if (int rc = check_buffers(who, rows, D, V, K, dtype, 0, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
   State st;
-  state_layout(rows, K, static_cast<char*>(state), &st);
+  state_layout(rows, D, K, dtype, static_cast<char*>(state), &st);
   int KP = 1;
   while (KP < K) KP *= 2;
   RR_DISPATCH_DTYPE(teacher_dtype, {
@@ -920,8 +1046,8 @@ extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtyp
                      workspace_bytes, s);
 }
 
-extern "C" int rr_linear_loss_bwd(const float* dloss, const void* hidden, const void* weight, int dtype, int64_t rows,
-                                  int64_t D, int64_t V, int64_t K, float z_loss, float temperature, int reduction,
+extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D,
+                                  int64_t V, int64_t K, float z_loss, float temperature, int reduction,
                                   const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
                                   size_t workspace_bytes, void* stream) {
   const char* who = "rr_linear_loss_bwd";
@@ -936,15 +1062,15 @@ extern "C" int rr_linear_loss_bwd(const float* dloss, const void* hidden, const 
     return rr::check_launch(who);
   }
   if (dloss == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
-  if (int rc = check_buffers(who, rows, D, V, K, dtype, 1, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
+  if (int rc = check_buffers(who, rows, D, V, K, dtype, 1, nullptr, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
   if (dhidden == nullptr && dweight == nullptr) return RR_OK;
   const Plan p = plan_of(rows, D, V, dtype);
   State st;
-  state_layout(rows, K, static_cast<char*>(const_cast<void*>(state)), &st);
+  state_layout(rows, D, K, dtype, static_cast<char*>(const_cast<void*>(state)), &st);
   BwdWs ws;
   bwd_layout(p, static_cast<char*>(workspace), &ws);
 #define LL_BACKWARD(X, OP, PX, PZ) \
-  backward<X, OP, PX, PZ>(p, dloss, hidden, weight, st, ws, (int)K, z_loss, temperature, reduction, dhidden, dweight, s)
+  backward<X, OP, PX, PZ>(p, dloss, weight, st, ws, (int)K, z_loss, temperature, reduction, dhidden, dweight, s)
   if (dtype == RR_BF16) return p.planes_z == 2 ? LL_BACKWARD(bf16, OpBf16, 1, 2) : LL_BACKWARD(bf16, OpBf16, 1, 1);
   if (dtype == RR_F16) return p.planes_z == 2 ? LL_BACKWARD(f16, OpF16, 1, 2) : LL_BACKWARD(f16, OpF16, 1, 1);
   return LL_BACKWARD(float, OpF16, 2, 2);

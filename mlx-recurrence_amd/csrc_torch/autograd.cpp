@@ -378,7 +378,7 @@ struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
     const int64_t rows = h_.size(0), D = h_.size(1), V = w_.size(0), K = t_ids.has_value() ? t_ids->size(1) : 1;
     const int dtc = dtype_code(dt);
     Tensor loss = reduction == 0 ? at::empty({rows}, h_.options().dtype(at::kFloat)) : at::empty({}, h_.options().dtype(at::kFloat));
-    const size_t sb = rr_linear_loss_state_bytes(rows, K), wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 0);
+    const size_t sb = rr_linear_loss_state_bytes(rows, D, K, dtc), wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 0);
     const Tensor state = workspace(sb, h_.options()), ws = workspace(wsb, h_.options());
     if (t_ids.has_value()) {
       const at::ScalarType tdt = common_dtype({&*t_logits});
@@ -392,7 +392,8 @@ struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
                              loss.data_ptr<float>(), P(state), sb, P(ws), wsb, stream_of(h_)),
             "rr_linear_ce_fwd");
     }
-    ctx->save_for_backward({h_, w_, state});
+    ctx->save_for_backward({w_, state});   // the state holds the rows of hidden that count
+    ctx->saved_data["rows"] = rows;
     ctx->saved_data["K"] = K;
     ctx->saved_data["zl"] = zl;
     ctx->saved_data["tau"] = tau;
@@ -402,18 +403,18 @@ struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &h_ = s[0], &w_ = s[1], &state = s[2];
-    const at::DeviceGuard guard(h_.device());
-    const int64_t rows = h_.size(0), D = h_.size(1), V = w_.size(0), K = ctx->saved_data["K"].toInt();
-    const int dtc = dtype_code(h_.scalar_type());
+    const Tensor &w_ = s[0], &state = s[1];
+    const at::DeviceGuard guard(w_.device());
+    const int64_t rows = ctx->saved_data["rows"].toInt(), D = w_.size(1), V = w_.size(0), K = ctx->saved_data["K"].toInt();
+    const int dtc = dtype_code(w_.scalar_type());
     const Tensor dloss = prep(grads[0], at::kFloat);
-    Tensor dh = ctx->needs_input_grad(0) ? at::empty_like(h_) : Tensor();
+    Tensor dh = ctx->needs_input_grad(0) ? at::empty({rows, D}, w_.options()) : Tensor();
     Tensor dw = ctx->needs_input_grad(1) ? at::empty_like(w_) : Tensor();
     const size_t wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 1);
-    const Tensor ws = workspace(wsb, h_.options());
-    check(rr_linear_loss_bwd(dloss.data_ptr<float>(), P(h_), P(w_), dtc, rows, D, V, K, (float)ctx->saved_data["zl"].toDouble(),
+    const Tensor ws = workspace(wsb, w_.options());
+    check(rr_linear_loss_bwd(dloss.data_ptr<float>(), P(w_), dtc, rows, D, V, K, (float)ctx->saved_data["zl"].toDouble(),
                              (float)ctx->saved_data["tau"].toDouble(), (int)ctx->saved_data["reduction"].toInt(), P(state),
-                             state.defined() ? (size_t)state.numel() : 0, P(dh), P(dw), P(ws), wsb, stream_of(h_)),
+                             state.defined() ? (size_t)state.numel() : 0, P(dh), P(dw), P(ws), wsb, stream_of(w_)),
           "rr_linear_loss_bwd");
     return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }

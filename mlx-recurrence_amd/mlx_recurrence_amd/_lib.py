@@ -84,13 +84,13 @@ _SIGS = {
                           + [_c_ptr] * 3),
     "rr_layer_norm_bwd_workspace_bytes": (_c_size, [_c_i64] * 2),
     "rr_layer_norm_bwd": (_c_int, [_c_ptr, _c_int] * 3 + [_c_ptr] * 2 + [_c_i64] * 2 + [_c_ptr] * 4 + [_c_size, _c_ptr]),
-    "rr_linear_loss_state_bytes": (_c_size, [_c_i64] * 2),
+    "rr_linear_loss_state_bytes": (_c_size, [_c_i64] * 3 + [_c_int]),
     "rr_linear_loss_workspace_bytes": (_c_size, [_c_i64] * 3 + [_c_int] * 2),
     "rr_linear_ce_fwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 3 + [_c_ptr, _c_i64, _c_f32, _c_int]
                          + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
     "rr_linear_kd_fwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 3 + [_c_ptr, _c_int, _c_ptr, _c_i64, _c_f32, _c_int]
                          + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
-    "rr_linear_loss_bwd": (_c_int, [_c_ptr] * 3 + [_c_int] + [_c_i64] * 4 + [_c_f32] * 2 + [_c_int, _c_ptr, _c_size]
+    "rr_linear_loss_bwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 4 + [_c_f32] * 2 + [_c_int, _c_ptr, _c_size]
                            + [_c_ptr] * 3 + [_c_size, _c_ptr]),
 }
 
@@ -532,7 +532,7 @@ def layer_norm_bwd(dy, x, w, w_dtype, mean, rstd, rows, D, dx, dw, db):
 
 def linear_loss_buffers(rows, D, V, K, dtype, device):
     """State (kept for the backward) and workspace of a forward."""
-    state = _alloc_ws(_ws_bytes("rr_linear_loss_state_bytes", (rows, K)), device)
+    state = _alloc_ws(_ws_bytes("rr_linear_loss_state_bytes", (rows, D, K, DTYPE_CODE[dtype])), device)
     return state, _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[dtype], 0)), device)
 
 
@@ -551,10 +551,10 @@ def linear_kd_fwd(hidden, weight, teacher_logits, teacher_ids, temperature, redu
                                    0 if ws is None else ws.numel(), stream_of(hidden)), "rr_linear_kd_fwd")
 
 
-def linear_loss_bwd(dloss, hidden, weight, K, z_loss, temperature, reduction, state, dhidden, dweight):
-    (rows, D), V = hidden.shape, weight.shape[0]
-    ws = _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[hidden.dtype], 1)), hidden.device)
-    _check(load().rr_linear_loss_bwd(ptr(dloss), ptr(hidden), ptr(weight), DTYPE_CODE[hidden.dtype], rows, D, V, K, z_loss,
-                                     temperature, reduction, ptr(state), 0 if state is None else state.numel(),
-                                     ptr(dhidden), ptr(dweight), ptr(ws), 0 if ws is None else ws.numel(),
-                                     stream_of(hidden)), "rr_linear_loss_bwd")
+def linear_loss_bwd(dloss, weight, rows, K, z_loss, temperature, reduction, state, dhidden, dweight):
+    V, D = weight.shape
+    ws = _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[weight.dtype], 1)), weight.device)
+    _check(load().rr_linear_loss_bwd(ptr(dloss), ptr(weight), DTYPE_CODE[weight.dtype], rows, D, V, K, z_loss, temperature,
+                                     reduction, ptr(state), 0 if state is None else state.numel(), ptr(dhidden),
+                                     ptr(dweight), ptr(ws), 0 if ws is None else ws.numel(), stream_of(weight)),
+           "rr_linear_loss_bwd")

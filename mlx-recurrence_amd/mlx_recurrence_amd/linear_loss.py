@@ -43,17 +43,17 @@ class _LinearLoss(torch.autograd.Function):
                 tdt = _lib.common_dtype(t_logits)
                 _lib.linear_kd_fwd(h_, w_, _lib.prep(t_logits, tdt), _lib.prep(t_ids, torch.int64), temperature, reduction,
                                    loss, state, ws)
-        ctx.save_for_backward(h_, w_, state)
-        ctx.args = (K, z_loss, temperature, reduction)
+        ctx.save_for_backward(w_, state)   # the state holds the rows of hidden that count
+        ctx.args = (rows, K, z_loss, temperature, reduction)
         return loss
 
     @staticmethod
     def backward(ctx, dloss):
-        h_, w_, state = ctx.saved_tensors
-        dh = torch.empty_like(h_) if ctx.needs_input_grad[0] else None
+        w_, state = ctx.saved_tensors
+        dh = w_.new_empty((ctx.args[0], w_.shape[1])) if ctx.needs_input_grad[0] else None
         dw = torch.empty_like(w_) if ctx.needs_input_grad[1] else None
-        with _lib.device_guard(h_.device):
-            _lib.linear_loss_bwd(_lib.prep(dloss, torch.float32), h_, w_, *ctx.args, state, dh, dw)
+        with _lib.device_guard(w_.device):
+            _lib.linear_loss_bwd(_lib.prep(dloss, torch.float32), w_, *ctx.args, state, dh, dw)
         return (dh, dw) + (None,) * 7
 
 

@@ -168,7 +168,7 @@ def test_c_abi_refusals():
     for bad in (dict(rows=-1), dict(D=0), dict(V=0), dict(dt=9), dict(red=3), dict(h=None), dict(w=None), dict(l=None),
                 dict(loss=None), dict(st=None), dict(ws=None), dict(h=odd), dict(w=odd)):
         assert ce(**bad) == _lib.RR_EINVAL, bad
-    for bad in (dict(sn=lib.rr_linear_loss_state_bytes(4, 1) - 1), dict(st=odd), dict(ws=odd),
+    for bad in (dict(sn=lib.rr_linear_loss_state_bytes(4, 8, 1, 1) - 1), dict(st=odd), dict(ws=odd),
                 dict(wn=lib.rr_linear_loss_workspace_bytes(4, 8, 10, 1, 0) - 1)):
         assert ce(**bad) == _lib.RR_EWORKSPACE, bad
     for bad in (dict(V=(1 << 24) + 1), dict(D=65537), dict(rows=1 << 24)):
@@ -179,9 +179,9 @@ def test_c_abi_refusals():
         assert kd(**bad) == _lib.RR_EINVAL, bad
     for bad in (dict(K=0), dict(K=1025)):
         assert kd(**bad) == _lib.RR_EUNSUPPORTED, bad
-    bw = lambda **k: lib.rr_linear_loss_bwd(*{**dict(dl=p, h=p, w=p, dt=1, rows=4, D=8, V=10, K=3, z=0.0, tau=1.0, red=1,  # noqa: E731,E501
+    bw = lambda **k: lib.rr_linear_loss_bwd(*{**dict(dl=p, w=p, dt=1, rows=4, D=8, V=10, K=3, z=0.0, tau=1.0, red=1,  # noqa: E731,E501
                                                      st=p, sn=big, dh=p, dw=p, ws=p, wn=big, s=None), **k}.values())
-    for bad in (dict(dl=None), dict(h=None), dict(st=None), dict(tau=-1.0), dict(red=-1)):
+    for bad in (dict(dl=None), dict(w=None), dict(st=None), dict(tau=-1.0), dict(red=-1)):
         assert bw(**bad) == _lib.RR_EINVAL, bad
     assert bw(wn=lib.rr_linear_loss_workspace_bytes(4, 8, 10, 1, 1) - 1) == _lib.RR_EWORKSPACE
     assert bw(dh=None, dw=None) == _lib.RR_OK
