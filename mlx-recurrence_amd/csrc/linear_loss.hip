@@ -415,21 +415,22 @@ __device__ __forceinline__ float rounded(float x) {
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Walks the entries of row `orig` whose column lies in this wave's v0 .. v0 + 16 MI
+// First of a row's K entries at column v0 or behind.
+__device__ __forceinline__ int first_entry(const int* ids, int K, int v0) {
+  int lo = 0, hi = K;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ids[mid] < v0) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+// Walks a row's entries from the lo-th on that lie in this wave's columns v0 .. v0 + 16 MI
 // and in this lane's quarter of the accumulator rows: f(k, element) with the element's
 // index 4 i + e.
 template <int MI, typename F>
-__device__ __forceinline__ void each_entry(const int* ids, int K, int v0, int quarter, bool on, F f) {
-  int lo = 0;
-  if (on) {
-    int hi = K;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (ids[mid] < v0) lo = mid + 1;
-      else hi = mid;
-    }
-  }
-  for (int k = lo; on && k < K; ++k) {
+__device__ __forceinline__ void each_entry(const int* ids, int K, int lo, int v0, int quarter, F f) {
+  for (int k = lo; k < K; ++k) {
     const int rel = ids[k] - v0;
     if (rel >= 16 * MI) break;
     if (((rel >> 2) & 3) == quarter) f(k, (rel >> 4) * 4 + (rel & 3));
@@ -479,31 +480,49 @@ logits_kernel(LogitArgs a) {
 
   float c = a.c;
   if constexpr (PX == 2) c /= scale_h(a.st.hdr) * scale_w(a.st.hdr);
-  const int vw = v0 + wm * P::MW;
-  float* red = reinterpret_cast<float*>(lds);   // forward: [WM][BN][2]
+  const int vw = v0 + wm * P::MW, left = a.V - vw;   // the wave's words, and how many there are
+  float* red = reinterpret_cast<float*>(lds);        // forward: [WM][BN][2]
+  // What the rows need, the loads of all blocks at once.
+  int64_t orig[P::NI];   // first of the row's entries
+  int lo[P::NI];
+  float2 co[P::NI];
+  float l2[P::NI];
+#pragma unroll
+  for (int j = 0; j < P::NI; ++j) {
+    const int t = min(t0 + wn * P::NW + 16 * j + (lane & 15), n - 1);
+    orig[j] = (int64_t)a.st.rows[t] * a.K;
+    if constexpr (GRAD) co[j] = a.coef[t], l2[j] = a.st.lse2[t];
+  }
+#pragma unroll
+  for (int j = 0; j < P::NI; ++j)
+    lo[j] = t0 + wn * P::NW + 16 * j + (lane & 15) < n ? first_entry(a.st.ids + orig[j], a.K, vw) : a.K;
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
     const int tl = wn * P::NW + 16 * j + (lane & 15);
-    const int t = t0 + tl;
-    const bool on = t < n;
-    const int64_t orig = on ? a.st.rows[t] : 0;
-    const int* ids = a.st.ids + orig * a.K;
+    const bool on = t0 + tl < n;
+    const int* ids = a.st.ids + orig[j];
+#pragma unroll
+    for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = rounded(acc[i][j][e] * c);
+    if (left < P::MW) {   // the vocabulary's last words
+#pragma unroll
+      for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = 16 * i + 4 * quarter + e < left ? acc[i][j][e] : -INFINITY;
+    }
     if constexpr (!GRAD) {
-      float m = -INFINITY;
+      float m = -INFINITY, part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = vw + 16 * i + 4 * quarter + e;
-          acc[i][j][e] = v < a.V ? rounded(acc[i][j][e] * c) : -INFINITY;
-          m = fmaxf(m, acc[i][j][e]);
-        }
-      float s = 0.f;
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, acc[i][j][e]);
 #pragma unroll
       for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s += m == -INFINITY ? acc[i][j][e] - m : exp2_fast(acc[i][j][e] - m);
-      if (m == -INFINITY && s != s) {   // no column of the vocabulary, or NaN among the logits
+        for (int e = 0; e < 4; ++e) part[e] += exp2_fast(acc[i][j][e] - m);
+      float s = (part[0] + part[1]) + (part[2] + part[3]);
+      if (m == -INFINITY) {   // no column of the vocabulary, or NaN among the logits
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < P::MI; ++i)
@@ -511,13 +530,13 @@ logits_kernel(LogitArgs a) {
           for (int e = 0; e < 4; ++e) bad |= acc[i][j][e] != acc[i][j][e];
         s = bad ? NAN : 0.f;
       }
-      each_entry<P::MI>(ids, a.K, vw, quarter, on, [&](int k, int el) {
+      each_entry<P::MI>(ids, a.K, lo[j], vw, quarter, [&](int k, int el) {
         float z = 0.f;
 #pragma unroll
         for (int i = 0; i < P::MI; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) z = el == i * 4 + e ? acc[i][j][e] : z;
-        a.st.z2[orig * a.K + k] = z;
+        a.st.z2[orig[j] + k] = z;
       });
       // the other quarters' words of the same row, then the waves along m
 #pragma unroll
@@ -532,32 +551,33 @@ logits_kernel(LogitArgs a) {
         red[(wm * BN + tl) * 2 + 1] = s;
       }
     } else {
-      const float2 co = on ? a.coef[t] : make_float2(0.f, 0.f);
-      const float l2 = on ? a.st.lse2[t] : 0.f;
 #pragma unroll
       for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = vw + 16 * i + 4 * quarter + e;
-          acc[i][j][e] = on && v < a.V ? exp2_fast(rounded(acc[i][j][e] * c) - l2) : 0.f;
-        }
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = exp2_fast(acc[i][j][e] - l2[j]);   // 0 behind the last word
       // q - p first, so that what is left of a sure label keeps its bits
-      each_entry<P::MI>(ids, a.K, vw, quarter, on, [&](int k, int el) {
-        const float p = a.st.p[orig * a.K + k], r = p * co.y;
+      each_entry<P::MI>(ids, a.K, lo[j], vw, quarter, [&](int k, int el) {
+        const float p = a.st.p[orig[j] + k], r = p * co[j].y;
 #pragma unroll
         for (int i = 0; i < P::MI; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = el == i * 4 + e ? acc[i][j][e] - p + r : acc[i][j][e];
       });
+#pragma unroll
+      for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = on ? co[j].x * acc[i][j][e] : 0.f;
+      if (left < P::MW) {   // not 0 x NaN
+#pragma unroll
+        for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = 16 * i + 4 * quarter + e < left ? acc[i][j][e] : 0.f;
+      }
       typedef uint16_t u16x4_e __attribute__((ext_vector_type(4)));
       typedef uint16_t u16x8_e __attribute__((ext_vector_type(8)));
       uint16_t* stage = lds + wave * 16 * (P::MW + 8);
       uint16_t* o = a.dz + (int64_t)(t0 + wn * P::NW + 16 * j) * a.ldz + (vw - a.v_first);
       auto store = [&](int r, int v, u16x8_e x) { *reinterpret_cast<u16x8_e*>(o + (int64_t)r * a.ldz + v) = x; };
-#pragma unroll
-      for (int i = 0; i < P::MI; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = on ? co.x * acc[i][j][e] : 0.f;
       store_block<P::MI>(stage, lane, [&](int i) {
         return u16x4_e{op_bits<Op>(acc[i][j][0]), op_bits<Op>(acc[i][j][1]), op_bits<Op>(acc[i][j][2]), op_bits<Op>(acc[i][j][3])};
       }, store);

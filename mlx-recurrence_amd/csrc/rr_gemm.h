@@ -245,11 +245,15 @@ struct Product {
     u16x8_t fa[MI], fb[2][NI];
     auto read_a = [&](int i, const uint16_t* buf, int ks) { fa[i] = TA::frag16(buf, wm * MW + 16 * i, ks, lane); };
     auto read_b = [&](int j, const uint16_t* buf, int ks) { fb[ks][j] = TB::frag16(buf + TA::ELEMS, wn * NW + 16 * j, ks, lane); };
-    // Row i of the products of k group ks.
-    auto row = [&](int i, int ks) {
+    // Row i of the products of k group ks; behind each product act(j).
+    auto row = [&](int i, int ks, auto act) {
 #pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = mma<Op>(fa[i], fb[ks][j], acc[i][j]);
-      keep_order();
+      for (int j = 0; j < NI; ++j) {
+        acc[i][j] = mma<Op>(fa[i], fb[ks][j], acc[i][j]);
+        keep_order();
+        act(j);
+        keep_order();
+      }
     };
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -270,30 +274,42 @@ struct Product {
       const uint16_t* other = lds + ((s + 1) & 1) * STEP;
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        row(i, 0);
-        if (i == 0) read_a(MI - 1, buf, 0);
-        else read_a(i - 1, buf, 1);
+        row(i, 0, [&](int j) {
+          if (j == 0) {
+            if (i == 0) read_a(MI - 1, buf, 0);
+            else read_a(i - 1, buf, 1);
+          }
+          if (j == 1) {
 #pragma unroll
-        for (int j = i * NI / MI; j < (i + 1) * NI / MI; ++j) read_b(j, buf, 1);
-        keep_order();
+            for (int f = i * NI / MI; f < (i + 1) * NI / MI; ++f) read_b(f, buf, 1);
+          }
+        });
       }
       next_step();
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        row(i, 1);
-        if (i == 0) {
-          read_a(MI - 1, buf, 1);
-          keep_order();
-          continue;
-        }
-        if (i == 1) loads_barrier();   // the buffer is read, the other full
-        read_a(i - 1, other, 0);
-        constexpr int R = MI - 1;      // behind the last step the fragments are of no step and not used
+        row(i, 1, [&](int j) {
+          constexpr int R = MI - 1;
+          if (i == 0) {
+            if (j == 0) read_a(MI - 1, buf, 1);
+            return;
+          }
+          if (j == 0) {
+            if (i == 1) loads_barrier();   // the buffer is read, the other full
+            read_a(i - 1, other, 0);
+          }
+          if (j == 1) {
 #pragma unroll
-        for (int j = (i - 1) * NI / R; j < i * NI / R; ++j) read_b(j, other, 0);
+            for (int f = (i - 1) * NI / R; f < i * NI / R; ++f) read_b(f, other, 0);
+          }
+          constexpr int Q = NI < 4 ? 1 : 3;   // products that the loads lie behind
+          if (j >= NI - Q) {
+            const int q = j - (NI - Q), l0 = (i - 1) * Steps::N / R, l1 = i * Steps::N / R;
 #pragma unroll
-        for (int l = (i - 1) * Steps::N / R; l < i * Steps::N / R; ++l) st.load(l, wave);
-        keep_order();
+            for (int l = 0; l < Steps::N; ++l)
+              if (l >= l0 + q * (l1 - l0) / Q && l < l0 + (q + 1) * (l1 - l0) / Q) st.load(l, wave);
+          }
+        });
       }
     }
     loads_barrier();   // the LDS is free
