@@ -55,13 +55,13 @@ constexpr int64_t kFewRows = 64;           // rows whose dz keeps a second plane
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Tiles: BM (words, or channels) x BN (rows, or words), WM x WN waves.  Tile256 moves the
-// fewest bytes a flop; two Tile128 share a CU, for products whose Tile256 would leave CUs
-// without work; Tile32 is for a few rows, whose products are bound by the weight's bytes.
+// fewest bytes a flop; tiles of 128 x 128 and 256 x 128 were no faster anywhere, not even
+// where 256 x 256 leaves CUs without work (1536 x 32000 x 768 forward and backward:
+// 294 us, 301 to 307 with them).  Tile32 is for a few rows, whose products are bound by the
+// weight's bytes (two workgroups a CU): 16 x 65536 x 5120 forward 137 us, 156 with Tile256.
 struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, THREADS = 512; };
-struct Tile128 { static constexpr int BM = 128, BN = 128, WM = 2, WN = 2, THREADS = 256; };
 struct Tile32 { static constexpr int BM = 256, BN = 32, WM = 4, WN = 1, THREADS = 256; };
-enum Tiles { kTile256, kTile128, kTile32 };
-constexpr int kEdge = 256;       // buffers hold whole tiles of any kind
+constexpr int kEdge = 256;       // BM of both; buffers hold whole tiles
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
@@ -113,26 +113,12 @@ struct Plan {
   bool copy_w;         // the weight is copied (planes, or rows that are not whole 16-byte chunks)
   int64_t Tp, Dp;      // rows to whole tiles, channels to whole k steps
   int64_t Vt, Dt;      // words and channels to whole tiles
-  Tiles logits, dh, dw;
+  bool few;            // Tile32 for the logits and dh
   // backward
   int64_t Vp;          // columns of a piece (whole tiles)
   int64_t splits;      // parts of a piece's columns that dh is added up in
 };
 constexpr int64_t kCus = 256;
-// Time of a product of `tiles` tiles of `steps` k steps each: full rounds of workgroups, in
-// steps of a Tile256.  A Tile128 has a quarter of its products; a pair of them that share a
-// CU takes 0.6 of its time where two quarters would be half.
-double rounds(Tiles t, int64_t tiles, double steps) {
-  const int64_t slots = t == kTile256 ? kCus : 2 * kCus;
-  return (double)((tiles + slots - 1) / slots) * steps * (t == kTile256 ? 1.0 : 0.6);
-}
-int64_t tiles_of(Tiles t, int64_t m, int64_t n) {
-  const int64_t e = t == kTile256 ? 256 : 128;
-  return up(m, e) / e * (up(n, e) / e);
-}
-Tiles choose(int64_t m, int64_t n) {
-  return rounds(kTile128, tiles_of(kTile128, m, n), 1.0) < rounds(kTile256, tiles_of(kTile256, m, n), 1.0) ? kTile128 : kTile256;
-}
 Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   Plan p{};
   p.T = T, p.D = D, p.V = V, p.dtype = dtype;
@@ -141,25 +127,22 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   // second plane, which costs nothing there (the weight's bytes bound the products).
   p.planes_z = p.planes == 2 || T <= kFewRows ? 2 : 1;
   p.copy_w = p.planes == 2 || D % 8 != 0;
-  const bool few = T <= Tile32::BN;
-  p.Tp = few ? Tile32::BN : up(T, kEdge), p.Dp = up(D, BK);
+  p.few = T <= Tile32::BN;
+  p.Tp = p.few ? Tile32::BN : up(T, kEdge), p.Dp = up(D, BK);
   p.Vt = up(V, kEdge), p.Dt = up(D, kEdge);
   const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * 2 * p.planes_z) / kEdge * kEdge));
   const int64_t pieces = (p.Vt + most - 1) / most;
   p.Vp = up((p.Vt + pieces - 1) / pieces, kEdge);
-  p.logits = few ? kTile32 : choose(p.Vp, T);
-  p.dw = choose(D, p.Vp);
-  // dh has few tiles: its sum over the piece's columns is cut in parts, each at the cost of
-  // writing and reading its part of dh (in steps of a Tile256, which take 1.5 us, at 4 TB/s).
-  const int64_t steps = p.Vp / BK * (p.planes + p.planes_z - 1);
-  const double part = (double)(std::min(p.Tp, up(T, 32)) * D * 8) / 4e12 / 1.5e-6;
+  // dh has few tiles: its sum over the piece's columns is cut in parts.  More parts fill the
+  // GPU's rounds better, each at the cost of writing and reading a dh in fp32 (here in k
+  // steps of a tile, 1.4 us, at 4 TB/s).
+  const int64_t tiles = p.Dt / kEdge * (p.few ? 1 : p.Tp / kEdge), slots = p.few ? 2 * kCus : kCus;
+  const double steps = (double)(p.Vp / BK * (p.planes + p.planes_z - 1));
+  const double part = (double)(T * D * 8) / 4e12 / 1.4e-6;
   double best = 0;
-  for (int t = few ? kTile32 : kTile256; t <= (few ? kTile32 : kTile128); ++t) {
-    const int64_t tiles = t == kTile32 ? p.Dt / Tile32::BM : tiles_of((Tiles)t, D, T);
-    for (int64_t n = 1; n <= 64 && n * 4 <= std::max<int64_t>(4, p.Vp / BK); ++n) {
-      const double cost = rounds((Tiles)t, tiles * n, (double)steps / (double)n) + (double)n * part;
-      if (best == 0 || cost < best) best = cost, p.dh = (Tiles)t, p.splits = n;
-    }
+  for (int64_t n = 1; n <= 64 && n * 4 <= std::max<int64_t>(4, p.Vp / BK); ++n) {
+    const double cost = (double)((tiles * n + slots - 1) / slots) * steps / (double)n + (double)n * part;
+    if (best == 0 || cost < best) best = cost, p.splits = n;
   }
   return p;
 }
@@ -177,7 +160,7 @@ size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
   };
   FwdWs t;
   t.w = reinterpret_cast<uint16_t*>(take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * 2 : 0));
-  t.part = reinterpret_cast<float2*>(take((size_t)(p.Vt / 128) * p.Tp * sizeof(float2)));
+  t.part = reinterpret_cast<float2*>(take((size_t)(p.Vt / kEdge) * p.Tp * sizeof(float2)));
   if (s != nullptr) *s = t;
   return off;
 }
@@ -852,7 +835,7 @@ int check_dims(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int 
     return rr::fail(RR_EUNSUPPORTED, w + ": at most " + std::to_string(kMaxVocab) + " words and " +
                                          std::to_string(kMaxChannels) + " channels");
   }
-  if (T >= ((int64_t)1 << 24) || up(V, 128) / 128 * (up(T, 128) / 128) >= (1 << 23)) {   // grids below 2^32 threads
+  if (T >= ((int64_t)1 << 24) || up(V, 256) / 256 * (up(T, 32) / 32) >= (1 << 23)) {   // grids below 2^32 threads
     return rr::fail(RR_EUNSUPPORTED, w + ": too many rows");
   }
   return RR_OK;
@@ -907,17 +890,10 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
   pack_weight<X>(p, weight, st, ws.w, s);
   LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
   a.part = ws.part;
-  int edge = 256;
-  if (p.logits == kTile256) {
-    launch_logits<Tile256, Op, false, PX, PX>(a, p.T, p.Vt, s);
-  } else if (p.logits == kTile128) {
-    launch_logits<Tile128, Op, false, PX, PX>(a, p.T, p.Vt, s);
-    edge = 128;
-  } else {
-    launch_logits<Tile32, Op, false, PX, PX>(a, p.T, p.Vt, s);
-  }
+  if (p.few) launch_logits<Tile32, Op, false, PX, PX>(a, p.T, p.Vt, s);
+  else launch_logits<Tile256, Op, false, PX, PX>(a, p.T, p.Vt, s);
   float* rows = reduction == 0 ? loss : st.loss;
-  row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, (int)(p.Vt / edge), p.Tp, K, labels, zl, tau, rows);
+  row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, (int)(p.Vt / kEdge), p.Tp, K, labels, zl, tau, rows);
   if (reduction != 0) sum_loss_kernel<<<1, 1024, 0, s>>>(st.loss, p.T, st.hdr, reduction == 1, loss);
   return rr::check_launch("rr_linear_loss");
 }
@@ -932,16 +908,14 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
     const int64_t cols = std::min(p.Vp, p.Vt - v);   // whole tiles
     LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
     a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp, a.plane_z = p.Tp * p.Vp, a.v_first = (int)v;
-    if (p.logits == kTile256) launch_logits<Tile256, Op, true, PX, PZ>(a, p.T, cols, s);
-    else if (p.logits == kTile128) launch_logits<Tile128, Op, true, PX, PZ>(a, p.T, cols, s);
+    if (!p.few) launch_logits<Tile256, Op, true, PX, PZ>(a, p.T, cols, s);
     else if constexpr (PZ == 2) launch_logits<Tile32, Op, true, PX, PZ>(a, p.T, cols, s);
     if (dh != nullptr) {
       DhArgs b{};
       b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = p.Vp, b.plane_w = a.plane_w, b.plane_z = a.plane_z;
       b.V = (int)(p.V - v), b.D = a.D, b.Dp = a.Dp, b.Tp = a.Tp, b.splits = (int)p.splits, b.cols = (int)cols;
       b.out = ws.dh, b.Dt = (int)p.Dt, b.first = v == 0, b.st = st;
-      if (p.dh == kTile256) launch_dh<Tile256, Op, PX, PZ>(b, p, s);
-      else if (p.dh == kTile128) launch_dh<Tile128, Op, PX, PZ>(b, p, s);
+      if (!p.few) launch_dh<Tile256, Op, PX, PZ>(b, p, s);
       else if constexpr (PZ == 2) launch_dh<Tile32, Op, PX, PZ>(b, p, s);
     }
     if (dw != nullptr) {
@@ -949,8 +923,7 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
       c.h = st.h, c.dz = ws.dz, c.ldh = p.Dp, c.ldz = p.Vp, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
       c.V = (int)(p.V - v), c.D = a.D, c.Dp = a.Dp, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
-      if (p.dw == kTile256) launch_dw<Tile256, Op, X, PX, PZ>(c, p, cols, s);
-      else launch_dw<Tile128, Op, X, PX, PZ>(c, p, cols, s);
+      launch_dw<Tile256, Op, X, PX, PZ>(c, p, cols, s);
     }
   }
   if (dh != nullptr) {
