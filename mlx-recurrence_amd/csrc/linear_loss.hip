@@ -24,7 +24,9 @@
 // fp32 inputs are split into two fp16 planes, x s = hi + lo (s a power of two that
 // brings the largest finite value of the tensor just below 2^15; the pair holds 22
 // bits), and a product is the three of the planes that are not below the last bit:
-// about fp32's own accuracy at a third of the fp16 rate, above the fp32 MFMA's.
+// about fp32's own accuracy at a third of the fp16 rate, above the fp32 MFMA's.  Making
+// the planes reads the weight twice and writes it once, which only many rows make up for:
+// up to kExactRows rows run on the fp32 MFMA, straight from the weight.
 // fp16 dz, and the planes of fp32's, carry a power of two that brings the largest
 // |dz| just below 2^14, so that small probabilities keep their bits; bf16 needs
 // none.
@@ -52,16 +54,21 @@ constexpr int64_t kPieceBytes = (int64_t)512 << 20;   // of dz, where the rows l
 constexpr int64_t kMinPiece = 2048;
 constexpr int64_t kMaxPiece = 1 << 20;       // a row of a tile's operand is at most so long
 constexpr int64_t kFewRows = 64;           // rows whose dz keeps a second plane
+constexpr int64_t kExactRows = 256;        // rows of fp32 that run on the fp32 MFMA
+constexpr int kPad = 64;                   // channels are padded to so many
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Tiles: BM (words, or channels) x BN (rows, or words), WM x WN waves.  Tile256 moves the
 // fewest bytes a flop; tiles of 128 x 128 and 256 x 128 were no faster anywhere, not even
 // where 256 x 256 leaves CUs without work (1536 x 32000 x 768 forward and backward:
-// 294 us, 301 to 307 with them).  Tile32 is for a few rows, whose products are bound by the
-// weight's bytes (two workgroups a CU): 16 x 65536 x 5120 forward 137 us, 156 with Tile256.
+// 294 us, 301 to 307 with them).  Tile64 and Tile32 are for a few rows, whose products are
+// bound by the weight's bytes (two workgroups a CU): 16 x 65536 x 5120 forward 137 us, 156
+// with Tile256.
 struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, THREADS = 512; };
+struct Tile64 { static constexpr int BM = 256, BN = 64, WM = 4, WN = 1, THREADS = 256; };
 struct Tile32 { static constexpr int BM = 256, BN = 32, WM = 4, WN = 1, THREADS = 256; };
-constexpr int kEdge = 256;       // BM of both; buffers hold whole tiles
+enum Tiles { kTile256, kTile64, kTile32 };
+constexpr int kEdge = 256;       // BM of all; buffers hold whole tiles
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
@@ -81,7 +88,7 @@ struct State {
   int* ids;      // [rows][K] the entries' columns, ascending; kAbsent past the last
   float* p;      // [rows][K] their weights
   float* z2;     // [rows][K] their logits, times log2(e) / tau
-  uint16_t* h;   // [planes][rows][Dp] the hidden states that count, as an operand
+  char* h;       // [planes][rows][Dp] the hidden states that count, as an operand
 };
 size_t state_layout(int64_t T, int64_t D, int64_t K, int dtype, char* base, State* s) {
   size_t off = 0;
@@ -99,7 +106,7 @@ size_t state_layout(int64_t T, int64_t D, int64_t K, int dtype, char* base, Stat
   t.ids = reinterpret_cast<int*>(take((size_t)T * K * 4));
   t.p = reinterpret_cast<float*>(take((size_t)T * K * 4));
   t.z2 = reinterpret_cast<float*>(take((size_t)T * K * 4));
-  t.h = reinterpret_cast<uint16_t*>(take((size_t)T * up(D, BK) * (dtype == RR_F32 ? 4 : 2)));
+  t.h = take((size_t)T * up(D, kPad) * (dtype == RR_F32 ? 4 : 2));
   if (s != nullptr) *s = t;
   return off;
 }
@@ -108,12 +115,14 @@ size_t state_layout(int64_t T, int64_t D, int64_t K, int dtype, char* base, Stat
 struct Plan {
   int64_t T, D, V;
   int dtype;
-  int planes;          // of the inputs: 2 for fp32
+  bool exact;          // fp32 on the fp32 MFMA
+  int eb;              // bytes of an operand's element
+  int planes;          // of the inputs: 2 for fp32 that is split
   int planes_z;        // of dz
   bool copy_w;         // the weight is copied (planes, or rows that are not whole 16-byte chunks)
   int64_t Tp, Dp;      // rows to whole tiles, channels to whole k steps
   int64_t Vt, Dt;      // words and channels to whole tiles
-  bool few;            // Tile32 for the logits and dh
+  Tiles rows, dw;      // tiles of the logits and dh, and of dw
   // backward
   int64_t Vp;          // columns of a piece (whole tiles)
   int64_t splits;      // parts of a piece's columns that dh is added up in
@@ -122,25 +131,29 @@ constexpr int64_t kCus = 256;
 Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   Plan p{};
   p.T = T, p.D = D, p.V = V, p.dtype = dtype;
-  p.planes = dtype == RR_F32 ? 2 : 1;
+  p.exact = dtype == RR_F32 && T <= kExactRows;
+  p.eb = p.exact ? 4 : 2;
+  p.planes = dtype == RR_F32 && !p.exact ? 2 : 1;
   // The rounding of dz to 16 bits averages out over the rows of dw; few rows get a
   // second plane, which costs nothing there (the weight's bytes bound the products).
-  p.planes_z = p.planes == 2 || T <= kFewRows ? 2 : 1;
-  p.copy_w = p.planes == 2 || D % 8 != 0;
-  p.few = T <= Tile32::BN;
-  p.Tp = p.few ? Tile32::BN : up(T, kEdge), p.Dp = up(D, BK);
+  p.planes_z = !p.exact && (p.planes == 2 || T <= kFewRows) ? 2 : 1;
+  p.copy_w = p.planes == 2 || D * p.eb % 16 != 0;
+  p.rows = T <= Tile32::BN ? kTile32 : T <= Tile64::BN || p.exact ? kTile64 : kTile256;
+  p.dw = T <= kExactRows ? kTile64 : kTile256;
+  p.Tp = p.rows == kTile32 ? Tile32::BN : up(T, kEdge), p.Dp = up(D, kPad);
   p.Vt = up(V, kEdge), p.Dt = up(D, kEdge);
-  const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * 2 * p.planes_z) / kEdge * kEdge));
+  const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * p.eb * p.planes_z) / kEdge * kEdge));
   const int64_t pieces = (p.Vt + most - 1) / most;
   p.Vp = up((p.Vt + pieces - 1) / pieces, kEdge);
   // dh has few tiles: its sum over the piece's columns is cut in parts.  More parts fill the
   // GPU's rounds better, each at the cost of writing and reading a dh in fp32 (here in k
   // steps of a tile, 1.4 us, at 4 TB/s).
-  const int64_t tiles = p.Dt / kEdge * (p.few ? 1 : p.Tp / kEdge), slots = p.few ? 2 * kCus : kCus;
-  const double steps = (double)(p.Vp / BK * (p.planes + p.planes_z - 1));
+  const int64_t tiles = p.Dt / kEdge * (p.rows == kTile256 ? p.Tp / 256 : p.rows == kTile64 ? up(T, 64) / 64 : 1);
+  const int64_t slots = p.rows == kTile256 ? kCus : 2 * kCus, all = p.Vp * p.eb / 128;
+  const double steps = (double)(all * (p.planes + p.planes_z - 1));
   const double part = (double)(T * D * 8) / 4e12 / 1.4e-6;
   double best = 0;
-  for (int64_t n = 1; n <= 64 && n * 4 <= std::max<int64_t>(4, p.Vp / BK); ++n) {
+  for (int64_t n = 1; n <= 64 && n * 4 <= std::max<int64_t>(4, all); ++n) {
     const double cost = (double)((tiles * n + slots - 1) / slots) * steps / (double)n + (double)n * part;
     if (best == 0 || cost < best) best = cost, p.splits = n;
   }
@@ -148,7 +161,7 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
 }
 
 struct FwdWs {
-  uint16_t* w;     // [planes][V][Dp] where the weight is copied
+  char* w;         // [planes][V][Dp] where the weight is copied
   float2* part;    // [word tiles][Tp] maximum and sum of a tile's row
 };
 size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
@@ -159,16 +172,16 @@ size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
     return at;
   };
   FwdWs t;
-  t.w = reinterpret_cast<uint16_t*>(take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * 2 : 0));
+  t.w = take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * p.eb : 0);
   t.part = reinterpret_cast<float2*>(take((size_t)(p.Vt / kEdge) * p.Tp * sizeof(float2)));
   if (s != nullptr) *s = t;
   return off;
 }
 struct BwdWs {
-  uint16_t* w;     // as forward
+  char* w;         // as forward
   float* scale;    // [0] the factor on both gradients
   float2* coef;    // [Tp] a row's factors (coef_kernel)
-  uint16_t* dz;    // [planes_z][Tp][Vp]
+  char* dz;        // [planes_z][Tp][Vp]
   float* dh;       // [splits][Tp][Dt]
 };
 size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
@@ -179,10 +192,10 @@ size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
     return at;
   };
   BwdWs t;
-  t.w = reinterpret_cast<uint16_t*>(take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * 2 : 0));
+  t.w = take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * p.eb : 0);
   t.scale = reinterpret_cast<float*>(take(256));
   t.coef = reinterpret_cast<float2*>(take((size_t)p.Tp * sizeof(float2)));
-  t.dz = reinterpret_cast<uint16_t*>(take((size_t)p.planes_z * p.Tp * p.Vp * 2));
+  t.dz = take((size_t)p.planes_z * p.Tp * p.Vp * p.eb);
   t.dh = reinterpret_cast<float*>(take((size_t)p.splits * p.Tp * p.Dt * 4));
   if (s != nullptr) *s = t;
   return off;
@@ -344,48 +357,53 @@ amax_kernel(const float* __restrict__ x, int64_t n_rows, int D, const int* rows,
   if ((threadIdx.x & 63) == 0 && m > 0.f) atomicMax(out, __float_as_uint(m));
 }
 
-// Rows as operands: copied (16-bit inputs) or split into two planes (fp32), padded
-// with zeros to Dp channels; through `rows` (the first hdr->n of them) where given.
-template <typename X>
+// Rows as operands: copied, or split into two planes (fp32 to fp16), padded with zeros to
+// Dp channels; through `rows` (the first hdr->n of them) where given.  plane: in bytes.
+template <typename X, typename Op>
 __global__ void __launch_bounds__(256)
 pack_kernel(const X* __restrict__ x, int64_t n_rows, int D, int Dp, const int* rows, const Header* hdr, int which,
-            uint16_t* __restrict__ out, int64_t plane) {
+            char* __restrict__ out, int64_t plane) {
+  constexpr bool SPLIT = sizeof(X) == 4 && __is_same(Op, OpF16);
   const int64_t n = rows != nullptr ? hdr->n : n_rows;
   float sc = 1.f;
-  if constexpr (sizeof(X) == 4) sc = which == 0 ? scale_h(hdr) : scale_w(hdr);
+  if constexpr (SPLIT) sc = which == 0 ? scale_h(hdr) : scale_w(hdr);
   for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const X* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
-    uint16_t* o = out + r * Dp;
+    char* o = out + r * Dp * kBytes<Op>;
     for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
       X v[8];
       load8(xr, c, D, v);
-      rr::u16x8_t hi, lo;
+      if constexpr (SPLIT) {
+        rr::u16x8_t hi, lo;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (sizeof(X) == 4) {
+        for (int e = 0; e < 8; ++e) {
           hi[e] = op_bits<OpF16>(v[e] * sc);
           lo[e] = op_bits<OpF16>(v[e] * sc - op_val<OpF16>(hi[e]));
-        } else {
-          hi[e] = __builtin_bit_cast(uint16_t, v[e]);
         }
+        *reinterpret_cast<rr::u16x8_t*>(o + c * 2) = hi;
+        *reinterpret_cast<rr::u16x8_t*>(o + plane + c * 2) = lo;
+      } else {
+        typedef uint32_t Words __attribute__((ext_vector_type(2 * sizeof(X))));
+        Words w;
+        __builtin_memcpy(&w, v, sizeof(w));
+        *reinterpret_cast<Words*>(o + c * sizeof(X)) = w;
       }
-      *reinterpret_cast<rr::u16x8_t*>(o + c) = hi;
-      if constexpr (sizeof(X) == 4) *reinterpret_cast<rr::u16x8_t*>(o + plane + c) = lo;
     }
   }
 }
 
 // ------------------------------------------------------------------ logits
+// (row lengths and planes of operands in bytes)
 struct LogitArgs {
-  const uint16_t* w;      // [V][ldw]
-  const uint16_t* h;      // [n][Dp]
+  const char* w;          // [V][ldw]
+  const char* h;          // [n][Dp]
   int64_t ldw, ldh, plane_w, plane_h;
   int V, D, Dp, K, Tp, nvt;   // nvt: tiles of this launch
   float c;                // log2(e) / tau
   State st;
   float2* part;           // forward
   const float2* coef;     // backward
-  uint16_t* dz;
+  char* dz;
   int64_t ldz, plane_z;
   int v_first;            // the piece's first column
 };
@@ -446,7 +464,7 @@ __global__ void __launch_bounds__(C::THREADS, 2)
 logits_kernel(LogitArgs a) {
   constexpr int BM = C::BM, BN = C::BN;
   using P = Product<Op, BM, BN, C::WM, C::WN, false, false>;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int n = a.st.hdr->n;
   int vt, tt;
   tile_of(blockIdx.x, a.nvt, gridDim.x / a.nvt, vt, tt);
@@ -458,7 +476,7 @@ logits_kernel(LogitArgs a) {
 
   typename P::Acc acc;
   const Operand A{a.w + (int64_t)v0 * a.ldw, a.ldw, a.plane_w, a.V - v0, (int)a.ldw};
-  const Operand B{a.h + (int64_t)t0 * a.ldh, a.ldh, a.plane_h, n - t0, a.Dp};
+  const Operand B{a.h + (int64_t)t0 * a.ldh, a.ldh, a.plane_h, n - t0, (int)a.ldh};
   P::template run<PX, PX>(acc, A, B, 0, a.Dp, lds);
 
   float c = a.c;
@@ -556,18 +574,20 @@ logits_kernel(LogitArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = 16 * i + 4 * quarter + e < left ? acc[i][j][e] : 0.f;
       }
-      typedef uint16_t u16x4_e __attribute__((ext_vector_type(4)));
-      typedef uint16_t u16x8_e __attribute__((ext_vector_type(8)));
-      uint16_t* stage = lds + wave * 16 * (P::MW + 8);
-      uint16_t* o = a.dz + (int64_t)(t0 + wn * P::NW + 16 * j) * a.ldz + (vw - a.v_first);
-      auto store = [&](int r, int v, u16x8_e x) { *reinterpret_cast<u16x8_e*>(o + (int64_t)r * a.ldz + v) = x; };
+      using Bits = typename std::conditional<P::EB == 4, float, uint16_t>::type;
+      typedef Bits Four __attribute__((ext_vector_type(4)));
+      typedef Bits Vec __attribute__((ext_vector_type(16 / P::EB)));
+      Bits* stage = reinterpret_cast<Bits*>(lds) + wave * 16 * (P::MW + 16 / P::EB);
+      char* o = a.dz + (int64_t)(t0 + wn * P::NW + 16 * j) * a.ldz + (vw - a.v_first) * P::EB;
+      auto store = [&](int r, int v, Vec x) { *reinterpret_cast<Vec*>(o + (int64_t)r * a.ldz + v * P::EB) = x; };
       store_block<P::MI>(stage, lane, [&](int i) {
-        return u16x4_e{op_bits<Op>(acc[i][j][0]), op_bits<Op>(acc[i][j][1]), op_bits<Op>(acc[i][j][2]), op_bits<Op>(acc[i][j][3])};
+        if constexpr (P::EB == 4) return acc[i][j];
+        else return Four{op_bits<Op>(acc[i][j][0]), op_bits<Op>(acc[i][j][1]), op_bits<Op>(acc[i][j][2]), op_bits<Op>(acc[i][j][3])};
       }, store);
       if constexpr (PZ == 2) {
         o += a.plane_z;
         store_block<P::MI>(stage, lane, [&](int i) {
-          u16x4_e lo;
+          Four lo;
 #pragma unroll
           for (int e = 0; e < 4; ++e) lo[e] = op_bits<Op>(acc[i][j][e] - op_val<Op>(op_bits<Op>(acc[i][j][e])));
           return lo;
@@ -691,8 +711,8 @@ coef_kernel(State st, const float* __restrict__ dloss, bool per_row, bool mean, 
 
 // dh^T tiles of one part of the piece: m = channels, n = rows, k = the piece's columns.
 struct DhArgs {
-  const uint16_t* w;     // at the piece's first row
-  const uint16_t* dz;
+  const char* w;         // at the piece's first row
+  const char* dz;
   int64_t ldw, ldz, plane_w, plane_z;
   int V, D, Dp, Tp, ndt, splits, cols;   // V: rows of w from the piece on; cols: the piece's columns to whole k steps
   float* out;            // [splits][Tp][Dt]
@@ -705,18 +725,18 @@ __global__ void __launch_bounds__(C::THREADS, 2)
 dh_kernel(DhArgs a) {
   constexpr int BM = C::BM, BN = C::BN;
   using P = Product<Op, BM, BN, C::WM, C::WN, true, false>;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int n = a.st.hdr->n;
   int dt, tt;
   const int tiles = gridDim.x / a.splits, sp = blockIdx.x / tiles;
   tile_of(blockIdx.x - sp * tiles, a.ndt, tiles / a.ndt, dt, tt);
   const int t0 = tt * BN, d0 = dt * BM;
   if (t0 >= n) return;
-  const int steps = a.cols / BK;
-  const int k0 = (int)((int64_t)steps * sp / a.splits) * BK, k1 = (int)((int64_t)steps * (sp + 1) / a.splits) * BK;
+  const int steps = a.cols / P::BK;
+  const int k0 = (int)((int64_t)steps * sp / a.splits) * P::BK, k1 = (int)((int64_t)steps * (sp + 1) / a.splits) * P::BK;
   typename P::Acc acc;
-  const Operand A{a.w + d0, a.ldw, a.plane_w, a.V, (int)a.ldw - d0};
-  const Operand B{a.dz + (int64_t)t0 * a.ldz, a.ldz, a.plane_z, a.Tp - t0, a.cols};
+  const Operand A{a.w + d0 * P::EB, a.ldw, a.plane_w, a.V, (int)a.ldw - d0 * P::EB};
+  const Operand B{a.dz + (int64_t)t0 * a.ldz, a.ldz, a.plane_z, a.Tp - t0, a.cols * P::EB};
   P::template run<PX, PZ>(acc, A, B, k0, k1, lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN, wn = wave % P::WN;
@@ -768,8 +788,8 @@ dh_out_kernel(State st, const float* __restrict__ part, int D, int64_t ldp, int6
 
 // dw^T tiles of the piece: m = channels, n = the piece's columns, k = rows.
 struct DwArgs {
-  const uint16_t* h;
-  const uint16_t* dz;
+  const char* h;
+  const char* dz;
   int64_t ldh, ldz, plane_h, plane_z;
   int V, D, Dp, ndt;     // V: rows of dw from the piece on
   const float* scale;
@@ -781,15 +801,15 @@ __global__ void __launch_bounds__(C::THREADS, 2)
 dw_kernel(DwArgs a) {
   constexpr int BM = C::BM, BN = C::BN;
   using P = Product<Op, BM, BN, C::WM, C::WN, true, true>;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[P::LDS_ELEMS];
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int n = a.st.hdr->n;
   int dt, vt;
   tile_of(blockIdx.x, a.ndt, gridDim.x / a.ndt, dt, vt);
   const int d0 = dt * BM, v0 = vt * BN;
   typename P::Acc acc;
-  const Operand A{a.h + d0, a.ldh, a.plane_h, n, a.Dp - d0};
-  const Operand B{a.dz + v0, a.ldz, a.plane_z, n, BN};
-  P::template run<PX, PZ>(acc, A, B, 0, (n + BK - 1) / BK * BK, lds);
+  const Operand A{a.h + d0 * P::EB, a.ldh, a.plane_h, n, (int)a.ldh - d0 * P::EB};
+  const Operand B{a.dz + (int64_t)v0 * P::EB, a.ldz, a.plane_z, n, BN * P::EB};
+  P::template run<PX, PZ>(acc, A, B, 0, (n + P::BK - 1) / P::BK * P::BK, lds);
   float f = a.scale[0];
   if constexpr (PX == 2) f /= scale_h(a.st.hdr);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -835,7 +855,7 @@ int check_dims(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int 
     return rr::fail(RR_EUNSUPPORTED, w + ": at most " + std::to_string(kMaxVocab) + " words and " +
                                          std::to_string(kMaxChannels) + " channels");
   }
-  if (T >= ((int64_t)1 << 24) || up(V, 256) / 256 * (up(T, 32) / 32) >= (1 << 23)) {   // grids below 2^32 threads
+  if (T >= ((int64_t)1 << 24) || up(V, 256) / 256 * (up(T, 64) / 64) >= (1 << 23)) {   // grids below 2^32 threads
     return rr::fail(RR_EUNSUPPORTED, w + ": too many rows");
   }
   return RR_OK;
@@ -843,19 +863,19 @@ int check_dims(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // The weight as an operand, where it is not one itself.
-template <typename X>
-void pack_weight(const Plan& p, const void* weight, const State& st, uint16_t* w, hipStream_t s) {
+template <typename X, typename Op>
+void pack_weight(const Plan& p, const void* weight, const State& st, char* w, hipStream_t s) {
   if (!p.copy_w) return;
-  pack_kernel<X><<<(unsigned)std::min<int64_t>(8192, p.V), 256, 0, s>>>(
-      static_cast<const X*>(weight), p.V, (int)p.D, (int)p.Dp, nullptr, st.hdr, 1, w, p.V * p.Dp);
+  pack_kernel<X, Op><<<(unsigned)std::min<int64_t>(8192, p.V), 256, 0, s>>>(
+      static_cast<const X*>(weight), p.V, (int)p.D, (int)p.Dp, nullptr, st.hdr, 1, w, p.V * p.Dp * p.eb);
 }
 
-LogitArgs logit_args(const Plan& p, const State& st, const void* weight, uint16_t* w, int K, float tau) {
+LogitArgs logit_args(const Plan& p, const State& st, const void* weight, char* w, int K, float tau) {
   LogitArgs a{};
-  a.w = p.copy_w ? w : static_cast<const uint16_t*>(weight);
+  a.w = p.copy_w ? w : static_cast<const char*>(weight);
   a.h = st.h;
-  a.ldw = p.copy_w ? p.Dp : p.D, a.ldh = p.Dp;
-  a.plane_w = p.V * p.Dp, a.plane_h = p.T * p.Dp;
+  a.ldw = (p.copy_w ? p.Dp : p.D) * p.eb, a.ldh = p.Dp * p.eb;
+  a.plane_w = p.V * a.ldw, a.plane_h = p.T * a.ldh;
   a.V = (int)p.V, a.D = (int)p.D, a.Dp = (int)p.Dp, a.K = K, a.Tp = (int)p.Tp;
   a.c = kLog2e / tau;
   a.st = st;
@@ -885,13 +905,19 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
     amax_kernel<<<1024, 256, 0, s>>>(static_cast<const float*>(hidden), p.T, (int)p.D, st.rows, st.hdr, &st.hdr->amax_h);
     amax_kernel<<<2048, 256, 0, s>>>(static_cast<const float*>(weight), p.V, (int)p.D, nullptr, st.hdr, &st.hdr->amax_w);
   }
-  pack_kernel<X><<<(unsigned)std::min<int64_t>(8192, p.T), 256, 0, s>>>(
-      static_cast<const X*>(hidden), p.T, (int)p.D, (int)p.Dp, st.rows, st.hdr, 0, st.h, p.T * p.Dp);
-  pack_weight<X>(p, weight, st, ws.w, s);
+  pack_kernel<X, Op><<<(unsigned)std::min<int64_t>(8192, p.T), 256, 0, s>>>(
+      static_cast<const X*>(hidden), p.T, (int)p.D, (int)p.Dp, st.rows, st.hdr, 0, st.h, p.T * p.Dp * p.eb);
+  pack_weight<X, Op>(p, weight, st, ws.w, s);
   LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
   a.part = ws.part;
-  if (p.few) launch_logits<Tile32, Op, false, PX, PX>(a, p.T, p.Vt, s);
-  else launch_logits<Tile256, Op, false, PX, PX>(a, p.T, p.Vt, s);
+  // (few rows are never split in planes, fp32 MFMA products never have many rows)
+  if constexpr (PX == 1) {
+    if (p.rows == kTile32) launch_logits<Tile32, Op, false, PX, PX>(a, p.T, p.Vt, s);
+    else if (p.rows == kTile64) launch_logits<Tile64, Op, false, PX, PX>(a, p.T, p.Vt, s);
+  }
+  if constexpr (!__is_same(Op, OpF32)) {
+    if (p.rows == kTile256) launch_logits<Tile256, Op, false, PX, PX>(a, p.T, p.Vt, s);
+  }
   float* rows = reduction == 0 ? loss : st.loss;
   row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, (int)(p.Vt / kEdge), p.Tp, K, labels, zl, tau, rows);
   if (reduction != 0) sum_loss_kernel<<<1, 1024, 0, s>>>(st.loss, p.T, st.hdr, reduction == 1, loss);
@@ -901,29 +927,43 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
 template <typename X, typename Op, int PX, int PZ>
 int backward(const Plan& p, const float* dloss, const void* weight, const State& st, const BwdWs& ws, int K, float zl,
              float tau, int reduction, void* dh, void* dw, hipStream_t s) {
-  pack_weight<X>(p, weight, st, ws.w, s);
-  coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, reduction == 1, tau, zl, !__is_same(Op, OpBf16), ws.coef,
+  pack_weight<X, Op>(p, weight, st, ws.w, s);
+  coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, reduction == 1, tau, zl, __is_same(Op, OpF16), ws.coef,
                                  ws.scale);
   for (int64_t v = 0; v < p.Vt; v += p.Vp) {
     const int64_t cols = std::min(p.Vp, p.Vt - v);   // whole tiles
     LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
-    a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp, a.plane_z = p.Tp * p.Vp, a.v_first = (int)v;
-    if (!p.few) launch_logits<Tile256, Op, true, PX, PZ>(a, p.T, cols, s);
-    else if constexpr (PZ == 2) launch_logits<Tile32, Op, true, PX, PZ>(a, p.T, cols, s);
+    a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp * p.eb, a.plane_z = p.Tp * a.ldz, a.v_first = (int)v;
+    constexpr bool kFew = __is_same(Op, OpF32) || (PX == 1 && PZ == 2);   // up to kFewRows, or kExactRows
+    if constexpr (kFew) {
+      if (p.rows == kTile32) launch_logits<Tile32, Op, true, PX, PZ>(a, p.T, cols, s);
+      else launch_logits<Tile64, Op, true, PX, PZ>(a, p.T, cols, s);
+    } else {
+      launch_logits<Tile256, Op, true, PX, PZ>(a, p.T, cols, s);
+    }
     if (dh != nullptr) {
       DhArgs b{};
-      b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = p.Vp, b.plane_w = a.plane_w, b.plane_z = a.plane_z;
+      b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = a.ldz, b.plane_w = a.plane_w, b.plane_z = a.plane_z;
       b.V = (int)(p.V - v), b.D = a.D, b.Dp = a.Dp, b.Tp = a.Tp, b.splits = (int)p.splits, b.cols = (int)cols;
       b.out = ws.dh, b.Dt = (int)p.Dt, b.first = v == 0, b.st = st;
-      if (!p.few) launch_dh<Tile256, Op, PX, PZ>(b, p, s);
-      else if constexpr (PZ == 2) launch_dh<Tile32, Op, PX, PZ>(b, p, s);
+      if constexpr (kFew) {
+        if (p.rows == kTile32) launch_dh<Tile32, Op, PX, PZ>(b, p, s);
+        else launch_dh<Tile64, Op, PX, PZ>(b, p, s);
+      } else {
+        launch_dh<Tile256, Op, PX, PZ>(b, p, s);
+      }
     }
     if (dw != nullptr) {
       DwArgs c{};
-      c.h = st.h, c.dz = ws.dz, c.ldh = p.Dp, c.ldz = p.Vp, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
+      c.h = st.h, c.dz = ws.dz, c.ldh = a.ldh, c.ldz = a.ldz, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
       c.V = (int)(p.V - v), c.D = a.D, c.Dp = a.Dp, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
-      launch_dw<Tile256, Op, X, PX, PZ>(c, p, cols, s);
+      if constexpr (PX == 1) {
+        if (p.dw == kTile64) launch_dw<Tile64, Op, X, PX, PZ>(c, p, cols, s);
+      }
+      if constexpr (!kFew) {
+        if (p.dw == kTile256) launch_dw<Tile256, Op, X, PX, PZ>(c, p, cols, s);
+      }
     }
   }
   if (dh != nullptr) {
@@ -952,6 +992,7 @@ int run_forward(const char* who, const void* hidden, const void* weight, int dty
   fwd_layout(p, static_cast<char*>(workspace), &ws);
   if (dtype == RR_BF16) return forward<bf16, OpBf16, 1>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
   if (dtype == RR_F16) return forward<f16, OpF16, 1>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
+  if (p.exact) return forward<float, OpF32, 1>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
   return forward<float, OpF16, 2>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
 }
 
@@ -1066,6 +1107,6 @@ extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dt
   backward<X, OP, PX, PZ>(p, dloss, weight, st, ws, (int)K, z_loss, temperature, reduction, dhidden, dweight, s)
   if (dtype == RR_BF16) return p.planes_z == 2 ? LL_BACKWARD(bf16, OpBf16, 1, 2) : LL_BACKWARD(bf16, OpBf16, 1, 1);
   if (dtype == RR_F16) return p.planes_z == 2 ? LL_BACKWARD(f16, OpF16, 1, 2) : LL_BACKWARD(f16, OpF16, 1, 1);
-  return LL_BACKWARD(float, OpF16, 2, 2);
+  return p.exact ? LL_BACKWARD(float, OpF32, 1, 1) : LL_BACKWARD(float, OpF16, 2, 2);
 #undef LL_BACKWARD
 }

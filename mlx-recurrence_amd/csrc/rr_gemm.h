@@ -1,18 +1,21 @@
 // rr_gemm.h — the tiled matrix product of the output-head losses on gfx950.
 //
-// acc[m][n] = sum_k A(m, k) B(n, k) for a BM x BN tile, 16-bit operands, fp32
-// accumulation on the 16x16x32 MFMA.  An operand lies in memory either with k
-// contiguous (its rows are m or n) or k-major (its rows are k); in LDS the tile
-// keeps the orientation it has in memory, and k-major tiles are read with the
-// transposing LDS read, so no operand is ever transposed in memory.
+// acc[m][n] = sum_k A(m, k) B(n, k) for a BM x BN tile, fp32 accumulation: 16-bit operands
+// on the 16x16x32 MFMA, fp32 operands on the fp32 16x16x4 MFMA.  An operand lies in
+// memory either with k contiguous (its rows are m or n) or k-major (its rows are k);
+// in LDS the tile keeps the orientation it has in memory, and k-major tiles are read
+// with the transposing LDS read (fp32: element by element), so no operand is ever
+// transposed in memory.
 //
-// LDS holds 16-byte chunks.  A fragment read takes the same chunk column of many
-// rows, whose addresses differ by a multiple of the row length, so chunk columns
-// are permuted by row (an XOR) to spread them over the banks:
-//   k contiguous  row r, 8 chunks of 8 k:      chunk c at c ^ ((r >> 1) & 7)
-//   k-major       row k, pieces of 16 columns: piece q at q ^ ((k & 3) + 4 ((k >> 3) & 1))
+// LDS holds 16-byte chunks, a step of 128 bytes of k (64 of 16 bits, 32 of fp32).  A
+// fragment read takes the same chunk column of many rows, whose addresses differ by a
+// multiple of the row length, so chunk columns are permuted by row (an XOR) to spread
+// them over the banks:
+//   k contiguous     row r, 8 chunks:              chunk c at c ^ ((r >> 1) & 7)
+//   k-major 16 bits  row k, pieces of 16 columns:  piece q at q ^ ((k & 3) + 4 ((k >> 3) & 1))
+//   k-major fp32     row k, pieces of 16 columns:  piece q at q ^ ((k >> 2) & 3)
 //
-// A step of 64 k is loaded by buffer loads that write LDS themselves (16 bytes a lane,
+// A step is loaded by buffer loads that write LDS themselves (16 bytes a lane,
 // the permutation made by the lanes' addresses), into one of two LDS buffers, while the
 // other is multiplied.  One barrier a step, behind the first two rows of blocks of its
 // second half, says both that the buffer has been read and that the other is full; the
@@ -34,19 +37,25 @@
 namespace rr {
 namespace gemm {
 
-constexpr int BK = 64;
-
 struct OpBf16 {};
 struct OpF16 {};
+struct OpF32 {};
+template <typename Op> constexpr int kBytes = __is_same(Op, OpF32) ? 4 : 2;    // of an element
+template <typename Op> constexpr int kStep = 128 / kBytes<Op>;                 // k of a step
 
 template <typename Op>
 __device__ __forceinline__ f32x4_t mma(const u16x8_t& a, const u16x8_t& b, f32x4_t c) {
   if constexpr (__is_same(Op, OpBf16)) {
     return mfma16(a, b, c);
-  } else {
+  } else if constexpr (__is_same(Op, OpF16)) {
     typedef _Float16 f16x8_t __attribute__((__vector_size__(16)));
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
                                                   0, 0);
+  } else {   // the e-th product takes k = 4 (lane / 16) + e from both sides
+    const f32x4_t x = __builtin_bit_cast(f32x4_t, a), y = __builtin_bit_cast(f32x4_t, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+    return c;
   }
 }
 
@@ -62,13 +71,13 @@ __device__ __forceinline__ float op_val(uint16_t b) {
   else return static_cast<float>(__builtin_bit_cast(_Float16, b));
 }
 
-// One operand of a tile: element (outer o, inner i) at p[o * ld + i]; outside
-// o < outer, i < inner it reads as 0.  k contiguous: o = the tile's row, i = k;
-// k-major: o = k, i = the tile's column.  ld and inner are multiples of 8, p
-// 16-byte aligned.  `plane`: elements from the high to the low plane of an
-// operand that is split in two.  ld <= 2^20, so that a tile spans less than 2^30 bytes.
+// One operand of a tile: element (outer o, inner i) at byte o * ld + i of p; outside
+// o < outer, i < inner it reads as 0.  k contiguous: o = the tile's row, i = k's byte;
+// k-major: o = k, i = the column's byte.  ld and inner are multiples of 16, p 16-byte
+// aligned.  `plane`: bytes from the high to the low plane of an operand that is split in
+// two.  ld <= 2^22, so that a tile spans at most 2^30 bytes.
 struct Operand {
-  const uint16_t* p;
+  const void* p;
   int64_t ld;
   int64_t plane;
   int outer, inner;
@@ -87,80 +96,87 @@ __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0)
 __device__ __forceinline__ void loads_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
-__device__ __forceinline__ uint32_t lds_byte(const uint16_t* p) {
-  return (uint32_t)__builtin_amdgcn_readfirstlane(
-      (int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint16_t*)p);
+__device__ __forceinline__ uint32_t lds_byte(const char* p) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p);
 }
 
-template <int ROWS, bool KMAJOR>
+// ROWS rows (k contiguous) or columns (k-major) of a step of elements of EB bytes.
+template <int ROWS, bool KMAJOR, int EB>
 struct Tile {
-  static constexpr int ELEMS = ROWS * BK;
-  static constexpr int CHUNKS = ELEMS / 8;
-  static constexpr int PER_ROW = KMAJOR ? ROWS / 8 : BK / 8;
-  static constexpr int PIECES = ROWS / 16;   // of a k-major row
+  static constexpr int BYTES = ROWS * 128;
+  static constexpr int CHUNKS = BYTES / 16;
+  static constexpr int PER_ROW = KMAJOR ? ROWS * EB / 16 : 8;
+  static constexpr int PIECE = EB;          // chunks of 16 columns of a k-major row
+  static constexpr int PIECES = ROWS / 16;
   static __device__ __forceinline__ int swz(int row) {
-    if constexpr (KMAJOR) return ((row & 3) | ((row >> 1) & 4)) & (PIECES - 1);
-    else return (row >> 1) & 7;
+    if constexpr (!KMAJOR) return (row >> 1) & 7;
+    else if constexpr (EB == 2) return ((row & 3) | ((row >> 1) & 4)) & (PIECES - 1);
+    else return ((row >> 2) & 3) & (PIECES - 1);
   }
   // Row and chunk column of the chunk that lies at 16-byte position P.
   static __device__ __forceinline__ void at(int P, int& row, int& col) {
     row = P / PER_ROW;
     const int c = P % PER_ROW;
-    if constexpr (KMAJOR) col = ((c >> 1) ^ swz(row)) * 2 + (c & 1);
+    if constexpr (KMAJOR) col = ((c / PIECE) ^ swz(row)) * PIECE + c % PIECE;
     else col = c ^ swz(row);
   }
-  // Fragment of rows (k contiguous) or columns (k-major) r0 .. r0 + 15, k = 32 ks ..:
-  // lane l holds row l % 16, k = 8 (l / 16) + e.
-  static __device__ __forceinline__ u16x8_t frag16(const uint16_t* t, int r0, int ks, int lane) {
+  // Fragment of rows (k contiguous) or columns (k-major) r0 .. r0 + 15, half ks of the step:
+  // lane l holds row l % 16 and the 16 bytes of k from chunk 4 ks + l / 16.
+  static __device__ __forceinline__ u16x8_t frag16(const char* t, int r0, int ks, int lane) {
     const int g = lane >> 4, i = lane & 15;
-    if constexpr (KMAJOR) {
+    if constexpr (!KMAJOR) {
+      const int r = r0 + i, c = 4 * ks + g;
+      return *reinterpret_cast<const u16x8_t*>(t + r * 128 + (c ^ swz(r)) * 16);
+    } else if constexpr (EB == 2) {
       const int k = 32 * ks + 8 * g + (i >> 2);
-      const uint16_t* a = t + k * ROWS + ((r0 >> 4) ^ swz(k)) * 16 + 4 * (i & 3);   // swz(k + 4) = swz(k)
-      const u16x4_t lo = tr_read4(a), hi = tr_read4(a + 4 * ROWS);
+      const uint16_t* a = reinterpret_cast<const uint16_t*>(t) + k * ROWS + ((r0 >> 4) ^ swz(k)) * 16 + 4 * (i & 3);
+      const u16x4_t lo = tr_read4(a), hi = tr_read4(a + 4 * ROWS);   // swz(k + 4) = swz(k)
       return u16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     } else {
-      const int r = r0 + i, c = 4 * ks + g;
-      return frag(t + r * BK + (c ^ swz(r)) * 8);
+      const int k = 16 * ks + 4 * g;
+      const float* a = reinterpret_cast<const float*>(t) + k * ROWS + ((r0 >> 4) ^ swz(k)) * 16 + i;
+      return __builtin_bit_cast(u16x8_t, f32x4_t{a[0], a[ROWS], a[2 * ROWS], a[3 * ROWS]});   // swz(k + 3) = swz(k)
     }
   }
 };
 
 // The loads of one operand's tile by the WAVES waves of a workgroup.
-template <int ROWS, bool KMAJOR, int WAVES>
+template <int ROWS, bool KMAJOR, int EB, int WAVES>
 struct Loader {
-  using T = Tile<ROWS, KMAJOR>;
+  using T = Tile<ROWS, KMAJOR, EB>;
+  static constexpr int STEP = 128 / EB;                // k of a step
   static constexpr int N = T::CHUNKS / (64 * WAVES);   // loads a thread and step
   static_assert(T::CHUNKS % (64 * WAVES) == 0 && WAVES % 2 == 0, "every thread loads the same number of chunks");
   static constexpr int kPast = 0x40000000;   // beyond any buffer here
   int voff[N];
-  int col;          // k contiguous: first k of this thread's chunks
+  int col;          // k contiguous: byte of this thread's chunks in a step
   int ldb, outer, inner;
   const char* at;   // the next step
 
   __device__ __forceinline__ void init(const Operand& o, int wave, int lane) {
-    ldb = (int)o.ld * 2, outer = o.outer, inner = o.inner;
+    ldb = (int)o.ld, outer = o.outer, inner = o.inner;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       int row, c;
       T::at((j * WAVES + wave) * 64 + lane, row, c);
-      voff[j] = KMAJOR && c * 8 >= inner ? kPast : row * ldb + c * 16;
-      col = c * 8;   // k contiguous: the same for every j, WAVES being even
+      voff[j] = KMAJOR && c * 16 >= inner ? kPast : row * ldb + c * 16;
+      col = c * 16;   // k contiguous: the same for every j, WAVES being even
     }
   }
-  __device__ __forceinline__ void seek(const uint16_t* p, int k) {
-    at = reinterpret_cast<const char*>(p) + (KMAJOR ? (int64_t)k * ldb : (int64_t)k * 2);
+  __device__ __forceinline__ void seek(const void* p, int k) {
+    at = static_cast<const char*>(p) + (KMAJOR ? (int64_t)k * ldb : (int64_t)k * EB);
   }
   // The buffer of the step that starts at k, and this thread's offset past its end.
   __device__ __forceinline__ void step(int k, i32x4_t& r, int& past) {
-    const int rows = KMAJOR ? min(outer - k, BK) : min(outer, ROWS);
-    const int bytes = rows <= 0 ? 0 : (rows - 1) * ldb + (KMAJOR ? inner : inner - k) * 2;
+    const int rows = KMAJOR ? min(outer - k, STEP) : min(outer, ROWS);
+    const int bytes = rows <= 0 ? 0 : (rows - 1) * ldb + (KMAJOR ? inner : inner - k * EB);
     const uint64_t b = reinterpret_cast<uint64_t>(at);
     r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
     r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff);
     r[2] = __builtin_amdgcn_readfirstlane(bytes);
     r[3] = 0x00020000;   // raw 32-bit buffer
-    past = !KMAJOR && k + col >= inner ? kPast : 0;   // the rest of a last step's row
-    at += KMAJOR ? (int64_t)BK * ldb : BK * 2;
+    past = !KMAJOR && k * EB + col >= inner ? kPast : 0;   // the rest of a last step's row
+    at += KMAJOR ? (int64_t)STEP * ldb : 128;
   }
   __device__ __forceinline__ void load(int j, i32x4_t r, int past, uint32_t lds, int wave) const {
     load_to_lds(r, voff[j] | past, lds + (uint32_t)(j * WAVES + wave) * 1024);
@@ -191,24 +207,25 @@ struct Product {
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int MW = BM / WM, NW = BN / WN;   // a wave's part
   static constexpr int MI = MW / 16, NI = NW / 16;
-  using TA = Tile<BM, AK_>;
-  using TB = Tile<BN, BK_MAJOR_>;
-  static constexpr int STEP = TA::ELEMS + TB::ELEMS;
-  static constexpr int LDS_ELEMS = 2 * STEP;
+  static constexpr int EB = kBytes<Op>, BK = kStep<Op>;
+  using TA = Tile<BM, AK_, EB>;
+  using TB = Tile<BN, BK_MAJOR_, EB>;
+  static constexpr int STEP = TA::BYTES + TB::BYTES;
+  static constexpr int LDS_BYTES = 2 * STEP;
   static_assert(MI >= 2, "the barrier of a step lies behind the second row of blocks");
   typedef f32x4_t Acc[MI][NI];
 
   // The step whose loads are under way.
   struct Steps {
-    Loader<BM, AK_, WAVES> a;
-    Loader<BN, BK_MAJOR_, WAVES> b;
+    Loader<BM, AK_, EB, WAVES> a;
+    Loader<BN, BK_MAJOR_, EB, WAVES> b;
     i32x4_t ra, rb;
     int pa, pb;
     uint32_t lds;
     static constexpr int N = decltype(a)::N + decltype(b)::N;
     __device__ __forceinline__ void load(int j, int wave) const {
       if (j < decltype(a)::N) a.load(j, ra, pa, lds, wave);
-      else b.load(j - decltype(a)::N, rb, pb, lds + TA::ELEMS * 2, wave);
+      else b.load(j - decltype(a)::N, rb, pb, lds + TA::BYTES, wave);
     }
   };
 
@@ -216,7 +233,7 @@ struct Product {
   // two, the three products that are not below the last bit: hi hi, hi lo, lo hi.
   template <int PA, int PB>
   static __device__ __forceinline__ void run(Acc& acc, const Operand& a, const Operand& b, int k0, int k1,
-                                             uint16_t* lds) {
+                                             char* lds) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 #pragma unroll
@@ -232,19 +249,19 @@ struct Product {
     int seg = 0, k = k1, loaded = 0;   // the step that is loaded next
     auto next_step = [&] {
       if (k == k1) {
-        st.a.seek(a.p + (PA == 2 && seg >= PB ? a.plane : 0), k0);
-        st.b.seek(b.p + (PB == 2 && seg == 1 ? b.plane : 0), k0);
+        st.a.seek(static_cast<const char*>(a.p) + (PA == 2 && seg >= PB ? a.plane : 0), k0);
+        st.b.seek(static_cast<const char*>(b.p) + (PB == 2 && seg == 1 ? b.plane : 0), k0);
         ++seg, k = k0;
       }
-      st.lds = base + (uint32_t)(loaded & 1) * (STEP * 2);
+      st.lds = base + (uint32_t)(loaded & 1) * STEP;
       st.a.step(k, st.ra, st.pa);
       st.b.step(k, st.rb, st.pb);
       if (loaded >= steps) st.ra[2] = st.rb[2] = 0;   // behind the last step: loads of nothing (zeros)
       k += BK, ++loaded;
     };
     u16x8_t fa[MI], fb[2][NI];
-    auto read_a = [&](int i, const uint16_t* buf, int ks) { fa[i] = TA::frag16(buf, wm * MW + 16 * i, ks, lane); };
-    auto read_b = [&](int j, const uint16_t* buf, int ks) { fb[ks][j] = TB::frag16(buf + TA::ELEMS, wn * NW + 16 * j, ks, lane); };
+    auto read_a = [&](int i, const char* buf, int ks) { fa[i] = TA::frag16(buf, wm * MW + 16 * i, ks, lane); };
+    auto read_b = [&](int j, const char* buf, int ks) { fb[ks][j] = TB::frag16(buf + TA::BYTES, wn * NW + 16 * j, ks, lane); };
     // Row i of the products of k group ks; behind each product act(j).
     auto row = [&](int i, int ks, auto act) {
 #pragma unroll
@@ -270,8 +287,8 @@ struct Product {
     // A row's fragment of A is read again, for the next k group, one row behind its last
     // use; the fragments of B have a set for each group.
     for (int s = 0; s < steps; ++s) {
-      const uint16_t* buf = lds + (s & 1) * STEP;
-      const uint16_t* other = lds + ((s + 1) & 1) * STEP;
+      const char* buf = lds + (s & 1) * STEP;
+      const char* other = lds + ((s + 1) & 1) * STEP;
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         row(i, 0, [&](int j) {
