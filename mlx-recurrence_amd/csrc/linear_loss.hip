@@ -122,7 +122,7 @@ struct Plan {
   bool copy_w;         // the weight is copied (planes, or rows that are not whole 16-byte chunks)
   int64_t Tp, Dp;      // rows to whole tiles, channels to whole k steps
   int64_t Vt, Dt;      // words and channels to whole tiles
-  Tiles rows, dw;      // tiles of the logits and dh, and of dw
+  Tiles rows;          // tiles of the logits and dh (dw: Tile256; with Tile64 5 % slower at 16 to 256 rows)
   // backward
   int64_t Vp;          // columns of a piece (whole tiles)
   int64_t splits;      // parts of a piece's columns that dh is added up in
@@ -139,7 +139,6 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   p.planes_z = !p.exact && (p.planes == 2 || T <= kFewRows) ? 2 : 1;
   p.copy_w = p.planes == 2 || D * p.eb % 16 != 0;
   p.rows = T <= Tile32::BN ? kTile32 : T <= Tile64::BN || p.exact ? kTile64 : kTile256;
-  p.dw = T <= kExactRows ? kTile64 : kTile256;
   p.Tp = p.rows == kTile32 ? Tile32::BN : up(T, kEdge), p.Dp = up(D, kPad);
   p.Vt = up(V, kEdge), p.Dt = up(D, kEdge);
   const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * p.eb * p.planes_z) / kEdge * kEdge));
@@ -958,12 +957,7 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
       c.h = st.h, c.dz = ws.dz, c.ldh = a.ldh, c.ldz = a.ldz, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
       c.V = (int)(p.V - v), c.D = a.D, c.Dp = a.Dp, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
-      if constexpr (PX == 1) {
-        if (p.dw == kTile64) launch_dw<Tile64, Op, X, PX, PZ>(c, p, cols, s);
-      }
-      if constexpr (!kFew) {
-        if (p.dw == kTile256) launch_dw<Tile256, Op, X, PX, PZ>(c, p, cols, s);
-      }
+      launch_dw<Tile256, Op, X, PX, PZ>(c, p, cols, s);
     }
   }
   if (dh != nullptr) {

@@ -166,18 +166,19 @@ struct Loader {
   __device__ __forceinline__ void seek(const void* p, int k) {
     at = static_cast<const char*>(p) + (KMAJOR ? (int64_t)k * ldb : (int64_t)k * EB);
   }
-  // The buffer of the step that starts at k, and this thread's offset past its end.
-  __device__ __forceinline__ void step(int k, i32x4_t& r, int& past) {
+  // The buffer of the step that starts at k, `plane` bytes on, and this thread's offset
+  // past its end.
+  __device__ __forceinline__ void step(int k, int64_t plane, i32x4_t& r, int& past) const {
     const int rows = KMAJOR ? min(outer - k, STEP) : min(outer, ROWS);
     const int bytes = rows <= 0 ? 0 : (rows - 1) * ldb + (KMAJOR ? inner : inner - k * EB);
-    const uint64_t b = reinterpret_cast<uint64_t>(at);
+    const uint64_t b = reinterpret_cast<uint64_t>(at + plane);
     r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
     r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff);
     r[2] = __builtin_amdgcn_readfirstlane(bytes);
     r[3] = 0x00020000;   // raw 32-bit buffer
     past = !KMAJOR && k * EB + col >= inner ? kPast : 0;   // the rest of a last step's row
-    at += KMAJOR ? (int64_t)STEP * ldb : 128;
   }
+  __device__ __forceinline__ void advance() { at += KMAJOR ? (int64_t)STEP * ldb : 128; }
   __device__ __forceinline__ void load(int j, i32x4_t r, int past, uint32_t lds, int wave) const {
     load_to_lds(r, voff[j] | past, lds + (uint32_t)(j * WAVES + wave) * 1024);
   }
@@ -240,24 +241,26 @@ struct Product {
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const int per = (k1 - k0) / BK, steps = per * (PA + PB - 1);
+    constexpr int SEGS = PA + PB - 1;   // products of planes, made step by step: what they share is read once
+    const int steps = (k1 - k0) / BK * SEGS;
     if (steps <= 0) return;
     Steps st;
     st.a.init(a, wave, lane);
     st.b.init(b, wave, lane);
+    st.a.seek(a.p, k0);
+    st.b.seek(b.p, k0);
     const uint32_t base = lds_byte(lds);
-    int seg = 0, k = k1, loaded = 0;   // the step that is loaded next
+    int seg = 0, k = k0, loaded = 0;    // the step that is loaded next
     auto next_step = [&] {
-      if (k == k1) {
-        st.a.seek(static_cast<const char*>(a.p) + (PA == 2 && seg >= PB ? a.plane : 0), k0);
-        st.b.seek(static_cast<const char*>(b.p) + (PB == 2 && seg == 1 ? b.plane : 0), k0);
-        ++seg, k = k0;
-      }
       st.lds = base + (uint32_t)(loaded & 1) * STEP;
-      st.a.step(k, st.ra, st.pa);
-      st.b.step(k, st.rb, st.pb);
+      st.a.step(k, PA == 2 && seg >= PB ? a.plane : 0, st.ra, st.pa);
+      st.b.step(k, PB == 2 && seg == 1 ? b.plane : 0, st.rb, st.pb);
       if (loaded >= steps) st.ra[2] = st.rb[2] = 0;   // behind the last step: loads of nothing (zeros)
-      k += BK, ++loaded;
+      ++loaded;
+      if (SEGS > 1 && ++seg < SEGS) return;
+      seg = 0, k += BK;
+      st.a.advance();
+      st.b.advance();
     };
     u16x8_t fa[MI], fb[2][NI];
     auto read_a = [&](int i, const char* buf, int ks) { fa[i] = TA::frag16(buf, wm * MW + 16 * i, ks, lane); };
