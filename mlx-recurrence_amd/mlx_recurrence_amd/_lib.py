@@ -115,7 +115,9 @@ def load() -> ctypes.CDLL:
         raise RuntimeError(f"{LIB_PATH} has ABI version {lib.rr_abi_version()}, this package needs {ABI_VERSION}; "
                            "rebuild it with `python mlx-recurrence_amd/build.py`")
     for name, (res, args) in _SIGS.items():
-        fn = getattr(lib, name)
+        fn = getattr(lib, name, None)
+        if fn is None:   # entry points were added under the same version
+            raise RuntimeError(f"{LIB_PATH} has no {name}; rebuild it with `python mlx-recurrence_amd/build.py`")
         fn.restype = res
         fn.argtypes = args
     _lib = lib
@@ -141,8 +143,8 @@ def autograd_ext():
             from . import _autograd as mod
         except ImportError:
             mod = None
-        if mod is not None and mod.abi_version() != load().rr_abi_version():
-            mod = None   # built against another revision of the library
+        if mod is not None and (mod.abi_version() != load().rr_abi_version() or not hasattr(mod, "linear_loss")):
+            mod = None   # built against another revision of the library, or from an older source
         _autograd_mod = mod
     return _autograd_mod
 

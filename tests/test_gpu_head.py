@@ -466,3 +466,51 @@ def test_python_and_cpp_bindings_agree(monkeypatch):
     monkeypatch.setattr(_lib, "autograd_ext", lambda: None)
     for a, b in zip(cpp, everything()):
         assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_example_learns():
+    """The example's model (norm, scan, norm, both losses together) learns the chain it is trained on."""
+    import importlib.util
+    import pathlib
+    path = pathlib.Path(__file__).resolve().parents[1] / "examples" / "train_head.py"
+    spec = importlib.util.spec_from_file_location("train_head", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    history = example.train(steps=30, vocab=300, width=64, batch=8, length=64, report=lambda line: print(line, flush=True))
+    first, last = history[0], history[-1]
+    assert all(math.isfinite(v) for pair in history for v in pair)
+    assert last[0] < 0.8 * first[0] and last[1] < 0.8 * first[1]
+
+
+def test_graph_replays():
+    """A step of the losses and the norm, captured in a HIP graph: every replay gives the eager bits."""
+    g, h, w, labels = head_inputs(300, 72, 1000, BF16, 31)
+    labels[::6] = -100
+    t, ids = teacher(g, 300, 9, 1000, labels.clamp(min=0))
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    scale = torch.ones(72, dtype=BF16, device="cuda").requires_grad_(True)
+    one = torch.ones((), device="cuda")
+
+    def step():
+        n = mr.layer_norm(h, scale)
+        ce, kd = mr.linear_cross_entropy(n, w, labels), mr.linear_distillation(n, w, t, ids, temperature=2.0)
+        return (ce, kd, *torch.autograd.grad((ce, kd), (h, w, scale), (one, one)))
+
+    eager = [a.detach().clone() for a in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        for a in out:
+            a.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(out, eager):
+            assert torch.equal(a, e)
+        for a, e in zip(step(), eager):
+            assert torch.equal(a, e)
