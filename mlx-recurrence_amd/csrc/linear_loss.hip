@@ -476,26 +476,27 @@ logits_kernel(LogitArgs a) {
   typename P::Acc acc;
   const Operand A{a.w + (int64_t)v0 * a.ldw, a.ldw, a.plane_w, a.V - v0, (int)a.ldw};
   const Operand B{a.h + (int64_t)t0 * a.ldh, a.ldh, a.plane_h, n - t0, (int)a.ldh};
-  P::template run<PX, PX>(acc, A, B, 0, a.Dp, lds);
+  // What the rows need, looked up while the first loads are under way.
+  const int vw = v0 + wm * P::MW, left = a.V - vw;   // the wave's words, and how many there are
+  int orig[P::NI];   // first of the row's entries
+  int lo[P::NI];     // first of them in the wave's words
+  float2 co[P::NI];
+  float l2[P::NI];
+  P::template run<PX, PX>(acc, A, B, 0, a.Dp, lds, [&] {
+#pragma unroll
+    for (int j = 0; j < P::NI; ++j) {
+      const int t = min(t0 + wn * P::NW + 16 * j + (lane & 15), n - 1);
+      orig[j] = a.st.rows[t] * a.K;
+      if constexpr (GRAD) co[j] = a.coef[t], l2[j] = a.st.lse2[t];
+    }
+#pragma unroll
+    for (int j = 0; j < P::NI; ++j)
+      lo[j] = t0 + wn * P::NW + 16 * j + (lane & 15) < n ? first_entry(a.st.ids + orig[j], a.K, vw) : a.K;
+  });
 
   float c = a.c;
   if constexpr (PX == 2) c /= scale_h(a.st.hdr) * scale_w(a.st.hdr);
-  const int vw = v0 + wm * P::MW, left = a.V - vw;   // the wave's words, and how many there are
   float* red = reinterpret_cast<float*>(lds);        // forward: [WM][BN][2]
-  // What the rows need, the loads of all blocks at once.
-  int64_t orig[P::NI];   // first of the row's entries
-  int lo[P::NI];
-  float2 co[P::NI];
-  float l2[P::NI];
-#pragma unroll
-  for (int j = 0; j < P::NI; ++j) {
-    const int t = min(t0 + wn * P::NW + 16 * j + (lane & 15), n - 1);
-    orig[j] = (int64_t)a.st.rows[t] * a.K;
-    if constexpr (GRAD) co[j] = a.coef[t], l2[j] = a.st.lse2[t];
-  }
-#pragma unroll
-  for (int j = 0; j < P::NI; ++j)
-    lo[j] = t0 + wn * P::NW + 16 * j + (lane & 15) < n ? first_entry(a.st.ids + orig[j], a.K, vw) : a.K;
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
     const int tl = wn * P::NW + 16 * j + (lane & 15);

@@ -232,9 +232,10 @@ struct Product {
 
   // k from k0 to k1 (multiples of BK).  PA, PB: the operands' planes; of two times
   // two, the three products that are not below the last bit: hi hi, hi lo, lo hi.
-  template <int PA, int PB>
-  static __device__ __forceinline__ void run(Acc& acc, const Operand& a, const Operand& b, int k0, int k1,
-                                             char* lds) {
+  // meanwhile(): what is done while the first loads are under way.
+  template <int PA, int PB, typename F>
+  static __device__ __forceinline__ void run(Acc& acc, const Operand& a, const Operand& b, int k0, int k1, char* lds,
+                                             F meanwhile) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 #pragma unroll
@@ -243,7 +244,10 @@ struct Product {
       for (int j = 0; j < NI; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     constexpr int SEGS = PA + PB - 1;   // products of planes, made step by step: what they share is read once
     const int steps = (k1 - k0) / BK * SEGS;
-    if (steps <= 0) return;
+    if (steps <= 0) {
+      meanwhile();
+      return;
+    }
     Steps st;
     st.a.init(a, wave, lane);
     st.b.init(b, wave, lane);
@@ -281,6 +285,7 @@ struct Product {
 #pragma unroll
       for (int j = 0; j < Steps::N; ++j) st.load(j, wave);
     }
+    meanwhile();
     loads_barrier();
 #pragma unroll
     for (int i = 0; i < MI; ++i) read_a(i, lds, 0);
@@ -333,6 +338,11 @@ struct Product {
       }
     }
     loads_barrier();   // the LDS is free
+  }
+
+  template <int PA, int PB>
+  static __device__ __forceinline__ void run(Acc& acc, const Operand& a, const Operand& b, int k0, int k1, char* lds) {
+    run<PA, PB>(acc, a, b, k0, k1, lds, [] {});
   }
 };
 
