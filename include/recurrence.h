@@ -390,14 +390,18 @@ int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, c
                       const float* mean, const float* rstd, int64_t rows, int64_t D, void* dx, void* dw, void* db,
                       void* workspace, size_t workspace_bytes, void* stream);
 
-/* Losses on the logits hidden [rows, D] x weight [V, D]^T, which are never stored:
+/* Losses on the logits hidden [rows, D] x weight [V, D]^T, which are not stored where
+ * they are many:
  * `reduction` 0 leaves a loss a row (loss [rows] fp32), 1 their mean over the rows
  * that count, 2 their sum (loss [1]; both 0 where no row counts).  The forward
  * leaves in `state` (16-byte aligned, rr_linear_loss_state_bytes) what
  * rr_linear_loss_bwd reads, the hidden states that count among it (the backward
- * needs `hidden` no more); its contents are the library's own.  K: teacher
- * entries a row, 1 to 1024; 1 for labels.  V <= 2^24, D <= 65536. */
-size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t K, int dtype);
+ * needs `hidden` no more); its contents are the library's own.  The logits are
+ * among it for up to 256 rows, and where they take at most 256 MiB or the weight's
+ * bytes and reading them costs less than their product.  grad = 0: the bytes that
+ * a forward without a backward needs.  K: teacher entries a row, 1 to 1024; 1 for
+ * labels.  V <= 2^24, D <= 65536. */
+size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t V, int64_t K, int dtype, int grad);
 
 /* Workspace of the forward (pass = 0) or backward (pass = 1); 0 for invalid
  * arguments.  The backward's holds a piece of the logits' gradient: about
@@ -429,8 +433,8 @@ int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtype, int64_t 
  * forward's weight and state, K = 1 and temperature = 1 for the cross entropy,
  * z_loss = 0 for the distillation.  dhidden [rows, D] and dweight [V, D] in
  * `dtype`, each null where not wanted; rows that do not count get dhidden 0. */
-int rr_linear_loss_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V, int64_t K, float z_loss, float temperature, int reduction,
-                       const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
+int rr_linear_loss_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                       int64_t K, float z_loss, float temperature, int reduction, const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
                        size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

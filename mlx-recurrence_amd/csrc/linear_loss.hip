@@ -44,6 +44,7 @@ namespace {
 
 using rr::bf16;
 using rr::f16;
+using rr::f32x4_t;
 using namespace rr::gemm;
 
 constexpr int kAbsent = 0x7fffffff;
@@ -55,6 +56,8 @@ constexpr int64_t kMinPiece = 2048;
 constexpr int64_t kMaxPiece = 1 << 20;       // a row of a tile's operand is at most so long
 constexpr int64_t kFewRows = 64;           // rows whose dz keeps a second plane
 constexpr int64_t kExactRows = 256;        // rows of fp32 that run on the fp32 MFMA
+constexpr int64_t kKeepBytes = (int64_t)256 << 20;    // of logits that are kept, or the weight's bytes
+constexpr int64_t kKeepChannels = 1280;    // from so many on (a third for planes) reading a logit costs less than its product
 constexpr int kPad = 64;                   // channels are padded to so many
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -89,8 +92,9 @@ struct State {
   float* p;      // [rows][K] their weights
   float* z2;     // [rows][K] their logits, times log2(e) / tau
   char* h;       // [planes][rows][Dp] the hidden states that count, as an operand
+  float* z;      // [rows][Vt] their logits, times log2(e) / tau, where they are kept
 };
-size_t state_layout(int64_t T, int64_t D, int64_t K, int dtype, char* base, State* s) {
+size_t state_layout(int64_t T, int64_t D, int64_t K, int dtype, int64_t z_words, char* base, State* s) {
   size_t off = 0;
   auto take = [&](size_t bytes) {
     char* at = base + off;
@@ -107,6 +111,8 @@ size_t state_layout(int64_t T, int64_t D, int64_t K, int dtype, char* base, Stat
   t.p = reinterpret_cast<float*>(take((size_t)T * K * 4));
   t.z2 = reinterpret_cast<float*>(take((size_t)T * K * 4));
   t.h = take((size_t)T * up(D, kPad) * (dtype == RR_F32 ? 4 : 2));
+  t.z = reinterpret_cast<float*>(take((size_t)T * z_words * 4));
+  if (z_words == 0) t.z = nullptr;
   if (s != nullptr) *s = t;
   return off;
 }
@@ -123,11 +129,25 @@ struct Plan {
   int64_t Tp, Dp;      // rows to whole tiles, channels to whole k steps
   int64_t Vt, Dt;      // words and channels to whole tiles
   Tiles rows;          // tiles of the logits and dh (dw: Tile256; with Tile64 5 % slower at 16 to 256 rows)
+  int64_t cuts;        // parts of the channels that the logits are added up in
+  bool keep;           // the forward leaves the logits for the backward
   // backward
   int64_t Vp;          // columns of a piece (whole tiles)
   int64_t splits;      // parts of a piece's columns that dh is added up in
 };
 constexpr int64_t kCus = 256;
+// How many parts the k steps of `tiles` tiles are cut in, `slots` workgroups running at one
+// time: more parts fill the GPU's rounds better, each at a cost of `part` (in steps), more
+// than one at a cost of `more`.  At least 4 of the `all` smallest ranges of k in each.
+int64_t best_parts(int64_t tiles, int64_t slots, double steps, double part, double more, int64_t all) {
+  int64_t best_n = 1;
+  double best = 0;
+  for (int64_t n = 1; n <= 64 && n * 4 <= std::max<int64_t>(4, all); ++n) {
+    const double cost = (double)((tiles * n + slots - 1) / slots) * steps / (double)n + (double)n * part + (n > 1 ? more : 0);
+    if (best == 0 || cost < best) best = cost, best_n = n;
+  }
+  return best_n;
+}
 Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   Plan p{};
   p.T = T, p.D = D, p.V = V, p.dtype = dtype;
@@ -141,27 +161,33 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   p.rows = T <= Tile32::BN ? kTile32 : T <= Tile64::BN || p.exact ? kTile64 : kTile256;
   p.Tp = p.rows == kTile32 ? Tile32::BN : up(T, kEdge), p.Dp = up(D, kPad);
   p.Vt = up(V, kEdge), p.Dt = up(D, kEdge);
+  const int64_t slots = p.rows == kTile256 ? kCus : 2 * kCus;   // workgroups at one time
+  const int64_t row_tiles = p.rows == kTile256 ? p.Tp / 256 : p.rows == kTile64 ? up(T, 64) / 64 : 1;
+  // Few tiles of many channels: their sums are cut in parts, each at the cost of writing
+  // and reading the logits in fp32 (in k steps of a tile, 1.4 us, at 4 TB/s), and all at
+  // that of one launch more.
+  {
+    const int64_t all = p.Dp * p.eb / 128;
+    const double steps = (double)all * (p.planes == 2 ? 3 : 1), part = (double)(T * V * 8) / 4e12 / 1.4e-6;
+    p.cuts = best_parts(p.Vt / kEdge * row_tiles, slots, steps, part, 4., all);
+  }
+  const int64_t z_bytes = T * p.Vt * 4;
+  p.keep = T <= kExactRows || p.cuts > 1 ||
+           (z_bytes <= std::max(kKeepBytes, V * D * (dtype == RR_F32 ? 4 : 2)) && D * (p.planes == 2 ? 3 : 1) >= kKeepChannels);
   const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * p.eb * p.planes_z) / kEdge * kEdge));
   const int64_t pieces = (p.Vt + most - 1) / most;
   p.Vp = up((p.Vt + pieces - 1) / pieces, kEdge);
-  // dh has few tiles: its sum over the piece's columns is cut in parts.  More parts fill the
-  // GPU's rounds better, each at the cost of writing and reading a dh in fp32 (here in k
-  // steps of a tile, 1.4 us, at 4 TB/s).
-  const int64_t tiles = p.Dt / kEdge * (p.rows == kTile256 ? p.Tp / 256 : p.rows == kTile64 ? up(T, 64) / 64 : 1);
-  const int64_t slots = p.rows == kTile256 ? kCus : 2 * kCus, all = p.Vp * p.eb / 128;
-  const double steps = (double)(all * (p.planes + p.planes_z - 1));
-  const double part = (double)(T * D * 8) / 4e12 / 1.4e-6;
-  double best = 0;
-  for (int64_t n = 1; n <= 64 && n * 4 <= std::max<int64_t>(4, all); ++n) {
-    const double cost = (double)((tiles * n + slots - 1) / slots) * steps / (double)n + (double)n * part;
-    if (best == 0 || cost < best) best = cost, p.splits = n;
-  }
+  // dh has few tiles: its sum over the piece's columns is cut in parts, as the logits' is.
+  const int64_t all = p.Vp * p.eb / 128;
+  p.splits = best_parts(p.Dt / kEdge * row_tiles, slots, (double)(all * (p.planes + p.planes_z - 1)),
+                        (double)(T * D * 8) / 4e12 / 1.4e-6, 0., all);
   return p;
 }
 
 struct FwdWs {
   char* w;         // [planes][V][Dp] where the weight is copied
   float2* part;    // [word tiles][Tp] maximum and sum of a tile's row
+  float* cut;      // [cuts][T][Vt] parts of the logits, where there are two or more
 };
 size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
   size_t off = 0;
@@ -173,6 +199,7 @@ size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
   FwdWs t;
   t.w = take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * p.eb : 0);
   t.part = reinterpret_cast<float2*>(take((size_t)(p.Vt / kEdge) * p.Tp * sizeof(float2)));
+  t.cut = reinterpret_cast<float*>(take(p.cuts > 1 ? (size_t)p.cuts * p.T * p.Vt * 4 : 0));
   if (s != nullptr) *s = t;
   return off;
 }
@@ -397,10 +424,13 @@ struct LogitArgs {
   const char* w;          // [V][ldw]
   const char* h;          // [n][Dp]
   int64_t ldw, ldh, plane_w, plane_h;
-  int V, D, Dp, K, Tp, nvt;   // nvt: tiles of this launch
+  int V, Dp, K, Tp, nvt;  // nvt: tiles of this launch
   float c;                // log2(e) / tau
   State st;
   float2* part;           // forward
+  float* z;               // forward: [n][ldzf] logits that are kept, or [cuts][ldcut] parts of them
+  int64_t ldzf, ldcut;
+  int cuts;
   const float2* coef;     // backward
   char* dz;
   int64_t ldz, plane_z;
@@ -458,15 +488,27 @@ __device__ __forceinline__ void store_block(T* lds, int lane, F value, S store) 
 }
 
 // z^T tiles: m = vocabulary, n = rows, so that a lane holds 4 MI logits of a row.
-template <typename C, typename Op, bool GRAD, int PX, int PZ>
+// kStats: the forward's maxima and sums, and the logits where they are kept; kCut: one part of
+// the sums, as it is; kGrad: the backward's dz.
+enum Mode { kStats, kCut, kGrad };
+template <typename C, typename Op, Mode MODE, int PX, int PZ>
 __global__ void __launch_bounds__(C::THREADS, 2)
 logits_kernel(LogitArgs a) {
+  constexpr bool GRAD = MODE == kGrad;
   constexpr int BM = C::BM, BN = C::BN;
   using P = Product<Op, BM, BN, C::WM, C::WN, false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int n = a.st.hdr->n;
   int vt, tt;
-  tile_of(blockIdx.x, a.nvt, gridDim.x / a.nvt, vt, tt);
+  int k0 = 0, k1 = a.Dp, cut = 0;
+  if constexpr (MODE == kCut) {
+    const int tiles = gridDim.x / a.cuts, steps = a.Dp / P::BK;
+    cut = blockIdx.x / tiles;
+    k0 = steps * cut / a.cuts * P::BK, k1 = steps * (cut + 1) / a.cuts * P::BK;
+    tile_of(blockIdx.x - cut * tiles, a.nvt, tiles / a.nvt, vt, tt);
+  } else {
+    tile_of(blockIdx.x, a.nvt, gridDim.x / a.nvt, vt, tt);
+  }
   const int t0 = tt * BN, v0 = a.v_first + vt * BM;
   if (t0 >= n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -482,7 +524,8 @@ logits_kernel(LogitArgs a) {
   int lo[P::NI];     // first of them in the wave's words
   float2 co[P::NI];
   float l2[P::NI];
-  P::template run<PX, PX>(acc, A, B, 0, a.Dp, lds, [&] {
+  P::template run<PX, PX>(acc, A, B, k0, k1, lds, [&] {
+    if constexpr (MODE == kCut) return;
 #pragma unroll
     for (int j = 0; j < P::NI; ++j) {
       const int t = min(t0 + wn * P::NW + 16 * j + (lane & 15), n - 1);
@@ -496,7 +539,21 @@ logits_kernel(LogitArgs a) {
 
   float c = a.c;
   if constexpr (PX == 2) c /= scale_h(a.st.hdr) * scale_w(a.st.hdr);
-  float* red = reinterpret_cast<float*>(lds);        // forward: [WM][BN][2]
+  float* fstage = reinterpret_cast<float*>(lds) + wave * 16 * (P::MW + 4);
+  float* red = reinterpret_cast<float*>(lds) + P::WAVES * 16 * (P::MW + 4);   // forward: [WM][BN][2]
+  static_assert((P::WAVES * 16 * (P::MW + 4) + P::WM * BN * 2) * 4 <= P::LDS_BYTES, "a tile's results go through its LDS");
+  auto store_z = [&](int j) {
+    const int t = t0 + wn * P::NW + 16 * j;
+    float* o = a.z + cut * a.ldcut + (int64_t)t * a.ldzf + vw;
+    store_block<P::MI>(fstage, lane, [&](int i) { return acc[i][j]; }, [&](int r, int v, f32x4_t x) {
+      if (t + r < n) *reinterpret_cast<f32x4_t*>(o + (int64_t)r * a.ldzf + v) = x;
+    });
+  };
+  if constexpr (MODE == kCut) {
+#pragma unroll
+    for (int j = 0; j < P::NI; ++j) store_z(j);
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
     const int tl = wn * P::NW + 16 * j + (lane & 15);
@@ -551,6 +608,7 @@ logits_kernel(LogitArgs a) {
         red[(wm * BN + tl) * 2] = m;
         red[(wm * BN + tl) * 2 + 1] = s;
       }
+      if (a.z != nullptr) store_z(j);
     } else {
 #pragma unroll
       for (int i = 0; i < P::MI; ++i)
@@ -606,6 +664,115 @@ logits_kernel(LogitArgs a) {
       }
       a.part[(int64_t)vt * a.Tp + t0 + tl] = make_float2(m, s);
     }
+  }
+}
+
+constexpr int kSeg = 2048;   // words of a row that a workgroup of the two kernels below takes, eight a thread
+
+// The parts of the logits added up: what kStats does for a tile, for a segment of a row.
+__global__ void __launch_bounds__(256)
+join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, int V, int64_t Vt, int K, bool planes, float c,
+            int64_t Tp, float2* __restrict__ part) {
+  __shared__ float red[2][4];
+  const int t = blockIdx.x;
+  if (t >= st.hdr->n) return;
+  const int tid = threadIdx.x, v0 = blockIdx.y * kSeg, v = v0 + tid * 8;
+  if (planes) c /= scale_h(st.hdr) * scale_w(st.hdr);
+  float z[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) z[e] = 0.f;
+  if (v < Vt) {   // Vt is a multiple of 8
+    const float* at = cut + (int64_t)t * Vt + v;
+#pragma unroll 4
+    for (int i = 0; i < cuts; ++i) {
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(at + i * ldcut), y = *reinterpret_cast<const f32x4_t*>(at + i * ldcut + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] += x[e], z[4 + e] += y[e];
+    }
+  }
+  float m = -INFINITY, s = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    z[e] = v + e < V ? rounded(z[e] * c) : -INFINITY;
+    m = fmaxf(m, z[e]);
+  }
+  if (st.z != nullptr && v < Vt) {
+    float* o = st.z + (int64_t)t * Vt + v;
+    *reinterpret_cast<f32x4_t*>(o) = f32x4_t{z[0], z[1], z[2], z[3]};
+    *reinterpret_cast<f32x4_t*>(o + 4) = f32x4_t{z[4], z[5], z[6], z[7]};
+  }
+  m = wave_max(m);
+  if ((tid & 63) == 0) red[0][tid >> 6] = m;
+  const int orig = st.rows[t] * K;
+  const int* ids = st.ids + orig;
+  for (int k = first_entry(ids, K, v0); k < K; ++k) {
+    const int rel = ids[k] - v0;
+    if (rel >= kSeg) break;
+    if (rel >> 3 != tid) continue;
+    float x = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x = (rel & 7) == e ? z[e] : x;
+    st.z2[orig + k] = x;
+  }
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  if (m != -INFINITY) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += exp2_fast(z[e] - m);
+  } else {   // NaN among the logits
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = z[e] != z[e] ? NAN : s;
+  }
+  s = wave_add(s);
+  if ((tid & 63) == 0) red[1][tid >> 6] = s;
+  __syncthreads();
+  if (tid == 0) part[(int64_t)blockIdx.y * Tp + t] = make_float2(m, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
+}
+
+// dz from the logits that were kept: what kGrad does for a tile, for a segment of a row.
+template <typename Op, int PZ>
+__global__ void __launch_bounds__(256)
+dz_kernel(State st, const float2* __restrict__ coef, int V, int64_t Vt, int K, int v_first, int cols, char* __restrict__ dz,
+          int64_t ldz, int64_t plane_z) {
+  const int t = blockIdx.x;
+  if (t >= st.hdr->n) return;
+  const int tid = threadIdx.x, rel0 = blockIdx.y * kSeg, at = rel0 + tid * 8, v0 = v_first + rel0, v = v0 + tid * 8;
+  const bool here = at < cols;   // both multiples of 8
+  const float2 co = coef[t];
+  const float l2 = st.lse2[t];
+  float z[8];
+  if (here) {
+    const float* i = st.z + (int64_t)t * Vt + v;
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(i), y = *reinterpret_cast<const f32x4_t*>(i + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = exp2_fast(x[e] - l2), z[4 + e] = exp2_fast(y[e] - l2);
+  }
+  const int orig = st.rows[t] * K;
+  const int* ids = st.ids + orig;
+  for (int k = first_entry(ids, K, v0); k < K; ++k) {
+    const int rel = ids[k] - v0;
+    if (rel >= kSeg) break;
+    if (rel >> 3 != tid) continue;
+    const float p = st.p[orig + k], r = p * co.y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = (rel & 7) == e ? z[e] - p + r : z[e];
+  }
+  if (!here) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) z[e] = v + e < V ? co.x * z[e] : 0.f;
+  char* o = dz + t * ldz + (int64_t)at * kBytes<Op>;
+  if constexpr (kBytes<Op> == 4) {
+    reinterpret_cast<f32x4_t*>(o)[0] = f32x4_t{z[0], z[1], z[2], z[3]};
+    reinterpret_cast<f32x4_t*>(o)[1] = f32x4_t{z[4], z[5], z[6], z[7]};
+  } else {
+    rr::u16x8_t hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      hi[e] = op_bits<Op>(z[e]);
+      lo[e] = op_bits<Op>(z[e] - op_val<Op>(hi[e]));
+    }
+    *reinterpret_cast<rr::u16x8_t*>(o) = hi;
+    if constexpr (PZ == 2) *reinterpret_cast<rr::u16x8_t*>(o + plane_z) = lo;
   }
 }
 
@@ -714,7 +881,7 @@ struct DhArgs {
   const char* w;         // at the piece's first row
   const char* dz;
   int64_t ldw, ldz, plane_w, plane_z;
-  int V, D, Dp, Tp, ndt, splits, cols;   // V: rows of w from the piece on; cols: the piece's columns to whole k steps
+  int V, Tp, ndt, splits, cols;   // V: rows of w from the piece on; cols: the piece's columns to whole k steps
   float* out;            // [splits][Tp][Dt]
   int Dt;
   bool first;
@@ -791,7 +958,7 @@ struct DwArgs {
   const char* h;
   const char* dz;
   int64_t ldh, ldz, plane_h, plane_z;
-  int V, D, Dp, ndt;     // V: rows of dw from the piece on
+  int V, D, ndt;         // V: rows of dw from the piece on
   const float* scale;
   void* out;             // dw at the piece's first row
   State st;
@@ -876,16 +1043,22 @@ LogitArgs logit_args(const Plan& p, const State& st, const void* weight, char* w
   a.h = st.h;
   a.ldw = (p.copy_w ? p.Dp : p.D) * p.eb, a.ldh = p.Dp * p.eb;
   a.plane_w = p.V * a.ldw, a.plane_h = p.T * a.ldh;
-  a.V = (int)p.V, a.D = (int)p.D, a.Dp = (int)p.Dp, a.K = K, a.Tp = (int)p.Tp;
+  a.V = (int)p.V, a.Dp = (int)p.Dp, a.K = K, a.Tp = (int)p.Tp;
   a.c = kLog2e / tau;
   a.st = st;
   return a;
 }
 // The logits of `cols` columns (whole tiles).
-template <typename C, typename Op, bool GRAD, int PX, int PZ>
+template <typename C, typename Op, Mode MODE, int PX, int PZ>
 void launch_logits(LogitArgs a, int64_t T, int64_t cols, hipStream_t s) {
   a.nvt = (int)(cols / C::BM);
-  logits_kernel<C, Op, GRAD, PX, PZ><<<(unsigned)(a.nvt * (up(T, C::BN) / C::BN)), C::THREADS, 0, s>>>(a);
+  logits_kernel<C, Op, MODE, PX, PZ><<<(unsigned)(a.nvt * (up(T, C::BN) / C::BN) * (MODE == kCut ? a.cuts : 1)), C::THREADS, 0, s>>>(a);
+}
+// The forward's, whole or in parts.
+template <typename C, typename Op, int PX>
+void launch_forward(const LogitArgs& a, const Plan& p, hipStream_t s) {
+  if (p.cuts > 1) launch_logits<C, Op, kCut, PX, PX>(a, p.T, p.Vt, s);
+  else launch_logits<C, Op, kStats, PX, PX>(a, p.T, p.Vt, s);
 }
 template <typename C, typename Op, int PX, int PZ>
 void launch_dh(DhArgs a, const Plan& p, hipStream_t s) {
@@ -910,16 +1083,23 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
   pack_weight<X, Op>(p, weight, st, ws.w, s);
   LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
   a.part = ws.part;
+  a.z = p.cuts > 1 ? ws.cut : st.z, a.ldzf = p.Vt, a.ldcut = p.T * p.Vt, a.cuts = (int)p.cuts;
   // (few rows are never split in planes, fp32 MFMA products never have many rows)
   if constexpr (PX == 1) {
-    if (p.rows == kTile32) launch_logits<Tile32, Op, false, PX, PX>(a, p.T, p.Vt, s);
-    else if (p.rows == kTile64) launch_logits<Tile64, Op, false, PX, PX>(a, p.T, p.Vt, s);
+    if (p.rows == kTile32) launch_forward<Tile32, Op, PX>(a, p, s);
+    else if (p.rows == kTile64) launch_forward<Tile64, Op, PX>(a, p, s);
   }
   if constexpr (!__is_same(Op, OpF32)) {
-    if (p.rows == kTile256) launch_logits<Tile256, Op, false, PX, PX>(a, p.T, p.Vt, s);
+    if (p.rows == kTile256) launch_forward<Tile256, Op, PX>(a, p, s);
+  }
+  int64_t parts = p.Vt / kEdge;
+  if (p.cuts > 1) {
+    parts = up(p.Vt, kSeg) / kSeg;
+    join_kernel<<<dim3((unsigned)p.T, (unsigned)parts), 256, 0, s>>>(st, ws.cut, a.cuts, a.ldcut, a.V, p.Vt, K, PX == 2, a.c,
+                                                                    p.Tp, ws.part);
   }
   float* rows = reduction == 0 ? loss : st.loss;
-  row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, (int)(p.Vt / kEdge), p.Tp, K, labels, zl, tau, rows);
+  row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, K, labels, zl, tau, rows);
   if (reduction != 0) sum_loss_kernel<<<1, 1024, 0, s>>>(st.loss, p.T, st.hdr, reduction == 1, loss);
   return rr::check_launch("rr_linear_loss");
 }
@@ -927,7 +1107,7 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
 template <typename X, typename Op, int PX, int PZ>
 int backward(const Plan& p, const float* dloss, const void* weight, const State& st, const BwdWs& ws, int K, float zl,
              float tau, int reduction, void* dh, void* dw, hipStream_t s) {
-  pack_weight<X, Op>(p, weight, st, ws.w, s);
+  if (dh != nullptr || !p.keep) pack_weight<X, Op>(p, weight, st, ws.w, s);
   coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, reduction == 1, tau, zl, __is_same(Op, OpF16), ws.coef,
                                  ws.scale);
   for (int64_t v = 0; v < p.Vt; v += p.Vp) {
@@ -935,16 +1115,16 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
     LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
     a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp * p.eb, a.plane_z = p.Tp * a.ldz, a.v_first = (int)v;
     constexpr bool kFew = __is_same(Op, OpF32) || (PX == 1 && PZ == 2);   // up to kFewRows, or kExactRows
-    if constexpr (kFew) {
-      if (p.rows == kTile32) launch_logits<Tile32, Op, true, PX, PZ>(a, p.T, cols, s);
-      else launch_logits<Tile64, Op, true, PX, PZ>(a, p.T, cols, s);
-    } else {
-      launch_logits<Tile256, Op, true, PX, PZ>(a, p.T, cols, s);
+    if (kFew || p.keep) {
+      dz_kernel<Op, PZ><<<dim3((unsigned)p.T, (unsigned)(up(cols, kSeg) / kSeg)), 256, 0, s>>>(
+          st, ws.coef, a.V, p.Vt, K, a.v_first, (int)cols, ws.dz, a.ldz, a.plane_z);
+    } else if constexpr (!kFew) {
+      launch_logits<Tile256, Op, kGrad, PX, PZ>(a, p.T, cols, s);
     }
     if (dh != nullptr) {
       DhArgs b{};
       b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = a.ldz, b.plane_w = a.plane_w, b.plane_z = a.plane_z;
-      b.V = (int)(p.V - v), b.D = a.D, b.Dp = a.Dp, b.Tp = a.Tp, b.splits = (int)p.splits, b.cols = (int)cols;
+      b.V = (int)(p.V - v), b.Tp = a.Tp, b.splits = (int)p.splits, b.cols = (int)cols;
       b.out = ws.dh, b.Dt = (int)p.Dt, b.first = v == 0, b.st = st;
       if constexpr (kFew) {
         if (p.rows == kTile32) launch_dh<Tile32, Op, PX, PZ>(b, p, s);
@@ -956,7 +1136,7 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
     if (dw != nullptr) {
       DwArgs c{};
       c.h = st.h, c.dz = ws.dz, c.ldh = a.ldh, c.ldz = a.ldz, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
-      c.V = (int)(p.V - v), c.D = a.D, c.Dp = a.Dp, c.scale = ws.scale;
+      c.V = (int)(p.V - v), c.D = (int)p.D, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
       launch_dw<Tile256, Op, X, PX, PZ>(c, p, cols, s);
     }
@@ -996,17 +1176,25 @@ int check_buffers(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, i
   const std::string w(who);
   if ((pass == 0 && hidden == nullptr) || weight == nullptr || state == nullptr || ws == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
   if (!aligned16(hidden) || !aligned16(weight)) return rr::fail(RR_EINVAL, w + ": buffers must be 16-byte aligned");
-  if (state_bytes < rr_linear_loss_state_bytes(T, D, K, dtype)) return rr::fail(RR_EWORKSPACE, w + ": state buffer too small");
+  if (state_bytes < rr_linear_loss_state_bytes(T, D, V, K, dtype, pass)) return rr::fail(RR_EWORKSPACE, w + ": state buffer too small");
   if (ws_bytes < rr_linear_loss_workspace_bytes(T, D, V, dtype, pass)) return rr::fail(RR_EWORKSPACE, w + ": workspace too small");
   if (!aligned16(state) || !aligned16(ws)) return rr::fail(RR_EWORKSPACE, w + ": state buffer or workspace misaligned");
   return RR_OK;
 }
 
+// The caller's state: with the logits where it has room for them.
+void lay_out_state(int64_t T, int64_t D, int64_t V, int64_t K, int dtype, void* state, size_t bytes, State* st) {
+  const bool grad = bytes >= rr_linear_loss_state_bytes(T, D, V, K, dtype, 1);
+  const Plan p = plan_of(T, D, V, dtype);
+  state_layout(T, D, K, dtype, grad && p.keep ? p.Vt : 0, static_cast<char*>(state), st);
+}
+
 }  // namespace
 
-extern "C" size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t K, int dtype) {
-  if (rows <= 0 || check_dims("rr_linear_loss_state_bytes", rows, D, 1, K, dtype, 0) != RR_OK) return 0;
-  return state_layout(rows, D, K, dtype, nullptr, nullptr);
+extern "C" size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t V, int64_t K, int dtype, int grad) {
+  if (rows <= 0 || check_dims("rr_linear_loss_state_bytes", rows, D, V, K, dtype, 0) != RR_OK) return 0;
+  const Plan p = plan_of(rows, D, V, dtype);
+  return state_layout(rows, D, K, dtype, grad && p.keep ? p.Vt : 0, nullptr, nullptr);
 }
 
 extern "C" size_t rr_linear_loss_workspace_bytes(int64_t rows, int64_t D, int64_t V, int dtype, int pass) {
@@ -1031,7 +1219,7 @@ extern "C" int rr_linear_ce_fwd(const void* hidden, const void* weight, int dtyp
   if (labels == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
   if (int rc = check_buffers(who, rows, D, V, 1, dtype, 0, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
   State st;
-  state_layout(rows, D, 1, dtype, static_cast<char*>(state), &st);
+  lay_out_state(rows, D, V, 1, dtype, state, state_bytes, &st);
   State in = st;
   if (reduction == 0) in.loss = loss;   // where rows that do not count leave their 0
   rows_kernel<true><<<1, 1024, 0, s>>>(labels, ignore_index, rows, (int)V, in);
@@ -1061,7 +1249,7 @@ extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtyp
   if (teacher_logits == nullptr || teacher_ids == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
   if (int rc = check_buffers(who, rows, D, V, K, dtype, 0, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
   State st;
-  state_layout(rows, D, K, dtype, static_cast<char*>(state), &st);
+  lay_out_state(rows, D, V, K, dtype, state, state_bytes, &st);
   int KP = 1;
   while (KP < K) KP *= 2;
   RR_DISPATCH_DTYPE(teacher_dtype, {
@@ -1095,7 +1283,7 @@ extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dt
   if (dhidden == nullptr && dweight == nullptr) return RR_OK;
   const Plan p = plan_of(rows, D, V, dtype);
   State st;
-  state_layout(rows, D, K, dtype, static_cast<char*>(const_cast<void*>(state)), &st);
+  lay_out_state(rows, D, V, K, dtype, const_cast<void*>(state), state_bytes, &st);
   BwdWs ws;
   bwd_layout(p, static_cast<char*>(workspace), &ws);
 #define LL_BACKWARD(X, OP, PX, PZ) \

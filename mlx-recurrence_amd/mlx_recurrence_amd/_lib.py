@@ -84,7 +84,7 @@ _SIGS = {
                           + [_c_ptr] * 3),
     "rr_layer_norm_bwd_workspace_bytes": (_c_size, [_c_i64] * 2),
     "rr_layer_norm_bwd": (_c_int, [_c_ptr, _c_int] * 3 + [_c_ptr] * 2 + [_c_i64] * 2 + [_c_ptr] * 4 + [_c_size, _c_ptr]),
-    "rr_linear_loss_state_bytes": (_c_size, [_c_i64] * 3 + [_c_int]),
+    "rr_linear_loss_state_bytes": (_c_size, [_c_i64] * 4 + [_c_int] * 2),
     "rr_linear_loss_workspace_bytes": (_c_size, [_c_i64] * 3 + [_c_int] * 2),
     "rr_linear_ce_fwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 3 + [_c_ptr, _c_i64, _c_f32, _c_int]
                          + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
@@ -532,9 +532,9 @@ def layer_norm_bwd(dy, x, w, w_dtype, mean, rstd, rows, D, dx, dw, db):
                                     0 if ws is None else ws.numel(), stream_of(x)), "rr_layer_norm_bwd")
 
 
-def linear_loss_buffers(rows, D, V, K, dtype, device):
-    """State (kept for the backward) and workspace of a forward."""
-    state = _alloc_ws(_ws_bytes("rr_linear_loss_state_bytes", (rows, D, K, DTYPE_CODE[dtype])), device)
+def linear_loss_buffers(rows, D, V, K, dtype, device, grad):
+    """State (kept for the backward, where there is to be one) and workspace of a forward."""
+    state = _alloc_ws(_ws_bytes("rr_linear_loss_state_bytes", (rows, D, V, K, DTYPE_CODE[dtype], int(grad))), device)
     return state, _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[dtype], 0)), device)
 
 

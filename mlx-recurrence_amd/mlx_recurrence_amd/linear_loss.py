@@ -28,7 +28,7 @@ class _LinearLoss(torch.autograd.Function):
     logits and ids [rows, K]."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, labels, t_logits, t_ids, ignore_index, z_loss, temperature, reduction):
+    def forward(ctx, hidden, weight, labels, t_logits, t_ids, ignore_index, z_loss, temperature, reduction, grad):
         dev = _lib.require_device(hidden, weight, labels, t_logits, t_ids)
         dt = hidden.dtype
         h_, w_ = _lib.prep(hidden, dt), _lib.prep(weight, dt)
@@ -36,7 +36,7 @@ class _LinearLoss(torch.autograd.Function):
         K = 1 if t_ids is None else t_ids.shape[1]
         loss = torch.empty((rows,) if reduction == 0 else (), dtype=torch.float32, device=dev)
         with _lib.device_guard(dev):
-            state, ws = _lib.linear_loss_buffers(rows, D, V, K, dt, dev)
+            state, ws = _lib.linear_loss_buffers(rows, D, V, K, dt, dev, grad)
             if t_ids is None:
                 _lib.linear_ce_fwd(h_, w_, _lib.prep(labels, torch.int64), ignore_index, z_loss, reduction, loss, state, ws)
             else:
@@ -54,7 +54,7 @@ class _LinearLoss(torch.autograd.Function):
         dw = torch.empty_like(w_) if ctx.needs_input_grad[1] else None
         with _lib.device_guard(w_.device):
             _lib.linear_loss_bwd(_lib.prep(dloss, torch.float32), w_, *ctx.args, state, dh, dw)
-        return (dh, dw) + (None,) * 7
+        return (dh, dw) + (None,) * 8
 
 
 def _check(hidden, weight, reduction):
@@ -80,7 +80,8 @@ def _apply(hidden, weight, *args):
     h, w = h if h.dtype == dt else h.to(dt), weight if weight.dtype == dt else weight.to(dt)
     ext = _lib.autograd_ext()
     # the same forward / backward as one C++ autograd node where it is built
-    loss = _LinearLoss.apply(h, w, *args) if ext is None else ext.linear_loss(h, w, *args)
+    grad = torch.is_grad_enabled() and (h.requires_grad or w.requires_grad)
+    loss = _LinearLoss.apply(h, w, *args, grad) if ext is None else ext.linear_loss(h, w, *args)
     return loss.reshape(lead) if len(lead) != 1 and loss.ndim == 1 else loss
 
 

@@ -168,7 +168,7 @@ def test_c_abi_refusals():
     for bad in (dict(rows=-1), dict(D=0), dict(V=0), dict(dt=9), dict(red=3), dict(h=None), dict(w=None), dict(l=None),
                 dict(loss=None), dict(st=None), dict(ws=None), dict(h=odd), dict(w=odd)):
         assert ce(**bad) == _lib.RR_EINVAL, bad
-    for bad in (dict(sn=lib.rr_linear_loss_state_bytes(4, 8, 1, 1) - 1), dict(st=odd), dict(ws=odd),
+    for bad in (dict(sn=lib.rr_linear_loss_state_bytes(4, 8, 10, 1, 1, 0) - 1), dict(st=odd), dict(ws=odd),
                 dict(wn=lib.rr_linear_loss_workspace_bytes(4, 8, 10, 1, 0) - 1)):
         assert ce(**bad) == _lib.RR_EWORKSPACE, bad
     for bad in (dict(V=(1 << 24) + 1), dict(D=65537), dict(rows=1 << 24)):
@@ -184,14 +184,19 @@ def test_c_abi_refusals():
     for bad in (dict(dl=None), dict(w=None), dict(st=None), dict(tau=-1.0), dict(red=-1)):
         assert bw(**bad) == _lib.RR_EINVAL, bad
     assert bw(wn=lib.rr_linear_loss_workspace_bytes(4, 8, 10, 1, 1) - 1) == _lib.RR_EWORKSPACE
+    # the state of a forward without a backward does not do for one
+    assert bw(sn=lib.rr_linear_loss_state_bytes(4, 8, 10, 3, 1, 1) - 1) == _lib.RR_EWORKSPACE
+    assert bw(sn=lib.rr_linear_loss_state_bytes(4, 8, 10, 3, 1, 0)) == _lib.RR_EWORKSPACE
     assert bw(dh=None, dw=None) == _lib.RR_OK
 
 
 @pytest.mark.parametrize("rows,D,V,dtype", [(8192, 2560, 65536, 1), (32768, 2560, 131072, 1), (1536, 768, 32000, 0),
                                             (1, 5120, 131072, 1), (100_000, 64, 32000, 2)])
-def test_the_logits_are_never_held(rows, D, V, dtype):
+def test_many_logits_are_not_held(rows, D, V, dtype):
     """The backward's workspace holds a piece of the logits' gradient, not all of it: beside the
-    copies of the inputs and dhidden's parts at most about 512 MiB, or 2048 columns of every row."""
+    copies of the inputs and dhidden's parts at most about 512 MiB, or 2048 columns of every row.
+    The state holds the logits of up to 256 rows, of more where they take 256 MiB or the weight's
+    bytes at most."""
     lib, planes = _lib.load(), 2 if dtype == 0 else 1
     rows_up = (rows + 255) // 256 * 256
     pieces = max(512 << 20, 2048 * rows_up * 2 * planes) + (256 * rows_up * 2 * planes)
@@ -199,3 +204,9 @@ def test_the_logits_are_never_held(rows, D, V, dtype):
     parts = 64 * rows_up * ((D + 255) // 256 * 256) * 4
     assert lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 1) <= pieces + copies + parts + (1 << 20)
     assert lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 0) <= copies + 8 * rows_up * (V + 255) // 32 + (1 << 20)
+    state = [lib.rr_linear_loss_state_bytes(rows, D, V, 4, dtype, grad) for grad in (0, 1)]
+    assert state[0] <= rows * (copies // (rows + (V if dtype == 0 else 0)) + 4 * 4 + 3 * 4 * 4) + (1 << 20)
+    logits = rows * ((V + 255) // 256 * 256) * 4
+    held = logits <= max(256 << 20, V * D * (4 if dtype == 0 else 2), 256 * V * 4)
+    assert state[1] - state[0] in ((0, logits) if held else (0,))
+    assert state[1] - state[0] == logits or rows > 256
