@@ -56,8 +56,13 @@ constexpr int64_t kMinPiece = 2048;
 constexpr int64_t kMaxPiece = 1 << 20;       // a row of a tile's operand is at most so long
 constexpr int64_t kFewRows = 64;           // rows whose dz keeps a second plane
 constexpr int64_t kExactRows = 256;        // rows of fp32 that run on the fp32 MFMA
-constexpr int64_t kKeepBytes = (int64_t)256 << 20;    // of logits that are kept, or the weight's bytes
-constexpr int64_t kKeepChannels = 1280;    // from so many on (a third for planes) reading a logit costs less than its product
+// Logits are kept where they take no more than 4 GiB (of 288) and, with many rows, writing and
+// reading one costs less than its product: forward and backward of 1024 x 32000 in bf16 with 768,
+// 1024 and 2560 channels 267, 293 and 568 us kept, 266, 298 and 633 formed again; 8192 x 65536
+// x 2560 7.6 and 8.9 ms.  (A product of planes costs three times as much.)  Few rows' are
+// always kept: their product is a whole reading of the weight.
+constexpr int64_t kKeepBytes = (int64_t)4 << 30;
+constexpr int64_t kKeepChannels = 1024;
 constexpr int kPad = 64;                   // channels are padded to so many
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -173,7 +178,7 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   }
   const int64_t z_bytes = T * p.Vt * 4;
   p.keep = T <= kExactRows || p.cuts > 1 ||
-           (z_bytes <= std::max(kKeepBytes, V * D * (dtype == RR_F32 ? 4 : 2)) && D * (p.planes == 2 ? 3 : 1) >= kKeepChannels);
+           (z_bytes <= kKeepBytes && D * (p.planes == 2 ? 3 : 1) >= kKeepChannels);
   const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * p.eb * p.planes_z) / kEdge * kEdge));
   const int64_t pieces = (p.Vt + most - 1) / most;
   p.Vp = up((p.Vt + pieces - 1) / pieces, kEdge);

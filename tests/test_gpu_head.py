@@ -266,6 +266,47 @@ def test_fp32_pieces():
     check_all(run_ce(h, w, labels, up), orc.cross_entropy(h, w, labels, up))
 
 
+# few tiles of many channels: the logits' sums are made in parts; words that are no whole segment of 2048
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,D,V", [(1, 5000, 300), (5, 3000, 700), (40, 2048, 5003), (200, 4096, 640), (300, 2050, 2100)])
+def test_sums_in_parts(rows, D, V, dtype):
+    g, h, w, labels = head_inputs(rows, D, V, dtype, rows + D + V)
+    labels[2::5] = -100
+    up = torch.rand(rows, generator=g, device="cuda") + 0.1
+    got = run_ce(h, w, labels, up, z_loss=1e-3, reduction="none")
+    check_all(got, orc.cross_entropy(h, w, labels, up, zl=1e-3, reduction="none"))
+    with torch.no_grad():   # without a backward the logits are not kept, the loss is the same
+        assert torch.equal(mr.linear_cross_entropy(h, w, labels, z_loss=1e-3, reduction="none"), got[0])
+    t, ids = teacher(g, rows, 70, V, labels.clamp(min=0))
+    ids[-1] = torch.arange(70, device="cuda") % 3 + V - 3
+    check_all(run_kd(h, w, t, ids, up, temperature=2.0, reduction="none"),
+              orc.distillation(h, w, t, ids, up, tau=2.0, reduction="none"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_sums_in_parts_of_what_is_not_finite(dtype):
+    _, h, w, labels = head_inputs(20, 3000, 300, dtype, 6)
+    h[3, 5], h[9, 1] = math.nan, math.inf
+    labels[12] = 300
+    loss, dh, dw = run_ce(h, w, labels, torch.ones(20, device="cuda"), reduction="none")
+    for r in (3, 9, 12):
+        assert not torch.isfinite(loss[r]) and torch.isnan(dh[r]).any()
+    assert torch.isnan(dw).any()
+    fine = [r for r in range(20) if r not in (3, 9, 12)]
+    want = orc.cross_entropy(h[fine], w, labels[fine], torch.ones(17, device="cuda"), reduction="none")
+    check("loss", loss[fine], want[0])
+    check("dhidden", dh[fine], want[1])
+
+
+@pytest.mark.parametrize("rows,D,V,dtype", [(8192, 1030, 33000, BF16), (4500, 360, 33000, F32)])
+def test_kept_logits_of_two_pieces(rows, D, V, dtype):
+    """Logits that the forward leaves, read by the backward in two pieces of the vocabulary."""
+    g, h, w, labels = head_inputs(rows, D, V, dtype, 15)
+    labels[::9] = -100
+    up = torch.tensor(1.0, device="cuda")
+    check_all(run_ce(h, w, labels, up, z_loss=1e-3), orc.cross_entropy(h, w, labels, up, zl=1e-3))
+
+
 def test_rows_that_do_not_count_are_not_read():
     for dtype in (F32, BF16, F16):
         g, h, w, labels = head_inputs(150, 64, 500, dtype, 3)

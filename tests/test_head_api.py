@@ -195,8 +195,8 @@ def test_c_abi_refusals():
 def test_many_logits_are_not_held(rows, D, V, dtype):
     """The backward's workspace holds a piece of the logits' gradient, not all of it: beside the
     copies of the inputs and dhidden's parts at most about 512 MiB, or 2048 columns of every row.
-    The state holds the logits of up to 256 rows, of more where they take 256 MiB or the weight's
-    bytes at most."""
+    The state holds the logits of up to 256 rows, of more where they take
+    4 GiB at most."""
     lib, planes = _lib.load(), 2 if dtype == 0 else 1
     rows_up = (rows + 255) // 256 * 256
     pieces = max(512 << 20, 2048 * rows_up * 2 * planes) + (256 * rows_up * 2 * planes)
@@ -207,6 +207,6 @@ def test_many_logits_are_not_held(rows, D, V, dtype):
     state = [lib.rr_linear_loss_state_bytes(rows, D, V, 4, dtype, grad) for grad in (0, 1)]
     assert state[0] <= rows * (copies // (rows + (V if dtype == 0 else 0)) + 4 * 4 + 3 * 4 * 4) + (1 << 20)
     logits = rows * ((V + 255) // 256 * 256) * 4
-    held = logits <= max(256 << 20, V * D * (4 if dtype == 0 else 2), 256 * V * 4)
+    held = rows <= 256 or logits <= 4 << 30
     assert state[1] - state[0] in ((0, logits) if held else (0,))
     assert state[1] - state[0] == logits or rows > 256
