@@ -139,6 +139,7 @@ struct Plan {
   // backward
   int64_t Vp;          // columns of a piece (whole tiles)
   int64_t splits;      // parts of a piece's columns that dh is added up in
+  int64_t cuts_w;      // parts of the rows that dw is added up in
 };
 constexpr int64_t kCus = 256;
 // How many parts the k steps of `tiles` tiles are cut in, `slots` workgroups running at one
@@ -186,6 +187,13 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   const int64_t all = p.Vp * p.eb / 128;
   p.splits = best_parts(p.Dt / kEdge * row_tiles, slots, (double)(all * (p.planes + p.planes_z - 1)),
                         (double)(T * D * 8) / 4e12 / 1.4e-6, 0., all);
+  // Few words and many rows: so is dw's sum over the rows (few rows are few steps).
+  p.cuts_w = 1;
+  if (T > kExactRows) {
+    const int64_t rows = up(T, 64) / 64;
+    p.cuts_w = best_parts(p.Dt / kEdge * (p.Vp / kEdge), kCus, (double)(rows * (p.planes + p.planes_z - 1)),
+                          (double)(p.Vp * D * 8) / 4e12 / 1.4e-6, 4., rows);
+  }
   return p;
 }
 
@@ -214,6 +222,7 @@ struct BwdWs {
   float2* coef;    // [Tp] a row's factors (coef_kernel)
   char* dz;        // [planes_z][Tp][Vp]
   float* dh;       // [splits][Tp][Dt]
+  float* dw;       // [cuts_w][Vp][Dt], where there are two or more
 };
 size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
   size_t off = 0;
@@ -228,6 +237,7 @@ size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
   t.coef = reinterpret_cast<float2*>(take((size_t)p.Tp * sizeof(float2)));
   t.dz = take((size_t)p.planes_z * p.Tp * p.Vp * p.eb);
   t.dh = reinterpret_cast<float*>(take((size_t)p.splits * p.Tp * p.Dt * 4));
+  t.dw = reinterpret_cast<float*>(take(p.cuts_w > 1 ? (size_t)p.cuts_w * p.Vp * p.Dt * 4 : 0));
   if (s != nullptr) *s = t;
   return off;
 }
@@ -929,21 +939,21 @@ dh_kernel(DhArgs a) {
   }
 }
 
-// dh of every row from its parts, in the inputs' type; 0 for rows that do not count.  A
-// workgroup per row and 1024 channels, four a thread.
-template <typename X>
+// A gradient from its parts, in the inputs' type: dh of every row (0 for rows that do not
+// count), or dw.  A workgroup per row and 1024 channels, four a thread.
+template <typename X, bool DH>
 __global__ void __launch_bounds__(256)
-dh_out_kernel(State st, const float* __restrict__ part, int D, int64_t ldp, int64_t stride, int splits,
-              const float* scale, X* __restrict__ dh) {
+sum_out_kernel(State st, const float* __restrict__ part, int D, int64_t ldp, int64_t stride, int splits,
+               const float* scale, X* __restrict__ out) {
   const int64_t row = blockIdx.x;
   const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (c >= D) return;
-  const int t = st.pos[row];
+  const int64_t t = DH ? st.pos[row] : row;
   float f = scale[0];
-  if constexpr (sizeof(X) == 4) f /= scale_w(st.hdr);
+  if constexpr (sizeof(X) == 4) f /= DH ? scale_w(st.hdr) : scale_h(st.hdr);
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (t >= 0) {
-    const float* at = part + (int64_t)t * ldp + c;   // ldp is whole tiles
+    const float* at = part + t * ldp + c;   // ldp is whole tiles
 #pragma unroll 4
     for (int i = 0; i < splits; ++i) {
       const float4 v = *reinterpret_cast<const float4*>(at + (int64_t)i * stride);
@@ -951,7 +961,7 @@ dh_out_kernel(State st, const float* __restrict__ part, int D, int64_t ldp, int6
     }
     s.x *= f, s.y *= f, s.z *= f, s.w *= f;
   }
-  X* o = dh + row * D + c;
+  X* o = out + row * D + c;
   const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -966,9 +976,12 @@ struct DwArgs {
   int V, D, ndt;         // V: rows of dw from the piece on
   const float* scale;
   void* out;             // dw at the piece's first row
+  float* part;           // CUT: [cuts][Vp][Dt]
+  int64_t ldp, ldcut;
+  int cuts;
   State st;
 };
-template <typename C, typename Op, typename X, int PX, int PZ>
+template <typename C, typename Op, typename X, int PX, int PZ, bool CUT>
 __global__ void __launch_bounds__(C::THREADS, 2)
 dw_kernel(DwArgs a) {
   constexpr int BM = C::BM, BN = C::BN;
@@ -976,16 +989,29 @@ dw_kernel(DwArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int n = a.st.hdr->n;
   int dt, vt;
-  tile_of(blockIdx.x, a.ndt, gridDim.x / a.ndt, dt, vt);
+  const int tiles = CUT ? gridDim.x / a.cuts : gridDim.x, cut = CUT ? blockIdx.x / tiles : 0;
+  tile_of(blockIdx.x - cut * tiles, a.ndt, tiles / a.ndt, dt, vt);
   const int d0 = dt * BM, v0 = vt * BN;
   typename P::Acc acc;
   const Operand A{a.h + d0 * P::EB, a.ldh, a.plane_h, n, (int)a.ldh - d0 * P::EB};
   const Operand B{a.dz + (int64_t)v0 * P::EB, a.ldz, a.plane_z, n, BN * P::EB};
-  P::template run<PX, PZ>(acc, A, B, 0, (n + P::BK - 1) / P::BK * P::BK, lds);
-  float f = a.scale[0];
-  if constexpr (PX == 2) f /= scale_h(a.st.hdr);
+  const int steps = (n + P::BK - 1) / P::BK;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN, wn = wave % P::WN;
+  if constexpr (CUT) {
+    const int k0 = (int)((int64_t)steps * cut / a.cuts) * P::BK, k1 = (int)((int64_t)steps * (cut + 1) / a.cuts) * P::BK;
+    P::template run<PX, PZ>(acc, A, B, k0, k1, lds);
+#pragma unroll
+    for (int j = 0; j < P::NI; ++j) {
+      float* o = a.part + cut * a.ldcut + (int64_t)(v0 + wn * P::NW + 16 * j) * a.ldp + d0 + wm * P::MW;
+      store_block<P::MI>(reinterpret_cast<float*>(lds) + wave * 16 * (P::MW + 4), lane, [&](int i) { return acc[i][j]; },
+                         [&](int r, int c, f32x4_t x) { *reinterpret_cast<f32x4_t*>(o + (int64_t)r * a.ldp + c) = x; });
+    }
+    return;
+  }
+  P::template run<PX, PZ>(acc, A, B, 0, steps * P::BK, lds);
+  float f = a.scale[0];
+  if constexpr (PX == 2) f /= scale_h(a.st.hdr);
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
     using Bits = typename std::conditional<sizeof(X) == 4, float, uint16_t>::type;   // of X
@@ -1070,10 +1096,15 @@ void launch_dh(DhArgs a, const Plan& p, hipStream_t s) {
   a.ndt = (int)(up(p.D, C::BM) / C::BM);
   dh_kernel<C, Op, PX, PZ><<<(unsigned)(a.ndt * (up(p.T, C::BN) / C::BN) * p.splits), C::THREADS, 0, s>>>(a);
 }
-template <typename C, typename Op, typename X, int PX, int PZ>
+template <typename C, typename Op, typename X, int PX, int PZ, bool CUT>
 void launch_dw(DwArgs a, const Plan& p, int64_t cols, hipStream_t s) {
   a.ndt = (int)(up(p.D, C::BM) / C::BM);
-  dw_kernel<C, Op, X, PX, PZ><<<(unsigned)(a.ndt * (cols / C::BN)), C::THREADS, 0, s>>>(a);
+  const unsigned tiles = (unsigned)(a.ndt * (cols / C::BN));
+  dw_kernel<C, Op, X, PX, PZ, CUT><<<CUT ? tiles * (unsigned)a.cuts : tiles, C::THREADS, 0, s>>>(a);
+  if constexpr (CUT) {
+    sum_out_kernel<X, false><<<dim3((unsigned)std::min<int64_t>(cols, a.V), (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
+        a.st, a.part, a.D, a.ldp, a.ldcut, a.cuts, a.scale, static_cast<X*>(a.out));
+  }
 }
 
 template <typename X, typename Op, int PX>
@@ -1143,11 +1174,16 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
       c.h = st.h, c.dz = ws.dz, c.ldh = a.ldh, c.ldz = a.ldz, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
       c.V = (int)(p.V - v), c.D = (int)p.D, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
-      launch_dw<Tile256, Op, X, PX, PZ>(c, p, cols, s);
+      c.part = ws.dw, c.ldp = p.Dt, c.ldcut = p.Vp * p.Dt, c.cuts = (int)p.cuts_w;
+      if (kFew || p.cuts_w == 1) {
+        launch_dw<Tile256, Op, X, PX, PZ, false>(c, p, cols, s);
+      } else if constexpr (!kFew) {
+        launch_dw<Tile256, Op, X, PX, PZ, true>(c, p, cols, s);
+      }
     }
   }
   if (dh != nullptr) {
-    dh_out_kernel<X><<<dim3((unsigned)p.T, (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
+    sum_out_kernel<X, true><<<dim3((unsigned)p.T, (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
         st, ws.dh, (int)p.D, p.Dt, p.Tp * p.Dt, (int)p.splits, ws.scale, static_cast<X*>(dh));
   }
   return rr::check_launch("rr_linear_loss_bwd");

@@ -284,6 +284,19 @@ def test_sums_in_parts(rows, D, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,D,V", [(1500, 65, 300), (3001, 200, 640), (5000, 1100, 129)])
+def test_dweight_in_parts(rows, D, V, dtype):
+    """Few words and many rows: dweight's sums over the rows that count, whose number only the device knows."""
+    g, h, w, labels = head_inputs(rows, D, V, dtype, rows + D + V)
+    for ignored in (0.0, 0.95, 1.0):
+        l2 = torch.where(torch.rand(rows, generator=g, device="cuda") < ignored, -100, labels)
+        up = torch.rand(rows, generator=g, device="cuda") + 0.1
+        got = run_ce(h, w, l2, up, reduction="none")
+        check_all(got, orc.cross_entropy(h, w, l2, up, reduction="none"))
+    assert not got[2].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_sums_in_parts_of_what_is_not_finite(dtype):
     _, h, w, labels = head_inputs(20, 3000, 300, dtype, 6)
     h[3, 5], h[9, 1] = math.nan, math.inf
