@@ -97,30 +97,9 @@ struct State {
   float* p;      // [rows][K] their weights
   float* z2;     // [rows][K] their logits, times log2(e) / tau
   char* h;       // [planes][rows][Dp] the hidden states that count, as an operand
+  char* w;       // [planes][V][Dp] where the weight is copied
   float* z;      // [rows][Vt] their logits, times log2(e) / tau, where they are kept
 };
-size_t state_layout(int64_t T, int64_t D, int64_t K, int dtype, int64_t z_words, char* base, State* s) {
-  size_t off = 0;
-  auto take = [&](size_t bytes) {
-    char* at = base + off;
-    off += (bytes + 255) / 256 * 256;
-    return at;
-  };
-  State t;
-  t.hdr = reinterpret_cast<Header*>(take(sizeof(Header)));
-  t.rows = reinterpret_cast<int*>(take((size_t)T * 4));
-  t.pos = reinterpret_cast<int*>(take((size_t)T * 4));
-  t.lse2 = reinterpret_cast<float*>(take((size_t)T * 4));
-  t.loss = reinterpret_cast<float*>(take((size_t)T * 4));
-  t.ids = reinterpret_cast<int*>(take((size_t)T * K * 4));
-  t.p = reinterpret_cast<float*>(take((size_t)T * K * 4));
-  t.z2 = reinterpret_cast<float*>(take((size_t)T * K * 4));
-  t.h = take((size_t)T * up(D, kPad) * (dtype == RR_F32 ? 4 : 2));
-  t.z = reinterpret_cast<float*>(take((size_t)T * z_words * 4));
-  if (z_words == 0) t.z = nullptr;
-  if (s != nullptr) *s = t;
-  return off;
-}
 
 // ------------------------------------------------------------------ plan
 struct Plan {
@@ -197,8 +176,32 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   return p;
 }
 
+size_t state_layout(const Plan& p, int64_t K, bool grad, char* base, State* s) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* at = base + off;
+    off += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  State t;
+  t.hdr = reinterpret_cast<Header*>(take(sizeof(Header)));
+  t.rows = reinterpret_cast<int*>(take((size_t)p.T * 4));
+  t.pos = reinterpret_cast<int*>(take((size_t)p.T * 4));
+  t.lse2 = reinterpret_cast<float*>(take((size_t)p.T * 4));
+  t.loss = reinterpret_cast<float*>(take((size_t)p.T * 4));
+  t.ids = reinterpret_cast<int*>(take((size_t)p.T * K * 4));
+  t.p = reinterpret_cast<float*>(take((size_t)p.T * K * 4));
+  t.z2 = reinterpret_cast<float*>(take((size_t)p.T * K * 4));
+  t.h = take((size_t)p.planes * p.T * p.Dp * p.eb);
+  t.w = take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * p.eb : 0);
+  const bool keep = grad && p.keep;
+  t.z = reinterpret_cast<float*>(take(keep ? (size_t)p.T * p.Vt * 4 : 0));
+  if (!keep) t.z = nullptr;
+  if (s != nullptr) *s = t;
+  return off;
+}
+
 struct FwdWs {
-  char* w;         // [planes][V][Dp] where the weight is copied
   float2* part;    // [word tiles][Tp] maximum and sum of a tile's row
   float* cut;      // [cuts][T][Vt] parts of the logits, where there are two or more
 };
@@ -210,14 +213,12 @@ size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
     return at;
   };
   FwdWs t;
-  t.w = take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * p.eb : 0);
   t.part = reinterpret_cast<float2*>(take((size_t)(p.Vt / kEdge) * p.Tp * sizeof(float2)));
   t.cut = reinterpret_cast<float*>(take(p.cuts > 1 ? (size_t)p.cuts * p.T * p.Vt * 4 : 0));
   if (s != nullptr) *s = t;
   return off;
 }
 struct BwdWs {
-  char* w;         // as forward
   float* scale;    // [0] the factor on both gradients
   float2* coef;    // [Tp] a row's factors (coef_kernel)
   char* dz;        // [planes_z][Tp][Vp]
@@ -232,7 +233,6 @@ size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
     return at;
   };
   BwdWs t;
-  t.w = take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * p.eb : 0);
   t.scale = reinterpret_cast<float*>(take(256));
   t.coef = reinterpret_cast<float2*>(take((size_t)p.Tp * sizeof(float2)));
   t.dz = take((size_t)p.planes_z * p.Tp * p.Vp * p.eb);
@@ -377,10 +377,13 @@ __device__ __forceinline__ void load8(const X* row, int c, int D, X (&v)[8]) {
   }
 }
 
-// Largest finite |x| of the rows (through `rows`, the first hdr->n of them, where given).
+// Largest finite |x| of the hidden states that count (blockIdx.y = 0) and of the weight (1).
 __global__ void __launch_bounds__(256)
-amax_kernel(const float* __restrict__ x, int64_t n_rows, int D, const int* rows, const Header* hdr, uint32_t* out) {
-  const int64_t n = rows != nullptr ? hdr->n : n_rows;
+amax_kernel(const float* __restrict__ hidden, const float* __restrict__ weight, int64_t V, int D, State st) {
+  const bool w = blockIdx.y == 1;
+  const float* x = w ? weight : hidden;
+  const int* rows = w ? nullptr : st.rows;
+  const int64_t n = w ? V : st.hdr->n;
   float m = 0.f;
   for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const float* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
@@ -395,19 +398,22 @@ amax_kernel(const float* __restrict__ x, int64_t n_rows, int D, const int* rows,
     }
   }
   m = wave_max(m);
-  if ((threadIdx.x & 63) == 0 && m > 0.f) atomicMax(out, __float_as_uint(m));
+  if ((threadIdx.x & 63) == 0 && m > 0.f) atomicMax(w ? &st.hdr->amax_w : &st.hdr->amax_h, __float_as_uint(m));
 }
 
-// Rows as operands: copied, or split into two planes (fp32 to fp16), padded with zeros to
-// Dp channels; through `rows` (the first hdr->n of them) where given.  plane: in bytes.
+// The hidden states that count (blockIdx.y = 0) and the weight (1) as operands: copied, or
+// split into two planes (fp32 to fp16), padded with zeros to Dp channels.
 template <typename X, typename Op>
 __global__ void __launch_bounds__(256)
-pack_kernel(const X* __restrict__ x, int64_t n_rows, int D, int Dp, const int* rows, const Header* hdr, int which,
-            char* __restrict__ out, int64_t plane) {
+pack_kernel(const X* __restrict__ hidden, const X* __restrict__ weight, int64_t T, int64_t V, int D, int Dp, State st) {
   constexpr bool SPLIT = sizeof(X) == 4 && __is_same(Op, OpF16);
-  const int64_t n = rows != nullptr ? hdr->n : n_rows;
+  const bool w = blockIdx.y == 1;
+  const X* x = w ? weight : hidden;
+  const int* rows = w ? nullptr : st.rows;
+  const int64_t n = w ? V : st.hdr->n, plane = (w ? V : T) * Dp * kBytes<Op>;
+  char* out = w ? st.w : st.h;
   float sc = 1.f;
-  if constexpr (SPLIT) sc = which == 0 ? scale_h(hdr) : scale_w(hdr);
+  if constexpr (SPLIT) sc = w ? scale_w(st.hdr) : scale_h(st.hdr);
   for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const X* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
     char* o = out + r * Dp * kBytes<Op>;
@@ -1060,17 +1066,9 @@ int check_dims(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int 
 }
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// The weight as an operand, where it is not one itself.
-template <typename X, typename Op>
-void pack_weight(const Plan& p, const void* weight, const State& st, char* w, hipStream_t s) {
-  if (!p.copy_w) return;
-  pack_kernel<X, Op><<<(unsigned)std::min<int64_t>(8192, p.V), 256, 0, s>>>(
-      static_cast<const X*>(weight), p.V, (int)p.D, (int)p.Dp, nullptr, st.hdr, 1, w, p.V * p.Dp * p.eb);
-}
-
-LogitArgs logit_args(const Plan& p, const State& st, const void* weight, char* w, int K, float tau) {
+LogitArgs logit_args(const Plan& p, const State& st, const void* weight, int K, float tau) {
   LogitArgs a{};
-  a.w = p.copy_w ? w : static_cast<const char*>(weight);
+  a.w = p.copy_w ? st.w : static_cast<const char*>(weight);
   a.h = st.h;
   a.ldw = (p.copy_w ? p.Dp : p.D) * p.eb, a.ldh = p.Dp * p.eb;
   a.plane_w = p.V * a.ldw, a.plane_h = p.T * a.ldh;
@@ -1110,14 +1108,15 @@ void launch_dw(DwArgs a, const Plan& p, int64_t cols, hipStream_t s) {
 template <typename X, typename Op, int PX>
 int forward(const Plan& p, const void* hidden, const void* weight, const State& st, const FwdWs& ws, int K, bool labels,
             float zl, float tau, int reduction, float* loss, hipStream_t s) {
+  const int64_t most = std::max(p.T, p.V);
   if constexpr (PX == 2) {
-    amax_kernel<<<1024, 256, 0, s>>>(static_cast<const float*>(hidden), p.T, (int)p.D, st.rows, st.hdr, &st.hdr->amax_h);
-    amax_kernel<<<2048, 256, 0, s>>>(static_cast<const float*>(weight), p.V, (int)p.D, nullptr, st.hdr, &st.hdr->amax_w);
+    amax_kernel<<<dim3((unsigned)std::min<int64_t>(2048, most), 2), 256, 0, s>>>(
+        static_cast<const float*>(hidden), static_cast<const float*>(weight), p.V, (int)p.D, st);
   }
-  pack_kernel<X, Op><<<(unsigned)std::min<int64_t>(8192, p.T), 256, 0, s>>>(
-      static_cast<const X*>(hidden), p.T, (int)p.D, (int)p.Dp, st.rows, st.hdr, 0, st.h, p.T * p.Dp * p.eb);
-  pack_weight<X, Op>(p, weight, st, ws.w, s);
-  LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
+  // the weight too where it is not an operand itself
+  pack_kernel<X, Op><<<dim3((unsigned)std::min<int64_t>(8192, p.copy_w ? most : p.T), p.copy_w ? 2 : 1), 256, 0, s>>>(
+      static_cast<const X*>(hidden), static_cast<const X*>(weight), p.T, p.V, (int)p.D, (int)p.Dp, st);
+  LogitArgs a = logit_args(p, st, weight, K, tau);
   a.part = ws.part;
   a.z = p.cuts > 1 ? ws.cut : st.z, a.ldzf = p.Vt, a.ldcut = p.T * p.Vt, a.cuts = (int)p.cuts;
   // (few rows are never split in planes, fp32 MFMA products never have many rows)
@@ -1143,12 +1142,11 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
 template <typename X, typename Op, int PX, int PZ>
 int backward(const Plan& p, const float* dloss, const void* weight, const State& st, const BwdWs& ws, int K, float zl,
              float tau, int reduction, void* dh, void* dw, hipStream_t s) {
-  if (dh != nullptr || !p.keep) pack_weight<X, Op>(p, weight, st, ws.w, s);
   coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, reduction == 1, tau, zl, __is_same(Op, OpF16), ws.coef,
                                  ws.scale);
   for (int64_t v = 0; v < p.Vt; v += p.Vp) {
     const int64_t cols = std::min(p.Vp, p.Vt - v);   // whole tiles
-    LogitArgs a = logit_args(p, st, weight, ws.w, K, tau);
+    LogitArgs a = logit_args(p, st, weight, K, tau);
     a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp * p.eb, a.plane_z = p.Tp * a.ldz, a.v_first = (int)v;
     constexpr bool kFew = __is_same(Op, OpF32) || (PX == 1 && PZ == 2);   // up to kFewRows, or kExactRows
     if (kFew || p.keep) {
@@ -1226,8 +1224,7 @@ int check_buffers(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, i
 // The caller's state: with the logits where it has room for them.
 void lay_out_state(int64_t T, int64_t D, int64_t V, int64_t K, int dtype, void* state, size_t bytes, State* st) {
   const bool grad = bytes >= rr_linear_loss_state_bytes(T, D, V, K, dtype, 1);
-  const Plan p = plan_of(T, D, V, dtype);
-  state_layout(T, D, K, dtype, grad && p.keep ? p.Vt : 0, static_cast<char*>(state), st);
+  state_layout(plan_of(T, D, V, dtype), K, grad, static_cast<char*>(state), st);
 }
 
 }  // namespace
@@ -1235,7 +1232,7 @@ void lay_out_state(int64_t T, int64_t D, int64_t V, int64_t K, int dtype, void* 
 extern "C" size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t V, int64_t K, int dtype, int grad) {
   if (rows <= 0 || check_dims("rr_linear_loss_state_bytes", rows, D, V, K, dtype, 0) != RR_OK) return 0;
   const Plan p = plan_of(rows, D, V, dtype);
-  return state_layout(rows, D, K, dtype, grad && p.keep ? p.Vt : 0, nullptr, nullptr);
+  return state_layout(p, K, grad != 0, nullptr, nullptr);
 }
 
 extern "C" size_t rr_linear_loss_workspace_bytes(int64_t rows, int64_t D, int64_t V, int dtype, int pass) {

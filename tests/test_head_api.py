@@ -194,7 +194,7 @@ def test_c_abi_refusals():
                                             (1, 5120, 131072, 1), (100_000, 64, 32000, 2)])
 def test_many_logits_are_not_held(rows, D, V, dtype):
     """The backward's workspace holds a piece of the logits' gradient, not all of it: beside the
-    copies of the inputs and dhidden's parts at most about 512 MiB, or 2048 columns of every row.
+    gradients' parts at most about 512 MiB, or 2048 columns of every row.
     The state holds the logits of up to 256 rows, of more where they take
     4 GiB at most."""
     lib, planes = _lib.load(), 2 if dtype == 0 else 1
@@ -202,10 +202,10 @@ def test_many_logits_are_not_held(rows, D, V, dtype):
     pieces = max(512 << 20, 2048 * rows_up * 2 * planes) + (256 * rows_up * 2 * planes)
     copies = planes * 2 * (rows + (V if dtype == 0 else 0)) * (D + 63) // 64 * 64
     parts = 64 * rows_up * ((D + 255) // 256 * 256) * 4
-    assert lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 1) <= pieces + copies + parts + (1 << 20)
-    assert lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 0) <= copies + 8 * rows_up * (V + 255) // 32 + (1 << 20)
+    assert lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 1) <= pieces + parts + (1 << 20)
+    assert lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 0) <= 8 * rows_up * (V + 255) // 32 + (1 << 20)
     state = [lib.rr_linear_loss_state_bytes(rows, D, V, 4, dtype, grad) for grad in (0, 1)]
-    assert state[0] <= rows * (copies // (rows + (V if dtype == 0 else 0)) + 4 * 4 + 3 * 4 * 4) + (1 << 20)
+    assert state[0] <= copies + rows * (4 * 4 + 3 * 4 * 4) + (1 << 20)   # K = 4 entries a row
     logits = rows * ((V + 255) // 256 * 256) * 4
     held = rows <= 256 or logits <= 4 << 30
     assert state[1] - state[0] in ((0, logits) if held else (0,))
