@@ -84,8 +84,10 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 // What the forward leaves for the backward, in one buffer of the caller's.
 struct Header {
   int n;                 // rows that count
-  uint32_t amax_h, amax_w;   // largest finite |hidden| (rows that count) and |weight|, as bits (fp32 inputs)
-  uint32_t pad[61];
+  uint32_t pad0[31];
+  uint32_t amax_h;       // largest finite |hidden| (rows that count) as bits (fp32 inputs)
+  uint32_t pad1[31];     // (a line of its own for each)
+  uint32_t amax_w;       // and |weight|
 };
 struct State {
   Header* hdr;
@@ -397,8 +399,15 @@ amax_kernel(const float* __restrict__ hidden, const float* __restrict__ weight, 
       }
     }
   }
+  __shared__ float buf[4];
   m = wave_max(m);
-  if ((threadIdx.x & 63) == 0 && m > 0.f) atomicMax(w ? &st.hdr->amax_w : &st.hdr->amax_h, __float_as_uint(m));
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  const uint32_t bits = __float_as_uint(fmaxf(fmaxf(buf[0], buf[1]), fmaxf(buf[2], buf[3])));
+  uint32_t* out = w ? &st.hdr->amax_w : &st.hdr->amax_h;
+  // an atomic a workgroup, and none where it changes nothing (4096 waves' took 40 us)
+  if (bits > __hip_atomic_load(out, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(out, bits);
 }
 
 // The hidden states that count (blockIdx.y = 0) and the weight (1) as operands: copied, or
@@ -695,6 +704,7 @@ __global__ void __launch_bounds__(256)
 join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, int V, int64_t Vt, int K, bool planes, float c,
             int64_t Tp, float2* __restrict__ part) {
   __shared__ float red[2][4];
+  __shared__ f32x4_t seg[kSeg / 4];
   const int t = blockIdx.x;
   if (t >= st.hdr->n) return;
   const int tid = threadIdx.x, v0 = blockIdx.y * kSeg, v = v0 + tid * 8;
@@ -722,20 +732,15 @@ join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, in
     *reinterpret_cast<f32x4_t*>(o) = f32x4_t{z[0], z[1], z[2], z[3]};
     *reinterpret_cast<f32x4_t*>(o + 4) = f32x4_t{z[4], z[5], z[6], z[7]};
   }
+  seg[2 * tid] = f32x4_t{z[0], z[1], z[2], z[3]}, seg[2 * tid + 1] = f32x4_t{z[4], z[5], z[6], z[7]};
   m = wave_max(m);
   if ((tid & 63) == 0) red[0][tid >> 6] = m;
-  const int orig = st.rows[t] * K;
-  const int* ids = st.ids + orig;
-  for (int k = first_entry(ids, K, v0); k < K; ++k) {
-    const int rel = ids[k] - v0;
-    if (rel >= kSeg) break;
-    if (rel >> 3 != tid) continue;
-    float x = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x = (rel & 7) == e ? z[e] : x;
-    st.z2[orig + k] = x;
-  }
   __syncthreads();
+  const int64_t orig = (int64_t)st.rows[t] * K;
+  for (int k = tid; k < K; k += 256) {
+    const int rel = st.ids[orig + k] - v0;
+    if (rel >= 0 && rel < kSeg) st.z2[orig + k] = reinterpret_cast<const float*>(seg)[rel];
+  }
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   if (m != -INFINITY) {
 #pragma unroll
@@ -761,26 +766,33 @@ dz_kernel(State st, const float2* __restrict__ coef, int V, int64_t Vt, int K, i
   const bool here = at < cols;   // both multiples of 8
   const float2 co = coef[t];
   const float l2 = st.lse2[t];
-  float z[8];
+  __shared__ f32x4_t seg[kSeg / 4];
   if (here) {
-    const float* i = st.z + (int64_t)t * Vt + v;
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(i), y = *reinterpret_cast<const f32x4_t*>(i + 4);
+    const f32x4_t* i = reinterpret_cast<const f32x4_t*>(st.z + (int64_t)t * Vt + v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) z[e] = exp2_fast(x[e] - l2), z[4 + e] = exp2_fast(y[e] - l2);
+    for (int q = 0; q < 2; ++q) {
+      const f32x4_t x = i[q];
+      seg[2 * tid + q] = f32x4_t{exp2_fast(x[0] - l2), exp2_fast(x[1] - l2), exp2_fast(x[2] - l2), exp2_fast(x[3] - l2)};
+    }
   }
-  const int orig = st.rows[t] * K;
+  __syncthreads();
+  const int64_t orig = (int64_t)st.rows[t] * K;
   const int* ids = st.ids + orig;
-  for (int k = first_entry(ids, K, v0); k < K; ++k) {
-    const int rel = ids[k] - v0;
-    if (rel >= kSeg) break;
-    if (rel >> 3 != tid) continue;
-    const float p = st.p[orig + k], r = p * co.y;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = (rel & 7) == e ? z[e] - p + r : z[e];
+  for (int k = tid; k < K; k += 256) {
+    const int id = ids[k], rel = id - v0;
+    if (rel < 0 || rel >= min(kSeg, cols - rel0) || (k > 0 && ids[k - 1] == id)) continue;
+    float q = reinterpret_cast<float*>(seg)[rel];
+    for (int j = k; j < K && ids[j] == id; ++j) {   // a word's entries
+      const float p = st.p[orig + j];
+      q = q - p + p * co.y;
+    }
+    reinterpret_cast<float*>(seg)[rel] = q;
   }
+  __syncthreads();
   if (!here) return;
+  float z[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) z[e] = v + e < V ? co.x * z[e] : 0.f;
+  for (int e = 0; e < 8; ++e) z[e] = v + e < V ? co.x * reinterpret_cast<const float*>(seg)[8 * tid + e] : 0.f;
   char* o = dz + t * ldz + (int64_t)at * kBytes<Op>;
   if constexpr (kBytes<Op> == 4) {
     reinterpret_cast<f32x4_t*>(o)[0] = f32x4_t{z[0], z[1], z[2], z[3]};
@@ -1110,7 +1122,7 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
             float zl, float tau, int reduction, float* loss, hipStream_t s) {
   const int64_t most = std::max(p.T, p.V);
   if constexpr (PX == 2) {
-    amax_kernel<<<dim3((unsigned)std::min<int64_t>(2048, most), 2), 256, 0, s>>>(
+    amax_kernel<<<dim3((unsigned)std::min<int64_t>(512, most), 2), 256, 0, s>>>(
         static_cast<const float*>(hidden), static_cast<const float*>(weight), p.V, (int)p.D, st);
   }
   // the weight too where it is not an operand itself
