@@ -140,6 +140,16 @@ struct Tile {
   }
 };
 
+// Bytes of a buffer that starts `skip` bytes into the first of `rows` rows and ends `inner`
+// bytes into the last: never negative, which the hardware would take for 4 GiB (a last step
+// may start behind the end of an only row).
+constexpr __host__ __device__ int buffer_bytes(int rows, int ld, int inner, int skip) {
+  const int b = rows <= 0 ? 0 : (rows - 1) * ld + inner - skip;
+  return b > 0 ? b : 0;
+}
+static_assert(buffer_bytes(1, 800, 800, 896) == 0 && buffer_bytes(2, 32, 32, 128) == 0 && buffer_bytes(0, 64, 64, 0) == 0 &&
+              buffer_bytes(3, 64, 64, 128) == 64, "a buffer ends with its operand");
+
 // The loads of one operand's tile by the WAVES waves of a workgroup.
 template <int ROWS, bool KMAJOR, int EB, int WAVES>
 struct Loader {
@@ -170,7 +180,7 @@ struct Loader {
   // past its end.
   __device__ __forceinline__ void step(int k, int64_t plane, i32x4_t& r, int& past) const {
     const int rows = KMAJOR ? min(outer - k, STEP) : min(outer, ROWS);
-    const int bytes = rows <= 0 ? 0 : (rows - 1) * ldb + (KMAJOR ? inner : inner - k * EB);
+    const int bytes = buffer_bytes(rows, ldb, inner, KMAJOR ? 0 : k * EB);
     const uint64_t b = reinterpret_cast<uint64_t>(at + plane);
     r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);
     r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xffff);
