@@ -10,12 +10,22 @@
 //   dh = dz w,  dw = dz^T h,  c the row's upstream gradient
 //
 // A label is a teacher with one entry of weight 1, so both run on the same
-// kernels.  The logits [rows, V] are never stored.  The forward forms them a tile
-// at a time and keeps each row's running maximum and sum per tile and the logits
-// of the row's entries.  The backward forms them again, a piece of the vocabulary
-// at a time, rounds that piece of dz to the operands' 16 bits (for fp32 inputs and
-// for few rows to two planes of them, below), and uses it for dw (complete for the
-// piece) and dh (added up over the pieces in fp32).
+// kernels.  The forward forms the logits a tile at a time and keeps each row's running
+// maximum and sum per tile and the logits of the row's entries; where that pays
+// (kKeepBytes and kKeepChannels below) it also leaves the logits themselves, in fp32.
+// The backward reads them, or forms them again, a piece of the vocabulary at a time,
+// rounds that piece of dz to the operands' 16 bits (for fp32 inputs and for few rows to
+// two planes of them, below), and uses it for dw (complete for the piece) and dh (added
+// up over the pieces in fp32).
+//
+// What bounds it: with many rows the products, two to four of 2 rows V D flops (8192 x
+// 65536 x 2560 bf16 forward and backward 7.45 ms, 1.1 PFLOP/s of the three it cannot do
+// without; a large product alone runs at 1.4); with few rows the weight's bytes, read
+// once forward and once backward and dw's written (16 x 65536 x 5120 bf16 forward 131 us, 5.1
+// TB/s, with the backward 545 us, 3.7 TB/s); below about 200 us the launches, 10 to 15.
+// Where a product has fewer tiles than CUs its sum is cut in parts that are joined by a
+// launch more (best_parts): the logits' over the channels, dh's over the words, dw's over the
+// rows (fp32, 209 rows of 3456 channels, 832 words, forward and backward: 543 us whole, 158 cut).
 //
 // Rows that count for nothing (an ignored label, no teacher entry) are left out
 // before the products: the rows that remain are gathered, in order, and their
@@ -63,6 +73,8 @@ constexpr int64_t kExactRows = 256;        // rows of fp32 that run on the fp32 
 // always kept: their product is a whole reading of the weight.
 constexpr int64_t kKeepBytes = (int64_t)4 << 30;
 constexpr int64_t kKeepChannels = 1024;
+constexpr int64_t kKeepChannels1 = 448;    // where the tiles are one round: 512 x 32000 x 768 159 us kept, 163 not,
+                                           // 1024 x 4096 x 512 103 and 110, 2048 x 8192 x 256 123 and 115
 constexpr int kPad = 64;                   // channels are padded to so many
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -160,7 +172,8 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   }
   const int64_t z_bytes = T * p.Vt * 4;
   p.keep = T <= kExactRows || p.cuts > 1 ||
-           (z_bytes <= kKeepBytes && D * (p.planes == 2 ? 3 : 1) >= kKeepChannels);
+           (z_bytes <= kKeepBytes &&
+            D * (p.planes == 2 ? 3 : 1) >= (p.Vt / kEdge * row_tiles <= kCus ? kKeepChannels1 : kKeepChannels));
   const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * p.eb * p.planes_z) / kEdge * kEdge));
   const int64_t pieces = (p.Vt + most - 1) / most;
   p.Vp = up((p.Vt + pieces - 1) / pieces, kEdge);
@@ -700,6 +713,9 @@ logits_kernel(LogitArgs a) {
 constexpr int kSeg = 2048;   // words of a row that a workgroup of the two kernels below takes, eight a thread
 
 // The parts of the logits added up: what kStats does for a tile, for a segment of a row.
+// Bound by the parts' bytes, or its launch.  The segment goes through LDS, so that an entry
+// is found by a thread of its own (each thread walking the row's 64 entries: 63 us at 3623 x
+// 865 words, 12 now).
 __global__ void __launch_bounds__(256)
 join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, int V, int64_t Vt, int K, bool planes, float c,
             int64_t Tp, float2* __restrict__ part) {
@@ -755,7 +771,8 @@ join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, in
   if (tid == 0) part[(int64_t)blockIdx.y * Tp + t] = make_float2(m, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
 }
 
-// dz from the logits that were kept: what kGrad does for a tile, for a segment of a row.
+// dz from the logits that were kept: what kGrad does for a tile, for a segment of a row (as
+// in join_kernel).  A word's entries are taken off in their order by the thread of the first.
 template <typename Op, int PZ>
 __global__ void __launch_bounds__(256)
 dz_kernel(State st, const float2* __restrict__ coef, int V, int64_t Vt, int K, int v_first, int cols, char* __restrict__ dz,
@@ -1210,9 +1227,8 @@ void zero(void* p, int64_t bytes, hipStream_t s) {
                                    bytes % 4 ? static_cast<uint16_t*>(p) + bytes / 2 - 1 : nullptr);
 }
 
-int run_forward(const char* who, const void* hidden, const void* weight, int dtype, int64_t T, int64_t D, int64_t V,
-                int64_t K, bool labels, float zl, float tau, int reduction, float* loss, const State& st, void* workspace,
-                size_t workspace_bytes, hipStream_t s) {
+int run_forward(const void* hidden, const void* weight, int dtype, int64_t T, int64_t D, int64_t V, int64_t K, bool labels,
+                float zl, float tau, int reduction, float* loss, const State& st, void* workspace, hipStream_t s) {
   const Plan p = plan_of(T, D, V, dtype);
   FwdWs ws;
   fwd_layout(p, static_cast<char*>(workspace), &ws);
@@ -1273,8 +1289,7 @@ extern "C" int rr_linear_ce_fwd(const void* hidden, const void* weight, int dtyp
   State in = st;
   if (reduction == 0) in.loss = loss;   // where rows that do not count leave their 0
   rows_kernel<true><<<1, 1024, 0, s>>>(labels, ignore_index, rows, (int)V, in);
-  return run_forward(who, hidden, weight, dtype, rows, D, V, 1, true, z_loss, 1.f, reduction, loss, st, workspace,
-                     workspace_bytes, s);
+  return run_forward(hidden, weight, dtype, rows, D, V, 1, true, z_loss, 1.f, reduction, loss, st, workspace, s);
 }
 
 extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
@@ -1309,8 +1324,7 @@ extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtyp
   State in = st;
   if (reduction == 0) in.loss = loss;
   rows_kernel<false><<<1, 1024, 0, s>>>(nullptr, 0, rows, (int)V, in);
-  return run_forward(who, hidden, weight, dtype, rows, D, V, K, false, 0.f, temperature, reduction, loss, st, workspace,
-                     workspace_bytes, s);
+  return run_forward(hidden, weight, dtype, rows, D, V, K, false, 0.f, temperature, reduction, loss, st, workspace, s);
 }
 
 extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D,

@@ -6,11 +6,12 @@ counterpart in the reference, which has the scans alone).
     linear_cross_entropy_reference, linear_distillation_reference      (plain torch)
 
 Both take the head's input and its weight in place of the logits ``hidden @
-weight.T``, which are formed tile by tile inside the kernels and never stored:
-for 8192 tokens and 65536 words the fp32 logits and their gradient would take
-4 GiB, the backward here works in pieces of half a GiB.  The products run on
-16-bit operands (fp32 inputs as two fp16 planes, to about fp32's accuracy) with
-fp32 accumulation; the loss is fp32.
+weight.T``, which are formed tile by tile inside the kernels.  Between forward and
+backward the logits of few rows, and where that is faster up to 4 GiB of them, stay in
+fp32; beyond that they are never stored, and the backward, whose gradient of the logits
+is a piece of half a GiB at a time, forms them again.  Without gradients none are kept.
+The products run on 16-bit operands with fp32 accumulation (fp32 inputs: up to 256
+rows in fp32, more as two fp16 planes, to about fp32's accuracy); the loss is fp32.
 """
 from __future__ import annotations
 
@@ -86,8 +87,8 @@ def _apply(hidden, weight, *args):
 
 
 def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, z_loss=0.0, reduction="mean"):
-    """Softmax cross entropy of ``hidden @ weight.T`` with `labels` on the GPU, without
-    storing the logits (fused forward + backward).
+    """Softmax cross entropy of ``hidden @ weight.T`` with `labels` on the GPU (fused
+    forward + backward).
 
     Per row, with ``z = hidden @ weight.T`` and ``lse = logsumexp(z)``::
 
@@ -119,8 +120,7 @@ def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, z_loss=0.
 
 
 def linear_distillation(hidden, weight, teacher_logits, teacher_ids, *, temperature=1.0, reduction="mean"):
-    """Distillation from a teacher's top logits on the GPU, without storing the
-    student's (fused forward + backward).
+    """Distillation from a teacher's top logits on the GPU (fused forward + backward).
 
     Per row, with p the softmax of ``teacher_logits / temperature`` over the row's
     entries and q that of ``hidden @ weight.T / temperature`` over the vocabulary::
