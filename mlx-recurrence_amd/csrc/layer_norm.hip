@@ -13,7 +13,7 @@
 //
 // A row belongs to TPR threads, eight consecutive elements per thread and step: a wave,
 // whose sums need no barrier, while its registers hold the row, else a workgroup.
-// Reached on an MI355X (a 2 GiB copy: 4.9 TB/s): 32768 x 2560 bf16 forward 4.5 TB/s,
+// Reached on an MI355X (a 2 GiB copy: 4.9 TB/s): 32768 x 2560 bf16 forward 4.8 TB/s,
 // backward 4.6 TB/s, the reduction of the parameters' gradients included; 1536 x 768
 // 5 and 11 us, one token 5 us, launches mostly.
 // Rows start at any element (odd D): the 16-byte accesses are made at the

@@ -72,7 +72,7 @@ constexpr int64_t kExactRows = 256;        // rows of fp32 that run on the fp32 
 // x 2560 7.6 and 8.9 ms.  (A product of planes costs three times as much.)  Few rows' are
 // always kept: their product is a whole reading of the weight.
 constexpr int64_t kKeepBytes = (int64_t)4 << 30;
-constexpr int64_t kKeepChannels = 1024;
+constexpr int64_t kKeepChannels = 896;
 constexpr int64_t kKeepChannels1 = 448;    // where the tiles are one round: 512 x 32000 x 768 159 us kept, 163 not,
                                            // 1024 x 4096 x 512 103 and 110, 2048 x 8192 x 256 123 and 115
 constexpr int kPad = 64;                   // channels are padded to so many
@@ -400,9 +400,11 @@ amax_kernel(const float* __restrict__ hidden, const float* __restrict__ weight, 
   const int* rows = w ? nullptr : st.rows;
   const int64_t n = w ? V : st.hdr->n;
   float m = 0.f;
-  for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < n; r += (int64_t)gridDim.x * 4) {   // a row a wave
     const float* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
-    for (int c = threadIdx.x * 8; c < D; c += 2048) {
+#pragma unroll 2
+    for (int c = lane * 8; c < D; c += 512) {
       float v[8];
       load8(xr, c, D, v);
 #pragma unroll
