@@ -4,7 +4,7 @@
 
 Embedding -> layer norm -> gated RG-LRU -> residual -> layer norm -> output head, whose losses
 (cross entropy on the next token, distillation from a teacher's top 16 logits) come straight
-from the hidden states: the logits are never stored.  The data are a random Markov chain and the
+from the hidden states.  The data are a random Markov chain and the
 teacher is the chain itself, so both losses have a known floor and fall towards it.  Needs an
 MI355X and the built library.
 """

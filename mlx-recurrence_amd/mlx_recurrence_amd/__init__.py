@@ -12,8 +12,8 @@ and, next to the scans, what a model of these layers ends in (no counterpart in
 the reference):
 
     norm         — layer norm
-    linear_loss  — cross entropy and distillation over a large vocabulary, from
-                   hidden states, without storing the logits
+    linear_loss  — cross entropy and distillation over a large vocabulary, straight
+                   from hidden states
 
 Each scan keeps the reference's signature, shape rules and fp32 state /
 accumulation, and is differentiable through ``torch.autograd``.  The compute
