@@ -52,7 +52,7 @@ SANITIZE_LINK = [arg for name in SANITIZERS for arg in ("-Xarch_host", "-fsaniti
 SANITIZE_FLAGS = [
     f"--offload-arch={ARCH}", "-O1", "-g", "-std=c++17", "-fPIC", "-Wno-unused-function",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    *SANITIZE_LINK, "-Xarch_host", "-fno-omit-frame-pointer", "-Xarch_device", "-O0",
+    *SANITIZE_LINK, "-Xarch_host", "-fno-omit-frame-pointer",
 ]
 
 
