@@ -92,6 +92,17 @@ constexpr int kEdge = 256;       // BM of all; buffers hold whole tiles
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
+// Parts of a caller's buffer, at multiples of 256 bytes (of none, where only its size is asked for).
+struct Carve {
+  char* base;
+  size_t off = 0;
+  char* operator()(size_t bytes) {
+    char* at = base == nullptr ? nullptr : base + off;
+    off += (bytes + 255) / 256 * 256;
+    return at;
+  }
+};
+
 // ------------------------------------------------------------------ state
 // What the forward leaves for the backward, in one buffer of the caller's.
 struct Header {
@@ -192,12 +203,7 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
 }
 
 size_t state_layout(const Plan& p, int64_t K, bool grad, char* base, State* s) {
-  size_t off = 0;
-  auto take = [&](size_t bytes) {
-    char* at = base + off;
-    off += (bytes + 255) / 256 * 256;
-    return at;
-  };
+  Carve take{base};
   State t;
   t.hdr = reinterpret_cast<Header*>(take(sizeof(Header)));
   t.rows = reinterpret_cast<int*>(take((size_t)p.T * 4));
@@ -213,7 +219,7 @@ size_t state_layout(const Plan& p, int64_t K, bool grad, char* base, State* s) {
   t.z = reinterpret_cast<float*>(take(keep ? (size_t)p.T * p.Vt * 4 : 0));
   if (!keep) t.z = nullptr;
   if (s != nullptr) *s = t;
-  return off;
+  return take.off;
 }
 
 struct FwdWs {
@@ -221,17 +227,12 @@ struct FwdWs {
   float* cut;      // [cuts][T][Vt] parts of the logits, where there are two or more
 };
 size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
-  size_t off = 0;
-  auto take = [&](size_t bytes) {
-    char* at = base + off;
-    off += (bytes + 255) / 256 * 256;
-    return at;
-  };
+  Carve take{base};
   FwdWs t;
   t.part = reinterpret_cast<float2*>(take((size_t)(p.Vt / kEdge) * p.Tp * sizeof(float2)));
   t.cut = reinterpret_cast<float*>(take(p.cuts > 1 ? (size_t)p.cuts * p.T * p.Vt * 4 : 0));
   if (s != nullptr) *s = t;
-  return off;
+  return take.off;
 }
 struct BwdWs {
   float* scale;    // [0] the factor on both gradients
@@ -241,12 +242,7 @@ struct BwdWs {
   float* dw;       // [cuts_w][Vp][Dt], where there are two or more
 };
 size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
-  size_t off = 0;
-  auto take = [&](size_t bytes) {
-    char* at = base + off;
-    off += (bytes + 255) / 256 * 256;
-    return at;
-  };
+  Carve take{base};
   BwdWs t;
   t.scale = reinterpret_cast<float*>(take(256));
   t.coef = reinterpret_cast<float2*>(take((size_t)p.Tp * sizeof(float2)));
@@ -254,7 +250,7 @@ size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
   t.dh = reinterpret_cast<float*>(take((size_t)p.splits * p.Tp * p.Dt * 4));
   t.dw = reinterpret_cast<float*>(take(p.cuts_w > 1 ? (size_t)p.cuts_w * p.Vp * p.Dt * 4 : 0));
   if (s != nullptr) *s = t;
-  return off;
+  return take.off;
 }
 
 // ------------------------------------------------------------------ rows and entries
