@@ -568,3 +568,33 @@ def test_graph_replays():
             assert torch.equal(a, e)
         for a, e in zip(step(), eager):
             assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,D,V", [(1, 8, 2), (20, 200, 257), (50, 3000, 300), (200, 100, 513), (300, 1000, 5003),
+                                      (700, 320, 4096), (3001, 200, 641)])
+def test_kernels_write_inside_their_buffers(rows, D, V, dtype, monkeypatch):
+    """State and workspaces of exactly the stated sizes between guards: nothing is written outside them, and
+    what they held before does not matter."""
+    buffers = []
+
+    def guarded(n, device):
+        whole = torch.full((n + 8192,), 0xA5, dtype=torch.uint8, device=device)
+        whole[4096:4096 + n] = 0xFF   # NaN as a float
+        buffers.append((whole, n))
+        return whole[4096:4096 + n]
+
+    g, h, w, labels = head_inputs(rows, D, V, dtype, rows + D + V)
+    labels[1::3] = -100
+    t, ids = teacher(g, rows, 9, V, labels.clamp(min=0))
+    up = torch.rand(rows, generator=g, device="cuda") + 0.1
+    want = (run_ce(h, w, labels, up, reduction="none"), run_kd(h, w, t, ids, up, reduction="none"))
+    monkeypatch.setattr(_lib, "autograd_ext", lambda: None)
+    monkeypatch.setattr(_lib, "_alloc_ws", guarded)
+    got = (run_ce(h, w, labels, up, reduction="none"), run_kd(h, w, t, ids, up, reduction="none"))
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+    assert len(buffers) == 6
+    for whole, n in buffers:
+        assert (whole[:4096] == 0xA5).all() and (whole[4096 + n:] == 0xA5).all()
