@@ -397,7 +397,7 @@ int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, c
  * leaves in `state` (16-byte aligned, rr_linear_loss_state_bytes) what
  * rr_linear_loss_bwd reads, the hidden states that count among it (the backward
  * needs `hidden` no more), and a copy of the weight where its rows are not whole
- * 16-byte pieces or fp32 is split; its contents are the library's own.  The logits
+ * 16-byte pieces; its contents are the library's own.  The logits
  * are among it for up to 256 rows, and for more where they take at most 4 GiB and reading
  * them costs less than their product.  grad = 0: the bytes that
  * a forward without a backward needs.  K: teacher entries a row, 1 to 1024; 1 for

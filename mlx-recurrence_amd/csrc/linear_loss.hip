@@ -14,8 +14,8 @@
 // maximum and sum per tile and the logits of the row's entries; where that pays
 // (kKeepBytes and kKeepChannels below) it also leaves the logits themselves, in fp32.
 // The backward reads them, or forms them again, a piece of the vocabulary at a time,
-// rounds that piece of dz to the operands' 16 bits (for fp32 inputs and for few rows to
-// two planes of them, below), and uses it for dw (complete for the piece) and dh (added
+// rounds that piece of dz to the operands' 16 bits (for few rows to two planes of them;
+// fp32 inputs: not at all), and uses it for dw (complete for the piece) and dh (added
 // up over the pieces in fp32).
 //
 // What bounds it: with many rows the products, two to four of 2 rows V D flops (8192 x
@@ -31,17 +31,15 @@
 // before the products: the rows that remain are gathered, in order, and their
 // number stays on the device.  What such a row's hidden state holds is not read.
 //
-// fp32 inputs are split into two fp16 planes, x s = hi + lo (s a power of two that
-// brings the largest finite value of the tensor just below 2^15; the pair holds 22
-// bits), and a product is the three of the planes that are not below the last bit:
-// about fp32's own accuracy at a third of the fp16 rate, above the fp32 MFMA's.  Making
-// the planes reads the weight twice and writes it once, which only many rows make up for:
-// up to kExactRows rows run on the fp32 MFMA, straight from the weight.
-// fp16 dz, and the planes of fp32's, carry a power of two that brings the largest
-// |dz| just below 2^14, so that small probabilities keep their bits; bf16 needs
-// none.
+// fp32 inputs run on the fp32 MFMA, at a ninth of the 16-bit rate, as they are: what a row, a
+// word or an upstream gradient gives does not depend on the sizes of the others.  (Two fp16
+// planes an operand, 22 bits below a power of two for the whole tensor, took half the time, but
+// hold nothing below 2^-40 of the largest value: one row 1e10 times the others' size put their
+// losses off by 0.1, and rare words' rows of dw had a few bits.)
+// fp16 dz carries a power of two that brings the largest |dz| just below 2^14, so that
+// small probabilities keep their bits; bf16 and fp32 need none.
 //
-// Everything is added up in a fixed order: no atomics but integer maxima.
+// Everything is added up in a fixed order, without atomics.
 #include "rr_common.h"
 #include "rr_gemm.h"
 #include "rr_mfma.h"
@@ -65,12 +63,13 @@ constexpr int64_t kPieceBytes = (int64_t)512 << 20;   // of dz, where the rows l
 constexpr int64_t kMinPiece = 2048;
 constexpr int64_t kMaxPiece = 1 << 20;       // a row of a tile's operand is at most so long
 constexpr int64_t kFewRows = 64;           // rows whose dz keeps a second plane
-constexpr int64_t kExactRows = 256;        // rows of fp32 that run on the fp32 MFMA
+constexpr int64_t kKeepRows = 256;         // rows whose logits are always kept
 // Logits are kept where they take no more than 4 GiB (of 288) and, with many rows, writing and
 // reading one costs less than its product: forward and backward of 1024 x 32000 in bf16 with 768,
 // 1024 and 2560 channels 267, 293 and 568 us kept, 266, 298 and 633 formed again; 8192 x 65536
-// x 2560 7.6 and 8.9 ms.  (A product of planes costs three times as much.)  Few rows' are
-// always kept: their product is a whole reading of the weight.
+// x 2560 7.6 and 8.9 ms.  fp32 products cost more, so theirs are kept from a twelfth of the
+// channels on: 1536 x 32000 with 64, 96 and 192 channels 588, 634 and 680 us kept, 583, 671 and
+// 762 formed again.  Few rows' are always kept: their product is a whole reading of the weight.
 constexpr int64_t kKeepBytes = (int64_t)4 << 30;
 constexpr int64_t kKeepChannels = 896;
 constexpr int64_t kKeepChannels1 = 448;    // where the tiles are one round: 512 x 32000 x 768 159 us kept, 163 not,
@@ -83,7 +82,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // where 256 x 256 leaves CUs without work (1536 x 32000 x 768 forward and backward:
 // 294 us, 301 to 307 with them).  Tile64 and Tile32 are for a few rows, whose products are
 // bound by the weight's bytes (two workgroups a CU): 16 x 65536 x 5120 forward 137 us, 156
-// with Tile256.
+// with Tile256.  fp32 has no tile above Tile64 but for dw: its products are slow enough to hide
+// the loads, and small tiles fill the last round (300 x 5003 x 1000 forward and backward 212
+// us, 274 with Tile256; 2048 x 32000 x 2048 5.86 and 5.77 ms).
 struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, THREADS = 512; };
 struct Tile64 { static constexpr int BM = 256, BN = 64, WM = 4, WN = 1, THREADS = 256; };
 struct Tile32 { static constexpr int BM = 256, BN = 32, WM = 4, WN = 1, THREADS = 256; };
@@ -107,10 +108,6 @@ struct Carve {
 // What the forward leaves for the backward, in one buffer of the caller's.
 struct Header {
   int n;                 // rows that count
-  uint32_t pad0[31];
-  uint32_t amax_h;       // largest finite |hidden| (rows that count) as bits (fp32 inputs)
-  uint32_t pad1[31];     // (a line of its own for each)
-  uint32_t amax_w;       // and |weight|
 };
 struct State {
   Header* hdr;
@@ -121,8 +118,8 @@ struct State {
   int* ids;      // [rows][K] the entries' columns, ascending; kAbsent past the last
   float* p;      // [rows][K] their weights
   float* z2;     // [rows][K] their logits, times log2(e) / tau
-  char* h;       // [planes][rows][Dp] the hidden states that count, as an operand
-  char* w;       // [planes][V][Dp] where the weight is copied
+  char* h;       // [rows][Dp] the hidden states that count, as an operand
+  char* w;       // [V][Dp] where the weight is copied
   float* z;      // [rows][Vt] their logits, times log2(e) / tau, where they are kept
 };
 
@@ -130,11 +127,10 @@ struct State {
 struct Plan {
   int64_t T, D, V;
   int dtype;
-  bool exact;          // fp32 on the fp32 MFMA
+  bool fp32;
   int eb;              // bytes of an operand's element
-  int planes;          // of the inputs: 2 for fp32 that is split
   int planes_z;        // of dz
-  bool copy_w;         // the weight is copied (planes, or rows that are not whole 16-byte chunks)
+  bool copy_w;         // the weight is copied: its rows are not whole 16-byte chunks
   int64_t Tp, Dp;      // rows to whole tiles, channels to whole k steps
   int64_t Vt, Dt;      // words and channels to whole tiles
   Tiles rows;          // tiles of the logits and dh (dw: Tile256; with Tile64 5 % slower at 16 to 256 rows)
@@ -161,14 +157,13 @@ int64_t best_parts(int64_t tiles, int64_t slots, double steps, double part, doub
 Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   Plan p{};
   p.T = T, p.D = D, p.V = V, p.dtype = dtype;
-  p.exact = dtype == RR_F32 && T <= kExactRows;
-  p.eb = p.exact ? 4 : 2;
-  p.planes = dtype == RR_F32 && !p.exact ? 2 : 1;
+  p.fp32 = dtype == RR_F32;
+  p.eb = p.fp32 ? 4 : 2;
   // The rounding of dz to 16 bits averages out over the rows of dw; few rows get a
   // second plane, which costs nothing there (the weight's bytes bound the products).
-  p.planes_z = !p.exact && (p.planes == 2 || T <= kFewRows) ? 2 : 1;
-  p.copy_w = p.planes == 2 || D * p.eb % 16 != 0;
-  p.rows = T <= Tile32::BN ? kTile32 : T <= Tile64::BN || p.exact ? kTile64 : kTile256;
+  p.planes_z = !p.fp32 && T <= kFewRows ? 2 : 1;
+  p.copy_w = D * p.eb % 16 != 0;
+  p.rows = T <= Tile32::BN ? kTile32 : T <= Tile64::BN || p.fp32 ? kTile64 : kTile256;
   p.Tp = p.rows == kTile32 ? Tile32::BN : up(T, kEdge), p.Dp = up(D, kPad);
   p.Vt = up(V, kEdge), p.Dt = up(D, kEdge);
   const int64_t slots = p.rows == kTile256 ? kCus : 2 * kCus;   // workgroups at one time
@@ -178,26 +173,25 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   // that of one launch more.
   {
     const int64_t all = p.Dp * p.eb / 128;
-    const double steps = (double)all * (p.planes == 2 ? 3 : 1), part = (double)(T * V * 8) / 4e12 / 1.4e-6;
-    p.cuts = best_parts(p.Vt / kEdge * row_tiles, slots, steps, part, 4., all);
+    const double part = (double)(T * V * 8) / 4e12 / 1.4e-6;
+    p.cuts = best_parts(p.Vt / kEdge * row_tiles, slots, (double)all, part, 4., all);
   }
   const int64_t z_bytes = T * p.Vt * 4;
-  p.keep = T <= kExactRows || p.cuts > 1 ||
+  p.keep = T <= kKeepRows || p.cuts > 1 ||
            (z_bytes <= kKeepBytes &&
-            D * (p.planes == 2 ? 3 : 1) >= (p.Vt / kEdge * row_tiles <= kCus ? kKeepChannels1 : kKeepChannels));
+            D * (p.fp32 ? 12 : 1) >= (p.Vt / kEdge * row_tiles <= kCus ? kKeepChannels1 : kKeepChannels));
   const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * p.eb * p.planes_z) / kEdge * kEdge));
   const int64_t pieces = (p.Vt + most - 1) / most;
   p.Vp = up((p.Vt + pieces - 1) / pieces, kEdge);
   // dh has few tiles: its sum over the piece's columns is cut in parts, as the logits' is.
   const int64_t all = p.Vp * p.eb / 128;
-  p.splits = best_parts(p.Dt / kEdge * row_tiles, slots, (double)(all * (p.planes + p.planes_z - 1)),
+  p.splits = best_parts(p.Dt / kEdge * row_tiles, slots, (double)(all * p.planes_z),
                         (double)(T * D * 8) / 4e12 / 1.4e-6, 0., all);
   // Few words and many rows: so is dw's sum over the rows (few rows are few steps).
   p.cuts_w = 1;
-  if (T > kExactRows) {
-    const int64_t rows = up(T, 64) / 64;
-    p.cuts_w = best_parts(p.Dt / kEdge * (p.Vp / kEdge), kCus, (double)(rows * (p.planes + p.planes_z - 1)),
-                          (double)(p.Vp * D * 8) / 4e12 / 1.4e-6, 4., rows);
+  if (T > kKeepRows) {
+    const int64_t steps = up(T * p.eb, 128) / 128;
+    p.cuts_w = best_parts(p.Dt / kEdge * (p.Vp / kEdge), kCus, (double)steps, (double)(p.Vp * D * 8) / 4e12 / 1.4e-6, 4., steps);
   }
   return p;
 }
@@ -213,8 +207,8 @@ size_t state_layout(const Plan& p, int64_t K, bool grad, char* base, State* s) {
   t.ids = reinterpret_cast<int*>(take((size_t)p.T * K * 4));
   t.p = reinterpret_cast<float*>(take((size_t)p.T * K * 4));
   t.z2 = reinterpret_cast<float*>(take((size_t)p.T * K * 4));
-  t.h = take((size_t)p.planes * p.T * p.Dp * p.eb);
-  t.w = take(p.copy_w ? (size_t)p.planes * p.V * p.Dp * p.eb : 0);
+  t.h = take((size_t)p.T * p.Dp * p.eb);
+  t.w = take(p.copy_w ? (size_t)p.V * p.Dp * p.eb : 0);
   const bool keep = grad && p.keep;
   t.z = reinterpret_cast<float*>(take(keep ? (size_t)p.T * p.Vt * 4 : 0));
   if (!keep) t.z = nullptr;
@@ -261,8 +255,6 @@ __device__ __forceinline__ float pow2_to(uint32_t amax_bits, int e) {
   const int x = (int)(amax_bits >> 23) - 127;   // floor(log2) of a normal value
   return ldexpf(1.f, max(-60, min(60, e - 1 - x)));
 }
-__device__ __forceinline__ float scale_h(const Header* h) { return pow2_to(h->amax_h, 15); }
-__device__ __forceinline__ float scale_w(const Header* h) { return pow2_to(h->amax_w, 15); }
 
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
@@ -370,7 +362,7 @@ rows_kernel(const int64_t* __restrict__ labels, int64_t ignore, int64_t T, int V
     }
     base += all;
   }
-  if (tid == 0) st.hdr->n = base, st.hdr->amax_h = 0, st.hdr->amax_w = 0;
+  if (tid == 0) st.hdr->n = base;
 }
 
 // Eight elements from column c of a row of D as they lie in memory, 0 past its end (a row
@@ -388,73 +380,25 @@ __device__ __forceinline__ void load8(const X* row, int c, int D, X (&v)[8]) {
   }
 }
 
-// Largest finite |x| of the hidden states that count (blockIdx.y = 0) and of the weight (1).
+// The hidden states that count (blockIdx.y = 0) and the weight (1) as operands: copied, padded
+// with zeros to Dp channels.
+template <typename X>
 __global__ void __launch_bounds__(256)
-amax_kernel(const float* __restrict__ hidden, const float* __restrict__ weight, int64_t V, int D, State st) {
-  const bool w = blockIdx.y == 1;
-  const float* x = w ? weight : hidden;
-  const int* rows = w ? nullptr : st.rows;
-  const int64_t n = w ? V : st.hdr->n;
-  float m = 0.f;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < n; r += (int64_t)gridDim.x * 4) {   // a row a wave
-    const float* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
-#pragma unroll 2
-    for (int c = lane * 8; c < D; c += 512) {
-      float v[8];
-      load8(xr, c, D, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = fabsf(v[e]);
-        if (a < INFINITY) m = fmaxf(m, a);   // neither infinite nor NaN
-      }
-    }
-  }
-  __shared__ float buf[4];
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  const uint32_t bits = __float_as_uint(fmaxf(fmaxf(buf[0], buf[1]), fmaxf(buf[2], buf[3])));
-  uint32_t* out = w ? &st.hdr->amax_w : &st.hdr->amax_h;
-  // an atomic a workgroup, and none where it changes nothing (4096 waves' took 40 us)
-  if (bits > __hip_atomic_load(out, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(out, bits);
-}
-
-// The hidden states that count (blockIdx.y = 0) and the weight (1) as operands: copied, or
-// split into two planes (fp32 to fp16), padded with zeros to Dp channels.
-template <typename X, typename Op>
-__global__ void __launch_bounds__(256)
-pack_kernel(const X* __restrict__ hidden, const X* __restrict__ weight, int64_t T, int64_t V, int D, int Dp, State st) {
-  constexpr bool SPLIT = sizeof(X) == 4 && __is_same(Op, OpF16);
+pack_kernel(const X* __restrict__ hidden, const X* __restrict__ weight, int64_t V, int D, int Dp, State st) {
   const bool w = blockIdx.y == 1;
   const X* x = w ? weight : hidden;
   const int* rows = w ? nullptr : st.rows;
-  const int64_t n = w ? V : st.hdr->n, plane = (w ? V : T) * Dp * kBytes<Op>;
-  char* out = w ? st.w : st.h;
-  float sc = 1.f;
-  if constexpr (SPLIT) sc = w ? scale_w(st.hdr) : scale_h(st.hdr);
+  const int64_t n = w ? V : st.hdr->n;
+  X* out = reinterpret_cast<X*>(w ? st.w : st.h);
   for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const X* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
-    char* o = out + r * Dp * kBytes<Op>;
     for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
       X v[8];
       load8(xr, c, D, v);
-      if constexpr (SPLIT) {
-        rr::u16x8_t hi, lo;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          hi[e] = op_bits<OpF16>(v[e] * sc);
-          lo[e] = op_bits<OpF16>(v[e] * sc - op_val<OpF16>(hi[e]));
-        }
-        *reinterpret_cast<rr::u16x8_t*>(o + c * 2) = hi;
-        *reinterpret_cast<rr::u16x8_t*>(o + plane + c * 2) = lo;
-      } else {
-        typedef uint32_t Words __attribute__((ext_vector_type(2 * sizeof(X))));
-        Words w;
-        __builtin_memcpy(&w, v, sizeof(w));
-        *reinterpret_cast<Words*>(o + c * sizeof(X)) = w;
-      }
+      typedef uint32_t Words __attribute__((ext_vector_type(2 * sizeof(X))));
+      Words q;
+      __builtin_memcpy(&q, v, sizeof(q));
+      *reinterpret_cast<Words*>(out + r * Dp + c) = q;
     }
   }
 }
@@ -464,7 +408,7 @@ pack_kernel(const X* __restrict__ hidden, const X* __restrict__ weight, int64_t 
 struct LogitArgs {
   const char* w;          // [V][ldw]
   const char* h;          // [n][Dp]
-  int64_t ldw, ldh, plane_w, plane_h;
+  int64_t ldw, ldh;
   int V, Dp, K, Tp, nvt;  // nvt: tiles of this launch
   float c;                // log2(e) / tau
   State st;
@@ -532,7 +476,7 @@ __device__ __forceinline__ void store_block(T* lds, int lane, F value, S store) 
 // kStats: the forward's maxima and sums, and the logits where they are kept; kCut: one part of
 // the sums, as it is; kGrad: the backward's dz.
 enum Mode { kStats, kCut, kGrad };
-template <typename C, typename Op, Mode MODE, int PX, int PZ>
+template <typename C, typename Op, Mode MODE, int PZ>
 __global__ void __launch_bounds__(C::THREADS, 2)
 logits_kernel(LogitArgs a) {
   constexpr bool GRAD = MODE == kGrad;
@@ -557,15 +501,15 @@ logits_kernel(LogitArgs a) {
   const int quarter = lane >> 4;
 
   typename P::Acc acc;
-  const Operand A{a.w + (int64_t)v0 * a.ldw, a.ldw, a.plane_w, a.V - v0, (int)a.ldw};
-  const Operand B{a.h + (int64_t)t0 * a.ldh, a.ldh, a.plane_h, n - t0, (int)a.ldh};
+  const Operand A{a.w + (int64_t)v0 * a.ldw, a.ldw, 0, a.V - v0, (int)a.ldw};
+  const Operand B{a.h + (int64_t)t0 * a.ldh, a.ldh, 0, n - t0, (int)a.ldh};
   // What the rows need, looked up while the first loads are under way.
   const int vw = v0 + wm * P::MW, left = a.V - vw;   // the wave's words, and how many there are
   int orig[P::NI];   // first of the row's entries
   int lo[P::NI];     // first of them in the wave's words
   float2 co[P::NI];
   float l2[P::NI];
-  P::template run<PX, PX>(acc, A, B, k0, k1, lds, [&] {
+  P::template run<1>(acc, A, B, k0, k1, lds, [&] {
     if constexpr (MODE == kCut) return;
 #pragma unroll
     for (int j = 0; j < P::NI; ++j) {
@@ -578,8 +522,6 @@ logits_kernel(LogitArgs a) {
       lo[j] = t0 + wn * P::NW + 16 * j + (lane & 15) < n ? first_entry(a.st.ids + orig[j], a.K, vw) : a.K;
   });
 
-  float c = a.c;
-  if constexpr (PX == 2) c /= scale_h(a.st.hdr) * scale_w(a.st.hdr);
   float* fstage = reinterpret_cast<float*>(lds) + wave * 16 * (P::MW + 4);
   float* red = reinterpret_cast<float*>(lds) + P::WAVES * 16 * (P::MW + 4);   // forward: [WM][BN][2]
   static_assert((P::WAVES * 16 * (P::MW + 4) + P::WM * BN * 2) * 4 <= P::LDS_BYTES, "a tile's results go through its LDS");
@@ -603,7 +545,7 @@ logits_kernel(LogitArgs a) {
 #pragma unroll
     for (int i = 0; i < P::MI; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][j][e] = rounded(acc[i][j][e] * c);
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = rounded(acc[i][j][e] * a.c);
     if (left < P::MW) {   // the vocabulary's last words
 #pragma unroll
       for (int i = 0; i < P::MI; ++i)
@@ -715,14 +657,13 @@ constexpr int kSeg = 2048;   // words of a row that a workgroup of the two kerne
 // is found by a thread of its own (each thread walking the row's 64 entries: 63 us at 3623 x
 // 865 words, 12 now).
 __global__ void __launch_bounds__(256)
-join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, int V, int64_t Vt, int K, bool planes, float c,
-            int64_t Tp, float2* __restrict__ part) {
+join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, int V, int64_t Vt, int K, float c, int64_t Tp,
+             float2* __restrict__ part) {
   __shared__ float red[2][4];
   __shared__ f32x4_t seg[kSeg / 4];
   const int t = blockIdx.x;
   if (t >= st.hdr->n) return;
   const int tid = threadIdx.x, v0 = blockIdx.y * kSeg, v = v0 + tid * 8;
-  if (planes) c /= scale_h(st.hdr) * scale_w(st.hdr);
   float z[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) z[e] = 0.f;
@@ -928,14 +869,14 @@ coef_kernel(State st, const float* __restrict__ dloss, bool per_row, bool mean, 
 struct DhArgs {
   const char* w;         // at the piece's first row
   const char* dz;
-  int64_t ldw, ldz, plane_w, plane_z;
+  int64_t ldw, ldz, plane_z;
   int V, Tp, ndt, splits, cols;   // V: rows of w from the piece on; cols: the piece's columns to whole k steps
   float* out;            // [splits][Tp][Dt]
   int Dt;
   bool first;
   State st;
 };
-template <typename C, typename Op, int PX, int PZ>
+template <typename C, typename Op, int PZ>
 __global__ void __launch_bounds__(C::THREADS, 2)
 dh_kernel(DhArgs a) {
   constexpr int BM = C::BM, BN = C::BN;
@@ -950,9 +891,9 @@ dh_kernel(DhArgs a) {
   const int steps = a.cols / P::BK;
   const int k0 = (int)((int64_t)steps * sp / a.splits) * P::BK, k1 = (int)((int64_t)steps * (sp + 1) / a.splits) * P::BK;
   typename P::Acc acc;
-  const Operand A{a.w + d0 * P::EB, a.ldw, a.plane_w, a.V, (int)a.ldw - d0 * P::EB};
+  const Operand A{a.w + d0 * P::EB, a.ldw, 0, a.V, (int)a.ldw - d0 * P::EB};
   const Operand B{a.dz + (int64_t)t0 * a.ldz, a.ldz, a.plane_z, a.Tp - t0, a.cols * P::EB};
-  P::template run<PX, PZ>(acc, A, B, k0, k1, lds);
+  P::template run<PZ>(acc, A, B, k0, k1, lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN, wn = wave % P::WN;
 #pragma unroll
@@ -982,8 +923,7 @@ sum_out_kernel(State st, const float* __restrict__ part, int D, int64_t ldp, int
   const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (c >= D) return;
   const int64_t t = DH ? st.pos[row] : row;
-  float f = scale[0];
-  if constexpr (sizeof(X) == 4) f /= DH ? scale_w(st.hdr) : scale_h(st.hdr);
+  const float f = scale[0];
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (t >= 0) {
     const float* at = part + t * ldp + c;   // ldp is whole tiles
@@ -1005,7 +945,7 @@ sum_out_kernel(State st, const float* __restrict__ part, int D, int64_t ldp, int
 struct DwArgs {
   const char* h;
   const char* dz;
-  int64_t ldh, ldz, plane_h, plane_z;
+  int64_t ldh, ldz, plane_z;
   int V, D, ndt;         // V: rows of dw from the piece on
   const float* scale;
   void* out;             // dw at the piece's first row
@@ -1014,7 +954,7 @@ struct DwArgs {
   int cuts;
   State st;
 };
-template <typename C, typename Op, typename X, int PX, int PZ, bool CUT>
+template <typename C, typename Op, typename X, int PZ, bool CUT>
 __global__ void __launch_bounds__(C::THREADS, 2)
 dw_kernel(DwArgs a) {
   constexpr int BM = C::BM, BN = C::BN;
@@ -1026,14 +966,14 @@ dw_kernel(DwArgs a) {
   tile_of(blockIdx.x - cut * tiles, a.ndt, tiles / a.ndt, dt, vt);
   const int d0 = dt * BM, v0 = vt * BN;
   typename P::Acc acc;
-  const Operand A{a.h + d0 * P::EB, a.ldh, a.plane_h, n, (int)a.ldh - d0 * P::EB};
+  const Operand A{a.h + d0 * P::EB, a.ldh, 0, n, (int)a.ldh - d0 * P::EB};
   const Operand B{a.dz + (int64_t)v0 * P::EB, a.ldz, a.plane_z, n, BN * P::EB};
   const int steps = (n + P::BK - 1) / P::BK;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN, wn = wave % P::WN;
   if constexpr (CUT) {
     const int k0 = (int)((int64_t)steps * cut / a.cuts) * P::BK, k1 = (int)((int64_t)steps * (cut + 1) / a.cuts) * P::BK;
-    P::template run<PX, PZ>(acc, A, B, k0, k1, lds);
+    P::template run<PZ>(acc, A, B, k0, k1, lds);
 #pragma unroll
     for (int j = 0; j < P::NI; ++j) {
       float* o = a.part + cut * a.ldcut + (int64_t)(v0 + wn * P::NW + 16 * j) * a.ldp + d0 + wm * P::MW;
@@ -1042,9 +982,8 @@ dw_kernel(DwArgs a) {
     }
     return;
   }
-  P::template run<PX, PZ>(acc, A, B, 0, steps * P::BK, lds);
-  float f = a.scale[0];
-  if constexpr (PX == 2) f /= scale_h(a.st.hdr);
+  P::template run<PZ>(acc, A, B, 0, steps * P::BK, lds);
+  const float f = a.scale[0];
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
     using Bits = typename std::conditional<sizeof(X) == 4, float, uint16_t>::type;   // of X
@@ -1098,67 +1037,57 @@ LogitArgs logit_args(const Plan& p, const State& st, const void* weight, int K, 
   a.w = p.copy_w ? st.w : static_cast<const char*>(weight);
   a.h = st.h;
   a.ldw = (p.copy_w ? p.Dp : p.D) * p.eb, a.ldh = p.Dp * p.eb;
-  a.plane_w = p.V * a.ldw, a.plane_h = p.T * a.ldh;
   a.V = (int)p.V, a.Dp = (int)p.Dp, a.K = K, a.Tp = (int)p.Tp;
   a.c = kLog2e / tau;
   a.st = st;
   return a;
 }
 // The logits of `cols` columns (whole tiles).
-template <typename C, typename Op, Mode MODE, int PX, int PZ>
+template <typename C, typename Op, Mode MODE, int PZ>
 void launch_logits(LogitArgs a, int64_t T, int64_t cols, hipStream_t s) {
   a.nvt = (int)(cols / C::BM);
-  logits_kernel<C, Op, MODE, PX, PZ><<<(unsigned)(a.nvt * (up(T, C::BN) / C::BN) * (MODE == kCut ? a.cuts : 1)), C::THREADS, 0, s>>>(a);
+  logits_kernel<C, Op, MODE, PZ><<<(unsigned)(a.nvt * (up(T, C::BN) / C::BN) * (MODE == kCut ? a.cuts : 1)), C::THREADS, 0, s>>>(a);
 }
 // The forward's, whole or in parts.
-template <typename C, typename Op, int PX>
+template <typename C, typename Op>
 void launch_forward(const LogitArgs& a, const Plan& p, hipStream_t s) {
-  if (p.cuts > 1) launch_logits<C, Op, kCut, PX, PX>(a, p.T, p.Vt, s);
-  else launch_logits<C, Op, kStats, PX, PX>(a, p.T, p.Vt, s);
+  if (p.cuts > 1) launch_logits<C, Op, kCut, 1>(a, p.T, p.Vt, s);
+  else launch_logits<C, Op, kStats, 1>(a, p.T, p.Vt, s);
 }
-template <typename C, typename Op, int PX, int PZ>
+template <typename C, typename Op, int PZ>
 void launch_dh(DhArgs a, const Plan& p, hipStream_t s) {
   a.ndt = (int)(up(p.D, C::BM) / C::BM);
-  dh_kernel<C, Op, PX, PZ><<<(unsigned)(a.ndt * (up(p.T, C::BN) / C::BN) * p.splits), C::THREADS, 0, s>>>(a);
+  dh_kernel<C, Op, PZ><<<(unsigned)(a.ndt * (up(p.T, C::BN) / C::BN) * p.splits), C::THREADS, 0, s>>>(a);
 }
-template <typename C, typename Op, typename X, int PX, int PZ, bool CUT>
+template <typename C, typename Op, typename X, int PZ, bool CUT>
 void launch_dw(DwArgs a, const Plan& p, int64_t cols, hipStream_t s) {
   a.ndt = (int)(up(p.D, C::BM) / C::BM);
   const unsigned tiles = (unsigned)(a.ndt * (cols / C::BN));
-  dw_kernel<C, Op, X, PX, PZ, CUT><<<CUT ? tiles * (unsigned)a.cuts : tiles, C::THREADS, 0, s>>>(a);
+  dw_kernel<C, Op, X, PZ, CUT><<<CUT ? tiles * (unsigned)a.cuts : tiles, C::THREADS, 0, s>>>(a);
   if constexpr (CUT) {
     sum_out_kernel<X, false><<<dim3((unsigned)std::min<int64_t>(cols, a.V), (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
         a.st, a.part, a.D, a.ldp, a.ldcut, a.cuts, a.scale, static_cast<X*>(a.out));
   }
 }
 
-template <typename X, typename Op, int PX>
+template <typename X, typename Op>
 int forward(const Plan& p, const void* hidden, const void* weight, const State& st, const FwdWs& ws, int K, bool labels,
             float zl, float tau, int reduction, float* loss, hipStream_t s) {
-  const int64_t most = std::max(p.T, p.V);
-  if constexpr (PX == 2) {
-    amax_kernel<<<dim3((unsigned)std::min<int64_t>(512, most), 2), 256, 0, s>>>(
-        static_cast<const float*>(hidden), static_cast<const float*>(weight), p.V, (int)p.D, st);
-  }
   // the weight too where it is not an operand itself
-  pack_kernel<X, Op><<<dim3((unsigned)std::min<int64_t>(8192, p.copy_w ? most : p.T), p.copy_w ? 2 : 1), 256, 0, s>>>(
-      static_cast<const X*>(hidden), static_cast<const X*>(weight), p.T, p.V, (int)p.D, (int)p.Dp, st);
+  const int64_t most = p.copy_w ? std::max(p.T, p.V) : p.T;
+  pack_kernel<X><<<dim3((unsigned)std::min<int64_t>(8192, most), p.copy_w ? 2 : 1), 256, 0, s>>>(
+      static_cast<const X*>(hidden), static_cast<const X*>(weight), p.V, (int)p.D, (int)p.Dp, st);
   LogitArgs a = logit_args(p, st, weight, K, tau);
   a.part = ws.part;
   a.z = p.cuts > 1 ? ws.cut : st.z, a.ldzf = p.Vt, a.ldcut = p.T * p.Vt, a.cuts = (int)p.cuts;
-  // (few rows are never split in planes, fp32 MFMA products never have many rows)
-  if constexpr (PX == 1) {
-    if (p.rows == kTile32) launch_forward<Tile32, Op, PX>(a, p, s);
-    else if (p.rows == kTile64) launch_forward<Tile64, Op, PX>(a, p, s);
-  }
-  if constexpr (!__is_same(Op, OpF32)) {
-    if (p.rows == kTile256) launch_forward<Tile256, Op, PX>(a, p, s);
-  }
+  if (p.rows == kTile32) launch_forward<Tile32, Op>(a, p, s);
+  else if (p.rows == kTile64) launch_forward<Tile64, Op>(a, p, s);
+  else if constexpr (!__is_same(Op, OpF32)) launch_forward<Tile256, Op>(a, p, s);
   int64_t parts = p.Vt / kEdge;
   if (p.cuts > 1) {
     parts = up(p.Vt, kSeg) / kSeg;
-    join_kernel<<<dim3((unsigned)p.T, (unsigned)parts), 256, 0, s>>>(st, ws.cut, a.cuts, a.ldcut, a.V, p.Vt, K, PX == 2, a.c,
-                                                                    p.Tp, ws.part);
+    join_kernel<<<dim3((unsigned)p.T, (unsigned)parts), 256, 0, s>>>(st, ws.cut, a.cuts, a.ldcut, a.V, p.Vt, K, a.c, p.Tp,
+                                                                    ws.part);
   }
   float* rows = reduction == 0 ? loss : st.loss;
   row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, K, labels, zl, tau, rows);
@@ -1166,7 +1095,7 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
   return rr::check_launch("rr_linear_loss");
 }
 
-template <typename X, typename Op, int PX, int PZ>
+template <typename X, typename Op, int PZ>
 int backward(const Plan& p, const float* dloss, const void* weight, const State& st, const BwdWs& ws, int K, float zl,
              float tau, int reduction, void* dh, void* dw, hipStream_t s) {
   coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, reduction == 1, tau, zl, __is_same(Op, OpF16), ws.coef,
@@ -1175,35 +1104,35 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
     const int64_t cols = std::min(p.Vp, p.Vt - v);   // whole tiles
     LogitArgs a = logit_args(p, st, weight, K, tau);
     a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp * p.eb, a.plane_z = p.Tp * a.ldz, a.v_first = (int)v;
-    constexpr bool kFew = __is_same(Op, OpF32) || (PX == 1 && PZ == 2);   // up to kFewRows, or kExactRows
+    constexpr bool kFp32 = __is_same(Op, OpF32), kFew = PZ == 2;   // up to kFewRows
     if (kFew || p.keep) {
       dz_kernel<Op, PZ><<<dim3((unsigned)p.T, (unsigned)(up(cols, kSeg) / kSeg)), 256, 0, s>>>(
           st, ws.coef, a.V, p.Vt, K, a.v_first, (int)cols, ws.dz, a.ldz, a.plane_z);
     } else if constexpr (!kFew) {
-      launch_logits<Tile256, Op, kGrad, PX, PZ>(a, p.T, cols, s);
+      launch_logits<typename std::conditional<kFp32, Tile64, Tile256>::type, Op, kGrad, PZ>(a, p.T, cols, s);
     }
     if (dh != nullptr) {
       DhArgs b{};
-      b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = a.ldz, b.plane_w = a.plane_w, b.plane_z = a.plane_z;
+      b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = a.ldz, b.plane_z = a.plane_z;
       b.V = (int)(p.V - v), b.Tp = a.Tp, b.splits = (int)p.splits, b.cols = (int)cols;
       b.out = ws.dh, b.Dt = (int)p.Dt, b.first = v == 0, b.st = st;
-      if constexpr (kFew) {
-        if (p.rows == kTile32) launch_dh<Tile32, Op, PX, PZ>(b, p, s);
-        else launch_dh<Tile64, Op, PX, PZ>(b, p, s);
+      if constexpr (kFew || kFp32) {
+        if (p.rows == kTile32) launch_dh<Tile32, Op, PZ>(b, p, s);
+        else launch_dh<Tile64, Op, PZ>(b, p, s);
       } else {
-        launch_dh<Tile256, Op, PX, PZ>(b, p, s);
+        launch_dh<Tile256, Op, PZ>(b, p, s);
       }
     }
     if (dw != nullptr) {
       DwArgs c{};
-      c.h = st.h, c.dz = ws.dz, c.ldh = a.ldh, c.ldz = a.ldz, c.plane_h = a.plane_h, c.plane_z = a.plane_z;
+      c.h = st.h, c.dz = ws.dz, c.ldh = a.ldh, c.ldz = a.ldz, c.plane_z = a.plane_z;
       c.V = (int)(p.V - v), c.D = (int)p.D, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
       c.part = ws.dw, c.ldp = p.Dt, c.ldcut = p.Vp * p.Dt, c.cuts = (int)p.cuts_w;
       if (kFew || p.cuts_w == 1) {
-        launch_dw<Tile256, Op, X, PX, PZ, false>(c, p, cols, s);
+        launch_dw<Tile256, Op, X, PZ, false>(c, p, cols, s);
       } else if constexpr (!kFew) {
-        launch_dw<Tile256, Op, X, PX, PZ, true>(c, p, cols, s);
+        launch_dw<Tile256, Op, X, PZ, true>(c, p, cols, s);
       }
     }
   }
@@ -1230,10 +1159,9 @@ int run_forward(const void* hidden, const void* weight, int dtype, int64_t T, in
   const Plan p = plan_of(T, D, V, dtype);
   FwdWs ws;
   fwd_layout(p, static_cast<char*>(workspace), &ws);
-  if (dtype == RR_BF16) return forward<bf16, OpBf16, 1>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
-  if (dtype == RR_F16) return forward<f16, OpF16, 1>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
-  if (p.exact) return forward<float, OpF32, 1>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
-  return forward<float, OpF16, 2>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
+  if (dtype == RR_BF16) return forward<bf16, OpBf16>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
+  if (dtype == RR_F16) return forward<f16, OpF16>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
+  return forward<float, OpF32>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
 }
 
 int check_buffers(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int dtype, int pass, const void* hidden,
@@ -1348,10 +1276,10 @@ extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dt
   lay_out_state(rows, D, V, K, dtype, const_cast<void*>(state), state_bytes, &st);
   BwdWs ws;
   bwd_layout(p, static_cast<char*>(workspace), &ws);
-#define LL_BACKWARD(X, OP, PX, PZ) \
-  backward<X, OP, PX, PZ>(p, dloss, weight, st, ws, (int)K, z_loss, temperature, reduction, dhidden, dweight, s)
-  if (dtype == RR_BF16) return p.planes_z == 2 ? LL_BACKWARD(bf16, OpBf16, 1, 2) : LL_BACKWARD(bf16, OpBf16, 1, 1);
-  if (dtype == RR_F16) return p.planes_z == 2 ? LL_BACKWARD(f16, OpF16, 1, 2) : LL_BACKWARD(f16, OpF16, 1, 1);
-  return p.exact ? LL_BACKWARD(float, OpF32, 1, 1) : LL_BACKWARD(float, OpF16, 2, 2);
+#define LL_BACKWARD(X, OP, PZ) \
+  backward<X, OP, PZ>(p, dloss, weight, st, ws, (int)K, z_loss, temperature, reduction, dhidden, dweight, s)
+  if (dtype == RR_BF16) return p.planes_z == 2 ? LL_BACKWARD(bf16, OpBf16, 2) : LL_BACKWARD(bf16, OpBf16, 1);
+  if (dtype == RR_F16) return p.planes_z == 2 ? LL_BACKWARD(f16, OpF16, 2) : LL_BACKWARD(f16, OpF16, 1);
+  return LL_BACKWARD(float, OpF32, 1);
 #undef LL_BACKWARD
 }

@@ -74,8 +74,8 @@ __device__ __forceinline__ float op_val(uint16_t b) {
 // One operand of a tile: element (outer o, inner i) at byte o * ld + i of p; outside
 // o < outer, i < inner it reads as 0.  k contiguous: o = the tile's row, i = k's byte;
 // k-major: o = k, i = the column's byte.  ld and inner are multiples of 16, p 16-byte
-// aligned.  `plane`: bytes from the high to the low plane of an operand that is split in
-// two.  ld <= 2^22, so that a tile spans at most 2^30 bytes.
+// aligned.  `plane`: bytes from the high to the low plane of a B that is split in two.
+// ld <= 2^22, so that a tile spans at most 2^30 bytes.
 struct Operand {
   const void* p;
   int64_t ld;
@@ -240,10 +240,9 @@ struct Product {
     }
   };
 
-  // k from k0 to k1 (multiples of BK).  PA, PB: the operands' planes; of two times
-  // two, the three products that are not below the last bit: hi hi, hi lo, lo hi.
+  // k from k0 to k1 (multiples of BK).  PB: planes of B, each multiplied by A.
   // meanwhile(): what is done while the first loads are under way.
-  template <int PA, int PB, typename F>
+  template <int PB, typename F>
   static __device__ __forceinline__ void run(Acc& acc, const Operand& a, const Operand& b, int k0, int k1, char* lds,
                                              F meanwhile) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -252,8 +251,7 @@ struct Product {
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    constexpr int SEGS = PA + PB - 1;   // products of planes, made step by step: what they share is read once
-    const int steps = (k1 - k0) / BK * SEGS;
+    const int steps = (k1 - k0) / BK * PB;   // the planes' products are made step by step
     if (steps <= 0) {
       meanwhile();
       return;
@@ -267,11 +265,11 @@ struct Product {
     int seg = 0, k = k0, loaded = 0;    // the step that is loaded next
     auto next_step = [&] {
       st.lds = base + (uint32_t)(loaded & 1) * STEP;
-      st.a.step(k, PA == 2 && seg >= PB ? a.plane : 0, st.ra, st.pa);
-      st.b.step(k, PB == 2 && seg == 1 ? b.plane : 0, st.rb, st.pb);
+      st.a.step(k, 0, st.ra, st.pa);
+      st.b.step(k, seg == 1 ? b.plane : 0, st.rb, st.pb);
       if (loaded >= steps) st.ra[2] = st.rb[2] = 0;   // behind the last step: loads of nothing (zeros)
       ++loaded;
-      if (SEGS > 1 && ++seg < SEGS) return;
+      if (PB > 1 && ++seg < PB) return;
       seg = 0, k += BK;
       st.a.advance();
       st.b.advance();
@@ -350,9 +348,9 @@ struct Product {
     loads_barrier();   // the LDS is free
   }
 
-  template <int PA, int PB>
+  template <int PB>
   static __device__ __forceinline__ void run(Acc& acc, const Operand& a, const Operand& b, int k0, int k1, char* lds) {
-    run<PA, PB>(acc, a, b, k0, k1, lds, [] {});
+    run<PB>(acc, a, b, k0, k1, lds, [] {});
   }
 };
 

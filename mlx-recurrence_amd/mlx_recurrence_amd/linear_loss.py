@@ -10,8 +10,7 @@ weight.T``, which are formed tile by tile inside the kernels.  Between forward a
 backward the logits of few rows, and where that is faster up to 4 GiB of them, stay in
 fp32; beyond that they are never stored, and the backward, whose gradient of the logits
 is a piece of half a GiB at a time, forms them again.  Without gradients none are kept.
-The products run on 16-bit operands with fp32 accumulation (fp32 inputs: up to 256
-rows in fp32, more as two fp16 planes, to about fp32's accuracy); the loss is fp32.
+The products run in the inputs' type with fp32 accumulation; the loss is fp32.
 """
 from __future__ import annotations
 

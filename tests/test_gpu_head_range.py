@@ -1,0 +1,133 @@
+"""Output head on the GPU over the range of its types: rows, words and upstream gradients of very different
+sizes in one call.  Every element is held to its own bound, from the sums that make it (in 64 bits, with
+absolute values), so that nothing large hides what is small.
+
+A sum of n products in fp32, in any order, is off by at most (n + 1) u S, with S the sum of the
+products' absolute values and u = 2^-24.  From that:
+  logits      E_t = (D + 16) u max_v S_tv         (16: the factor log2(e) and the exponentials, a few u each)
+  loss        2 E_t + 16 u |lse|                  (a logit, and the lse of logits so far off)
+  dhidden     (V + 16) u sum_v |dz||w| + 4 E_t sum_v |c| q |w|          (q is off by the factor exp(2 E_t),
+  dweight     (rows + 16) u sum_t |dz||h| + sum_t 4 E_t |c_t| q |h|      less than 1 + 4 E_t below E_t = 1 / 4)
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import mlx_recurrence_amd as mr
+from tests import head_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(shape, generator=g, device="cuda")
+
+
+def run_ce(h, w, labels, up, **kw):
+    h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = mr.linear_cross_entropy(h, w, labels, reduction="none", **kw)
+    return (loss.detach(), *torch.autograd.grad(loss, (h, w), up))
+
+
+def parts(h, w, labels, up):
+    """64-bit q, |dz| and each logit's sum of absolute products."""
+    h, w = h.double(), w.double()
+    q = torch.softmax(h @ w.T, 1)
+    dz = q.clone()
+    dz[torch.arange(len(h)), labels] -= 1
+    return q, (dz * up.double()[:, None]).abs(), h.abs() @ w.abs().T
+
+
+def check_fp32(got, h, w, labels, up, kw=None):
+    u = 2.0 ** -24
+    want = orc.cross_entropy(h, w, labels, up, reduction="none")
+    q, dz, s = parts(h, w, labels, up)
+    e = (h.shape[1] + 16) * u * s.max(1).values
+    qe = q * torch.where(e < 0.25, 4 * e, math.inf)[:, None] * up.double().abs()[:, None]
+    qe = torch.where(q > 0, qe, 0).nan_to_num(posinf=1e300)
+    lse = torch.logsumexp(h.double() @ w.double().T, 1)
+    bounds = (2 * e + 16 * u * lse.abs(),
+              (len(w) + 16) * u * (dz @ w.double().abs()) + qe @ w.double().abs(),
+              (len(h) + 16) * u * (dz.T @ h.double().abs()) + qe.T @ h.double().abs())
+    for name, a, b, most in zip(("loss", "dhidden", "dweight"), got, want, bounds):
+        assert bool(torch.isfinite(a).all()), f"{name}: not finite"
+        off = (a.double() - b).abs() / (most + 1e-35)
+        worst = float(off.max())
+        assert worst <= 1, f"{name}: {worst:.3g} times the bound at {tuple(int(i) for i in (off == worst).nonzero()[0])}"
+
+
+def head(rows, D, V, seed, dtype=F32):
+    g = gen(seed)
+    w = randn(g, V, D) * (2 / math.sqrt(D))
+    labels = torch.randint(0, V, (rows,), generator=g, device="cuda")
+    return (randn(g, rows, D) + 0.5 * w[labels]).to(dtype), w.to(dtype), labels
+
+
+# On either side of 256 rows; one more size where the logits are formed again.
+FP32_SIZES = [(200, 256, 2000), (300, 256, 2000), (700, 64, 1500)]
+
+
+@pytest.mark.parametrize("rows,D,V", FP32_SIZES)
+@pytest.mark.parametrize("size", [1.0, 1e8, 1e13])
+def test_fp32_one_large_row(rows, D, V, size):
+    h, w, labels = head(rows, D, V, 1)
+    h[0] *= size
+    up = torch.ones(rows, device="cuda")
+    check_fp32(run_ce(h, w, labels, up), h, w, labels, up)
+
+
+@pytest.mark.parametrize("rows,D,V", FP32_SIZES)
+@pytest.mark.parametrize("size", [1e4, 1e8, 1e13])
+def test_fp32_one_large_word(rows, D, V, size):
+    h, w, labels = head(rows, D, V, 2)
+    w[5] *= size
+    h[:, 0] = 1 / size
+    w[5, 1:] = 0   # its logits stay near 1, so every row has something of it
+    labels[labels == 5] = 6
+    up = torch.ones(rows, device="cuda")
+    check_fp32(run_ce(h, w, labels, up), h, w, labels, up)
+
+
+@pytest.mark.parametrize("rows,D,V", FP32_SIZES)
+def test_fp32_channels_of_other_sizes(rows, D, V):
+    """Channels large in the states and small in the weight: products near 1 of factors far apart."""
+    h, w, labels = head(rows, D, V, 3)
+    f = torch.exp2(torch.arange(D, device="cuda") % 7 * 10.0 - 30)
+    up = torch.ones(rows, device="cuda")
+    check_fp32(run_ce(h * f, w / f, labels, up), h * f, w / f, labels, up)
+
+
+@pytest.mark.parametrize("rows,D,V", FP32_SIZES)
+def test_fp32_rare_words(rows, D, V):
+    """Words of probability 1e-3 to 1e-18: their rows of dweight are as exact as any other."""
+    h, w, labels = head(rows, D, V, 4)
+    h[:, 0] = 4.0
+    w[:, 0] = -torch.arange(V, device="cuda") % 100 / 10.0
+    labels = labels // 100 * 100
+    up = torch.ones(rows, device="cuda")
+    check_fp32(run_ce(h, w, labels, up), h, w, labels, up)
+
+
+@pytest.mark.parametrize("rows,D,V", FP32_SIZES)
+def test_fp32_upstreams_of_other_sizes(rows, D, V):
+    h, w, labels = head(rows, D, V, 5)
+    up = torch.logspace(0, -20, rows, device="cuda")
+    check_fp32(run_ce(h, w, labels, up), h, w, labels, up)
+
+
+@pytest.mark.parametrize("rows", [120, 300])
+@pytest.mark.parametrize("scale_h,scale_w", [(1e-24, 1e24), (1e25, 1e-25), (1.0, 1e-30), (1e-30, 1.0)])
+def test_fp32_extreme_scales(rows, scale_h, scale_w):
+    h, w, labels = head(rows, 100, 600, 6)
+    h, w = h * scale_h, w * scale_w
+    up = torch.ones(rows, device="cuda")
+    check_fp32(run_ce(h, w, labels, up), h, w, labels, up)
