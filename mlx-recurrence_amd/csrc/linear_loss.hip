@@ -37,7 +37,9 @@
 // hold nothing below 2^-40 of the largest value: one row 1e10 times the others' size put their
 // losses off by 0.1, and rare words' rows of dw had a few bits.)
 // fp16 dz carries a power of two that brings the largest |dz| just below 2^14, so that
-// small probabilities keep their bits; bf16 and fp32 need none.
+// small probabilities keep their bits; bf16 and fp32 need none.  Where each row has an
+// upstream gradient of its own the power is the row's own too: dh's rows are divided by it
+// at the end, and dw reads the hidden states divided by it (a copy, for dw sums over rows).
 //
 // Everything is added up in a fixed order, without atomics.
 #include "rr_common.h"
@@ -118,6 +120,7 @@ struct State {
   int* ids;      // [rows][K] the entries' columns, ascending; kAbsent past the last
   float* p;      // [rows][K] their weights
   float* z2;     // [rows][K] their logits, times log2(e) / tau
+  float* amax;   // [rows] largest finite |hidden| of a row that counts (fp16)
   char* h;       // [rows][Dp] the hidden states that count, as an operand
   char* w;       // [V][Dp] where the weight is copied
   float* z;      // [rows][Vt] their logits, times log2(e) / tau, where they are kept
@@ -207,6 +210,7 @@ size_t state_layout(const Plan& p, int64_t K, bool grad, char* base, State* s) {
   t.ids = reinterpret_cast<int*>(take((size_t)p.T * K * 4));
   t.p = reinterpret_cast<float*>(take((size_t)p.T * K * 4));
   t.z2 = reinterpret_cast<float*>(take((size_t)p.T * K * 4));
+  t.amax = reinterpret_cast<float*>(take(p.dtype == RR_F16 ? (size_t)p.T * 4 : 0));
   t.h = take((size_t)p.T * p.Dp * p.eb);
   t.w = take(p.copy_w ? (size_t)p.V * p.Dp * p.eb : 0);
   const bool keep = grad && p.keep;
@@ -229,8 +233,10 @@ size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
   return take.off;
 }
 struct BwdWs {
-  float* scale;    // [0] the factor on both gradients
+  float* scale;    // the factors on dw and on dh
   float2* coef;    // [Tp] a row's factors (coef_kernel)
+  float* unscale;  // [Tp] the inverse of a row's power of two (fp16)
+  char* h;         // [T][Dp] the hidden states times that (fp16)
   char* dz;        // [planes_z][Tp][Vp]
   float* dh;       // [splits][Tp][Dt]
   float* dw;       // [cuts_w][Vp][Dt], where there are two or more
@@ -240,6 +246,8 @@ size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
   BwdWs t;
   t.scale = reinterpret_cast<float*>(take(256));
   t.coef = reinterpret_cast<float2*>(take((size_t)p.Tp * sizeof(float2)));
+  t.unscale = reinterpret_cast<float*>(take(p.dtype == RR_F16 ? (size_t)p.Tp * 4 : 0));
+  t.h = take(p.dtype == RR_F16 ? (size_t)p.T * p.Dp * p.eb : 0);
   t.dz = take((size_t)p.planes_z * p.Tp * p.Vp * p.eb);
   t.dh = reinterpret_cast<float*>(take((size_t)p.splits * p.Tp * p.Dt * 4));
   t.dw = reinterpret_cast<float*>(take(p.cuts_w > 1 ? (size_t)p.cuts_w * p.Vp * p.Dt * 4 : 0));
@@ -249,11 +257,11 @@ size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
 
 // ------------------------------------------------------------------ rows and entries
 // A power of two that brings a largest value of these bits into [2^(e - 1), 2^e)
-// (1 where there is none); kept within 2^+-60 so that products of two stay finite.
+// (1 where there is none), both it and its inverse a normal value.
 __device__ __forceinline__ float pow2_to(uint32_t amax_bits, int e) {
   if (amax_bits == 0) return 1.f;
   const int x = (int)(amax_bits >> 23) - 127;   // floor(log2) of a normal value
-  return ldexpf(1.f, max(-60, min(60, e - 1 - x)));
+  return ldexpf(1.f, max(-126, min(126, e - 1 - x)));
 }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -381,7 +389,7 @@ __device__ __forceinline__ void load8(const X* row, int c, int D, X (&v)[8]) {
 }
 
 // The hidden states that count (blockIdx.y = 0) and the weight (1) as operands: copied, padded
-// with zeros to Dp channels.
+// with zeros to Dp channels.  fp16: and the largest finite |hidden| of each row.
 template <typename X>
 __global__ void __launch_bounds__(256)
 pack_kernel(const X* __restrict__ hidden, const X* __restrict__ weight, int64_t V, int D, int Dp, State st) {
@@ -390,15 +398,32 @@ pack_kernel(const X* __restrict__ hidden, const X* __restrict__ weight, int64_t 
   const int* rows = w ? nullptr : st.rows;
   const int64_t n = w ? V : st.hdr->n;
   X* out = reinterpret_cast<X*>(w ? st.w : st.h);
+  __shared__ float buf[4];
   for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const X* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
+    float m = 0.f;
     for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
       X v[8];
       load8(xr, c, D, v);
+      if constexpr (__is_same(X, f16)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float a = fabsf(rr::to_f32(v[e]));
+          if (a < INFINITY) m = fmaxf(m, a);   // neither infinite nor NaN
+        }
+      }
       typedef uint32_t Words __attribute__((ext_vector_type(2 * sizeof(X))));
       Words q;
       __builtin_memcpy(&q, v, sizeof(q));
       *reinterpret_cast<Words*>(out + r * Dp + c) = q;
+    }
+    if constexpr (__is_same(X, f16)) {
+      if (w) continue;
+      m = wave_max(m);
+      __syncthreads();   // the last row's reads of buf are done
+      if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
+      __syncthreads();
+      if (threadIdx.x == 0) st.amax[r] = fmaxf(fmaxf(buf[0], buf[1]), fmaxf(buf[2], buf[3]));
     }
   }
 }
@@ -832,25 +857,35 @@ sum_loss_kernel(const float* __restrict__ loss, int64_t T, const Header* hdr, bo
 
 // ------------------------------------------------------------------ gradients
 // coef[t] = (c f, 1 - 1 / f) with f = 1 + 2 zl lse, so that a row of dz is
-// c f (q - p + p (1 - 1 / f)), and the factor on both gradients, scale[0].  One upstream
+// c f (q - p + p (1 - 1 / f)), and the factors on dw and dh, scale[0] and [1].  One upstream
 // gradient for all rows goes into that factor and c = 1: -1 at a label is exact in 16
 // bits, where -c would be off by the same rounding in every row.  Otherwise c is the
 // row's.  `scaled`: c carries the power of two that brings the largest of them below
-// 2^14, and the factor its inverse.  One workgroup.
+// 2^14, and the factors its inverse; or each row's own does, whose inverse is left in
+// unscale (0 where dz is 0), and dw's factor undoes that of the copy of the hidden states
+// (scale_h_kernel), which brings the largest of those below 2^15.  One workgroup.
 __global__ void __launch_bounds__(1024)
 coef_kernel(State st, const float* __restrict__ dloss, bool per_row, bool mean, float factor, float zl, bool scaled,
-            float2* __restrict__ coef, float* scale) {
+            float2* __restrict__ coef, float* __restrict__ unscale, float* scale) {
   __shared__ float buf[16];
   const int n = st.hdr->n;
+  const bool each = scaled && per_row;
   float m = 0.f;
   for (int t = threadIdx.x; t < n; t += 1024) {
     const float c = per_row ? dloss[st.rows[t]] * factor : 1.f;
     const float x = 2.f * zl * st.lse2[t] * kLn2;
     float f = 1.f + x;
     if (f == 0.f) f = 1e-30f;
-    coef[t] = make_float2(c * f, x / f);
     const float a = fmaxf(fabsf(c * f), fabsf(c));   // |dz| <= 2 a
-    if (a < INFINITY) m = fmaxf(m, a);
+    float sc = 1.f, v = a;
+    if (each) {
+      float un = 1.f;
+      if (a < INFINITY) sc = pow2_to(__float_as_uint(a), 14), un = a == 0.f ? 0.f : 1.f / sc;
+      unscale[t] = un;
+      v = st.amax[t] * un;
+    }
+    coef[t] = make_float2(c * f * sc, x / f);
+    if (v < INFINITY) m = fmaxf(m, v);
   }
   float sc = 1.f;
   if (scaled) {   // the same for the whole workgroup
@@ -859,10 +894,31 @@ coef_kernel(State st, const float* __restrict__ dloss, bool per_row, bool mean, 
     __syncthreads();
     m = 0.f;
     for (int w = 0; w < 16; ++w) m = fmaxf(m, buf[w]);
-    sc = pow2_to(__float_as_uint(m), 14);
-    for (int t = threadIdx.x; t < n; t += 1024) coef[t].x *= sc;   // this thread's own
+    sc = pow2_to(__float_as_uint(m), each ? 15 : 14);
+    if (!each)
+      for (int t = threadIdx.x; t < n; t += 1024) coef[t].x *= sc;   // this thread's own
   }
-  if (threadIdx.x == 0) scale[0] = (per_row ? 1.f : dloss[0] * factor * (mean ? 1.f / (float)max(1, n) : 1.f)) / sc;
+  if (threadIdx.x != 0) return;
+  const float f = per_row ? 1.f : dloss[0] * factor * (mean ? 1.f / (float)max(1, n) : 1.f);
+  scale[0] = f / sc, scale[1] = each ? f : f / sc;
+}
+
+// The hidden states divided by their rows' powers of two, times dw's (a row a workgroup).
+__global__ void __launch_bounds__(256)
+scale_h_kernel(State st, const float* __restrict__ unscale, const float* scale, int Dp, f16* __restrict__ out) {
+  const int t = blockIdx.x;
+  if (t >= st.hdr->n) return;
+  const float k = unscale[t] / scale[0];
+  const f16* h = reinterpret_cast<const f16*>(st.h) + (int64_t)t * Dp;
+  for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
+    f16 v[8];
+    load8(h, c, Dp, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = rr::from_f32<f16>(rr::to_f32(v[e]) * k);
+    rr::u16x8_t q;
+    __builtin_memcpy(&q, v, sizeof(q));
+    *reinterpret_cast<rr::u16x8_t*>(out + (int64_t)t * Dp + c) = q;
+  }
 }
 
 // dh^T tiles of one part of the piece: m = channels, n = rows, k = the piece's columns.
@@ -918,14 +974,14 @@ dh_kernel(DhArgs a) {
 template <typename X, bool DH>
 __global__ void __launch_bounds__(256)
 sum_out_kernel(State st, const float* __restrict__ part, int D, int64_t ldp, int64_t stride, int splits,
-               const float* scale, X* __restrict__ out) {
+               const float* scale, const float* unscale, X* __restrict__ out) {
   const int64_t row = blockIdx.x;
   const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (c >= D) return;
   const int64_t t = DH ? st.pos[row] : row;
-  const float f = scale[0];
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (t >= 0) {
+    const float f = scale[0] * (unscale != nullptr ? unscale[t] : 1.f);
     const float* at = part + t * ldp + c;   // ldp is whole tiles
 #pragma unroll 4
     for (int i = 0; i < splits; ++i) {
@@ -1066,7 +1122,7 @@ void launch_dw(DwArgs a, const Plan& p, int64_t cols, hipStream_t s) {
   dw_kernel<C, Op, X, PZ, CUT><<<CUT ? tiles * (unsigned)a.cuts : tiles, C::THREADS, 0, s>>>(a);
   if constexpr (CUT) {
     sum_out_kernel<X, false><<<dim3((unsigned)std::min<int64_t>(cols, a.V), (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
-        a.st, a.part, a.D, a.ldp, a.ldcut, a.cuts, a.scale, static_cast<X*>(a.out));
+        a.st, a.part, a.D, a.ldp, a.ldcut, a.cuts, a.scale, nullptr, static_cast<X*>(a.out));
   }
 }
 
@@ -1098,8 +1154,12 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
 template <typename X, typename Op, int PZ>
 int backward(const Plan& p, const float* dloss, const void* weight, const State& st, const BwdWs& ws, int K, float zl,
              float tau, int reduction, void* dh, void* dw, hipStream_t s) {
+  const bool each = __is_same(Op, OpF16) && reduction == 0;   // a power of two for each row's dz
   coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, reduction == 1, tau, zl, __is_same(Op, OpF16), ws.coef,
-                                 ws.scale);
+                                 ws.unscale, ws.scale);
+  if (each && dw != nullptr) {
+    scale_h_kernel<<<(unsigned)p.T, 256, 0, s>>>(st, ws.unscale, ws.scale, (int)p.Dp, reinterpret_cast<f16*>(ws.h));
+  }
   for (int64_t v = 0; v < p.Vt; v += p.Vp) {
     const int64_t cols = std::min(p.Vp, p.Vt - v);   // whole tiles
     LogitArgs a = logit_args(p, st, weight, K, tau);
@@ -1125,7 +1185,7 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
     }
     if (dw != nullptr) {
       DwArgs c{};
-      c.h = st.h, c.dz = ws.dz, c.ldh = a.ldh, c.ldz = a.ldz, c.plane_z = a.plane_z;
+      c.h = each ? ws.h : st.h, c.dz = ws.dz, c.ldh = a.ldh, c.ldz = a.ldz, c.plane_z = a.plane_z;
       c.V = (int)(p.V - v), c.D = (int)p.D, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
       c.part = ws.dw, c.ldp = p.Dt, c.ldcut = p.Vp * p.Dt, c.cuts = (int)p.cuts_w;
@@ -1138,7 +1198,7 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
   }
   if (dh != nullptr) {
     sum_out_kernel<X, true><<<dim3((unsigned)p.T, (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
-        st, ws.dh, (int)p.D, p.Dt, p.Tp * p.Dt, (int)p.splits, ws.scale, static_cast<X*>(dh));
+        st, ws.dh, (int)p.D, p.Dt, p.Tp * p.Dt, (int)p.splits, ws.scale + 1, each ? ws.unscale : nullptr, static_cast<X*>(dh));
   }
   return rr::check_launch("rr_linear_loss_bwd");
 }

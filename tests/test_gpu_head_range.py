@@ -131,3 +131,60 @@ def test_fp32_extreme_scales(rows, scale_h, scale_w):
     h, w = h * scale_h, w * scale_w
     up = torch.ones(rows, device="cuda")
     check_fp32(run_ce(h, w, labels, up), h, w, labels, up)
+
+
+# fp16 outputs, row by row in the 2-norm.  u = 2^-11 (half a unit in the last place), 2^-25 half of fp16's least step:
+#   dhidden  u |dh_t| + u sum_v |dz_tv| |w_v| + 2^-25 sqrt(D)         its rounding, that of dz, and what fp16 cannot hold
+#   dweight  u |dw_v| + 2 u sum_t |dz_tv| |h_t| + 2^-25 sqrt(D)       and that of a state times its row's power of two
+# and an eighth on top for the sums in fp32.
+def check_f16(got, h, w, dz, want):
+    u, (h, w) = 2.0 ** -11, (h.double(), w.double())
+    least = 2.0 ** -25 * math.sqrt(h.shape[1])
+    for name, a, b, terms in (("dhidden", got[1], want[1], dz @ w.norm(dim=1)), ("dweight", got[2], want[2], 2 * (dz.T @ h.norm(dim=1)))):
+        assert bool(torch.isfinite(a).all()), f"{name}: not finite"
+        off = (a.double() - b).norm(dim=1) / (1.125 * u * (b.norm(dim=1) + terms) + least)
+        assert float(off.max()) <= 1, f"{name}: {float(off.max()):.3g} times the bound in row {int(off.argmax())}"
+
+
+@pytest.mark.parametrize("rows,D,V", [(40, 64, 2000), (300, 64, 2000), (700, 200, 3000)])
+def test_fp16_upstreams_of_other_sizes(rows, D, V):
+    """Upstream gradients from 5e3 to 5e-5: the gradients of the smallest are still fp16's normal values."""
+    g = gen(7)
+    w = (2 * randn(g, V, D)).to(F16)
+    h = (0.05 * randn(g, rows, D)).to(F16)
+    labels = torch.randint(0, V, (rows,), generator=g, device="cuda")
+    up = torch.logspace(math.log10(5e3), math.log10(5e-5), rows, device="cuda")
+    _, dz, _ = parts(h, w, labels, up)
+    check_f16(run_ce(h, w, labels, up), h, w, dz, orc.cross_entropy(h, w, labels, up, reduction="none"))
+
+
+@pytest.mark.parametrize("rows,D,V", [(40, 64, 1000), (300, 64, 1000)])
+def test_fp16_words_of_rows_with_a_small_upstream(rows, D, V):
+    """Rows of a large upstream that are sure of their word leave the gradients of the others' words alone."""
+    g = gen(8)
+    w = randn(g, V, D).to(F16)
+    labels = torch.randint(0, V, (rows,), generator=g, device="cuda")
+    h = randn(g, rows, D)
+    h[::2] = 4 * w[labels[::2]].float()
+    h = h.to(F16)
+    up = torch.where(torch.arange(rows, device="cuda") % 2 == 0, 5e3, 1e-4)
+    _, dz, _ = parts(h, w, labels, up)
+    assert float(dz[::2].max()) < 1e-6 * float(dz[1::2].max())
+    check_f16(run_ce(h, w, labels, up), h, w, dz, orc.cross_entropy(h, w, labels, up, reduction="none"))
+
+
+@pytest.mark.parametrize("rows", [40, 300])
+def test_fp16_distillation_upstreams_of_other_sizes(rows):
+    g = gen(9)
+    w, h = (2 * randn(g, 1500, 72)).to(F16), (0.05 * randn(g, rows, 72)).to(F16)
+    t = 2 * randn(g, rows, 6)
+    ids = torch.stack([torch.randperm(1500, generator=g, device="cuda")[:6] for _ in range(rows)])
+    up = torch.logspace(math.log10(2e3), math.log10(5e-5), rows, device="cuda")
+    up[3] = 0
+    hl, wl = h.requires_grad_(True), w.requires_grad_(True)
+    loss = mr.linear_distillation(hl, wl, t, ids, temperature=2.0, reduction="none")
+    got = (loss, *torch.autograd.grad(loss, (hl, wl), up))
+    h, w = h.detach(), w.detach()
+    dz = 2 * up.double()[:, None] * (torch.softmax(h.double() @ w.double().T / 2, 1)
+                                     .scatter_add(1, ids, -torch.softmax(t.double() / 2, 1)))
+    check_f16(got, h, w, dz.abs(), orc.distillation(h, w, t, ids, up, tau=2.0, reduction="none"))
