@@ -423,7 +423,7 @@ int rr_linear_ce_fwd(const void* hidden, const void* weight, int dtype, int64_t 
  * entries and q that of z / temperature over the vocabulary,
  *   loss = temperature^2 * sum_k p_k (log p_k - log q[id_k]).
  * An entry with a negative id or a logit of -inf is absent; a row without entries
- * counts for nothing.  An id >= V makes the row's loss, and every gradient, NaN.
+ * counts for nothing.  Any other entry's id >= V makes the row's loss, and every gradient, NaN.
  * The teacher gets no gradient. */
 int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
                      const void* teacher_logits, int teacher_dtype, const int64_t* teacher_ids, int64_t K,

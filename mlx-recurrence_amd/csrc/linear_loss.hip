@@ -276,8 +276,8 @@ __device__ __forceinline__ float wave_add(float v) {
 }
 
 // A row's teacher entries by column (a wave per row): ids ascending, absent ones
-// (id < 0 or a logit of -inf) last, and their softmax weights.  An id past the
-// vocabulary makes the row's weights, and with them its loss and gradients, NaN.
+// (id < 0 or a logit of -inf) last, and their softmax weights.  The id of an entry past
+// the vocabulary makes the row's weights, and with them its loss and gradients, NaN.
 // pos[row] = 1 where the row has an entry.
 template <typename E>
 __global__ void __launch_bounds__(64)
@@ -295,8 +295,10 @@ entries_kernel(const E* __restrict__ logits, const int64_t* __restrict__ ids_in,
     if (k < K) {
       const int64_t raw = ids_in[row * K + k];
       const float x = rr::to_f32(logits[row * K + k]) * inv_tau;
-      if (raw >= V) worst = NAN;
-      if (raw >= 0 && raw < V && x != -INFINITY) i = (int)raw, v = x;
+      if (raw >= 0 && x != -INFINITY) {
+        if (raw < V) i = (int)raw, v = x;
+        else worst = NAN;
+      }
     }
     id[k] = i, t[k] = v;
   }

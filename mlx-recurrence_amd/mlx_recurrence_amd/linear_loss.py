@@ -132,8 +132,9 @@ def linear_distillation(hidden, weight, teacher_logits, teacher_ids, *, temperat
         teacher_logits: [..., K] the teacher's logits, K up to 1024, in any order.
         teacher_ids:    [..., K] their words, integers below V.  An entry with a negative
                         id or a logit of -inf is absent; a row without entries gives no
-                        loss and no gradient and is not counted by the mean.  An id of V
-                        or more makes the row's loss (and every gradient) NaN.
+                        loss and no gradient and is not counted by the mean.  Any other
+                        entry's id of V or more makes the row's loss (and every
+                        gradient) NaN.
         temperature:    of both softmaxes.
         reduction:      as for linear_cross_entropy.
 

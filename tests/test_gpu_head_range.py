@@ -188,3 +188,30 @@ def test_fp16_distillation_upstreams_of_other_sizes(rows):
     dz = 2 * up.double()[:, None] * (torch.softmax(h.double() @ w.double().T / 2, 1)
                                      .scatter_add(1, ids, -torch.softmax(t.double() / 2, 1)))
     check_f16(got, h, w, dz.abs(), orc.distillation(h, w, t, ids, up, tau=2.0, reduction="none"))
+
+
+def run_kd(h, w, t, ids, tau):
+    h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = mr.linear_distillation(h, w, t, ids, temperature=tau, reduction="none")
+    return (loss.detach(), *torch.autograd.grad(loss, (h, w), torch.ones_like(loss)))
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_absent_entries_may_have_any_id(dtype):
+    """A logit of -inf is no entry whatever its id, a negative id none whatever its logit."""
+    h, w, first = head(70, 40, 300, 10, dtype)
+    ids = first[:, None].repeat(1, 5)
+    ids[:, 1:] = (ids[:, 1:] + torch.arange(1, 5, device="cuda")) % 300
+    t = randn(gen(11), 70, 5)
+    t[::2, 3:], t[4] = -math.inf, -math.inf
+    gone = t == -math.inf
+    want = run_kd(h, w, t, ids.masked_fill(gone, -1), 1.5)
+    assert bool(torch.isfinite(want[0]).all()) and float(want[0][4]) == 0
+    for bad in (300, 1 << 20, 1 << 40, -(1 << 40)):
+        assert same(run_kd(h, w, t, ids.masked_fill(gone, bad), 1.5), want), bad
+    assert same(run_kd(h, w, t.masked_fill(gone, math.nan), ids.masked_fill(gone, -5), 1.5), want)
+    assert bool(torch.isnan(run_kd(h, w, t, torch.where(gone, ids, 300), 1.5)[0][0]))   # an entry that is there
