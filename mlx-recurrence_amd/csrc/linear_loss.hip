@@ -276,12 +276,13 @@ __device__ __forceinline__ float wave_add(float v) {
 }
 
 // A row's teacher entries by column (a wave per row): ids ascending, absent ones
-// (id < 0 or a logit of -inf) last, and their softmax weights.  The id of an entry past
+// (id < 0 or a logit of -inf) last, and their softmax weights: the temperature divides
+// differences of logits, which a large one of the type's range outlasts.  The id of an entry past
 // the vocabulary makes the row's weights, and with them its loss and gradients, NaN.
 // pos[row] = 1 where the row has an entry.
 template <typename E>
 __global__ void __launch_bounds__(64)
-entries_kernel(const E* __restrict__ logits, const int64_t* __restrict__ ids_in, int K, int KP, int V, float inv_tau,
+entries_kernel(const E* __restrict__ logits, const int64_t* __restrict__ ids_in, int K, int KP, int V, float tau,
                int* __restrict__ ids, float* __restrict__ p, int* __restrict__ pos) {
   extern __shared__ char sm[];
   int* id = reinterpret_cast<int*>(sm);
@@ -294,7 +295,7 @@ entries_kernel(const E* __restrict__ logits, const int64_t* __restrict__ ids_in,
     float v = -INFINITY;
     if (k < K) {
       const int64_t raw = ids_in[row * K + k];
-      const float x = rr::to_f32(logits[row * K + k]) * inv_tau;
+      const float x = rr::to_f32(logits[row * K + k]);
       if (raw >= 0 && x != -INFINITY) {
         if (raw < V) i = (int)raw, v = x;
         else worst = NAN;
@@ -322,11 +323,11 @@ entries_kernel(const E* __restrict__ logits, const int64_t* __restrict__ ids_in,
   const bool any = id[0] != kAbsent;
   float s = 0.f;
   for (int k = lane; k < K; k += 64)
-    if (id[k] != kAbsent) s += expf(t[k] - m);
+    if (id[k] != kAbsent) s += expf((t[k] - m) / tau);
   s = wave_add(s) + wave_add(worst);
   for (int k = lane; k < K; k += 64) {
     ids[row * K + k] = id[k];
-    p[row * K + k] = id[k] != kAbsent ? expf(t[k] - m) / s : s != s ? NAN : 0.f;
+    p[row * K + k] = id[k] != kAbsent ? expf((t[k] - m) / tau) / s : s != s ? NAN : 0.f;
   }
   if (lane == 0) pos[row] = any || s != s ? 1 : 0;
 }
@@ -1307,7 +1308,7 @@ extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtyp
   while (KP < K) KP *= 2;
   RR_DISPATCH_DTYPE(teacher_dtype, {
     entries_kernel<InT><<<(unsigned)rows, 64, (size_t)KP * 8, s>>>(static_cast<const InT*>(teacher_logits), teacher_ids, (int)K,
-                                                                  KP, (int)V, 1.f / temperature, st.ids, st.p, st.pos);
+                                                                  KP, (int)V, temperature, st.ids, st.p, st.pos);
   });
   State in = st;
   if (reduction == 0) in.loss = loss;

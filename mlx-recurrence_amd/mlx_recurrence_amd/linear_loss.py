@@ -185,8 +185,10 @@ def linear_distillation_reference(hidden, weight, teacher_logits, teacher_ids, *
     there = (teacher_ids >= 0) & (teacher_logits != -math.inf)
     valid = there.any(-1)
     z = _logits(hidden, weight, valid) / temperature
-    t = torch.where(there, teacher_logits.to(z.dtype) / temperature, -math.inf)
-    logp = torch.log_softmax(torch.where(valid[..., None], t, 0), -1)
+    t = torch.where(there, teacher_logits.to(z.dtype), -math.inf)
+    t = torch.where(valid[..., None], t, 0)
+    logp = torch.log_softmax((t - t.detach().amax(-1, keepdim=True)) / temperature, -1)
+    p = logp.exp()
     logq = z.gather(-1, torch.where(there, teacher_ids, 0).long()) - torch.logsumexp(z, -1, keepdim=True)
-    loss = (logp.exp() * (torch.where(there, logp, 0) - logq)).sum(-1)
+    loss = (p * (torch.where(p > 0, logp, 0) - logq)).sum(-1)
     return _reduce(temperature ** 2 * loss, valid, reduction)

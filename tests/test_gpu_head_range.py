@@ -215,3 +215,25 @@ def test_absent_entries_may_have_any_id(dtype):
         assert same(run_kd(h, w, t, ids.masked_fill(gone, bad), 1.5), want), bad
     assert same(run_kd(h, w, t.masked_fill(gone, math.nan), ids.masked_fill(gone, -5), 1.5), want)
     assert bool(torch.isnan(run_kd(h, w, t, torch.where(gone, ids, 300), 1.5)[0][0]))   # an entry that is there
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("tau", [0.25, 1.0, 4.0])
+def test_teacher_logits_of_the_largest_and_lowest_values(dtype, tau):
+    """The type's lowest value is an entry like any other, also divided by a temperature below 1: equal logits,
+    whatever they are, are an even split, and one far below another has weight 0."""
+    h, w, first = head(20, 40, 300, 12)
+    ids = torch.stack([first, (first + 7) % 300, (first + 50) % 300], 1)
+    t = torch.zeros(20, 3, device="cuda", dtype=dtype)
+    want = run_kd(h, w, t, ids, tau)
+    for value in (torch.finfo(dtype).min, torch.finfo(dtype).max, 1000.0):
+        assert same(run_kd(h, w, torch.full_like(t, value), ids, tau), want), value
+    one = t.clone()
+    one[:, 2] = -math.inf
+    for low in (torch.finfo(dtype).min, -6e4):
+        two = one.clone()
+        two[:, 2] = low
+        assert same(run_kd(h, w, two, ids, tau), run_kd(h, w, one, ids, tau)), low
+    one[:, 0], t[:, 0] = torch.finfo(dtype).max, torch.finfo(dtype).max
+    t[:, 1:], one[:, 1:] = torch.finfo(dtype).min, -math.inf
+    assert same(run_kd(h, w, t, ids, tau), run_kd(h, w, one, ids, tau))
