@@ -77,3 +77,5 @@ __all__ = [
     "linear_distillation",
     "linear_distillation_reference",
 ]
+
+__version__ = "0.3.0+gfx950"
