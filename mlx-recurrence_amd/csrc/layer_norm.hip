@@ -37,6 +37,10 @@ using rr::f16;
 
 constexpr int64_t kMaxChannels = 32768;   // 1024 threads, 4 steps of 8 elements
 constexpr int kPartRows = 512;            // partial rows of dw and db at most
+// Workgroups of a forward launch at most: HIP launches fewer than 2^32 threads.  (One launch whose
+// workgroups stride over the rows took 97 us in place of 68 at 32768 x 2560: the loop
+// keeps the weight and the bias in registers.)
+constexpr int64_t kMaxBlocks = 1 << 21;
 
 // Eight consecutive elements as they lie in memory (any alignment of T).
 template <typename T>
@@ -359,9 +363,15 @@ extern "C" int rr_layer_norm_fwd(const void* x, int x_dtype, const void* w, cons
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   const Shape sh = shape_of(D, false, x_dtype == RR_F32);
-  const int nb = (int)(sh.tpr == 64 ? (rows + 3) / 4 : rows);
-  LN_TYPES(LN_SHAPE(false, ln_fwd_kernel, nb, static_cast<const X*>(x), w, b, w_dtype, rows, (int)D, eps, static_cast<Y*>(y), mean,
-                    rstd))
+  const int64_t rpb = sh.tpr == 64 ? 4 : 1;
+  for (int64_t r = 0; r < rows; r += kMaxBlocks * rpb) {
+    const int64_t n = std::min(rows - r, kMaxBlocks * rpb);
+    float* const mean_r = mean == nullptr ? nullptr : mean + r;
+    float* const rstd_r = mean == nullptr ? nullptr : rstd + r;
+    const int nb = (int)((n + rpb - 1) / rpb);
+    LN_TYPES(LN_SHAPE(false, ln_fwd_kernel, nb, static_cast<const X*>(x) + r * D, w, b, w_dtype, n, (int)D, eps,
+                      static_cast<Y*>(y) + r * D, mean_r, rstd_r))
+  }
   return rr::check_launch("rr_layer_norm_fwd");
 }
 
