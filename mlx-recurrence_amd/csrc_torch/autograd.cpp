@@ -14,6 +14,7 @@
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include <cstdint>
 #include <string>
@@ -360,7 +361,11 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
 Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& w, const c10::optional<Tensor>& b, double eps, int64_t out) {
   const Tensor wt = opt(w), bt = opt(b);
   require_device({&x, &wt, &bt});
-  if (records({&x, &wt, &bt})) return LayerNormFn::apply(x, w, b, eps, out);
+  // (apply refuses tangents of forward-mode differentiation, which the call below would drop)
+  using torch::autograd::isFwGradDefined;
+  if (records({&x, &wt, &bt}) || isFwGradDefined(x) || isFwGradDefined(w) || isFwGradDefined(b)) {
+    return LayerNormFn::apply(x, w, b, eps, out);
+  }
   const at::DeviceGuard guard(x.device());
   return layer_norm_fwd(prep(x, x.scalar_type()), wt.defined() ? prep(wt, wt.scalar_type()) : wt,
                         bt.defined() ? prep(bt, bt.scalar_type()) : bt, eps, out, nullptr);

@@ -1,0 +1,50 @@
+"""What the output head does not offer (GPU): forward-mode differentiation is refused, by both
+bindings, never left out in silence."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwad
+
+import mlx_recurrence_amd as mr
+from mlx_recurrence_amd import _lib
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["cpp", "python"])
+def binding(request, monkeypatch):
+    assert _lib.autograd_ext() is not None
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "autograd_ext", lambda: None)
+
+
+def tensors():
+    g = torch.Generator(device="cuda").manual_seed(1)
+    return [torch.randn(s, generator=g, device="cuda") for s in ((12, 16), (16,), (16,), (30, 16))]
+
+
+LABELS = list(range(12))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad", [True, False])
+def test_layer_norm_refuses_forward_mode(which, grad, binding):
+    args = tensors()[:3]
+    with fwad.dual_level(), torch.set_grad_enabled(grad):
+        args[which] = fwad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="jvp"):
+            mr.layer_norm(*args)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_losses_refuse_forward_mode(which, binding):
+    x, _, _, w = tensors()
+    labels = torch.tensor(LABELS, device="cuda")
+    with fwad.dual_level():
+        args = [x, w]
+        args[which] = fwad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="jvp"):
+            mr.linear_cross_entropy(*args, labels)
+        with pytest.raises(RuntimeError, match="jvp"):
+            mr.linear_distillation(*args, x[:, :4], labels[:, None].repeat(1, 4))
