@@ -303,6 +303,12 @@ std::tuple<Tensor, Tensor> gla_scan(const Tensor& q, const Tensor& k, const Tens
 at::ScalarType dtype_of(int64_t code) {
   return code == RR_F32 ? at::kFloat : code == RR_BF16 ? at::kBFloat16 : at::kHalf;
 }
+// A backward that is itself recorded would give gradients that are constants to autograd
+// (mlx_recurrence_amd._lib.refuse_second_derivatives).
+void refuse_second_derivatives() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "mlx_recurrence_amd: the output head has no second derivatives "
+              "(a backward with create_graph=True)");
+}
 Tensor opt(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
 // x of one of the three input types; weight and bias, where given, of one type.
@@ -336,6 +342,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_second_derivatives();
     const variable_list s = ctx->get_saved_variables();
     const Tensor &x_ = s[0], &w_ = s[1], &stats = s[2];
     const at::DeviceGuard guard(x_.device());
@@ -408,6 +415,7 @@ struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_second_derivatives();
     const variable_list s = ctx->get_saved_variables();
     const Tensor &w_ = s[0], &state = s[1];
     const at::DeviceGuard guard(w_.device());

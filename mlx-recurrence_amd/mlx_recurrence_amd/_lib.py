@@ -519,6 +519,13 @@ def gdn_bwd(dy, dfinal, q, k, v, alpha, beta, h0, ckpt, seg, dq, dk, dv, dalpha,
 
 
 # ---------------------------------------------------------------- output head
+def refuse_second_derivatives():
+    """For a backward: one that is itself recorded would give gradients that are constants to autograd."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("mlx_recurrence_amd: the output head has no second derivatives "
+                           "(a backward with create_graph=True)")
+
+
 def layer_norm_fwd(x, w, b, w_dtype, rows, D, eps, y, mean, rstd):
     _check(load().rr_layer_norm_fwd(ptr(x), DTYPE_CODE[x.dtype], ptr(w), ptr(b), DTYPE_CODE[w_dtype], rows, D, eps, ptr(y),
                                     DTYPE_CODE[y.dtype], ptr(mean), ptr(rstd), stream_of(x)), "rr_layer_norm_fwd")

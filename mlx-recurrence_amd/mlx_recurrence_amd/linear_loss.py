@@ -49,6 +49,7 @@ class _LinearLoss(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dloss):
+        _lib.refuse_second_derivatives()
         w_, state = ctx.saved_tensors
         dh = w_.new_empty((ctx.args[0], w_.shape[1])) if ctx.needs_input_grad[0] else None
         dw = torch.empty_like(w_) if ctx.needs_input_grad[1] else None
@@ -106,7 +107,8 @@ def linear_cross_entropy(hidden, weight, labels, *, ignore_index=-100, z_loss=0.
                       "none".
 
     Returns:
-        loss:         fp32, a scalar or [...] for "none".  Gradients flow to hidden and weight.
+        loss:         fp32, a scalar or [...] for "none".  Gradients flow to hidden and weight
+                      (first derivatives only).
     """
     _check(hidden, weight, reduction)
     if tuple(labels.shape) != tuple(hidden.shape[:-1]):
@@ -140,7 +142,7 @@ def linear_distillation(hidden, weight, teacher_logits, teacher_ids, *, temperat
 
     Returns:
         loss:           fp32, a scalar or [...] for "none".  Gradients flow to hidden and
-                        weight, none to the teacher.
+                        weight (first derivatives only), none to the teacher.
     """
     _check(hidden, weight, reduction)
     lead = tuple(hidden.shape[:-1])

@@ -39,6 +39,7 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _lib.refuse_second_derivatives()
         x_, w_, mean, rstd = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         D = x_.shape[-1]
@@ -68,7 +69,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, out_dtype=None):
                    three input types.
 
     Returns:
-        y:         x's shape.  Gradients flow to x, weight and bias.
+        y:         x's shape.  Gradients flow to x, weight and bias (first derivatives only).
     """
     if x.ndim < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must be [..., D] with D > 0, got shape {tuple(x.shape)}")

@@ -1,4 +1,4 @@
-"""What the output head does not offer (GPU): forward-mode differentiation is refused, by both
+"""What the output head's gradients do not offer (GPU): forward-mode and second derivatives are refused, by both
 bindings, never left out in silence."""
 from __future__ import annotations
 
@@ -48,3 +48,19 @@ def test_losses_refuse_forward_mode(which, binding):
             mr.linear_cross_entropy(*args, labels)
         with pytest.raises(RuntimeError, match="jvp"):
             mr.linear_distillation(*args, x[:, :4], labels[:, None].repeat(1, 4))
+
+
+@pytest.mark.parametrize("op", ["norm", "ce", "kd"])
+def test_second_derivatives_are_refused(op, binding):
+    x, s, b, w = (t.requires_grad_(True) for t in tensors())
+    labels = torch.tensor(LABELS, device="cuda")
+    if op == "norm":
+        leaves, out = (x, s, b), mr.layer_norm(x, s, b).sin().sum()
+    elif op == "ce":
+        leaves, out = (x, w), mr.linear_cross_entropy(x, w, labels)
+    else:
+        leaves, out = (x, w), mr.linear_distillation(x, w, x[:, :4], labels[:, None].repeat(1, 4))
+    with pytest.raises(RuntimeError, match="no second derivatives"):
+        torch.autograd.grad(out, leaves, create_graph=True)
+    first = torch.autograd.grad(out, leaves, retain_graph=True)
+    assert all(bool(torch.isfinite(a).all()) and a.grad_fn is None for a in first)
