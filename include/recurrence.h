@@ -390,8 +390,7 @@ int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, c
                       const float* mean, const float* rstd, int64_t rows, int64_t D, void* dx, void* dw, void* db,
                       void* workspace, size_t workspace_bytes, void* stream);
 
-/* Losses on the logits hidden [rows, D] x weight [V, D]^T, which are not stored where
- * they are many:
+/* Losses on the logits hidden [rows, D] x weight [V, D]^T, which are formed tile by tile.
  * `reduction` 0 leaves a loss a row (loss [rows] fp32), 1 their mean over the rows
  * that count, 2 their sum (loss [1]; both 0 where no row counts).  The forward
  * leaves in `state` (16-byte aligned, rr_linear_loss_state_bytes) what
@@ -405,8 +404,12 @@ int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, c
 size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t V, int64_t K, int dtype, int grad);
 
 /* Workspace of the forward (pass = 0) or backward (pass = 1); 0 for invalid
- * arguments.  The backward's holds a piece of the logits' gradient: about
- * 512 MiB at most, and 2048 columns of the vocabulary at least. */
+ * arguments.  The forward's holds two floats a row and 256 words and, where tiles are
+ * few and their sums are made in parts, at most 256 MiB of those parts of the logits.
+ * The backward's holds a piece of the logits' gradient (512 MiB, or 2048 columns of the
+ * vocabulary where those are more), dhidden's sums in fp32 (once, or in parts of at most
+ * 256 MiB), at most 256 MiB of parts of dweight's, and for fp16 a copy of the hidden
+ * states that count. */
 size_t rr_linear_loss_workspace_bytes(int64_t rows, int64_t D, int64_t V, int dtype, int pass);
 
 /* Cross entropy: with z = hidden weight^T and lse = log sum exp z of a row,

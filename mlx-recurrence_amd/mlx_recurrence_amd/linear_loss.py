@@ -8,8 +8,9 @@ counterpart in the reference, which has the scans alone).
 Both take the head's input and its weight in place of the logits ``hidden @
 weight.T``, which are formed tile by tile inside the kernels.  Between forward and
 backward the logits of few rows, and where that is faster up to 4 GiB of them, stay in
-fp32; beyond that they are never stored, and the backward, whose gradient of the logits
-is a piece of half a GiB at a time, forms them again.  Without gradients none are kept.
+fp32; beyond that the backward, whose gradient of the logits is a piece of half a GiB at
+a time, forms them again.  Without gradients none are kept (a few tiles' logits may be
+summed from parts, of at most 256 MiB, during the call).
 The products run in the inputs' type with fp32 accumulation; the loss is fp32.
 """
 from __future__ import annotations

@@ -1,0 +1,63 @@
+"""What the losses hold in memory (CPU: the sizes that the library asks its caller for)."""
+import pytest
+
+from mlx_recurrence_amd import _lib
+
+F32, BF16, F16 = 0, 1, 2
+MIB = 1 << 20
+
+
+def up(a, b):
+    return (a + b - 1) // b * b
+
+
+def sizes(rows, D, V, dtype, K=1):
+    lib = _lib.load()
+    return (lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 0), lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 1),
+            *(lib.rr_linear_loss_state_bytes(rows, D, V, K, dtype, grad) for grad in (0, 1)))
+
+
+SHAPES = [(T, D, V) for T in (1, 16, 40, 100, 256, 300, 756, 3000, 8192, 32768, 262144) for D in (64, 768, 2560, 7429, 16384, 65536)
+          for V in (500, 5003, 32000, 65536, 141063, 262144) if T * D <= 1 << 31 and V * D <= 1 << 32]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_forward_workspace_holds_no_logits_beyond_256_mib(dtype):
+    """A maximum and a sum per row and 256 words, and where the sums are made in parts at most 256 MiB of those."""
+    for T, D, V in SHAPES:
+        stats = up(V, 256) // 256 * up(T, 256) * 8
+        assert sizes(T, D, V, dtype)[0] <= stats + 256 * MIB + 4096, (T, D, V)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_backward_workspace_holds_a_piece_of_the_gradient(dtype):
+    """A piece of the logits' gradient: 512 MiB, or 2048 words of every row where those are more (two planes for up to 64
+    rows of 16 bits).  Beside it fp32 sums of dhidden and, where dweight's are made in parts, of those: one copy, or
+    parts of at most 256 MiB.  fp16: a copy of the hidden states."""
+    size = 4 if dtype == F32 else 2
+    for T, D, V in SHAPES:
+        planes = 2 if dtype != F32 and T <= 64 else 1
+        rows = 32 if T <= 32 else up(T, 256)
+        piece = max(512 * MIB, 2048 * rows * size * planes)
+        sums = max(rows * up(D, 256) * 4, 256 * MIB) + 256 * MIB
+        copy = T * up(D, 64) * 2 if dtype == F16 else 0
+        got = sizes(T, D, V, dtype)[1]
+        assert got <= piece + sums + copy + rows * 16 + 4096, (T, D, V)
+        if rows * up(V, 256) * size * planes > piece + sums + MIB:   # less than the whole gradient
+            assert got - copy - rows * 16 < rows * up(V, 256) * size * planes, (T, D, V)
+
+
+# rows, D, V, dtype, whether the logits are kept for the backward
+@pytest.mark.parametrize("rows,D,V,dtype,kept", [
+    (1, 5120, 131072, BF16, True), (16, 5120, 65536, BF16, True), (256, 64, 65536, F16, True),   # few rows
+    (1536, 768, 32000, BF16, False), (1536, 768, 32000, F32, True), (8192, 2560, 65536, BF16, True),
+    (32768, 2560, 131072, BF16, False), (8192, 4096, 131328, F16, False),   # more than 4 GiB
+    (100_000, 64, 32000, F16, False), (8192, 64, 65536, F32, False), (777, 513, 10007, BF16, True),
+])
+def test_state_holds_the_logits_where_it_says(rows, D, V, dtype, kept):
+    state = sizes(rows, D, V, dtype, K=4)[2:]
+    size = 4 if dtype == F32 else 2
+    logits = rows * up(V, 256) * 4
+    assert state[1] - state[0] == (up(logits, 256) if kept else 0)
+    copies = (rows + (V if D * size % 16 else 0)) * up(D, 64) * size
+    assert state[0] <= copies + rows * (5 * 4 + 3 * 4 * 4) + 4096   # indices, lse, loss; four entries a row
