@@ -396,10 +396,12 @@ int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, c
  * leaves in `state` (16-byte aligned, rr_linear_loss_state_bytes) what
  * rr_linear_loss_bwd reads, the hidden states that count among it (the backward
  * needs `hidden` no more), and a copy of the weight where its rows are not whole
- * 16-byte pieces; its contents are the library's own.  The logits
- * are among it for up to 256 rows, and for more where they take at most 4 GiB and reading
- * them costs less than their product.  grad = 0: the bytes that
- * a forward without a backward needs.  K: teacher entries a row, 1 to 1024; 1 for
+ * 16-byte pieces; its contents are the library's own.  The logits are among it in fp32 for
+ * up to 256 rows and where their sums were made in parts (at most 128 MiB), and, where the
+ * buffer has room, for more rows if they take at most 4 GiB and reading them costs less than
+ * their product.  The bytes of a state: grad = 0 for a forward without a backward, 1 with that
+ * room, 2 without it (the backward forms the logits again).  A state is passed to the backward
+ * with the size that the forward was given.  K: teacher entries a row, 1 to 1024; 1 for
  * labels.  V <= 2^24, D <= 65536. */
 size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t V, int64_t K, int dtype, int grad);
 

@@ -12,7 +12,8 @@
 // A label is a teacher with one entry of weight 1, so both run on the same
 // kernels.  The forward forms the logits a tile at a time and keeps each row's running
 // maximum and sum per tile and the logits of the row's entries; where that pays
-// (kKeepBytes and kKeepChannels below) it also leaves the logits themselves, in fp32.
+// (kKeepBytes and kKeepChannels below) and the caller has room it also leaves the logits
+// themselves, in fp32.
 // The backward reads them, or forms them again, a piece of the vocabulary at a time,
 // rounds that piece of dz to the operands' 16 bits (for few rows to two planes of them;
 // fp32 inputs: not at all), and uses it for dw (complete for the piece) and dh (added
@@ -139,7 +140,8 @@ struct Plan {
   int64_t Vt, Dt;      // words and channels to whole tiles
   Tiles rows;          // tiles of the logits and dh (dw: Tile256; with Tile64 5 % slower at 16 to 256 rows)
   int64_t cuts;        // parts of the channels that the logits are added up in
-  bool keep;           // the forward leaves the logits for the backward
+  bool keep_few;       // the forward leaves the logits for the backward whatever the caller's room
+  bool keep;           // or where there is room
   // backward
   int64_t Vp;          // columns of a piece (whole tiles)
   int64_t splits;      // parts of a piece's columns that dh is added up in
@@ -184,7 +186,8 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
     p.cuts = best_parts(p.Vt / kEdge * row_tiles, slots, (double)all, part, 4., all, T * p.Vt * 4);
   }
   const int64_t z_bytes = T * p.Vt * 4;
-  p.keep = T <= kKeepRows || p.cuts > 1 ||
+  p.keep_few = T <= kKeepRows || p.cuts > 1;   // (parts are small, and summed once for both)
+  p.keep = p.keep_few ||
            (z_bytes <= kKeepBytes &&
             D * (p.fp32 ? 12 : 1) >= (p.Vt / kEdge * row_tiles <= kCus ? kKeepChannels1 : kKeepChannels));
   const int64_t most = std::min(kMaxPiece, std::max(kMinPiece, kPieceBytes / (p.Tp * p.eb * p.planes_z) / kEdge * kEdge));
@@ -204,7 +207,8 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   return p;
 }
 
-size_t state_layout(const Plan& p, int64_t K, bool grad, char* base, State* s) {
+// grad: 0 no backward, 1 logits where they are kept, 2 only those that always are.
+size_t state_layout(const Plan& p, int64_t K, int grad, char* base, State* s) {
   Carve take{base};
   State t;
   t.hdr = reinterpret_cast<Header*>(take(sizeof(Header)));
@@ -218,7 +222,7 @@ size_t state_layout(const Plan& p, int64_t K, bool grad, char* base, State* s) {
   t.amax = reinterpret_cast<float*>(take(p.dtype == RR_F16 ? (size_t)p.T * 4 : 0));
   t.h = take((size_t)p.T * p.Dp * p.eb);
   t.w = take(p.copy_w ? (size_t)p.V * p.Dp * p.eb : 0);
-  const bool keep = grad && p.keep;
+  const bool keep = grad == 1 ? p.keep : grad == 2 && p.keep_few;
   t.z = reinterpret_cast<float*>(take(keep ? (size_t)p.T * p.Vt * 4 : 0));
   if (!keep) t.z = nullptr;
   if (s != nullptr) *s = t;
@@ -1173,7 +1177,7 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
     LogitArgs a = logit_args(p, st, weight, K, tau);
     a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp * p.eb, a.plane_z = p.Tp * a.ldz, a.v_first = (int)v;
     constexpr bool kFp32 = __is_same(Op, OpF32), kFew = PZ == 2;   // up to kFewRows
-    if (kFew || p.keep) {
+    if (kFew || st.z != nullptr) {
       dz_kernel<Op, PZ><<<dim3((unsigned)p.T, (unsigned)(up(cols, kSeg) / kSeg)), 256, 0, s>>>(
           st, ws.coef, a.V, p.Vt, K, a.v_first, (int)cols, ws.dz, a.ldz, a.plane_z);
     } else if constexpr (!kFew) {
@@ -1237,24 +1241,25 @@ int check_buffers(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, i
   const std::string w(who);
   if ((pass == 0 && hidden == nullptr) || weight == nullptr || state == nullptr || ws == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
   if (!aligned16(hidden) || !aligned16(weight)) return rr::fail(RR_EINVAL, w + ": buffers must be 16-byte aligned");
-  if (state_bytes < rr_linear_loss_state_bytes(T, D, V, K, dtype, pass)) return rr::fail(RR_EWORKSPACE, w + ": state buffer too small");
+  if (state_bytes < rr_linear_loss_state_bytes(T, D, V, K, dtype, pass == 0 ? 0 : 2)) return rr::fail(RR_EWORKSPACE, w + ": state buffer too small");
   if (ws_bytes < rr_linear_loss_workspace_bytes(T, D, V, dtype, pass)) return rr::fail(RR_EWORKSPACE, w + ": workspace too small");
   if (!aligned16(state) || !aligned16(ws)) return rr::fail(RR_EWORKSPACE, w + ": state buffer or workspace misaligned");
   return RR_OK;
 }
 
-// The caller's state: with the logits where it has room for them.
+// The caller's state: with the logits that it has room for.
 void lay_out_state(int64_t T, int64_t D, int64_t V, int64_t K, int dtype, void* state, size_t bytes, State* st) {
-  const bool grad = bytes >= rr_linear_loss_state_bytes(T, D, V, K, dtype, 1);
-  state_layout(plan_of(T, D, V, dtype), K, grad, static_cast<char*>(state), st);
+  const Plan p = plan_of(T, D, V, dtype);
+  const int grad = bytes >= state_layout(p, K, 1, nullptr, nullptr) ? 1 : bytes >= state_layout(p, K, 2, nullptr, nullptr) ? 2 : 0;
+  state_layout(p, K, grad, static_cast<char*>(state), st);
 }
 
 }  // namespace
 
 extern "C" size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t V, int64_t K, int dtype, int grad) {
-  if (rows <= 0 || check_dims("rr_linear_loss_state_bytes", rows, D, V, K, dtype, 0) != RR_OK) return 0;
+  if (rows <= 0 || grad < 0 || grad > 2 || check_dims("rr_linear_loss_state_bytes", rows, D, V, K, dtype, 0) != RR_OK) return 0;
   const Plan p = plan_of(rows, D, V, dtype);
-  return state_layout(p, K, grad != 0, nullptr, nullptr);
+  return state_layout(p, K, grad, nullptr, nullptr);
 }
 
 extern "C" size_t rr_linear_loss_workspace_bytes(int64_t rows, int64_t D, int64_t V, int dtype, int pass) {

@@ -380,18 +380,19 @@ Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& w, const c10::op
 
 // ------------------------------------------------------------------ losses from hidden states
 // hidden [rows, D] and weight [V, D] of one type; labels [rows], or teacher logits and ids [rows, K].
+// grad: of rr_linear_loss_state_bytes.
 struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
                         const c10::optional<Tensor>& labels, const c10::optional<Tensor>& t_logits,
                         const c10::optional<Tensor>& t_ids, int64_t ignore, double zl, double tau, int64_t reduction,
-                        bool grad) {
+                        int64_t grad) {
     const at::DeviceGuard guard(hidden.device());
     const at::ScalarType dt = hidden.scalar_type();
     const Tensor h_ = prep(hidden, dt), w_ = prep(weight, dt);
     const int64_t rows = h_.size(0), D = h_.size(1), V = w_.size(0), K = t_ids.has_value() ? t_ids->size(1) : 1;
     const int dtc = dtype_code(dt);
     Tensor loss = reduction == 0 ? at::empty({rows}, h_.options().dtype(at::kFloat)) : at::empty({}, h_.options().dtype(at::kFloat));
-    const size_t sb = rr_linear_loss_state_bytes(rows, D, V, K, dtc, grad), wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 0);
+    const size_t sb = rr_linear_loss_state_bytes(rows, D, V, K, dtc, (int)grad), wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 0);
     const Tensor state = workspace(sb, h_.options()), ws = workspace(wsb, h_.options());
     if (t_ids.has_value()) {
       const at::ScalarType tdt = common_dtype({&*t_logits});
@@ -436,10 +437,9 @@ struct LinearLossFn : public torch::autograd::Function<LinearLossFn> {
 
 Tensor linear_loss(const Tensor& hidden, const Tensor& weight, const c10::optional<Tensor>& labels,
                    const c10::optional<Tensor>& t_logits, const c10::optional<Tensor>& t_ids, int64_t ignore, double zl,
-                   double tau, int64_t reduction) {
+                   double tau, int64_t reduction, int64_t grad) {
   const Tensor a = opt(labels), b = opt(t_logits), c = opt(t_ids);
   require_device({&hidden, &weight, &a, &b, &c});
-  const bool grad = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad());
   return LinearLossFn::apply(hidden, weight, labels, t_logits, t_ids, ignore, zl, tau, reduction, grad);
 }
 

@@ -540,8 +540,9 @@ def layer_norm_bwd(dy, x, w, w_dtype, mean, rstd, rows, D, dx, dw, db):
 
 
 def linear_loss_buffers(rows, D, V, K, dtype, device, grad):
-    """State (kept for the backward, where there is to be one) and workspace of a forward."""
-    state = _alloc_ws(_ws_bytes("rr_linear_loss_state_bytes", (rows, D, V, K, DTYPE_CODE[dtype], int(grad))), device)
+    """State (kept for the backward; grad: 0 without one, 1 with room for the logits, 2 without) and workspace
+    of a forward."""
+    state = _alloc_ws(_ws_bytes("rr_linear_loss_state_bytes", (rows, D, V, K, DTYPE_CODE[dtype], grad)), device)
     return state, _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[dtype], 0)), device)
 
 

@@ -61,3 +61,28 @@ def test_state_holds_the_logits_where_it_says(rows, D, V, dtype, kept):
     assert state[1] - state[0] == (up(logits, 256) if kept else 0)
     copies = (rows + (V if D * size % 16 else 0)) * up(D, 64) * size
     assert state[0] <= copies + rows * (5 * 4 + 3 * 4 * 4) + 4096   # indices, lse, loss; four entries a row
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_state_without_room_for_the_logits(dtype):
+    """grad = 2: the logits of up to 256 rows and of sums made in parts (128 MiB at most), no others."""
+    lib = _lib.load()
+    for T, D, V in SHAPES:
+        without, small, full = (lib.rr_linear_loss_state_bytes(T, D, V, 1, dtype, grad) for grad in (0, 2, 1))
+        logits = up(T * up(V, 256) * 4, 256)
+        assert without <= small <= full and small - without in (0, logits)
+        if T <= 256:
+            assert small == full == without + logits
+        else:
+            assert small == without or logits <= 128 * MIB, (T, D, V)
+    assert lib.rr_linear_loss_state_bytes(8, 8, 8, 1, dtype, 3) == 0 == lib.rr_linear_loss_state_bytes(8, 8, 8, 1, dtype, -1)
+
+
+def test_backward_takes_a_state_of_either_size():
+    """Refusals by the state's size (found before any work is enqueued: no pointer is read)."""
+    lib, p = _lib.load(), 16
+    for rows, D, V in ((8192, 2560, 65536), (4, 8, 10)):
+        size = [lib.rr_linear_loss_state_bytes(rows, D, V, 1, 1, grad) for grad in (0, 1, 2)]
+        run = lambda n: lib.rr_linear_loss_bwd(p, p, 1, rows, D, V, 1, 0.0, 1.0, 1, p, n, None, None, p, 1 << 40, None)  # noqa: E731,E501
+        assert run(size[1]) == run(size[2]) == _lib.RR_OK
+        assert run(size[2] - 1) == _lib.RR_EWORKSPACE
