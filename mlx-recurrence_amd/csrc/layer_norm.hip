@@ -311,8 +311,8 @@ constexpr bool reached(bool bwd, bool fp32, int tpr, int nv) {
 }
 // Workgroups of the backward: two rows a wave (or workgroup) where that leaves fewer than
 // kPartRows partial rows.
-int64_t bwd_blocks(int64_t rows, int64_t D) {
-  const int64_t rpb = D <= 64 * 8 * wave_pieces(true, false) ? 8 : 2;
+int64_t bwd_blocks(int64_t rows, int64_t D, bool fp32) {
+  const int64_t rpb = shape_of(D, true, fp32).tpr == 64 ? 8 : 2;
   return std::max<int64_t>(1, std::min<int64_t>(kPartRows, (rows + rpb - 1) / rpb));
 }
 
@@ -377,7 +377,7 @@ extern "C" int rr_layer_norm_fwd(const void* x, int x_dtype, const void* w, cons
 
 extern "C" size_t rr_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t D) {
   if (rows <= 0 || D <= 0 || D > kMaxChannels) return 0;
-  return (size_t)bwd_blocks(rows, D) * 2 * (size_t)D * sizeof(float);
+  return (size_t)bwd_blocks(rows, D, true) * 2 * (size_t)D * sizeof(float);   // fp32's, at least those of 16 bits
 }
 
 extern "C" int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, const void* w, int w_dtype,
@@ -386,7 +386,7 @@ extern "C" int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int
   if (int rc = check_args("rr_layer_norm_bwd", rows, D, x_dtype, y_dtype, w_dtype)) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool params = dw != nullptr || db != nullptr;
-  const int64_t nb = rows == 0 ? 0 : bwd_blocks(rows, D);
+  const int64_t nb = rows == 0 ? 0 : bwd_blocks(rows, D, x_dtype == RR_F32);
   if (rows > 0) {
     if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr) {
       return rr::fail(RR_EINVAL, "rr_layer_norm_bwd: null pointer");

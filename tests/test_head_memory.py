@@ -86,3 +86,11 @@ def test_backward_takes_a_state_of_either_size():
         run = lambda n: lib.rr_linear_loss_bwd(p, p, 1, rows, D, V, 1, 0.0, 1.0, 1, p, n, None, None, p, 1 << 40, None)  # noqa: E731,E501
         assert run(size[1]) == run(size[2]) == _lib.RR_OK
         assert run(size[2] - 1) == _lib.RR_EWORKSPACE
+
+
+@pytest.mark.parametrize("rows,D,partial", [(1, 8, 1), (100, 1000, 13), (100, 1536, 13), (100, 1537, 50), (512, 2048, 256), (512, 2560, 256),
+                                            (512, 2561, 256), (9000, 64, 512), (9000, 5120, 512), (3, 32768, 2)])
+def test_layer_norm_backward_workspace(rows, D, partial):
+    """Two partial rows (dweight's and dbias's) a workgroup, for two rows a wave or, where a workgroup takes a row, two
+    rows a workgroup: the most that any input type's form needs (fp32 has a wave a row up to 1536 channels)."""
+    assert _lib.load().rr_layer_norm_bwd_workspace_bytes(rows, D) == partial * 2 * D * 4
