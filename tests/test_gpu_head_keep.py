@@ -31,6 +31,8 @@ def test_gradients_with_and_without_kept_logits(rows, D, V, dtype):
                                                                       keep_logits=keep))):
         kept, formed = loss(True), loss(False)
         assert torch.equal(kept, formed)
+        with torch.no_grad():
+            assert torch.equal(loss(True), kept)
         for out in (kept, formed):
             check_all((out.detach(), *torch.autograd.grad(out, (h, w), up)), want)
 
