@@ -440,7 +440,8 @@ int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtype, int64_t 
  * z_loss = 0 for the distillation.  dhidden [rows, D] and dweight [V, D] in
  * `dtype`, each null where not wanted; rows that do not count get dhidden 0. */
 int rr_linear_loss_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
-                       int64_t K, float z_loss, float temperature, int reduction, const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
+                       int64_t K, float z_loss, float temperature, int reduction, const void* state,
+                       size_t state_bytes, void* dhidden, void* dweight, void* workspace,
                        size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -43,8 +43,7 @@ HIPCC_FLAGS = [
 # (argument validation, workspace sizing, the tile schedule and workspace
 # bound walks) under AddressSanitizer + UndefinedBehaviorSanitizer, for the
 # CPU tests.  Only host code is instrumented (each -fsanitize= behind
-# -Xarch_host); the device code is built unoptimised, since this library never
-# launches a kernel.  Loaded by setting MLX_RECURRENCE_AMD_LIB to its path with
+# -Xarch_host); this library never launches a kernel.  Loaded by setting MLX_RECURRENCE_AMD_LIB to its path with
 # the ASan runtime preloaded (tests/test_host_sanitize.py).
 SANITIZE_DIR = BUILD / "sanitize"
 SANITIZERS = ("address", "undefined")
