@@ -911,7 +911,8 @@ coef_kernel(State st, const float* __restrict__ dloss, bool per_row, bool mean, 
       for (int t = threadIdx.x; t < n; t += 1024) coef[t].x *= sc;   // this thread's own
   }
   if (threadIdx.x != 0) return;
-  const float f = per_row ? 1.f : dloss[0] * factor * (mean ? 1.f / (float)max(1, n) : 1.f);
+  // (no row counts: 0, whatever the upstream gradient)
+  const float f = per_row ? 1.f : n == 0 ? 0.f : dloss[0] * factor * (mean ? 1.f / (float)n : 1.f);
   scale[0] = f / sc, scale[1] = each ? f : f / sc;
 }
 

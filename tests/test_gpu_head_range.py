@@ -237,3 +237,19 @@ def test_teacher_logits_of_the_largest_and_lowest_values(dtype, tau):
     one[:, 0], t[:, 0] = torch.finfo(dtype).max, torch.finfo(dtype).max
     t[:, 1:], one[:, 1:] = torch.finfo(dtype).min, -math.inf
     assert same(run_kd(h, w, t, ids, tau), run_kd(h, w, one, ids, tau))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("rows", [40, 300])
+def test_no_row_counts_whatever_the_upstream(rows, reduction, dtype):
+    """A sum over no row, divided by their number: the upstream gradient is not finite, the gradients are 0."""
+    h, w, labels = head(rows, 40, 300, 13, dtype)
+    none = torch.full((rows, 2), -1, device="cuda")
+    for value in (math.inf, math.nan):
+        for f in (lambda a, b: mr.linear_cross_entropy(a, b, torch.full_like(labels, -100), reduction=reduction),
+                  lambda a, b: mr.linear_distillation(a, b, torch.zeros(rows, 2, device="cuda"), none, reduction=reduction)):
+            leaves = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+            loss = f(*leaves)
+            for grad in torch.autograd.grad(loss, leaves, torch.full_like(loss, value)):
+                assert not grad.any()
