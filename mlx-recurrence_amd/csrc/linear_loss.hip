@@ -148,6 +148,13 @@ struct Plan {
   int64_t cuts_w;      // parts of the rows that dw is added up in
 };
 constexpr int64_t kCus = 256;
+// Seconds of a k step of a round of tiles, against which the parts' bytes (at 4 TB/s, written and read)
+// and a launch are weighed: fp32's at 1.4 us too took 210 us at 300 x 5003 x 1000 forward and backward, 185
+// now, 5.4 and 4.9 ms at 4678 x 30720 x 535 (but 694 and 719 us at 512 x 32000 x 768).
+constexpr double kStep = 1.4e-6;        // Tile256 of 16 bits (smaller tiles: the weight's bytes)
+constexpr double kStepF32 = 3.5e-6;     // Tile64, two a CU
+constexpr double kStepF32Dw = 7e-6;     // Tile256
+constexpr double kLaunch = 5.6e-6;
 // How many parts the k steps of `tiles` tiles are cut in, `slots` workgroups running at one
 // time: more parts fill the GPU's rounds better, each at a cost of `part` (in steps), more
 // than one at a cost of `more`.  At least 4 of the `all` smallest ranges of k in each, and two or
@@ -178,12 +185,12 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   const int64_t slots = p.rows == kTile256 ? kCus : 2 * kCus;   // workgroups at one time
   const int64_t row_tiles = p.rows == kTile256 ? p.Tp / 256 : p.rows == kTile64 ? up(T, 64) / 64 : 1;
   // Few tiles of many channels: their sums are cut in parts, each at the cost of writing
-  // and reading the logits in fp32 (in k steps of a tile, 1.4 us, at 4 TB/s), and all at
-  // that of one launch more.
+  // and reading the logits in fp32, and all at that of one launch more.
+  const double step = p.fp32 ? kStepF32 : kStep;
   {
     const int64_t all = p.Dp * p.eb / 128;
-    const double part = (double)(T * V * 8) / 4e12 / 1.4e-6;
-    p.cuts = best_parts(p.Vt / kEdge * row_tiles, slots, (double)all, part, 4., all, T * p.Vt * 4);
+    const double part = (double)(T * V * 8) / 4e12 / step;
+    p.cuts = best_parts(p.Vt / kEdge * row_tiles, slots, (double)all, part, kLaunch / step, all, T * p.Vt * 4);
   }
   const int64_t z_bytes = T * p.Vt * 4;
   p.keep_few = T <= kKeepRows || p.cuts > 1;   // (parts are small, and summed once for both)
@@ -196,13 +203,14 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   // dh has few tiles: its sum over the piece's columns is cut in parts, as the logits' is.
   const int64_t all = p.Vp * p.eb / 128;
   p.splits = best_parts(p.Dt / kEdge * row_tiles, slots, (double)(all * p.planes_z),
-                        (double)(T * D * 8) / 4e12 / 1.4e-6, 0., all, p.Tp * p.Dt * 4);
+                        (double)(T * D * 8) / 4e12 / step, 0., all, p.Tp * p.Dt * 4);
   // Few words and many rows: so is dw's sum over the rows (few rows are few steps).
   p.cuts_w = 1;
   if (T > kKeepRows) {
     const int64_t steps = up(T * p.eb, 128) / 128;
-    p.cuts_w = best_parts(p.Dt / kEdge * (p.Vp / kEdge), kCus, (double)steps, (double)(p.Vp * D * 8) / 4e12 / 1.4e-6, 4., steps,
-                          p.Vp * p.Dt * 4);
+    const double step_w = p.fp32 ? kStepF32Dw : kStep;
+    p.cuts_w = best_parts(p.Dt / kEdge * (p.Vp / kEdge), kCus, (double)steps, (double)(p.Vp * D * 8) / 4e12 / step_w,
+                          kLaunch / step_w, steps, p.Vp * p.Dt * 4);
   }
   return p;
 }
