@@ -5,8 +5,8 @@
 //   backward  g = dy w;  dx = r (g - mean(g) - xh mean(g xh))
 //             dw = sum over rows of dy xh;  db = sum over rows of dy
 //
-// The rows are streamed once: a row stays in the registers of its threads
-// between the statistics and the output, so the variance is that of the
+// The rows are streamed once: a row stays in the registers of its threads (up to 8192
+// channels, below) between the statistics and the output, so the variance is that of the
 // differences (two passes over registers, no cancellation) and HBM sees x (and
 // dy) once and y (dx) once.  The kernels are bound by those bytes, a single
 // token by its launch.
@@ -15,7 +15,9 @@
 // whose sums need no barrier, while its registers hold the row, else a workgroup.
 // Reached on an MI355X (a 2 GiB copy: 4.9 TB/s): 32768 x 2560 bf16 forward 4.8 TB/s,
 // backward 4.6 TB/s, the reduction of the parameters' gradients included; 1536 x 768
-// 5 and 11 us, one token 5 us, launches mostly.
+// 5 and 11 us, one token 5 us, launches mostly.  A workgroup a row: backward 5.0 TB/s at
+// 16384 x 5120, 3.3 at 16384 x 2688 (a third of the lanes idle); beyond 8192 channels its 1024
+// threads' registers spill: 2.7 TB/s at 4096 x 16384, 0.7 at 2048 x 32768.
 // Rows start at any element (odd D): the 16-byte accesses are made at the
 // element type's alignment, which global memory allows, and only a row's last
 // piece is element by element.
