@@ -64,3 +64,52 @@ def test_second_derivatives_are_refused(op, binding):
         torch.autograd.grad(out, leaves, create_graph=True)
     first = torch.autograd.grad(out, leaves, retain_graph=True)
     assert all(bool(torch.isfinite(a).all()) and a.grad_fn is None for a in first)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_under_checkpointing(reentrant, binding):
+    """Recomputed forwards run with gradients on inside a backward: that is no second derivative."""
+    from torch.utils.checkpoint import checkpoint
+    x, s, b, w = (t.requires_grad_(True) for t in tensors())
+    labels = torch.tensor(LABELS, device="cuda")
+
+    def f(x, s, b, w):
+        return mr.linear_cross_entropy(mr.layer_norm(x, s, b), w, labels)
+
+    want = torch.autograd.grad(f(x, s, b, w), (x, s, b, w))
+    checkpoint(f, x, s, b, w, use_reentrant=reentrant).backward()
+    for leaf, e in zip((x, s, b, w), want):
+        assert torch.equal(leaf.grad, e)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_graph_replays_of_losses_a_row(dtype):
+    """reduction="none" and logits that are formed again, captured in a HIP graph: every replay gives the eager bits."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    h, w = (torch.randn(s, generator=g, device="cuda").to(dtype).requires_grad_(True) for s in ((300, 72), (1000, 72)))
+    labels = torch.randint(0, 1000, (300,), generator=g, device="cuda")
+    labels[::6] = -100
+    up = torch.logspace(2, -4, 300, device="cuda")
+
+    def step():
+        loss = mr.linear_cross_entropy(h, w, labels, reduction="none", keep_logits=False)
+        return (loss, *torch.autograd.grad(loss, (h, w), up))
+
+    eager = [a.detach().clone() for a in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        for a in out:
+            a.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(out, eager):
+            assert torch.equal(a, e)
+        for a, e in zip(step(), eager):
+            assert torch.equal(a, e)
