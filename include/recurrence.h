@@ -444,6 +444,46 @@ int rr_linear_loss_bwd(const float* dloss, const void* weight, int dtype, int64_
                        size_t state_bytes, void* dhidden, void* dweight, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* Losses on the log-probabilities of the labels, logp = z[label] - log sum exp z with
+ * z = hidden weight^T / temperature: labels, ignore_index, reduction, state, workspace and
+ * their sizes (K = 1) are those of rr_linear_ce_fwd.  Rows that are ignored count for
+ * nothing, whatever their hidden state, advantage and log-probabilities hold.
+ *
+ * The log-probabilities themselves, [rows] fp32, 0 for an ignored row. */
+int rr_linear_logp_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                       const int64_t* labels, int64_t ignore_index, float temperature, float* log_probs,
+                       void* state, size_t state_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A clipped policy loss with a KL term.  With r = exp(logp - old) and d = ref - logp of a row,
+ * and A its advantage (advantages[row / rows_per_advantage]),
+ *   loss = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight (exp(d) - d - 1).
+ * old_log_probs null: r = 1, with logp's gradient.  ref_log_probs is read where kl_weight is not 0.
+ * The widths may be infinite (no clipping).  A ratio on a border of the clipping has its gradient. */
+int rr_linear_policy_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                         const int64_t* labels, int64_t ignore_index, float temperature, const float* advantages,
+                         int64_t rows_per_advantage, const float* old_log_probs, const float* ref_log_probs,
+                         float clip_low, float clip_high, float kl_weight, int reduction, float* loss, void* state,
+                         size_t state_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A preference loss: rows are [pairs][2][L], the preferred sequence of each pair first.  With S
+ * the sum of a sequence's logp over its tokens that count and ref_log_probs [pairs][2] (null: 0),
+ *   m = beta ((S_1 - ref_1) - (S_2 - ref_2)),
+ *   loss = -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m),
+ * a loss a pair ([pairs] for reduction 0).  A pair without a token that counts gives 0 and is not counted
+ * by the mean; a pair with a NaN among its log-probabilities is NaN as a whole. */
+int rr_linear_preference_fwd(const void* hidden, const void* weight, int dtype, int64_t pairs, int64_t L, int64_t D,
+                             int64_t V, const int64_t* labels, int64_t ignore_index, const float* ref_log_probs,
+                             float beta, float label_smoothing, int reduction, float* loss, void* state,
+                             size_t state_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of the three: dloss fp32 ([rows / rows_per_loss] for reduction 0, else [1]) with
+ * rows_per_loss 1, or 2 L for the preference loss (whose temperature is 1); of_log_probs is 1 for
+ * rr_linear_logp_fwd (reduction 0), else 0.  The rest as for rr_linear_loss_bwd. */
+int rr_linear_logp_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                       float temperature, int64_t rows_per_loss, int of_log_probs, int reduction, const void* state,
+                       size_t state_bytes, void* dhidden, void* dweight, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

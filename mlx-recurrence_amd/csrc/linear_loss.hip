@@ -1,5 +1,6 @@
 // linear_loss.hip — losses over a large vocabulary straight from hidden states, on
-// gfx950: cross entropy on labels and distillation from a teacher's top logits.
+// gfx950: cross entropy on labels, distillation from a teacher's top logits, and the
+// losses on the labels' log-probabilities.
 //
 //   z = h w^T  [rows, V];  s = z / tau;  lse = log sum_v exp(s_v);  q = exp(s - lse)
 //   cross entropy (tau = 1)  loss = lse - z_label + zl lse^2
@@ -9,8 +10,16 @@
 //                            dz = c tau (q - sum_{k: id_k = v} p_k)
 //   dh = dz w,  dw = dz^T h,  c the row's upstream gradient
 //
-// A label is a teacher with one entry of weight 1, so both run on the same
-// kernels.  The forward forms the logits a tile at a time and keeps each row's running
+//   log-probabilities        logp = s_label - lse;  dz = c / tau (1[v = label] - q)
+//   clipped policy           r = exp(logp - old), d = ref - logp
+//                            loss = -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl (exp(d) - d - 1)
+//                            c = -[r not clipped] r A + kl (1 - exp(d))
+//   preference               S = sum of a sequence's logp, m = beta ((S_1 - ref_1) - (S_2 - ref_2)) of a pair
+//                            loss = -(1 - eps) log sigmoid(m) - eps log sigmoid(-m)
+//                            c = +- beta (eps sigmoid(m) - (1 - eps) sigmoid(-m)) for all tokens of a sequence
+//
+// A label is a teacher with one entry of weight 1, so all run on the same
+// kernels; what the last two put on a log-probability is left by the forward, a value a row.  The forward forms the logits a tile at a time and keeps each row's running
 // maximum and sum per tile and the logits of the row's entries; where that pays
 // (kKeepBytes and kKeepChannels below) and the caller has room it also leaves the logits
 // themselves, in fp32.
@@ -113,6 +122,7 @@ struct Carve {
 // What the forward leaves for the backward, in one buffer of the caller's.
 struct Header {
   int n;                 // rows that count
+  int count;             // what the mean is over: those rows, or the pairs that count
 };
 struct State {
   Header* hdr;
@@ -122,7 +132,8 @@ struct State {
   float* loss;   // [rows]
   int* ids;      // [rows][K] the entries' columns, ascending; kAbsent past the last
   float* p;      // [rows][K] their weights
-  float* z2;     // [rows][K] their logits, times log2(e) / tau
+  float* z2;     // [rows][K] their logits, times log2(e) / tau; the policy and the preference loss leave
+                 // the derivative of a row's loss by -logp there instead, for the backward
   float* amax;   // [rows] largest finite |hidden| of a row that counts (fp16)
   char* h;       // [rows][Dp] the hidden states that count, as an operand
   char* w;       // [V][Dp] where the weight is copied
@@ -251,7 +262,7 @@ size_t fwd_layout(const Plan& p, char* base, FwdWs* s) {
   return take.off;
 }
 struct BwdWs {
-  float* scale;    // the factors on dw and on dh
+  float* scale;    // the factors on dw and on dh, and dw's power of two
   float2* coef;    // [Tp] a row's factors (coef_kernel)
   float* unscale;  // [Tp] the inverse of a row's power of two (fp16)
   char* h;         // [T][Dp] the hidden states times that (fp16)
@@ -391,7 +402,7 @@ rows_kernel(const int64_t* __restrict__ labels, int64_t ignore, int64_t T, int V
     }
     base += all;
   }
-  if (tid == 0) st.hdr->n = base;
+  if (tid == 0) st.hdr->n = base, st.hdr->count = base;
 }
 
 // Eight elements from column c of a row of D as they lie in memory, 0 past its end (a row
@@ -811,15 +822,10 @@ dz_kernel(State st, const float2* __restrict__ coef, int V, int64_t Vt, int K, i
   }
 }
 
-// Per row (a wave each): the tiles' maxima and sums to the row's lse, and its loss.
-__global__ void __launch_bounds__(256)
-row_loss_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, int K, bool labels, float zl, float tau,
-                float* __restrict__ out) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
-  if (t >= st.hdr->n) return;
-  const int64_t row = st.rows[t];
-  float m = -INFINITY, s = 0.f;
+// The tiles' maxima and sums of a row to the row's, by a wave.
+__device__ __forceinline__ void join_tiles(const float2* __restrict__ part, int nvt, int64_t Tp, int64_t t, int lane, float& m,
+                                           float& s) {
+  m = -INFINITY, s = 0.f;
   for (int v = lane; v < nvt; v += 64) {
     const float2 x = part[(int64_t)v * Tp + t];
     const float mm = fmaxf(m, x.x);
@@ -833,6 +839,18 @@ row_loss_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, 
     s = (m == mm ? s : s * exp2f(m - mm)) + (m2 == mm ? s2 : s2 * exp2f(m2 - mm));
     m = mm;
   }
+}
+
+// Per row (a wave each): the tiles' maxima and sums to the row's lse, and its loss.
+__global__ void __launch_bounds__(256)
+row_loss_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, int K, bool labels, float zl, float tau,
+                float* __restrict__ out) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+  if (t >= st.hdr->n) return;
+  const int64_t row = st.rows[t];
+  float m, s;
+  join_tiles(part, nvt, Tp, t, lane, m, s);
   const float l2 = m + log2f(s);
   float loss = 0.f;
   for (int k = lane; k < K; k += 64) {
@@ -858,6 +876,105 @@ row_loss_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, 
   }
 }
 
+// What a policy's loss reads of each row.
+struct Policy {
+  const float* advantages;   // [rows / per]
+  int64_t per;
+  const float* old;          // [rows]; null: the log-probabilities of this call
+  const float* ref;          // [rows], where kl is not 0
+  float lo, hi, kl;          // borders of the ratio, weight of the KL term
+};
+
+// exp(d) - d - 1, which is d^2 / 2 and more: close to 0 from its series (below 1/4 its next term is
+// 1e-8 of it), where the difference would leave few bits.
+__device__ __forceinline__ float exp_rest(float d) {
+  if (fabsf(d) < 0.25f)
+    return 0.5f * d * d * (1.f + d * (1.f / 3) * (1.f + d * (1.f / 4) * (1.f + d * (1.f / 5) * (1.f + d * (1.f / 6) * (1.f + d * (1.f / 7))))));
+  return d > 60.f ? expm1f(d) : expm1f(d) - d;   // (not inf - inf)
+}
+
+// Per row (a wave each): the tiles' maxima and sums to the row's lse and its label's
+// log-probability, to `out`; or, POLICY, its loss, and the derivative by -logp for the
+// backward.  A ratio on a border of the clipping counts as inside it; without an advantage the
+// ratio counts for nothing, however large.
+template <bool POLICY>
+__global__ void __launch_bounds__(256)
+row_logp_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, Policy a, float* __restrict__ out) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+  if (t >= st.hdr->n) return;
+  const int64_t row = st.rows[t];
+  float m, s;
+  join_tiles(part, nvt, Tp, t, lane, m, s);
+  if (lane != 0) return;
+  const float log2s = log2f(s);
+  // (the maximum goes first: what is left is small and keeps its bits)
+  const float logp = st.ids[row] == kAbsent ? NAN : ((st.z2[row] - m) - log2s) * kLn2;
+  float value = logp;
+  if constexpr (POLICY) {
+    const float A = a.advantages[row / a.per];
+    const float r = a.old == nullptr ? (logp != logp ? logp : 1.f) : expf(logp - a.old[row]);
+    float by = 0.f;   // by logp
+    if (A == 0.f) {
+      value = r != r ? r : 0.f;
+    } else {
+      const bool clipped = A > 0.f ? r > a.hi : r < a.lo;
+      value = -(clipped ? (A > 0.f ? a.hi : a.lo) : r) * A;
+      by = clipped ? 0.f : value;
+    }
+    if (a.kl != 0.f) {
+      const float d = a.ref[row] - logp;
+      value += a.kl * exp_rest(d);
+      by -= a.kl * expm1f(d);
+    }
+    st.z2[row] = -by;
+  }
+  out[row] = value;
+  st.lse2[t] = value != value ? NAN : m + log2s;   // the backward's row is NaN where the loss is
+}
+
+// The loss of each pair of sequences (a workgroup each) from their tokens' log-probabilities in
+// st.loss, and its derivative by each token's -logp.  Sums and the loss are in 64 bits: a
+// sequence's sum is in the thousands where the difference of two of them decides.  A pair without
+// a token that counts counts for nothing.  counted: null, or whether each does.
+__global__ void __launch_bounds__(256)
+pair_kernel(State st, const float* __restrict__ ref, int64_t L, double beta, double eps, float* __restrict__ out,
+            int* __restrict__ counted) {
+  __shared__ double sum[4];
+  __shared__ int any[4];
+  __shared__ float by;
+  const int64_t pair = blockIdx.x, first = pair * 2 * L;
+  const int tid = threadIdx.x, side = tid >> 7;   // half of the threads take one sequence, half the other
+  double s = 0;
+  int n = 0;
+  for (int64_t i = tid & 127; i < L; i += 128) {
+    const int64_t row = first + side * L + i;
+    if (st.pos[row] < 0) continue;
+    s += (double)st.loss[row], n = 1;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64), n |= __shfl_xor(n, o, 64);
+  if ((tid & 63) == 0) sum[tid >> 6] = s, any[tid >> 6] = n;
+  __syncthreads();
+  const bool counts = (any[0] | any[1] | any[2] | any[3]) != 0;
+  if (tid == 0) {
+    double m = (sum[0] + sum[1]) - (sum[2] + sum[3]);
+    if (ref != nullptr) m -= (double)ref[2 * pair] - (double)ref[2 * pair + 1];
+    m *= beta;
+    const double e = exp(-fabs(m)), rest = log1p(e);   // -log sigmoid(m) = max(-m, 0) + rest
+    const double up = 1 / (1 + e), down = e / (1 + e);   // sigmoid(|m|), sigmoid(-|m|)
+    double loss = (1 - eps) * (fmax(-m, 0.) + rest);
+    if (eps != 0) loss += eps * (fmax(m, 0.) + rest);   // (not 0 x inf)
+    by = (float)(beta * (m < 0 ? (1 - eps) * up - eps * down : (1 - eps) * down - eps * up));
+    out[pair] = counts ? (float)loss : 0.f;
+    if (counted != nullptr) counted[pair] = counts ? 1 : 0;
+  }
+  __syncthreads();
+  if (!counts) return;
+  const float d = side == 0 ? by : -by;
+  for (int64_t i = tid & 127; i < L; i += 128) st.z2[first + side * L + i] = d;
+}
+
 // The sum of the rows' losses, over the number that count where `mean` (0 without any).  A
 // launch of its own: the fences by which row_loss_kernel's last workgroup could do it
 // took 160 us at 8192 rows.
@@ -876,6 +993,27 @@ sum_loss_kernel(const float* __restrict__ loss, int64_t T, const Header* hdr, bo
   out[0] = mean ? s / (float)max(1, hdr->n) : s;
 }
 
+// The same of pairs, whose number that count it finds.
+__global__ void __launch_bounds__(1024)
+sum_pairs_kernel(const float* __restrict__ loss, const int* __restrict__ counted, int64_t pairs, Header* hdr, bool mean,
+                 float* out) {
+  __shared__ float buf[16];
+  __shared__ int count[16];
+  float s = 0.f;
+  int n = 0;
+  for (int64_t i = threadIdx.x; i < pairs; i += 1024) s += loss[i], n += counted[i];
+  s = wave_add(s);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = s, count[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  s = 0.f, n = 0;
+  for (int w = 0; w < 16; ++w) s += buf[w], n += count[w];
+  hdr->count = n;
+  out[0] = mean ? s / (float)max(1, n) : s;
+}
+
 // ------------------------------------------------------------------ gradients
 // coef[t] = (c f, 1 - 1 / f) with f = 1 + 2 zl lse, so that a row of dz is
 // c f (q - p + p (1 - 1 / f)), and the factors on dw and dh, scale[0] and [1].  One upstream
@@ -884,16 +1022,19 @@ sum_loss_kernel(const float* __restrict__ loss, int64_t T, const Header* hdr, bo
 // row's.  `scaled`: c carries the power of two that brings the largest of them below
 // 2^14, and the factors its inverse; or each row's own does, whose inverse is left in
 // unscale (0 where dz is 0), and dw's factor undoes that of the copy of the hidden states
-// (scale_h_kernel), which brings the largest of those below 2^15.  One workgroup.
+// (scale_h_kernel), which brings the largest of those below 2^15.  The loss of a pair is that
+// of `group` rows; weights: null, or each row's derivative by -logp, which c carries.  One workgroup.
 __global__ void __launch_bounds__(1024)
-coef_kernel(State st, const float* __restrict__ dloss, bool per_row, bool mean, float factor, float zl, bool scaled,
-            float2* __restrict__ coef, float* __restrict__ unscale, float* scale) {
+coef_kernel(State st, const float* __restrict__ dloss, bool per_row, int group, const float* __restrict__ weights, bool mean,
+            float factor, float zl, bool scaled, float2* __restrict__ coef, float* __restrict__ unscale, float* scale) {
   __shared__ float buf[16];
   const int n = st.hdr->n;
-  const bool each = scaled && per_row;
+  const bool each = scaled && (per_row || weights != nullptr);
   float m = 0.f;
   for (int t = threadIdx.x; t < n; t += 1024) {
-    const float c = per_row ? dloss[st.rows[t]] * factor : 1.f;
+    const int row = st.rows[t];
+    float c = per_row ? dloss[group == 1 ? row : row / group] * factor : 1.f;
+    if (weights != nullptr) c *= weights[row];
     const float x = 2.f * zl * st.lse2[t] * kLn2;
     float f = 1.f + x;
     if (f == 0.f) f = 1e-30f;
@@ -921,8 +1062,8 @@ coef_kernel(State st, const float* __restrict__ dloss, bool per_row, bool mean, 
   }
   if (threadIdx.x != 0) return;
   // (no row counts: 0, whatever the upstream gradient)
-  const float f = per_row ? 1.f : n == 0 ? 0.f : dloss[0] * factor * (mean ? 1.f / (float)n : 1.f);
-  scale[0] = f / sc, scale[1] = each ? f : f / sc;
+  const float f = per_row ? 1.f : n == 0 ? 0.f : dloss[0] * factor * (mean ? 1.f / (float)st.hdr->count : 1.f);
+  scale[0] = f / sc, scale[1] = each ? f : f / sc, scale[2] = sc;
 }
 
 // The hidden states divided by their rows' powers of two, times dw's (a row a workgroup).
@@ -930,7 +1071,7 @@ __global__ void __launch_bounds__(256)
 scale_h_kernel(State st, const float* __restrict__ unscale, const float* scale, int Dp, f16* __restrict__ out) {
   const int t = blockIdx.x;
   if (t >= st.hdr->n) return;
-  const float k = unscale[t] / scale[0];
+  const float k = unscale[t] * scale[2];
   const f16* h = reinterpret_cast<const f16*>(st.h) + (int64_t)t * Dp;
   for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
     f16 v[8];
@@ -1148,14 +1289,25 @@ void launch_dw(DwArgs a, const Plan& p, int64_t cols, hipStream_t s) {
   }
 }
 
+// What a call computes from the logits.
+enum Kind { kLabels, kTeacher, kLogp, kPolicy, kPreference };
+struct Loss {
+  Kind kind;
+  float tau, zl;
+  Policy policy;
+  const float* ref;      // of pairs
+  int64_t L;             // tokens of a pair's sequence
+  double beta, eps;
+};
+
 template <typename X, typename Op>
-int forward(const Plan& p, const void* hidden, const void* weight, const State& st, const FwdWs& ws, int K, bool labels,
-            float zl, float tau, int reduction, float* loss, hipStream_t s) {
+int forward(const Plan& p, const void* hidden, const void* weight, const State& st, const FwdWs& ws, int K, const Loss& l,
+            int reduction, float* loss, hipStream_t s) {
   // the weight too where it is not an operand itself
   const int64_t most = p.copy_w ? std::max(p.T, p.V) : p.T;
   pack_kernel<X><<<dim3((unsigned)std::min<int64_t>(8192, most), p.copy_w ? 2 : 1), 256, 0, s>>>(
       static_cast<const X*>(hidden), static_cast<const X*>(weight), p.V, (int)p.D, (int)p.Dp, st);
-  LogitArgs a = logit_args(p, st, weight, K, tau);
+  LogitArgs a = logit_args(p, st, weight, K, l.tau);
   a.part = ws.part;
   a.z = p.cuts > 1 ? ws.cut : st.z, a.ldzf = p.Vt, a.ldcut = p.T * p.Vt, a.cuts = (int)p.cuts;
   if (p.rows == kTile32) launch_forward<Tile32, Op>(a, p, s);
@@ -1167,24 +1319,48 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
     join_kernel<<<dim3((unsigned)p.T, (unsigned)parts), 256, 0, s>>>(st, ws.cut, a.cuts, a.ldcut, a.V, p.Vt, K, a.c, p.Tp,
                                                                     ws.part);
   }
+  const unsigned waves = (unsigned)((p.T + 3) / 4);
   float* rows = reduction == 0 ? loss : st.loss;
-  row_loss_kernel<<<(unsigned)((p.T + 3) / 4), 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, K, labels, zl, tau, rows);
+  if (l.kind == kPreference) {
+    row_logp_kernel<false><<<waves, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, st.loss);
+    const int64_t pairs = p.T / (2 * l.L);
+    float* each = reduction == 0 ? loss : reinterpret_cast<float*>(ws.part);   // a float2 a row is there and done with
+    int* counted = reduction == 0 ? nullptr : reinterpret_cast<int*>(each + pairs);
+    pair_kernel<<<(unsigned)pairs, 256, 0, s>>>(st, l.ref, l.L, l.beta, l.eps, each, counted);
+    if (reduction != 0) sum_pairs_kernel<<<1, 1024, 0, s>>>(each, counted, pairs, st.hdr, reduction == 1, loss);
+    return rr::check_launch("rr_linear_preference");
+  }
+  if (l.kind == kPolicy) {
+    row_logp_kernel<true><<<waves, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, l.policy, rows);
+  } else if (l.kind == kLogp) {
+    row_logp_kernel<false><<<waves, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, rows);
+  } else {
+    row_loss_kernel<<<waves, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, K, l.kind == kLabels, l.zl, l.tau, rows);
+  }
   if (reduction != 0) sum_loss_kernel<<<1, 1024, 0, s>>>(st.loss, p.T, st.hdr, reduction == 1, loss);
   return rr::check_launch("rr_linear_loss");
 }
 
+// What the backward has to know of a loss: dz is `factor` times (f q - p) and a row's upstream gradient,
+// one for `group` rows, and with `weighted` what the forward left for the row.
+struct LossGrad {
+  float tau, factor, zl;
+  int group;
+  bool weighted;
+};
+
 template <typename X, typename Op, int PZ>
-int backward(const Plan& p, const float* dloss, const void* weight, const State& st, const BwdWs& ws, int K, float zl,
-             float tau, int reduction, void* dh, void* dw, hipStream_t s) {
-  const bool each = __is_same(Op, OpF16) && reduction == 0;   // a power of two for each row's dz
-  coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, reduction == 1, tau, zl, __is_same(Op, OpF16), ws.coef,
-                                 ws.unscale, ws.scale);
+int backward(const Plan& p, const float* dloss, const void* weight, const State& st, const BwdWs& ws, int K, const LossGrad& l,
+             int reduction, void* dh, void* dw, hipStream_t s) {
+  const bool each = __is_same(Op, OpF16) && (reduction == 0 || l.weighted);   // a power of two for each row's dz
+  coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, l.group, l.weighted ? st.z2 : nullptr, reduction == 1, l.factor,
+                                 l.zl, __is_same(Op, OpF16), ws.coef, ws.unscale, ws.scale);
   if (each && dw != nullptr) {
     scale_h_kernel<<<(unsigned)p.T, 256, 0, s>>>(st, ws.unscale, ws.scale, (int)p.Dp, reinterpret_cast<f16*>(ws.h));
   }
   for (int64_t v = 0; v < p.Vt; v += p.Vp) {
     const int64_t cols = std::min(p.Vp, p.Vt - v);   // whole tiles
-    LogitArgs a = logit_args(p, st, weight, K, tau);
+    LogitArgs a = logit_args(p, st, weight, K, l.tau);
     a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp * p.eb, a.plane_z = p.Tp * a.ldz, a.v_first = (int)v;
     constexpr bool kFp32 = __is_same(Op, OpF32), kFew = PZ == 2;   // up to kFewRows
     if (kFew || st.z != nullptr) {
@@ -1236,14 +1412,14 @@ void zero(void* p, int64_t bytes, hipStream_t s) {
                                    bytes % 4 ? static_cast<uint16_t*>(p) + bytes / 2 - 1 : nullptr);
 }
 
-int run_forward(const void* hidden, const void* weight, int dtype, int64_t T, int64_t D, int64_t V, int64_t K, bool labels,
-                float zl, float tau, int reduction, float* loss, const State& st, void* workspace, hipStream_t s) {
+int run_forward(const void* hidden, const void* weight, int dtype, int64_t T, int64_t D, int64_t V, int64_t K, const Loss& l,
+                int reduction, float* loss, const State& st, void* workspace, hipStream_t s) {
   const Plan p = plan_of(T, D, V, dtype);
   FwdWs ws;
   fwd_layout(p, static_cast<char*>(workspace), &ws);
-  if (dtype == RR_BF16) return forward<bf16, OpBf16>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
-  if (dtype == RR_F16) return forward<f16, OpF16>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
-  return forward<float, OpF32>(p, hidden, weight, st, ws, (int)K, labels, zl, tau, reduction, loss, s);
+  if (dtype == RR_BF16) return forward<bf16, OpBf16>(p, hidden, weight, st, ws, (int)K, l, reduction, loss, s);
+  if (dtype == RR_F16) return forward<f16, OpF16>(p, hidden, weight, st, ws, (int)K, l, reduction, loss, s);
+  return forward<float, OpF32>(p, hidden, weight, st, ws, (int)K, l, reduction, loss, s);
 }
 
 int check_buffers(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int dtype, int pass, const void* hidden,
@@ -1298,7 +1474,8 @@ extern "C" int rr_linear_ce_fwd(const void* hidden, const void* weight, int dtyp
   State in = st;
   if (reduction == 0) in.loss = loss;   // where rows that do not count leave their 0
   rows_kernel<true><<<1, 1024, 0, s>>>(labels, ignore_index, rows, (int)V, in);
-  return run_forward(hidden, weight, dtype, rows, D, V, 1, true, z_loss, 1.f, reduction, loss, st, workspace, s);
+  Loss l{kLabels, 1.f, z_loss};
+  return run_forward(hidden, weight, dtype, rows, D, V, 1, l, reduction, loss, st, workspace, s);
 }
 
 extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
@@ -1333,19 +1510,47 @@ extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtyp
   State in = st;
   if (reduction == 0) in.loss = loss;
   rows_kernel<false><<<1, 1024, 0, s>>>(nullptr, 0, rows, (int)V, in);
-  return run_forward(hidden, weight, dtype, rows, D, V, K, false, 0.f, temperature, reduction, loss, st, workspace, s);
+  Loss l{kTeacher, temperature, 0.f};
+  return run_forward(hidden, weight, dtype, rows, D, V, K, l, reduction, loss, st, workspace, s);
 }
 
-extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D,
-                                  int64_t V, int64_t K, float z_loss, float temperature, int reduction,
-                                  const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
-  const char* who = "rr_linear_loss_bwd";
-  if (int rc = check_dims(who, rows, D, V, K, dtype, reduction)) return rc;
-  if (!(temperature > 0.f) || !(temperature < 1e30f)) {
-    return rr::fail(RR_EINVAL, std::string(who) + ": temperature must be positive and finite");
+namespace {
+
+bool bad_temperature(float t) { return !(t > 0.f) || !(t < 1e30f); }
+
+// The forward of the losses on the labels' log-probabilities, `losses` of them where none are added up.
+int forward_logp(const char* who, const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                 const int64_t* labels, int64_t ignore_index, const Loss& l, int reduction, float* loss, int64_t losses,
+                 void* state, size_t state_bytes, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  if (int rc = check_dims(who, rows, D, V, 1, dtype, reduction)) return rc;
+  const std::string w(who);
+  if (bad_temperature(l.tau)) return rr::fail(RR_EINVAL, w + ": temperature must be positive and finite");
+  if (losses > 0 || reduction != 0) {
+    if (loss == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
   }
-  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows == 0) {
+    zero(loss, reduction != 0 ? 4 : losses * 4, s);
+    return rr::check_launch(who);
+  }
+  if (labels == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
+  if (l.kind == kPolicy && (l.policy.advantages == nullptr || (l.policy.kl != 0.f && l.policy.ref == nullptr))) {
+    return rr::fail(RR_EINVAL, w + ": null pointer");
+  }
+  if (int rc = check_buffers(who, rows, D, V, 1, dtype, 0, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
+  State st;
+  lay_out_state(rows, D, V, 1, dtype, state, state_bytes, &st);
+  State in = st;
+  if (reduction == 0 && l.kind != kPreference) in.loss = loss;   // where rows that do not count leave their 0
+  rows_kernel<true><<<1, 1024, 0, s>>>(labels, ignore_index, rows, (int)V, in);
+  return run_forward(hidden, weight, dtype, rows, D, V, 1, l, reduction, loss, st, workspace, s);
+}
+
+// The backward of all losses.
+int run_backward(const char* who, const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                 int64_t K, const LossGrad& l, int reduction, const void* state, size_t state_bytes, void* dhidden,
+                 void* dweight, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  if (int rc = check_dims(who, rows, D, V, K, dtype, reduction)) return rc;
+  if (bad_temperature(l.tau)) return rr::fail(RR_EINVAL, std::string(who) + ": temperature must be positive and finite");
   const int64_t es = dtype == RR_F32 ? 4 : 2;
   if (rows == 0) {
     zero(dweight, V * D * es, s);
@@ -1359,10 +1564,76 @@ extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dt
   lay_out_state(rows, D, V, K, dtype, const_cast<void*>(state), state_bytes, &st);
   BwdWs ws;
   bwd_layout(p, static_cast<char*>(workspace), &ws);
-#define LL_BACKWARD(X, OP, PZ) \
-  backward<X, OP, PZ>(p, dloss, weight, st, ws, (int)K, z_loss, temperature, reduction, dhidden, dweight, s)
+#define LL_BACKWARD(X, OP, PZ) backward<X, OP, PZ>(p, dloss, weight, st, ws, (int)K, l, reduction, dhidden, dweight, s)
   if (dtype == RR_BF16) return p.planes_z == 2 ? LL_BACKWARD(bf16, OpBf16, 2) : LL_BACKWARD(bf16, OpBf16, 1);
   if (dtype == RR_F16) return p.planes_z == 2 ? LL_BACKWARD(f16, OpF16, 2) : LL_BACKWARD(f16, OpF16, 1);
   return LL_BACKWARD(float, OpF32, 1);
 #undef LL_BACKWARD
+}
+
+}  // namespace
+
+extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D,
+                                  int64_t V, int64_t K, float z_loss, float temperature, int reduction,
+                                  const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  const LossGrad l{temperature, temperature, z_loss, 1, false};
+  return run_backward("rr_linear_loss_bwd", dloss, weight, dtype, rows, D, V, K, l, reduction, state, state_bytes, dhidden,
+                      dweight, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int rr_linear_logp_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                                  const int64_t* labels, int64_t ignore_index, float temperature, float* log_probs,
+                                  void* state, size_t state_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  const Loss l{kLogp, temperature, 0.f};
+  return forward_logp("rr_linear_logp_fwd", hidden, weight, dtype, rows, D, V, labels, ignore_index, l, 0, log_probs, rows,
+                      state, state_bytes, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int rr_linear_policy_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                                    const int64_t* labels, int64_t ignore_index, float temperature,
+                                    const float* advantages, int64_t rows_per_advantage, const float* old_log_probs,
+                                    const float* ref_log_probs, float clip_low, float clip_high, float kl_weight,
+                                    int reduction, float* loss, void* state, size_t state_bytes, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  const std::string w = "rr_linear_policy_fwd";
+  if (!(clip_low >= 0.f) || !(clip_high >= 0.f)) return rr::fail(RR_EINVAL, w + ": the clipping's widths must not be negative");
+  if (!(kl_weight >= 0.f) || !(kl_weight < INFINITY)) return rr::fail(RR_EINVAL, w + ": kl_weight must be finite and not negative");
+  if (rows_per_advantage <= 0) return rr::fail(RR_EINVAL, w + ": an advantage is for one row or more");
+  Loss l{kPolicy, temperature, 0.f};
+  l.policy = {advantages, rows_per_advantage, old_log_probs, ref_log_probs, 1.f - clip_low, 1.f + clip_high, kl_weight};
+  return forward_logp(w.c_str(), hidden, weight, dtype, rows, D, V, labels, ignore_index, l, reduction, loss, rows, state,
+                      state_bytes, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int rr_linear_preference_fwd(const void* hidden, const void* weight, int dtype, int64_t pairs, int64_t L,
+                                        int64_t D, int64_t V, const int64_t* labels, int64_t ignore_index,
+                                        const float* ref_log_probs, float beta, float label_smoothing, int reduction,
+                                        float* loss, void* state, size_t state_bytes, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  const std::string w = "rr_linear_preference_fwd";
+  if (pairs < 0 || L < 0) return rr::fail(RR_EINVAL, w + ": pairs and tokens must be >= 0");
+  if (pairs >= ((int64_t)1 << 23) || L >= ((int64_t)1 << 23)) return rr::fail(RR_EUNSUPPORTED, w + ": too many rows");
+  if (!(beta > 0.f) || !(beta < INFINITY)) return rr::fail(RR_EINVAL, w + ": beta must be positive and finite");
+  if (!(label_smoothing >= 0.f) || !(label_smoothing <= 0.5f)) return rr::fail(RR_EINVAL, w + ": label_smoothing must be in [0, 0.5]");
+  Loss l{kPreference, 1.f, 0.f};
+  l.ref = ref_log_probs, l.L = L, l.beta = beta, l.eps = label_smoothing;
+  return forward_logp(w.c_str(), hidden, weight, dtype, pairs * 2 * L, D, V, labels, ignore_index, l, reduction, loss, pairs,
+                      state, state_bytes, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int rr_linear_logp_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
+                                  float temperature, int64_t rows_per_loss, int of_log_probs, int reduction,
+                                  const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  const std::string w = "rr_linear_logp_bwd";
+  if (rows_per_loss <= 0 || rows_per_loss >= ((int64_t)1 << 24)) return rr::fail(RR_EINVAL, w + ": a loss is of one row or more");
+  const bool itself = of_log_probs != 0;
+  if (itself && (rows_per_loss != 1 || reduction != 0)) {
+    return rr::fail(RR_EINVAL, w + ": log-probabilities have a gradient a row");
+  }
+  // (the log-probabilities' own derivative by -logp is -1)
+  const LossGrad l{temperature, (itself ? -1.f : 1.f) / temperature, 0.f, (int)rows_per_loss, !itself};
+  return run_backward(w.c_str(), dloss, weight, dtype, rows, D, V, 1, l, reduction, state, state_bytes, dhidden, dweight,
+                      workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }

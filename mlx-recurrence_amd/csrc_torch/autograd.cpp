@@ -18,6 +18,7 @@
 
 #include <cstdint>
 #include <string>
+#include <vector>
 
 #include "../../include/recurrence.h"
 
@@ -443,6 +444,81 @@ Tensor linear_loss(const Tensor& hidden, const Tensor& weight, const c10::option
   return LinearLossFn::apply(hidden, weight, labels, t_logits, t_ids, ignore, zl, tau, reduction, grad);
 }
 
+// ------------------------------------------------------------------ losses on log-probabilities
+// hidden [rows, D] and weight [V, D] of one type, labels [rows].  `kind` 0: the log-probabilities; 1: the
+// policy loss of advantages [rows / per], old and ref [rows]; 2: the preference loss of pairs of
+// sequences of `per` tokens, ref [pairs, 2].  values: temperature, and for 1 the clipping's widths and
+// the KL term's weight, for 2 beta and the smoothing.
+struct LinearLogpFn : public torch::autograd::Function<LinearLogpFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& labels,
+                        const c10::optional<Tensor>& advantages, const c10::optional<Tensor>& old,
+                        const c10::optional<Tensor>& ref, int64_t kind, int64_t losses, int64_t per, int64_t ignore,
+                        std::vector<double> values, int64_t reduction, int64_t grad) {
+    const at::DeviceGuard guard(hidden.device());
+    const at::ScalarType dt = hidden.scalar_type();
+    const Tensor h_ = prep(hidden, dt), w_ = prep(weight, dt), l_ = prep(labels, at::kLong);
+    const Tensor a_ = advantages.has_value() ? prep(*advantages, at::kFloat) : Tensor();
+    const Tensor o_ = old.has_value() ? prep(*old, at::kFloat) : Tensor();
+    const Tensor r_ = ref.has_value() ? prep(*ref, at::kFloat) : Tensor();
+    const int64_t rows = h_.size(0), D = h_.size(1), V = w_.size(0);
+    const int dtc = dtype_code(dt);
+    const auto f32 = h_.options().dtype(at::kFloat);
+    Tensor loss = reduction == 0 ? at::empty({losses}, f32) : at::empty({}, f32);
+    const size_t sb = rr_linear_loss_state_bytes(rows, D, V, 1, dtc, (int)grad), wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 0);
+    const Tensor state = workspace(sb, h_.options()), ws = workspace(wsb, h_.options());
+    const int64_t* lp = l_.data_ptr<int64_t>();
+    const float tau = (float)values[0];
+    void* s = stream_of(h_);
+    if (kind == 0) {
+      check(rr_linear_logp_fwd(P(h_), P(w_), dtc, rows, D, V, lp, ignore, tau, MF(loss), P(state), sb, P(ws), wsb, s),
+            "rr_linear_logp_fwd");
+    } else if (kind == 1) {
+      check(rr_linear_policy_fwd(P(h_), P(w_), dtc, rows, D, V, lp, ignore, tau, PF(a_), per, PF(o_), PF(r_), (float)values[1],
+                                 (float)values[2], (float)values[3], (int)reduction, MF(loss), P(state), sb, P(ws), wsb, s),
+            "rr_linear_policy_fwd");
+    } else {
+      check(rr_linear_preference_fwd(P(h_), P(w_), dtc, losses, per, D, V, lp, ignore, PF(r_), (float)values[1],
+                                     (float)values[2], (int)reduction, MF(loss), P(state), sb, P(ws), wsb, s),
+            "rr_linear_preference_fwd");
+    }
+    ctx->save_for_backward({w_, state});   // the state holds the rows of hidden that count
+    ctx->saved_data["rows"] = rows;
+    ctx->saved_data["kind"] = kind;
+    ctx->saved_data["group"] = kind == 2 && per > 0 ? 2 * per : (int64_t)1;
+    ctx->saved_data["tau"] = values[0];
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_second_derivatives();
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &w_ = s[0], &state = s[1];
+    const at::DeviceGuard guard(w_.device());
+    const int64_t rows = ctx->saved_data["rows"].toInt(), D = w_.size(1), V = w_.size(0);
+    const int dtc = dtype_code(w_.scalar_type());
+    const Tensor dloss = prep(grads[0], at::kFloat);
+    Tensor dh = ctx->needs_input_grad(0) ? at::empty({rows, D}, w_.options()) : Tensor();
+    Tensor dw = ctx->needs_input_grad(1) ? at::empty_like(w_) : Tensor();
+    const size_t wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 1);
+    const Tensor ws = workspace(wsb, w_.options());
+    check(rr_linear_logp_bwd(dloss.data_ptr<float>(), P(w_), dtc, rows, D, V, (float)ctx->saved_data["tau"].toDouble(),
+                             ctx->saved_data["group"].toInt(), ctx->saved_data["kind"].toInt() == 0 ? 1 : 0,
+                             (int)ctx->saved_data["reduction"].toInt(), P(state), state.defined() ? (size_t)state.numel() : 0,
+                             P(dh), P(dw), P(ws), wsb, stream_of(w_)),
+          "rr_linear_logp_bwd");
+    return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor linear_logp(const Tensor& hidden, const Tensor& weight, const Tensor& labels, const c10::optional<Tensor>& advantages,
+                   const c10::optional<Tensor>& old, const c10::optional<Tensor>& ref, int64_t kind, int64_t losses, int64_t per,
+                   int64_t ignore, std::vector<double> values, int64_t reduction, int64_t grad) {
+  const Tensor a = opt(advantages), o = opt(old), r = opt(ref);
+  require_device({&hidden, &weight, &labels, &a, &o, &r});
+  return LinearLogpFn::apply(hidden, weight, labels, advantages, old, ref, kind, losses, per, ignore, values, reduction, grad);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
@@ -451,6 +527,7 @@ PYBIND11_MODULE(_autograd, m) {
   m.def("gla_scan", &gla_scan, "GLA scan (y, final state) as one C++ autograd node");
   m.def("layer_norm", &layer_norm, "layer norm as one C++ autograd node");
   m.def("linear_loss", &linear_loss, "cross entropy or distillation from hidden states as one C++ autograd node");
+  m.def("linear_logp", &linear_logp, "log-probabilities from hidden states, or a loss on them, as one C++ autograd node");
   // the header revision this module was compiled against (not the loaded
   // library's, which the Python loader compares it with)
   m.def("abi_version", [] { return RR_ABI_VERSION; });

@@ -14,6 +14,8 @@ the reference):
     norm         — layer norm
     linear_loss  — cross entropy and distillation over a large vocabulary, straight
                    from hidden states
+    linear_logp  — log-probabilities, a clipped policy loss and a preference loss, the
+                   same way
 
 Each scan keeps the reference's signature, shape rules and fp32 state /
 accumulation, and is differentiable through ``torch.autograd``.  The compute
@@ -38,6 +40,8 @@ from .gdn import gated_deltanet_scan, gated_deltanet_scan_with_state, gated_delt
 from .norm import layer_norm, layer_norm_reference
 from .linear_loss import (linear_cross_entropy, linear_cross_entropy_reference, linear_distillation,
                           linear_distillation_reference)
+from .linear_logp import (linear_log_probs, linear_log_probs_reference, linear_policy_loss, linear_policy_loss_reference,
+                          linear_preference_loss, linear_preference_loss_reference)
 
 __all__ = [
     "ssd_scan",
@@ -76,6 +80,12 @@ __all__ = [
     "linear_cross_entropy_reference",
     "linear_distillation",
     "linear_distillation_reference",
+    "linear_log_probs",
+    "linear_log_probs_reference",
+    "linear_policy_loss",
+    "linear_policy_loss_reference",
+    "linear_preference_loss",
+    "linear_preference_loss_reference",
 ]
 
 __version__ = "0.3.0+gfx950"

@@ -92,6 +92,14 @@ _SIGS = {
                          + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
     "rr_linear_loss_bwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 4 + [_c_f32] * 2 + [_c_int, _c_ptr, _c_size]
                            + [_c_ptr] * 3 + [_c_size, _c_ptr]),
+    "rr_linear_logp_fwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 3 + [_c_ptr, _c_i64, _c_f32]
+                           + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
+    "rr_linear_policy_fwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 3 + [_c_ptr, _c_i64, _c_f32, _c_ptr, _c_i64]
+                             + [_c_ptr] * 2 + [_c_f32] * 3 + [_c_int] + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
+    "rr_linear_preference_fwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 4 + [_c_ptr, _c_i64, _c_ptr] + [_c_f32] * 2
+                                 + [_c_int] + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
+    "rr_linear_logp_bwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 3 + [_c_f32, _c_i64] + [_c_int] * 2
+                           + [_c_ptr, _c_size] + [_c_ptr] * 3 + [_c_size, _c_ptr]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGS)
@@ -143,7 +151,7 @@ def autograd_ext():
             from . import _autograd as mod
         except ImportError:
             mod = None
-        if mod is not None and (mod.abi_version() != load().rr_abi_version() or not hasattr(mod, "linear_loss")):
+        if mod is not None and (mod.abi_version() != load().rr_abi_version() or not hasattr(mod, "linear_logp")):
             mod = None   # built against another revision of the library, or from an older source
         _autograd_mod = mod
     return _autograd_mod
@@ -568,3 +576,39 @@ def linear_loss_bwd(dloss, weight, rows, K, z_loss, temperature, reduction, stat
                                      reduction, ptr(state), 0 if state is None else state.numel(), ptr(dhidden),
                                      ptr(dweight), ptr(ws), 0 if ws is None else ws.numel(), stream_of(weight)),
            "rr_linear_loss_bwd")
+
+
+def _sized(t):
+    return ptr(t), 0 if t is None else t.numel()
+
+
+def linear_logp_fwd(hidden, weight, labels, ignore_index, temperature, out, state, ws):
+    (rows, D), V = hidden.shape, weight.shape[0]
+    _check(load().rr_linear_logp_fwd(ptr(hidden), ptr(weight), DTYPE_CODE[hidden.dtype], rows, D, V, ptr(labels), ignore_index,
+                                     temperature, ptr(out), *_sized(state), *_sized(ws), stream_of(hidden)),
+           "rr_linear_logp_fwd")
+
+
+def linear_policy_fwd(hidden, weight, labels, ignore_index, temperature, advantages, per, old, ref, clip_low, clip_high,
+                      kl_weight, reduction, loss, state, ws):
+    (rows, D), V = hidden.shape, weight.shape[0]
+    _check(load().rr_linear_policy_fwd(ptr(hidden), ptr(weight), DTYPE_CODE[hidden.dtype], rows, D, V, ptr(labels),
+                                       ignore_index, temperature, ptr(advantages), per, ptr(old), ptr(ref), clip_low,
+                                       clip_high, kl_weight, reduction, ptr(loss), *_sized(state), *_sized(ws),
+                                       stream_of(hidden)), "rr_linear_policy_fwd")
+
+
+def linear_preference_fwd(hidden, weight, labels, ignore_index, pairs, L, ref, beta, label_smoothing, reduction, loss, state,
+                          ws):
+    V, D = weight.shape
+    _check(load().rr_linear_preference_fwd(ptr(hidden), ptr(weight), DTYPE_CODE[hidden.dtype], pairs, L, D, V, ptr(labels),
+                                           ignore_index, ptr(ref), beta, label_smoothing, reduction, ptr(loss),
+                                           *_sized(state), *_sized(ws), stream_of(hidden)), "rr_linear_preference_fwd")
+
+
+def linear_logp_bwd(dloss, weight, rows, temperature, rows_per_loss, of_log_probs, reduction, state, dhidden, dweight):
+    V, D = weight.shape
+    ws = _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[weight.dtype], 1)), weight.device)
+    _check(load().rr_linear_logp_bwd(ptr(dloss), ptr(weight), DTYPE_CODE[weight.dtype], rows, D, V, temperature,
+                                     rows_per_loss, of_log_probs, reduction, *_sized(state), ptr(dhidden), ptr(dweight),
+                                     *_sized(ws), stream_of(weight)), "rr_linear_logp_bwd")
