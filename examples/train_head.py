@@ -1,10 +1,10 @@
 """A small recurrent language model trained on labels and on a teacher's top logits.
 
-    python examples/train_head.py [--steps 60] [--vocab 2000] [--width 256]
+    python examples/train_head.py [--steps 60] [--vocab 2000] [--width 256] [--max-norm inf]
 
 Embedding -> layer norm -> gated RG-LRU -> residual -> layer norm -> output head, whose losses
 (cross entropy on the next token, distillation from a teacher's top 16 logits) come straight
-from the hidden states.  The data are a random Markov chain and the
+from the hidden states; the gradients are clipped by their norm.  The data are a random Markov chain and the
 teacher is the chain itself, so both losses have a known floor and fall towards it.  Needs an
 MI355X and the built library.
 """
@@ -72,7 +72,8 @@ def sample(ids, logits, batch, length, g):
     return torch.stack(tokens, 1)
 
 
-def train(steps=60, vocab=2000, width=256, batch=16, length=128, temperature=2.0, report=print):
+def train(steps=60, vocab=2000, width=256, batch=16, length=128, temperature=2.0, report=print,
+          max_norm=math.inf):
     device = torch.device("cuda:0")
     ids, logits = chain(vocab, device)
     g = torch.Generator(device=device).manual_seed(2)
@@ -90,10 +91,12 @@ def train(steps=60, vocab=2000, width=256, batch=16, length=128, temperature=2.0
         kd = mr.linear_distillation(hidden, head, logits[inputs], t_ids, temperature=temperature)
         optimiser.zero_grad(set_to_none=True)
         (ce + kd).backward()
+        norm = mr.clip_grad_norm([p.grad for p in model.parameters()], max_norm)
         optimiser.step()
         history.append((ce.detach(), kd.detach()))
         if step % 10 == 0 or step == steps - 1:
-            report(f"step {step:4d}  cross entropy {float(ce.detach()):.3f}  distillation {float(kd.detach()):.3f}")
+            report(f"step {step:4d}  cross entropy {float(ce.detach()):.3f}  distillation {float(kd.detach()):.3f}"
+                   f"  gradients' norm {float(norm):.3f}")
     p = torch.softmax(logits, -1)
     report(f"floor      cross entropy {float(-(p * p.log()).sum(-1).mean()):.3f}  distillation 0; "
            f"an untrained head: {math.log(vocab):.3f}")
@@ -105,5 +108,6 @@ if __name__ == "__main__":
     ap.add_argument("--steps", type=int, default=60)
     ap.add_argument("--vocab", type=int, default=2000)
     ap.add_argument("--width", type=int, default=256)
+    ap.add_argument("--max-norm", type=float, default=math.inf)
     a = ap.parse_args()
-    train(a.steps, a.vocab, a.width)
+    train(a.steps, a.vocab, a.width, max_norm=a.max_norm)

@@ -484,6 +484,22 @@ int rr_linear_logp_bwd(const float* dloss, const void* weight, int dtype, int64_
                        size_t state_bytes, void* dhidden, void* dweight, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* ------------------------------------------------------- norm of gradients --
+ * What a training step ends in (no reference counterpart): the norm of `count` tensors taken
+ * together, n = sqrt(sum of all squares), and their scaling down to a largest norm,
+ * out = g max_norm / n where n > max_norm, else g.  grads and out: device addresses in host
+ * memory, of numel[i] contiguous values of dtypes[i] each, at any multiple of an element's size;
+ * out[i] may be grads[i], and nothing else of what is written may share memory with another
+ * tensor.  The arrays are not read after the call returns.  norm: one fp32 on the device.
+ * Sums and products are in 64 bits, added in a fixed order.  A norm that is not finite leaves the
+ * values as they are.  max_norm >= 0, infinity: nothing is scaled. */
+size_t rr_grad_norm_workspace_bytes(int64_t count);
+int rr_grad_norm(int64_t count, const void* const* grads, const int64_t* numel, const int* dtypes, float* norm,
+                 void* workspace, size_t workspace_bytes, void* stream);
+int rr_clip_grad_norm(int64_t count, const void* const* grads, void* const* out, const int64_t* numel,
+                      const int* dtypes, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,360 @@
+// grad_norm.hip — the norm of many tensors taken together, and their scaling down to a
+// largest norm, on gfx950.
+//
+//   n = sqrt(sum over all tensors of g^2);  f = max / n where n > max, else 1;  out = f g
+//
+// Two launches for up to 128 tensors: the first leaves a partial sum a workgroup, every
+// workgroup of the second adds those up (in the same order, so all have the same f) and
+// scales its share.  The table of tensors travels in the kernels' arguments: nothing is copied
+// to the device and nothing waits, so a call can be captured in a graph.
+//
+// Sums are in 64 bits, and so is the product: squares of any fp32 value neither overflow nor
+// vanish, and what is left is the rounding to the output's type.
+#include "rr_common.h"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+#include <vector>
+
+namespace {
+
+using rr::bf16;
+using rr::f16;
+
+constexpr int kTensors = 128;      // of a launch: the table is below the 4 KiB that arguments may take
+constexpr int kThreads = 256;
+constexpr int kVec = 8;            // values a thread takes at a time
+constexpr int kStep = kThreads * kVec;
+constexpr int kGroups = 2048;      // workgroups at one time: eight a CU
+
+struct Table {
+  const void* in[kTensors];
+  void* out[kTensors];
+  int64_t n[kTensors];
+  int first[kTensors + 1];         // chunks of the tensors in front of each
+  uint8_t type[kTensors];
+  int tensors, chunk;              // values of a chunk
+};
+static_assert(sizeof(Table) <= 3800, "arguments of a launch");
+
+// The tensor of a chunk: the last whose first chunk is not behind it.
+__device__ __forceinline__ int tensor_of(const Table& t, int c) {
+  int lo = 0, hi = t.tensors - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Eight values as they lie in memory, from any element on.
+template <typename X>
+struct Eight {
+  typedef uint32_t Words __attribute__((ext_vector_type(2 * sizeof(X))));
+  typedef Words Any __attribute__((aligned(sizeof(X))));
+  X v[kVec];
+  __device__ __forceinline__ void load(const X* p) {
+    const Words w = *reinterpret_cast<const Any*>(p);
+    __builtin_memcpy(v, &w, sizeof(w));
+  }
+  __device__ __forceinline__ void store(X* p) const {
+    Words w;
+    __builtin_memcpy(&w, v, sizeof(w));
+    *reinterpret_cast<Any*>(p) = w;
+  }
+};
+
+__device__ __forceinline__ double wave_add(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// Of the whole workgroup, to all of its threads.
+__device__ __forceinline__ double group_add(double v, double* buf) {
+  v = wave_add(v);
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (buf[0] + buf[1]) + (buf[2] + buf[3]);
+}
+
+template <typename X>
+__device__ __forceinline__ double squares(const X* p, int n) {
+  double a[4] = {0, 0, 0, 0};
+  int i = threadIdx.x * kVec;
+  constexpr int kDeep = 4;   // loads on their way at one time
+  for (; i + (kDeep - 1) * kStep + kVec <= n; i += kDeep * kStep) {
+    Eight<X> x[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) x[d].load(p + i + d * kStep);
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const double g = (double)rr::to_f32(x[d].v[e]);
+        a[e & 3] = fma(g, g, a[e & 3]);
+      }
+  }
+  for (; i + kVec <= n; i += kStep) {
+    Eight<X> x;
+    x.load(p + i);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const double g = (double)rr::to_f32(x.v[e]);
+      a[e & 3] = fma(g, g, a[e & 3]);
+    }
+  }
+  for (int e = 0; i + e < n && e < kVec; ++e) {
+    const double g = (double)rr::to_f32(p[i + e]);
+    a[0] = fma(g, g, a[0]);
+  }
+  return (a[0] + a[1]) + (a[2] + a[3]);
+}
+
+template <typename X>
+__device__ __forceinline__ X scaled(X g, double f) { return rr::from_f32<X>((float)((double)rr::to_f32(g) * f)); }
+
+template <typename X>
+__device__ __forceinline__ void scale(const X* p, X* o, int n, double f) {
+  int i = threadIdx.x * kVec;
+  constexpr int kDeep = 4;
+  for (; i + (kDeep - 1) * kStep + kVec <= n; i += kDeep * kStep) {
+    Eight<X> x[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) x[d].load(p + i + d * kStep);
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) x[d].v[e] = scaled(x[d].v[e], f);
+      x[d].store(o + i + d * kStep);
+    }
+  }
+  for (; i + kVec <= n; i += kStep) {
+    Eight<X> x;
+    x.load(p + i);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x.v[e] = scaled(x.v[e], f);
+    x.store(o + i);
+  }
+  for (int e = 0; i + e < n && e < kVec; ++e) o[i + e] = scaled(p[i + e], f);
+}
+
+// What a chunk is: its tensor, where it starts there and how many values it has.
+struct Chunk {
+  int i, n;
+  int64_t at;
+};
+__device__ __forceinline__ Chunk chunk_of(const Table& t, int c) {
+  Chunk k;
+  k.i = __builtin_amdgcn_readfirstlane(tensor_of(t, c));
+  k.at = (int64_t)(c - t.first[k.i]) * t.chunk;
+  k.n = (int)min((int64_t)t.chunk, t.n[k.i] - k.at);
+  return k;
+}
+
+__global__ void __launch_bounds__(kThreads)
+squares_kernel(Table t, int chunks, double* __restrict__ part) {
+  __shared__ double buf[4];
+  double s = 0;
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const Chunk k = chunk_of(t, c);
+    const void* p = t.in[k.i];
+    if (t.type[k.i] == RR_F32) s += squares(static_cast<const float*>(p) + k.at, k.n);
+    else if (t.type[k.i] == RR_BF16) s += squares(static_cast<const bf16*>(p) + k.at, k.n);
+    else s += squares(static_cast<const f16*>(p) + k.at, k.n);
+  }
+  s = group_add(s, buf);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+// The norm from the partial sums, by a workgroup.
+__device__ __forceinline__ double norm_of(const double* __restrict__ part, int parts, double* buf) {
+  double s = 0;
+  for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
+  return sqrt(group_add(s, buf));
+}
+
+__global__ void __launch_bounds__(kThreads)
+norm_kernel(const double* __restrict__ part, int parts, float* norm) {
+  __shared__ double buf[4];
+  const double n = norm_of(part, parts, buf);
+  if (threadIdx.x == 0) *norm = (float)n;
+}
+
+// The last chunks come first: they are what the caches still hold of the first launch.
+__global__ void __launch_bounds__(kThreads)
+scale_kernel(Table t, int chunks, const double* __restrict__ part, int parts, double most, float* norm) {
+  __shared__ double buf[4];
+  const double n = norm_of(part, parts, buf);
+  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+  const double f = n > most && n < INFINITY ? most / n : 1.;
+  for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+    const Chunk k = chunk_of(t, c);
+    const void* p = t.in[k.i];
+    void* o = t.out[k.i];
+    if (f == 1. && p == o) continue;
+    if (t.type[k.i] == RR_F32) scale(static_cast<const float*>(p) + k.at, static_cast<float*>(o) + k.at, k.n, f);
+    else if (t.type[k.i] == RR_BF16) scale(static_cast<const bf16*>(p) + k.at, static_cast<bf16*>(o) + k.at, k.n, f);
+    else scale(static_cast<const f16*>(p) + k.at, static_cast<f16*>(o) + k.at, k.n, f);
+  }
+}
+
+// ------------------------------------------------------------------ host
+struct Launch {
+  Table table;
+  int chunks, groups;
+};
+
+int64_t bytes_of(int64_t n, int dtype) { return n * (dtype == RR_F32 ? 4 : 2); }
+
+int check_tensors(const char* who, int64_t count, const void* const* grads, const int64_t* numel, const int* dtypes) {
+  const std::string w(who);
+  if (count < 0 || count > (1 << 24)) return rr::fail(RR_EINVAL, w + ": 0 to 2^24 tensors");
+  if (count > 0 && (grads == nullptr || numel == nullptr || dtypes == nullptr)) return rr::fail(RR_EINVAL, w + ": null pointer");
+  for (int64_t i = 0; i < count; ++i) {
+    if (!rr::valid_dtype(dtypes[i])) return rr::fail(RR_EINVAL, w + ": unsupported dtype");
+    if (numel[i] < 0 || numel[i] > ((int64_t)1 << 48)) return rr::fail(RR_EINVAL, w + ": a tensor's size is out of range");
+    if (numel[i] == 0) continue;
+    if (grads[i] == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
+    if (reinterpret_cast<uintptr_t>(grads[i]) % bytes_of(1, dtypes[i]) != 0) return rr::fail(RR_EINVAL, w + ": misaligned tensor");
+  }
+  return RR_OK;
+}
+
+// What is written must not be another's: neither written nor read.
+int check_disjoint(const char* who, int64_t count, const void* const* grads, void* const* out, const int64_t* numel,
+                   const int* dtypes) {
+  const std::string w(who);
+  struct Range {
+    uintptr_t at, end;
+    int64_t i;
+  };
+  std::vector<Range> written;
+  for (int64_t i = 0; i < count; ++i) {
+    if (numel[i] == 0) continue;
+    if (out[i] == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
+    const uintptr_t at = reinterpret_cast<uintptr_t>(out[i]);
+    if (at % bytes_of(1, dtypes[i]) != 0) return rr::fail(RR_EINVAL, w + ": misaligned tensor");
+    written.push_back({at, at + (uintptr_t)bytes_of(numel[i], dtypes[i]), i});
+  }
+  std::sort(written.begin(), written.end(), [](const Range& a, const Range& b) { return a.at < b.at; });
+  for (size_t k = 1; k < written.size(); ++k)
+    if (written[k].at < written[k - 1].end) return rr::fail(RR_EINVAL, w + ": two of the tensors to write share memory");
+  for (int64_t i = 0; i < count; ++i) {
+    if (numel[i] == 0 || grads[i] == out[i]) continue;   // (what is written in place shares nothing, as just seen)
+    const uintptr_t at = reinterpret_cast<uintptr_t>(grads[i]), end = at + (uintptr_t)bytes_of(numel[i], dtypes[i]);
+    auto k = std::upper_bound(written.begin(), written.end(), at, [](uintptr_t v, const Range& r) { return v < r.end; });
+    if (k != written.end() && k->at < end) return rr::fail(RR_EINVAL, w + ": a tensor to write shares memory with another to read");
+  }
+  return RR_OK;
+}
+
+int64_t launches_of(int64_t count) { return std::max<int64_t>(1, (count + kTensors - 1) / kTensors); }
+
+// The launches over the tensors: chunks of 2048 to 16384 values, so that many small tensors make
+// enough of them and large ones not too many to look up; workgroups in proportion to their chunks.
+int plan(const char* who, int64_t count, const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
+         std::vector<Launch>* launches) {
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) total += numel[i];
+  int chunk = kStep;
+  while (chunk < 8 * kStep && total / chunk > 4 * kGroups) chunk *= 2;
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < count; ++i) chunks += (numel[i] + chunk - 1) / chunk;
+  if (chunks >= ((int64_t)1 << 31)) return rr::fail(RR_EUNSUPPORTED, std::string(who) + ": too many values");
+  Launch l{};
+  auto flush = [&] {
+    Table& t = l.table;
+    if (t.tensors == 0) return;
+    l.chunks = t.first[t.tensors];
+    l.groups = (int)std::min<int64_t>(l.chunks, std::max<int64_t>(1, kGroups * (int64_t)l.chunks / chunks));
+    launches->push_back(l);
+    l = Launch{};
+  };
+  for (int64_t i = 0; i < count; ++i) {
+    if (numel[i] == 0) continue;
+    Table& t = l.table;
+    t.chunk = chunk;
+    t.in[t.tensors] = grads[i], t.out[t.tensors] = out == nullptr ? nullptr : out[i];
+    t.n[t.tensors] = numel[i], t.type[t.tensors] = (uint8_t)dtypes[i];
+    t.first[t.tensors + 1] = t.first[t.tensors] + (int)((numel[i] + chunk - 1) / chunk);
+    if (++t.tensors == kTensors) flush();
+  }
+  flush();
+  return RR_OK;
+}
+
+int run_norm(const std::vector<Launch>& launches, double* part, hipStream_t s) {
+  int parts = 0;
+  for (const Launch& l : launches) {
+    squares_kernel<<<(unsigned)l.groups, kThreads, 0, s>>>(l.table, l.chunks, part + parts);
+    parts += l.groups;
+  }
+  return parts;
+}
+
+int check_workspace(const char* who, int64_t count, const void* ws, size_t ws_bytes, const float* norm) {
+  const std::string w(who);
+  if (norm == nullptr || ws == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
+  if (ws_bytes < rr_grad_norm_workspace_bytes(count)) return rr::fail(RR_EWORKSPACE, w + ": workspace too small");
+  if (reinterpret_cast<uintptr_t>(ws) % 16 != 0) return rr::fail(RR_EWORKSPACE, w + ": workspace misaligned");
+  return RR_OK;
+}
+
+// (std::vector may throw; nothing leaves a C entry)
+template <typename F>
+int guarded(const char* who, F f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return rr::fail(RR_EINVAL, std::string(who) + ": " + e.what());
+  }
+}
+
+}  // namespace
+
+extern "C" size_t rr_grad_norm_workspace_bytes(int64_t count) {
+  if (count < 0 || count > (1 << 24)) return 0;
+  return (size_t)(kGroups + launches_of(count)) * sizeof(double);   // a launch's share of the workgroups is at least one
+}
+
+extern "C" int rr_grad_norm(int64_t count, const void* const* grads, const int64_t* numel, const int* dtypes, float* norm,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "rr_grad_norm";
+  return guarded(who, [&]() -> int {
+    if (int rc = check_tensors(who, count, grads, numel, dtypes)) return rc;
+    if (int rc = check_workspace(who, count, workspace, workspace_bytes, norm)) return rc;
+    std::vector<Launch> launches;
+    if (int rc = plan(who, count, grads, nullptr, numel, dtypes, &launches)) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    double* part = static_cast<double*>(workspace);
+    const int parts = run_norm(launches, part, s);
+    norm_kernel<<<1, kThreads, 0, s>>>(part, parts, norm);
+    return rr::check_launch(who);
+  });
+}
+
+extern "C" int rr_clip_grad_norm(int64_t count, const void* const* grads, void* const* out, const int64_t* numel,
+                                 const int* dtypes, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  const char* who = "rr_clip_grad_norm";
+  return guarded(who, [&]() -> int {
+    if (int rc = check_tensors(who, count, grads, numel, dtypes)) return rc;
+    if (!(max_norm >= 0)) return rr::fail(RR_EINVAL, std::string(who) + ": max_norm must not be negative");
+    if (count > 0 && out == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
+    if (int rc = check_workspace(who, count, workspace, workspace_bytes, norm)) return rc;
+    if (int rc = check_disjoint(who, count, grads, out, numel, dtypes)) return rc;
+    std::vector<Launch> launches;
+    if (int rc = plan(who, count, grads, out, numel, dtypes, &launches)) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    double* part = static_cast<double*>(workspace);
+    const int parts = run_norm(launches, part, s);
+    if (launches.empty()) norm_kernel<<<1, kThreads, 0, s>>>(part, 0, norm);
+    for (size_t k = 0; k < launches.size(); ++k) {
+      const Launch& l = launches[k];
+      scale_kernel<<<(unsigned)l.groups, kThreads, 0, s>>>(l.table, l.chunks, part, parts, max_norm, k == 0 ? norm : nullptr);
+    }
+    return rr::check_launch(who);
+  });
+}

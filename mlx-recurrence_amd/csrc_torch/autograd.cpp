@@ -16,8 +16,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/utils.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/recurrence.h"
@@ -519,6 +521,79 @@ Tensor linear_logp(const Tensor& hidden, const Tensor& weight, const Tensor& lab
   return LinearLogpFn::apply(hidden, weight, labels, advantages, old, ref, kind, losses, per, ignore, values, reduction, grad);
 }
 
+// ------------------------------------------------------------------ norm of gradients
+// The norm of all of `grads` together; with `clip` they leave scaled to max_norm at most, in place or,
+// where `outs` has tensors, there (mlx_recurrence_amd.grad_norm._run, which checks the same).
+Tensor grad_norm(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs, bool clip, double max_norm) {
+  const at::Device dev = grads[0].device();
+  const size_t n = grads.size();
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& g = grads[i];
+    if (g.layout() != at::kStrided) throw pybind11::type_error("gradients must be dense tensors");
+    require_device({&grads[0], &g});
+    if (at::GradMode::is_enabled() && g.requires_grad()) {
+      throw pybind11::value_error("the norm of gradients is not differentiable; call it under torch.no_grad()");
+    }
+    const at::ScalarType t = g.scalar_type();
+    if (t != at::kFloat && t != at::kBFloat16 && t != at::kHalf) {
+      throw pybind11::type_error("gradients must be float32, bfloat16 or float16");
+    }
+    if (outs.empty()) continue;
+    const Tensor& o = outs[i];
+    if (o.layout() != at::kStrided || o.sizes() != g.sizes() || o.scalar_type() != t) {
+      throw pybind11::value_error("out must have a tensor of each gradient's shape and type");
+    }
+    require_device({&g, &o});
+  }
+  const at::DeviceGuard guard(dev);
+  std::vector<const void*> in(n);
+  std::vector<void*> to(n);
+  std::vector<int64_t> numel(n);
+  std::vector<int> types(n);
+  std::vector<Tensor> held;                                // what lives until the launches are made
+  std::vector<std::pair<Tensor, Tensor>> back;             // copies to go back to tensors with gaps
+  std::vector<const void*> gaps;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& g = grads[i];
+    const bool dense = g.is_non_overlapping_and_dense();
+    Tensor src = g;
+    if (!dense) held.push_back(src = g.contiguous());
+    in[i] = src.data_ptr(), numel[i] = src.numel(), types[i] = dtype_code(src.scalar_type());
+    if (!clip) continue;
+    const Tensor& o = outs.empty() ? g : outs[i];
+    if (o.is_non_overlapping_and_dense() && o.strides() == src.strides()) {
+      to[i] = o.data_ptr();
+      continue;
+    }
+    for (int64_t d = 0; d < o.dim(); ++d) {
+      if (o.stride(d) == 0 && o.size(d) > 1) throw pybind11::value_error("a tensor to write has its values more than once");
+    }
+    gaps.push_back(o.data_ptr());
+    const Tensor tmp = outs.empty() ? src : at::empty_like(src);
+    to[i] = tmp.data_ptr();
+    back.emplace_back(o, tmp);
+  }
+  std::sort(gaps.begin(), gaps.end());
+  if (std::adjacent_find(gaps.begin(), gaps.end()) != gaps.end()) {
+    throw pybind11::value_error("two of the tensors to write share memory");
+  }
+  Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
+  const size_t wsb = rr_grad_norm_workspace_bytes((int64_t)n);
+  const Tensor ws = workspace(wsb, norm.options());
+  if (!clip) {
+    check(rr_grad_norm((int64_t)n, in.data(), numel.data(), types.data(), MF(norm), P(ws), wsb, stream_of(norm)), "rr_grad_norm");
+    return norm;
+  }
+  check(rr_clip_grad_norm((int64_t)n, in.data(), to.data(), numel.data(), types.data(), max_norm, MF(norm), P(ws), wsb,
+                          stream_of(norm)),
+        "rr_clip_grad_norm");
+  const at::NoGradGuard no_grad;
+  for (const auto& [o, tmp] : back) o.copy_(tmp);
+  // (copy_ has counted its own)
+  for (size_t i = 0; i < n; ++i) (outs.empty() ? grads[i] : outs[i]).unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
@@ -528,6 +603,7 @@ PYBIND11_MODULE(_autograd, m) {
   m.def("layer_norm", &layer_norm, "layer norm as one C++ autograd node");
   m.def("linear_loss", &linear_loss, "cross entropy or distillation from hidden states as one C++ autograd node");
   m.def("linear_logp", &linear_logp, "log-probabilities from hidden states, or a loss on them, as one C++ autograd node");
+  m.def("grad_norm", &grad_norm, "the norm of tensors taken together, and their clipping by it");
   // the header revision this module was compiled against (not the loaded
   // library's, which the Python loader compares it with)
   m.def("abi_version", [] { return RR_ABI_VERSION; });

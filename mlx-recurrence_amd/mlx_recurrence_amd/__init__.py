@@ -16,6 +16,7 @@ the reference):
                    from hidden states
     linear_logp  — log-probabilities, a clipped policy loss and a preference loss, the
                    same way
+    grad_norm    — the norm of a step's gradients, and their clipping by it
 
 Each scan keeps the reference's signature, shape rules and fp32 state /
 accumulation, and is differentiable through ``torch.autograd``.  The compute
@@ -40,6 +41,7 @@ from .gdn import gated_deltanet_scan, gated_deltanet_scan_with_state, gated_delt
 from .norm import layer_norm, layer_norm_reference
 from .linear_loss import (linear_cross_entropy, linear_cross_entropy_reference, linear_distillation,
                           linear_distillation_reference)
+from .grad_norm import (clip_grad_norm, clip_grad_norm_reference, global_grad_norm, global_grad_norm_reference)
 from .linear_logp import (linear_log_probs, linear_log_probs_reference, linear_policy_loss, linear_policy_loss_reference,
                           linear_preference_loss, linear_preference_loss_reference)
 
@@ -80,6 +82,10 @@ __all__ = [
     "linear_cross_entropy_reference",
     "linear_distillation",
     "linear_distillation_reference",
+    "clip_grad_norm",
+    "clip_grad_norm_reference",
+    "global_grad_norm",
+    "global_grad_norm_reference",
     "linear_log_probs",
     "linear_log_probs_reference",
     "linear_policy_loss",

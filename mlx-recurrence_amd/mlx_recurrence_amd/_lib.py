@@ -100,6 +100,9 @@ _SIGS = {
                                  + [_c_int] + [_c_ptr] * 2 + [_c_size, _c_ptr, _c_size, _c_ptr]),
     "rr_linear_logp_bwd": (_c_int, [_c_ptr] * 2 + [_c_int] + [_c_i64] * 3 + [_c_f32, _c_i64] + [_c_int] * 2
                            + [_c_ptr, _c_size] + [_c_ptr] * 3 + [_c_size, _c_ptr]),
+    "rr_grad_norm_workspace_bytes": (_c_size, [_c_i64]),
+    "rr_grad_norm": (_c_int, [_c_i64] + [_c_ptr] * 5 + [_c_size, _c_ptr]),
+    "rr_clip_grad_norm": (_c_int, [_c_i64] + [_c_ptr] * 4 + [ctypes.c_double] + [_c_ptr] * 2 + [_c_size, _c_ptr]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGS)
@@ -151,7 +154,7 @@ def autograd_ext():
             from . import _autograd as mod
         except ImportError:
             mod = None
-        if mod is not None and (mod.abi_version() != load().rr_abi_version() or not hasattr(mod, "linear_logp")):
+        if mod is not None and (mod.abi_version() != load().rr_abi_version() or not hasattr(mod, "grad_norm")):
             mod = None   # built against another revision of the library, or from an older source
         _autograd_mod = mod
     return _autograd_mod
@@ -612,3 +615,19 @@ def linear_logp_bwd(dloss, weight, rows, temperature, rows_per_loss, of_log_prob
     _check(load().rr_linear_logp_bwd(ptr(dloss), ptr(weight), DTYPE_CODE[weight.dtype], rows, D, V, temperature,
                                      rows_per_loss, of_log_probs, reduction, *_sized(state), ptr(dhidden), ptr(dweight),
                                      *_sized(ws), stream_of(weight)), "rr_linear_logp_bwd")
+
+
+# ---------------------------------------------------------------- norm of gradients
+def grad_norm(grads, out, max_norm, norm):
+    """rr_grad_norm, or with `out` rr_clip_grad_norm, of tensors whose values lie in memory without gaps."""
+    n = len(grads)
+    ptrs = (_c_ptr * n)(*(t.data_ptr() for t in grads))
+    numel = (_c_i64 * n)(*(t.numel() for t in grads))
+    types = (_c_int * n)(*(DTYPE_CODE[t.dtype] for t in grads))
+    ws = _alloc_ws(_ws_bytes("rr_grad_norm_workspace_bytes", (n,)), norm.device)
+    if out is None:
+        _check(load().rr_grad_norm(n, ptrs, numel, types, ptr(norm), ptr(ws), ws.numel(), stream_of(norm)), "rr_grad_norm")
+        return
+    outs = (_c_ptr * n)(*(t.data_ptr() for t in out))
+    _check(load().rr_clip_grad_norm(n, ptrs, outs, numel, types, max_norm, ptr(norm), ptr(ws), ws.numel(), stream_of(norm)),
+           "rr_clip_grad_norm")

@@ -1,0 +1,133 @@
+"""grad_norm.py — the norm of a step's gradients taken together, and their clipping by it (no
+counterpart in the reference, which has the scans alone).
+
+    global_grad_norm(grads)                          -> norm
+    clip_grad_norm(grads, max_norm)                  -> norm, grads scaled in place
+    global_grad_norm_reference, clip_grad_norm_reference      (plain torch)
+
+Any number of tensors of any sizes and of the three input types together, in two launches for
+each 128 of them; nothing waits for the device.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+
+
+def _dense(t):
+    """Whether the values lie in memory without gaps, in any order of the axes."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _run(grads, outs, clip, max_norm):
+    """The C++ module's grad_norm for where it is not built."""
+    dev = _lib.require_device(*grads, *outs)
+    for i, g in enumerate(grads):
+        if g.layout != torch.strided:
+            raise TypeError("gradients must be dense tensors")
+        if torch.is_grad_enabled() and g.requires_grad:
+            raise ValueError("the norm of gradients is not differentiable; call it under torch.no_grad()")
+        if g.dtype not in _lib.DTYPE_CODE:
+            raise TypeError("gradients must be float32, bfloat16 or float16")
+        if outs and (outs[i].layout != torch.strided or outs[i].shape != g.shape or outs[i].dtype != g.dtype):
+            raise ValueError("out must have a tensor of each gradient's shape and type")
+    with _lib.device_guard(dev), torch.no_grad():
+        src = [g if _dense(g) else g.contiguous() for g in grads]
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        if not clip:
+            _lib.grad_norm(src, None, 0.0, norm)
+            return norm
+        written = outs or grads
+        to, back = [], []
+        for o, s in zip(written, src):
+            if _dense(o) and o.stride() == s.stride():
+                to.append(o)
+                continue
+            if any(st == 0 and sz > 1 for st, sz in zip(o.stride(), o.shape)):
+                raise ValueError("a tensor to write has its values more than once")
+            to.append(torch.empty_like(s) if outs else s)
+            back.append((o, to[-1]))
+        if len({o.data_ptr() for o, _ in back}) < len(back):
+            raise ValueError("two of the tensors to write share memory")
+        _lib.grad_norm(src, to, max_norm, norm)
+        for o, t in back:
+            o.copy_(t)
+        torch.autograd.graph.increment_version(written)
+    return norm
+
+
+def _tensors(grads):
+    grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
+    if not grads:
+        raise ValueError("no gradients to take a norm of")
+    return grads
+
+
+def global_grad_norm(grads):
+    """The 2-norm of all values of `grads` together, on the GPU.
+
+    Args:
+        grads:  tensors of any shapes and of the three input types, on one device (or one
+                tensor); entries that are None, of parameters without a gradient, are left out.
+
+    Returns:
+        norm:   fp32 scalar on the device.  Sums are in 64 bits, in a fixed order.
+    """
+    grads = _tensors(grads)
+    ext = _lib.autograd_ext()
+    return _run(grads, (), False, 0.0) if ext is None else ext.grad_norm(grads, (), False, 0.0)
+
+
+def clip_grad_norm(grads, max_norm, *, out=None):
+    """Scale `grads` in place so that their norm, taken together, is at most `max_norm`, on the GPU.
+
+    ``g *= max_norm / norm`` where ``norm > max_norm``; otherwise they are not touched.  A norm
+    that is infinite or NaN leaves them as they are: the caller sees it in what is returned.
+
+    Args:
+        grads:     as for global_grad_norm; tensors that share memory are refused.
+        max_norm:  the largest norm, 0 or more (math.inf: take the norm alone).
+        out:       tensors of the same shapes and types to write to, in place of `grads` (each
+                   a tensor of its own, or the gradient itself).
+
+    Returns:
+        norm:      before the clipping, as global_grad_norm's.  Not differentiable.
+    """
+    if not float(max_norm) >= 0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    if out is None:
+        grads, outs = _tensors(grads), ()
+    else:
+        grads, outs = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (grads, out))
+        if len(grads) != len(outs):
+            raise ValueError(f"out must have a tensor for each gradient, got {len(outs)} for {len(grads)}")
+        outs = [o for g, o in zip(grads, outs) if g is not None]
+        grads = _tensors(grads)
+        if any(o is None for o in outs):
+            raise ValueError("out must have a tensor of each gradient's shape and type")
+    ext = _lib.autograd_ext()
+    return _run(grads, outs, True, float(max_norm)) if ext is None else ext.grad_norm(grads, outs, True, float(max_norm))
+
+
+# ------------------------------------------------------------------ plain forms
+def global_grad_norm_reference(grads):
+    """global_grad_norm as plain torch ops in 64 bits.  Runs on any device."""
+    return torch.stack([g.detach().double().square().sum() for g in _tensors(grads)]).sum().sqrt().float()
+
+
+def clip_grad_norm_reference(grads, max_norm):
+    """clip_grad_norm as plain torch ops in 64 bits: (norm, scaled copies).  Runs on any device."""
+    grads = _tensors(grads)
+    norm = torch.stack([g.detach().double().square().sum() for g in grads]).sum().sqrt()
+    factor = torch.where((norm > max_norm) & (norm < math.inf), max_norm / norm, 1.0)
+    return norm.float(), [(g.detach().double() * factor).float().to(g.dtype) for g in grads]
