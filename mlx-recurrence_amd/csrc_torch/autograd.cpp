@@ -523,15 +523,34 @@ Tensor linear_logp(const Tensor& hidden, const Tensor& weight, const Tensor& lab
 
 // ------------------------------------------------------------------ norm of gradients
 // The norm of all of `grads` together; with `clip` they leave scaled to max_norm at most, in place or,
-// where `outs` has tensors, there (mlx_recurrence_amd.grad_norm._run, which checks the same).
-Tensor grad_norm(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs, bool clip, double max_norm) {
+// where `outs` is a list of as many, there (mlx_recurrence_amd.grad_norm._run, which checks the same).
+// The tensors are taken from Python's lists as they are: converting a list of 300 takes longer than its
+// kernels.
+Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::list>& out_list, bool clip, double max_norm) {
+  std::vector<Tensor> grads, outs;
+  const Py_ssize_t all = PyList_GET_SIZE(grad_list.ptr());
+  grads.reserve(all);
+  if (out_list.has_value()) outs.reserve(all);
+  for (Py_ssize_t i = 0; i < all; ++i) {
+    PyObject* g = PyList_GET_ITEM(grad_list.ptr(), i);
+    if (g == Py_None) continue;
+    if (!THPVariable_Check(g)) throw pybind11::type_error("gradients must be tensors or None");
+    grads.push_back(THPVariable_Unpack(g));
+    if (!out_list.has_value()) continue;
+    PyObject* o = PyList_GET_ITEM(out_list->ptr(), i);
+    if (!THPVariable_Check(o)) throw pybind11::value_error("out must have a tensor of each gradient's shape and type");
+    outs.push_back(THPVariable_Unpack(o));
+  }
+  if (grads.empty()) throw pybind11::value_error("no gradients to take a norm of");
   const at::Device dev = grads[0].device();
   const size_t n = grads.size();
+  const bool recording = at::GradMode::is_enabled();
+  require_device({&grads[0]});
   for (size_t i = 0; i < n; ++i) {
     const Tensor& g = grads[i];
     if (g.layout() != at::kStrided) throw pybind11::type_error("gradients must be dense tensors");
-    require_device({&grads[0], &g});
-    if (at::GradMode::is_enabled() && g.requires_grad()) {
+    if (g.device() != dev) require_device({&grads[0], &g});
+    if (recording && g.requires_grad()) {
       throw pybind11::value_error("the norm of gradients is not differentiable; call it under torch.no_grad()");
     }
     const at::ScalarType t = g.scalar_type();
@@ -543,7 +562,7 @@ Tensor grad_norm(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
     if (o.layout() != at::kStrided || o.sizes() != g.sizes() || o.scalar_type() != t) {
       throw pybind11::value_error("out must have a tensor of each gradient's shape and type");
     }
-    require_device({&g, &o});
+    if (o.device() != dev) require_device({&g, &o});
   }
   const at::DeviceGuard guard(dev);
   std::vector<const void*> in(n);

@@ -31,7 +31,15 @@ def _dense(t):
 
 def _run(grads, outs, clip, max_norm):
     """The C++ module's grad_norm for where it is not built."""
-    dev = _lib.require_device(*grads, *outs)
+    if outs is not None:
+        outs = [o for g, o in zip(grads, outs) if g is not None]
+        if not all(isinstance(o, torch.Tensor) for o in outs):
+            raise ValueError("out must have a tensor of each gradient's shape and type")
+    grads = [g for g in grads if g is not None]
+    if not all(isinstance(g, torch.Tensor) for g in grads):
+        raise TypeError("gradients must be tensors or None")
+    if not grads:
+        raise ValueError("no gradients to take a norm of")
     for i, g in enumerate(grads):
         if g.layout != torch.strided:
             raise TypeError("gradients must be dense tensors")
@@ -41,6 +49,7 @@ def _run(grads, outs, clip, max_norm):
             raise TypeError("gradients must be float32, bfloat16 or float16")
         if outs and (outs[i].layout != torch.strided or outs[i].shape != g.shape or outs[i].dtype != g.dtype):
             raise ValueError("out must have a tensor of each gradient's shape and type")
+    dev = _lib.require_device(*grads, *(outs or ()))
     with _lib.device_guard(dev), torch.no_grad():
         src = [g if _dense(g) else g.contiguous() for g in grads]
         norm = torch.empty((), dtype=torch.float32, device=dev)
@@ -66,8 +75,12 @@ def _run(grads, outs, clip, max_norm):
     return norm
 
 
+def _listed(tensors):
+    return tensors if isinstance(tensors, list) else [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+
+
 def _tensors(grads):
-    grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
+    grads = [g for g in _listed(grads) if g is not None]
     if not grads:
         raise ValueError("no gradients to take a norm of")
     return grads
@@ -83,9 +96,8 @@ def global_grad_norm(grads):
     Returns:
         norm:   fp32 scalar on the device.  Sums are in 64 bits, in a fixed order.
     """
-    grads = _tensors(grads)
     ext = _lib.autograd_ext()
-    return _run(grads, (), False, 0.0) if ext is None else ext.grad_norm(grads, (), False, 0.0)
+    return (_run if ext is None else ext.grad_norm)(_listed(grads), None, False, 0.0)
 
 
 def clip_grad_norm(grads, max_norm, *, out=None):
@@ -105,18 +117,11 @@ def clip_grad_norm(grads, max_norm, *, out=None):
     """
     if not float(max_norm) >= 0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    if out is None:
-        grads, outs = _tensors(grads), ()
-    else:
-        grads, outs = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (grads, out))
-        if len(grads) != len(outs):
-            raise ValueError(f"out must have a tensor for each gradient, got {len(outs)} for {len(grads)}")
-        outs = [o for g, o in zip(grads, outs) if g is not None]
-        grads = _tensors(grads)
-        if any(o is None for o in outs):
-            raise ValueError("out must have a tensor of each gradient's shape and type")
+    grads, outs = _listed(grads), None if out is None else _listed(out)
+    if outs is not None and len(grads) != len(outs):
+        raise ValueError(f"out must have a tensor for each gradient, got {len(outs)} for {len(grads)}")
     ext = _lib.autograd_ext()
-    return _run(grads, outs, True, float(max_norm)) if ext is None else ext.grad_norm(grads, outs, True, float(max_norm))
+    return (_run if ext is None else ext.grad_norm)(grads, outs, True, float(max_norm))
 
 
 # ------------------------------------------------------------------ plain forms
