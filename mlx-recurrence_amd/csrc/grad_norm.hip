@@ -244,30 +244,57 @@ int check_tensors(const char* who, int64_t count, const void* const* grads, cons
   return RR_OK;
 }
 
+// Tensors one behind the other in memory, in and out: one run of values.
+struct Run {
+  const char* in;
+  char* out;
+  int64_t n;
+  int type;
+  int64_t bytes() const { return bytes_of(n, type); }
+};
+int runs_of(const char* who, int64_t count, const void* const* grads, void* const* out, const int64_t* numel,
+            const int* dtypes, std::vector<Run>* runs) {
+  const std::string w(who);
+  for (int64_t i = 0; i < count; ++i) {
+    if (numel[i] == 0) continue;
+    const char* in = static_cast<const char*>(grads[i]);
+    char* to = out == nullptr ? nullptr : static_cast<char*>(out[i]);
+    if (out != nullptr) {
+      if (to == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
+      if (reinterpret_cast<uintptr_t>(to) % bytes_of(1, dtypes[i]) != 0) return rr::fail(RR_EINVAL, w + ": misaligned tensor");
+    }
+    if (!runs->empty()) {
+      Run& r = runs->back();
+      if (r.type == dtypes[i] && in == r.in + r.bytes() && (out == nullptr || to == r.out + r.bytes())) {
+        r.n += numel[i];
+        continue;
+      }
+    }
+    runs->push_back({in, to, numel[i], dtypes[i]});
+  }
+  return RR_OK;
+}
+
 // What is written must not be another's: neither written nor read.
-int check_disjoint(const char* who, int64_t count, const void* const* grads, void* const* out, const int64_t* numel,
-                   const int* dtypes) {
+int check_disjoint(const char* who, const std::vector<Run>& runs) {
   const std::string w(who);
   struct Range {
     uintptr_t at, end;
-    int64_t i;
   };
   std::vector<Range> written;
-  for (int64_t i = 0; i < count; ++i) {
-    if (numel[i] == 0) continue;
-    if (out[i] == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
-    const uintptr_t at = reinterpret_cast<uintptr_t>(out[i]);
-    if (at % bytes_of(1, dtypes[i]) != 0) return rr::fail(RR_EINVAL, w + ": misaligned tensor");
-    written.push_back({at, at + (uintptr_t)bytes_of(numel[i], dtypes[i]), i});
+  written.reserve(runs.size());
+  for (const Run& r : runs) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(r.out);
+    written.push_back({at, at + (uintptr_t)r.bytes()});
   }
   auto before = [](const Range& a, const Range& b) { return a.at < b.at; };
   if (!std::is_sorted(written.begin(), written.end(), before)) std::sort(written.begin(), written.end(), before);
   for (size_t k = 1; k < written.size(); ++k)
     if (written[k].at < written[k - 1].end) return rr::fail(RR_EINVAL, w + ": two of the tensors to write share memory");
-  for (int64_t i = 0; i < count; ++i) {
-    if (numel[i] == 0 || grads[i] == out[i]) continue;   // (what is written in place shares nothing, as just seen)
-    const uintptr_t at = reinterpret_cast<uintptr_t>(grads[i]), end = at + (uintptr_t)bytes_of(numel[i], dtypes[i]);
-    auto k = std::upper_bound(written.begin(), written.end(), at, [](uintptr_t v, const Range& r) { return v < r.end; });
+  for (const Run& r : runs) {
+    if (r.in == r.out) continue;   // (what is written in place shares nothing, as just seen)
+    const uintptr_t at = reinterpret_cast<uintptr_t>(r.in), end = at + (uintptr_t)r.bytes();
+    auto k = std::upper_bound(written.begin(), written.end(), at, [](uintptr_t v, const Range& x) { return v < x.end; });
     if (k != written.end() && k->at < end) return rr::fail(RR_EINVAL, w + ": a tensor to write shares memory with another to read");
   }
   return RR_OK;
@@ -278,32 +305,10 @@ int64_t launches_of(int64_t count) { return std::max<int64_t>(1, (count + kTenso
 // The launches over the tensors.  Chunks are of 2048 to 16384 values, so that many small tensors make
 // enough of them and large ones not too many to look up (of 4096 at most: 660 us where it takes 552); workgroups
 // are in proportion to chunks.  *bytes: of all values.
-int plan(const char* who, int64_t count, const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes,
-         std::vector<Launch>* launches, int64_t* bytes) {
-  struct Run {   // tensors one behind the other in memory
-    const char* in;
-    char* out;
-    int64_t n;
-    int type;
-  };
-  std::vector<Run> runs;
+int plan(const char* who, const std::vector<Run>& runs, std::vector<Launch>* launches, int64_t* bytes) {
   int64_t total = 0;
   *bytes = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    if (numel[i] == 0) continue;
-    const char* in = static_cast<const char*>(grads[i]);
-    char* to = out == nullptr ? nullptr : static_cast<char*>(out[i]);
-    total += numel[i], *bytes += bytes_of(numel[i], dtypes[i]);
-    if (!runs.empty()) {
-      Run& r = runs.back();
-      const int64_t past = bytes_of(r.n, r.type);
-      if (r.type == dtypes[i] && in == r.in + past && (out == nullptr || to == r.out + past)) {
-        r.n += numel[i];
-        continue;
-      }
-    }
-    runs.push_back({in, to, numel[i], dtypes[i]});
-  }
+  for (const Run& r : runs) total += r.n, *bytes += r.bytes();
   int chunk = kStep;
   while (chunk < 8 * kStep && total / chunk > 4 * kGroups) chunk *= 2;
   int64_t chunks = 0;
@@ -326,7 +331,7 @@ int plan(const char* who, int64_t count, const void* const* grads, void* const* 
     t.in[t.tensors] = r.in, t.out[t.tensors] = r.out, t.n[t.tensors] = r.n, t.type[t.tensors] = (uint8_t)r.type;
     t.first[t.tensors + 1] = t.first[t.tensors] + mine;
     if (cold > 0) t.warm = t.first[t.tensors] + (int)std::min<int64_t>(mine, cold / bytes_of(chunk, r.type));
-    cold -= bytes_of(r.n, r.type);
+    cold -= r.bytes();
     if (++t.tensors == kTensors) flush();
   }
   flush();
@@ -373,9 +378,11 @@ extern "C" int rr_grad_norm(int64_t count, const void* const* grads, const int64
   return guarded(who, [&]() -> int {
     if (int rc = check_tensors(who, count, grads, numel, dtypes)) return rc;
     if (int rc = check_workspace(who, count, workspace, workspace_bytes, norm)) return rc;
+    std::vector<Run> runs;
     std::vector<Launch> launches;
     int64_t bytes = 0;
-    if (int rc = plan(who, count, grads, nullptr, numel, dtypes, &launches, &bytes)) return rc;
+    if (int rc = runs_of(who, count, grads, nullptr, numel, dtypes, &runs)) return rc;
+    if (int rc = plan(who, runs, &launches, &bytes)) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     double* part = static_cast<double*>(workspace);
     const int parts = run_norm(launches, part, s);
@@ -393,10 +400,12 @@ extern "C" int rr_clip_grad_norm(int64_t count, const void* const* grads, void* 
     if (!(max_norm >= 0)) return rr::fail(RR_EINVAL, std::string(who) + ": max_norm must not be negative");
     if (count > 0 && out == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
     if (int rc = check_workspace(who, count, workspace, workspace_bytes, norm)) return rc;
-    if (int rc = check_disjoint(who, count, grads, out, numel, dtypes)) return rc;
+    std::vector<Run> runs;
     std::vector<Launch> launches;
     int64_t bytes = 0;
-    if (int rc = plan(who, count, grads, out, numel, dtypes, &launches, &bytes)) return rc;
+    if (int rc = runs_of(who, count, grads, out, numel, dtypes, &runs)) return rc;
+    if (int rc = check_disjoint(who, runs)) return rc;
+    if (int rc = plan(who, runs, &launches, &bytes)) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     double* part = static_cast<double*>(workspace);
     const int parts = run_norm(launches, part, s);

@@ -123,6 +123,7 @@ struct Carve {
 struct Header {
   int n;                 // rows that count
   int count;             // what the mean is over: those rows, or the pairs that count
+  float top;             // the largest of the rows' derivatives that the forward left (State.z2)
 };
 struct State {
   Header* hdr;
@@ -420,6 +421,74 @@ __device__ __forceinline__ void load8(const X* row, int c, int D, X (&v)[8]) {
   }
 }
 
+// A row of an operand by a workgroup: copied, padded with zeros to Dp channels.  amax: null, or where
+// fp16's largest finite |value| goes.
+template <typename X>
+__device__ __forceinline__ void pack_row(const X* xr, int D, int Dp, X* out, float* amax, float* buf) {
+  float m = 0.f;
+  for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
+    X v[8];
+    load8(xr, c, D, v);
+    if constexpr (__is_same(X, f16)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = fabsf(rr::to_f32(v[e]));
+        if (a < INFINITY) m = fmaxf(m, a);   // neither infinite nor NaN
+      }
+    }
+    typedef uint32_t Words __attribute__((ext_vector_type(2 * sizeof(X))));
+    Words q;
+    __builtin_memcpy(&q, v, sizeof(q));
+    *reinterpret_cast<Words*>(out + c) = q;
+  }
+  if constexpr (__is_same(X, f16)) {
+    if (amax == nullptr) return;
+    m = wave_max(m);
+    __syncthreads();   // the last row's reads of buf are done
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) *amax = fmaxf(fmaxf(buf[0], buf[1]), fmaxf(buf[2], buf[3]));
+  }
+}
+
+// rows_kernel<true> and pack_kernel in one launch, for few rows: a workgroup a row, which
+// finds its place by reading the labels in front of it (1536 rows of 768 channels: 9.7 us in two
+// launches, 6.2 in one; with 2048 rows that is 16 MB from the caches).
+constexpr int64_t kRowsInOne = 2048;
+template <typename X>
+__global__ void __launch_bounds__(256)
+rows_pack_kernel(const X* __restrict__ hidden, const X* __restrict__ weight, const int64_t* __restrict__ labels,
+                 int64_t ignore, int T, int V, int D, int Dp, State st, float* __restrict__ loss) {
+  __shared__ float buf[4];
+  __shared__ int counts[4];
+  const int tid = threadIdx.x;
+  if (blockIdx.y == 1) {
+    for (int64_t r = blockIdx.x; r < V; r += gridDim.x) pack_row(weight + r * D, D, Dp, reinterpret_cast<X*>(st.w) + r * Dp, nullptr, buf);
+    return;
+  }
+  const int row = blockIdx.x;
+  if (row >= T) return;
+  int before = 0;
+  for (int i = tid; i < row; i += 256) before += labels[i] != ignore ? 1 : 0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+  if ((tid & 63) == 0) counts[tid >> 6] = before;
+  __syncthreads();
+  const int at = (counts[0] + counts[1]) + (counts[2] + counts[3]);
+  const int64_t l = labels[row];
+  const bool in = l != ignore;
+  if (tid == 0) {
+    const bool ok = l >= 0 && l < V;
+    st.ids[row] = ok ? (int)l : kAbsent;
+    st.p[row] = ok || !in ? 1.f : NAN;
+    st.pos[row] = in ? at : -1;
+    if (in) st.rows[at] = row;
+    if (!in) loss[row] = 0.f;
+    if (row == T - 1) st.hdr->n = st.hdr->count = at + (in ? 1 : 0);
+  }
+  if (in) pack_row(hidden + (int64_t)row * D, D, Dp, reinterpret_cast<X*>(st.h) + (int64_t)at * Dp, st.amax + at, buf);
+}
+
 // The hidden states that count (blockIdx.y = 0) and the weight (1) as operands: copied, padded
 // with zeros to Dp channels.  fp16: and the largest finite |hidden| of each row.
 template <typename X>
@@ -433,31 +502,28 @@ pack_kernel(const X* __restrict__ hidden, const X* __restrict__ weight, int64_t 
   __shared__ float buf[4];
   for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const X* xr = x + (rows != nullptr ? (int64_t)rows[r] : r) * D;
-    float m = 0.f;
-    for (int c = threadIdx.x * 8; c < Dp; c += 2048) {
-      X v[8];
-      load8(xr, c, D, v);
-      if constexpr (__is_same(X, f16)) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float a = fabsf(rr::to_f32(v[e]));
-          if (a < INFINITY) m = fmaxf(m, a);   // neither infinite nor NaN
-        }
-      }
-      typedef uint32_t Words __attribute__((ext_vector_type(2 * sizeof(X))));
-      Words q;
-      __builtin_memcpy(&q, v, sizeof(q));
-      *reinterpret_cast<Words*>(out + r * Dp + c) = q;
-    }
-    if constexpr (__is_same(X, f16)) {
-      if (w) continue;
-      m = wave_max(m);
-      __syncthreads();   // the last row's reads of buf are done
-      if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
-      __syncthreads();
-      if (threadIdx.x == 0) st.amax[r] = fmaxf(fmaxf(buf[0], buf[1]), fmaxf(buf[2], buf[3]));
-    }
+    pack_row(xr, D, Dp, out + r * Dp, w ? nullptr : st.amax + r, buf);
   }
+}
+
+// What multiplies a row of dz where nothing has to be known of the other rows (the losses on
+// log-probabilities in bf16 and fp32): found where dz is made, coef_kernel's launch saved (2.4 us of 146
+// for 512 rows of 768 channels and 32000 words, 8 of 6300 for 8192).
+struct Upstream {
+  const float* dloss;   // [losses], or one for all
+  float factor;
+  int group;            // rows of a loss
+  bool per_row, mean, weighted;
+  float* scale;         // the factors on dw and on dh
+};
+__device__ __forceinline__ float row_factor(const Upstream& u, const State& st, int row) {
+  const float c = u.per_row ? u.dloss[u.group == 1 ? row : row / u.group] * u.factor : 1.f;
+  return u.weighted ? (u.per_row ? c * st.z2[row] : st.z2[row] / st.hdr->top) : c;
+}
+__device__ __forceinline__ void leave_scale(const Upstream& u, const State& st) {
+  float f = 1.f;   // (no row counts: 0, whatever the upstream gradient)
+  if (!u.per_row) f = st.hdr->n == 0 ? 0.f : u.dloss[0] * u.factor * (u.mean ? 1.f / (float)st.hdr->count : 1.f) * st.hdr->top;
+  u.scale[0] = f, u.scale[1] = f;
 }
 
 // ------------------------------------------------------------------ logits
@@ -473,7 +539,8 @@ struct LogitArgs {
   float* z;               // forward: [n][ldzf] logits that are kept, or [cuts][ldcut] parts of them
   int64_t ldzf, ldcut;
   int cuts;
-  const float2* coef;     // backward
+  const float2* coef;     // backward: of coef_kernel, or null
+  Upstream up;
   char* dz;
   int64_t ldz, plane_z;
   int v_first;            // the piece's first column
@@ -552,6 +619,9 @@ logits_kernel(LogitArgs a) {
     tile_of(blockIdx.x, a.nvt, gridDim.x / a.nvt, vt, tt);
   }
   const int t0 = tt * BN, v0 = a.v_first + vt * BM;
+  if constexpr (GRAD) {
+    if (a.coef == nullptr && blockIdx.x == 0 && threadIdx.x == 0) leave_scale(a.up, a.st);
+  }
   if (t0 >= n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN, wn = wave % P::WN;
@@ -572,7 +642,10 @@ logits_kernel(LogitArgs a) {
     for (int j = 0; j < P::NI; ++j) {
       const int t = min(t0 + wn * P::NW + 16 * j + (lane & 15), n - 1);
       orig[j] = a.st.rows[t] * a.K;
-      if constexpr (GRAD) co[j] = a.coef[t], l2[j] = a.st.lse2[t];
+      if constexpr (GRAD) {
+        co[j] = a.coef != nullptr ? a.coef[t] : make_float2(row_factor(a.up, a.st, orig[j]), 0.f);   // (K is 1)
+        l2[j] = a.st.lse2[t];
+      }
     }
 #pragma unroll
     for (int j = 0; j < P::NI; ++j)
@@ -771,13 +844,14 @@ join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, in
 // in join_kernel).  A word's entries are taken off in their order by the thread of the first.
 template <typename Op, int PZ>
 __global__ void __launch_bounds__(256)
-dz_kernel(State st, const float2* __restrict__ coef, int V, int64_t Vt, int K, int v_first, int cols, char* __restrict__ dz,
-          int64_t ldz, int64_t plane_z) {
+dz_kernel(State st, const float2* __restrict__ coef, Upstream up, int V, int64_t Vt, int K, int v_first, int cols,
+          char* __restrict__ dz, int64_t ldz, int64_t plane_z) {
   const int t = blockIdx.x;
+  if (coef == nullptr && t == 0 && blockIdx.y == 0 && threadIdx.x == 0) leave_scale(up, st);
   if (t >= st.hdr->n) return;
   const int tid = threadIdx.x, rel0 = blockIdx.y * kSeg, at = rel0 + tid * 8, v0 = v_first + rel0, v = v0 + tid * 8;
   const bool here = at < cols;   // both multiples of 8
-  const float2 co = coef[t];
+  const float2 co = coef != nullptr ? coef[t] : make_float2(row_factor(up, st, st.rows[t]), 0.f);
   const float l2 = st.lse2[t];
   __shared__ f32x4_t seg[kSeg / 4];
   if (here) {
@@ -822,10 +896,15 @@ dz_kernel(State st, const float2* __restrict__ coef, int V, int64_t Vt, int K, i
   }
 }
 
-// The tiles' maxima and sums of a row to the row's, by a wave.
-__device__ __forceinline__ void join_tiles(const float2* __restrict__ part, int nvt, int64_t Tp, int64_t t, int lane, float& m,
-                                           float& s) {
-  m = -INFINITY, s = 0.f;
+// Per row (a wave each): the tiles' maxima and sums to the row's lse, and its loss.
+__global__ void __launch_bounds__(256)
+row_loss_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, int K, bool labels, float zl, float tau,
+                float* __restrict__ out) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+  if (t >= st.hdr->n) return;
+  const int64_t row = st.rows[t];
+  float m = -INFINITY, s = 0.f;
   for (int v = lane; v < nvt; v += 64) {
     const float2 x = part[(int64_t)v * Tp + t];
     const float mm = fmaxf(m, x.x);
@@ -839,18 +918,6 @@ __device__ __forceinline__ void join_tiles(const float2* __restrict__ part, int 
     s = (m == mm ? s : s * exp2f(m - mm)) + (m2 == mm ? s2 : s2 * exp2f(m2 - mm));
     m = mm;
   }
-}
-
-// Per row (a wave each): the tiles' maxima and sums to the row's lse, and its loss.
-__global__ void __launch_bounds__(256)
-row_loss_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, int K, bool labels, float zl, float tau,
-                float* __restrict__ out) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
-  if (t >= st.hdr->n) return;
-  const int64_t row = st.rows[t];
-  float m, s;
-  join_tiles(part, nvt, Tp, t, lane, m, s);
   const float l2 = m + log2f(s);
   float loss = 0.f;
   for (int k = lane; k < K; k += 64) {
@@ -893,20 +960,48 @@ __device__ __forceinline__ float exp_rest(float d) {
   return d > 60.f ? expm1f(d) : expm1f(d) - d;   // (not inf - inf)
 }
 
-// Per row (a wave each): the tiles' maxima and sums to the row's lse and its label's
-// log-probability, to `out`; or, POLICY, its loss, and the derivative by -logp for the
-// backward.  A ratio on a border of the clipping counts as inside it; without an advantage the
-// ratio counts for nothing, however large.
+// Per row: the tiles' maxima and sums to the row's lse and its label's log-probability, to
+// `out`; or, POLICY, its loss, and the derivative by -logp for the backward.  A ratio on a border
+// of the clipping counts as inside it; without an advantage the ratio counts for nothing,
+// however large.  A workgroup takes 16 rows, 16 threads each, so that a wave's loads are whole
+// lines (8192 rows of 256 tiles: 16.4 us a wave a row, 10.3 so; 1152 of 125: 5.6 and 5.0).
+constexpr int kLogpRows = 16;
 template <bool POLICY>
 __global__ void __launch_bounds__(256)
 row_logp_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, Policy a, float* __restrict__ out) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
-  if (t >= st.hdr->n) return;
+  __shared__ float2 buf[4][kLogpRows];
+  const int n = st.hdr->n, t0 = (int)blockIdx.x * kLogpRows;
+  if (t0 >= n) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, mine = threadIdx.x & (kLogpRows - 1);
+  const int t = t0 + mine;
+  float m = -INFINITY, s = 0.f;
+  auto part_of = [](float m2, float s2, float mm) { return m2 == mm ? s2 : s2 * exp2_fast(m2 - mm); };   // (not inf - inf)
+  auto join = [&](float m2, float s2) {
+    const float mm = fmaxf(m, m2);
+    s = part_of(m, s, mm) + part_of(m2, s2, mm);
+    m = mm;
+  };
+  // eight tiles at a time: their loads, their exponentials
+  const float2* at = part + (t < n ? t : t0);
+  for (int v0 = threadIdx.x / kLogpRows; v0 < nvt; v0 += 128) {
+    float2 x[8];
+    float mm = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v0 + 16 * i < nvt ? at[(int64_t)(v0 + 16 * i) * Tp] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mm = fmaxf(mm, x[i].x);
+    s = part_of(m, s, mm), m = mm;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += part_of(x[i].x, x[i].y, mm);
+  }
+#pragma unroll
+  for (int o = kLogpRows; o < 64; o *= 2) join(__shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+  if (lane < kLogpRows) buf[wave][lane] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x >= kLogpRows || t >= n) return;
+  m = buf[0][mine].x, s = buf[0][mine].y;
+  for (int w = 1; w < 4; ++w) join(buf[w][mine].x, buf[w][mine].y);
   const int64_t row = st.rows[t];
-  float m, s;
-  join_tiles(part, nvt, Tp, t, lane, m, s);
-  if (lane != 0) return;
   const float log2s = log2f(s);
   // (the maximum goes first: what is left is small and keeps its bits)
   const float logp = st.ids[row] == kAbsent ? NAN : ((st.z2[row] - m) - log2s) * kLn2;
@@ -933,46 +1028,130 @@ row_logp_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, 
   st.lse2[t] = value != value ? NAN : m + log2s;   // the backward's row is NaN where the loss is
 }
 
-// The loss of each pair of sequences (a workgroup each) from their tokens' log-probabilities in
-// st.loss, and its derivative by each token's -logp.  Sums and the loss are in 64 bits: a
-// sequence's sum is in the thousands where the difference of two of them decides.  A pair without
-// a token that counts counts for nothing.  counted: null, or whether each does.
+// A pair's loss from its sequences' sums, and its derivative by -logp of a token of the first.  In 64
+// bits, as the sums are: a sequence's is in the thousands where the difference of two of them decides.
+struct Preference {
+  const float* ref;   // [pairs][2], or null
+  int64_t L;          // tokens of a sequence
+  double beta, eps;
+};
+__device__ __forceinline__ float pair_loss(const Preference& a, double m, int64_t pair, float& by) {
+  if (a.ref != nullptr) m -= (double)a.ref[2 * pair] - (double)a.ref[2 * pair + 1];
+  m *= a.beta;
+  const double e = exp(-fabs(m)), rest = log1p(e);   // -log sigmoid(m) = max(-m, 0) + rest
+  const double up = 1 / (1 + e), down = e / (1 + e);   // sigmoid(|m|), sigmoid(-|m|)
+  double loss = (1 - a.eps) * (fmax(-m, 0.) + rest);
+  if (a.eps != 0) loss += a.eps * (fmax(m, 0.) + rest);   // (not 0 x inf)
+  by = (float)(a.beta * (m < 0 ? (1 - a.eps) * up - a.eps * down : (1 - a.eps) * down - a.eps * up));
+  return (float)loss;
+}
+
+// Of a whole workgroup, what the losses are closed by: their sum, how many count, the largest
+// |derivative|; to its first thread.
+struct Close {
+  float sum, top;
+  int count;
+};
+template <int WAVES>
+__device__ __forceinline__ Close close_up(Close c) {
+  __shared__ Close buf[WAVES];
+  c.sum = wave_add(c.sum), c.top = wave_max(c.top);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) c.count += __shfl_xor(c.count, o, 64);
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = c;
+  __syncthreads();
+  Close all{0.f, 0.f, 0};
+  for (int w = 0; w < WAVES; ++w) all.sum += buf[w].sum, all.top = fmaxf(all.top, buf[w].top), all.count += buf[w].count;
+  return all;
+}
+// (a top whose inverse is no normal value: 1)
+__device__ __forceinline__ float usable(float top) { return top > 0x1p-100f ? top : 1.f; }
+__device__ __forceinline__ float finite_abs(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.f; }
+
+// The losses of the pairs from their tokens' log-probabilities in st.loss, and their derivative
+// by each token's -logp.  A pair without a token that counts counts for nothing.  One launch for few
+// tokens: `waves` of the workgroup's 16 take a pair, half of them a sequence (512 tokens: 7.1 us in
+// two launches, 6.2 in one; 8192: 11.5 and 13.9).  each: null, or where the pairs' losses go;
+// out: null, or where their sum or mean does.
+constexpr int64_t kTokensInOne = 2048;
+__global__ void __launch_bounds__(1024)
+pairs_kernel(State st, Preference a, int64_t pairs, int waves, bool mean, float* __restrict__ each, float* __restrict__ out) {
+  __shared__ double sum[16];
+  __shared__ int any[16];
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const int at_once = 16 / waves, half = waves * 32;   // threads of a sequence
+  const int mine = tid / (2 * half), k = tid % half, side = tid / half & 1;
+  Close c{0.f, 0.f, 0};
+  for (int64_t p0 = 0; p0 < pairs; p0 += at_once) {
+    const int64_t pair = p0 + mine, first = (pair * 2 + side) * a.L;
+    double s = 0;
+    int n = 0;
+    if (pair < pairs) {
+      for (int64_t i = k; i < a.L; i += half) {
+        if (st.pos[first + i] < 0) continue;
+        s += (double)st.loss[first + i], n = 1;
+      }
+    }
+    // a wave is of one sequence, or, where it has a pair, its halves are
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor(s, o, 64), n |= __shfl_xor(n, o, 64);
+    n |= __shfl_xor(n, 32, 64);
+    const double other = __shfl_xor(s, 32, 64);
+    const double both = waves == 1 ? ((tid & 32) == 0 ? s - other : other - s) : s + other;
+    __syncthreads();   // the last turn's reads are done
+    if ((tid & 63) == 0) sum[wave] = both, any[wave] = n;
+    __syncthreads();
+    if (pair >= pairs) continue;
+    double m = 0;
+    int counts = 0;
+    for (int w = 0; w < waves; ++w) {
+      const double v = sum[mine * waves + w];
+      m += waves == 1 || w < waves / 2 ? v : -v;
+      counts |= any[mine * waves + w];
+    }
+    float by = 0.f;
+    const float loss = counts ? pair_loss(a, m, pair, by) : 0.f;
+    if (tid % (2 * half) == 0) {
+      if (each != nullptr) each[pair] = loss;
+      c.sum += loss, c.count += counts, c.top = fmaxf(c.top, finite_abs(by));
+    }
+    if (!counts) continue;
+    for (int64_t i = k; i < a.L; i += half) st.z2[first + i] = side == 0 ? by : -by;
+  }
+  if (out == nullptr) return;
+  c = close_up<16>(c);
+  if (tid != 0) return;
+  st.hdr->count = c.count, st.hdr->top = usable(c.top);
+  out[0] = mean ? c.sum / (float)max(1, c.count) : c.sum;
+}
+
+// The same for many tokens, a workgroup a pair.  counted and bys: null, or whether each counts and its |derivative|.
 __global__ void __launch_bounds__(256)
-pair_kernel(State st, const float* __restrict__ ref, int64_t L, double beta, double eps, float* __restrict__ out,
-            int* __restrict__ counted) {
+pair_kernel(State st, Preference a, float* __restrict__ each, int* __restrict__ counted, float* __restrict__ bys) {
   __shared__ double sum[4];
   __shared__ int any[4];
-  __shared__ float by;
-  const int64_t pair = blockIdx.x, first = pair * 2 * L;
+  const int64_t pair = blockIdx.x;
   const int tid = threadIdx.x, side = tid >> 7;   // half of the threads take one sequence, half the other
+  const int64_t first = (pair * 2 + side) * a.L;
   double s = 0;
   int n = 0;
-  for (int64_t i = tid & 127; i < L; i += 128) {
-    const int64_t row = first + side * L + i;
-    if (st.pos[row] < 0) continue;
-    s += (double)st.loss[row], n = 1;
+  for (int64_t i = tid & 127; i < a.L; i += 128) {
+    if (st.pos[first + i] < 0) continue;
+    s += (double)st.loss[first + i], n = 1;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64), n |= __shfl_xor(n, o, 64);
   if ((tid & 63) == 0) sum[tid >> 6] = s, any[tid >> 6] = n;
   __syncthreads();
   const bool counts = (any[0] | any[1] | any[2] | any[3]) != 0;
+  float by = 0.f;
+  const float loss = counts ? pair_loss(a, (sum[0] + sum[1]) - (sum[2] + sum[3]), pair, by) : 0.f;
   if (tid == 0) {
-    double m = (sum[0] + sum[1]) - (sum[2] + sum[3]);
-    if (ref != nullptr) m -= (double)ref[2 * pair] - (double)ref[2 * pair + 1];
-    m *= beta;
-    const double e = exp(-fabs(m)), rest = log1p(e);   // -log sigmoid(m) = max(-m, 0) + rest
-    const double up = 1 / (1 + e), down = e / (1 + e);   // sigmoid(|m|), sigmoid(-|m|)
-    double loss = (1 - eps) * (fmax(-m, 0.) + rest);
-    if (eps != 0) loss += eps * (fmax(m, 0.) + rest);   // (not 0 x inf)
-    by = (float)(beta * (m < 0 ? (1 - eps) * up - eps * down : (1 - eps) * down - eps * up));
-    out[pair] = counts ? (float)loss : 0.f;
-    if (counted != nullptr) counted[pair] = counts ? 1 : 0;
+    each[pair] = loss;
+    if (counted != nullptr) counted[pair] = counts ? 1 : 0, bys[pair] = finite_abs(by);
   }
-  __syncthreads();
   if (!counts) return;
-  const float d = side == 0 ? by : -by;
-  for (int64_t i = tid & 127; i < L; i += 128) st.z2[first + side * L + i] = d;
+  for (int64_t i = tid & 127; i < a.L; i += 128) st.z2[first + i] = side == 0 ? by : -by;
 }
 
 // The sum of the rows' losses, over the number that count where `mean` (0 without any).  A
@@ -993,25 +1172,31 @@ sum_loss_kernel(const float* __restrict__ loss, int64_t T, const Header* hdr, bo
   out[0] = mean ? s / (float)max(1, hdr->n) : s;
 }
 
+// The same of a policy's losses, with the largest of the rows' derivatives.
+__global__ void __launch_bounds__(1024)
+sum_policy_kernel(State st, int T, bool mean, float* out) {
+  Close c{0.f, 0.f, 0};
+#pragma unroll 4
+  for (int i = threadIdx.x; i < T; i += 1024) {
+    if (st.pos[i] < 0) continue;
+    c.sum += st.loss[i], c.top = fmaxf(c.top, finite_abs(st.z2[i]));
+  }
+  c = close_up<16>(c);
+  if (threadIdx.x != 0) return;
+  st.hdr->top = usable(c.top);
+  out[0] = mean ? c.sum / (float)max(1, st.hdr->n) : c.sum;
+}
+
 // The same of pairs, whose number that count it finds.
 __global__ void __launch_bounds__(1024)
-sum_pairs_kernel(const float* __restrict__ loss, const int* __restrict__ counted, int64_t pairs, Header* hdr, bool mean,
-                 float* out) {
-  __shared__ float buf[16];
-  __shared__ int count[16];
-  float s = 0.f;
-  int n = 0;
-  for (int64_t i = threadIdx.x; i < pairs; i += 1024) s += loss[i], n += counted[i];
-  s = wave_add(s);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = s, count[threadIdx.x >> 6] = n;
-  __syncthreads();
+sum_pairs_kernel(const float* __restrict__ loss, const int* __restrict__ counted, const float* __restrict__ bys, int64_t pairs,
+                 Header* hdr, bool mean, float* out) {
+  Close c{0.f, 0.f, 0};
+  for (int64_t i = threadIdx.x; i < pairs; i += 1024) c.sum += loss[i], c.top = fmaxf(c.top, bys[i]), c.count += counted[i];
+  c = close_up<16>(c);
   if (threadIdx.x != 0) return;
-  s = 0.f, n = 0;
-  for (int w = 0; w < 16; ++w) s += buf[w], n += count[w];
-  hdr->count = n;
-  out[0] = mean ? s / (float)max(1, n) : s;
+  hdr->count = c.count, hdr->top = usable(c.top);
+  out[0] = mean ? c.sum / (float)max(1, c.count) : c.sum;
 }
 
 // ------------------------------------------------------------------ gradients
@@ -1042,26 +1227,7 @@ coef_kernel(State st, const float* __restrict__ dloss, bool per_row, int group, 
     const float c = per_row ? dloss[group == 1 ? row : row / group] * factor : 1.f;
     return weights != nullptr ? c * weights[row] : c;
   };
-  // The largest of the workgroup's values, to all of it.
-  auto largest = [&](float v) {
-    v = wave_max(v);
-    __syncthreads();   // the last call's reads of buf are done
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.f;
-    for (int w = 0; w < 16; ++w) v = fmaxf(v, buf[w]);
-    return v;
-  };
-  float top = 1.f;
-  if (weights != nullptr) {
-    float v = 0.f;
-    for (int t = threadIdx.x; t < n; t += 1024) {
-      const float c = fabsf(c_of(t));
-      if (c < INFINITY) v = fmaxf(v, c);
-    }
-    v = largest(v);
-    if (v > 0x1p-100f) top = v;   // (its inverse is a normal value)
-  }
+  const float top = weights != nullptr && !per_row ? st.hdr->top : 1.f;
   float m = 0.f;
   for (int t = threadIdx.x; t < n; t += 1024) {
     const float c = c_of(t) / top;
@@ -1081,7 +1247,11 @@ coef_kernel(State st, const float* __restrict__ dloss, bool per_row, int group, 
   }
   float sc = 1.f;
   if (scaled) {   // the same for the whole workgroup
-    m = largest(m);
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = 0.f;
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, buf[w]);
     sc = pow2_to(__float_as_uint(m), each ? 15 : 14);
     if (!each)
       for (int t = threadIdx.x; t < n; t += 1024) coef[t].x *= sc;   // this thread's own
@@ -1321,10 +1491,10 @@ enum Kind { kLabels, kTeacher, kLogp, kPolicy, kPreference };
 struct Loss {
   Kind kind;
   float tau, zl;
+  const int64_t* labels;   // null: a teacher, whose entries and rows have been found
+  int64_t ignore;
   Policy policy;
-  const float* ref;      // of pairs
-  int64_t L;             // tokens of a pair's sequence
-  double beta, eps;
+  Preference pairs;
 };
 
 template <typename X, typename Op>
@@ -1332,8 +1502,18 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
             int reduction, float* loss, hipStream_t s) {
   // the weight too where it is not an operand itself
   const int64_t most = p.copy_w ? std::max(p.T, p.V) : p.T;
-  pack_kernel<X><<<dim3((unsigned)std::min<int64_t>(8192, most), p.copy_w ? 2 : 1), 256, 0, s>>>(
-      static_cast<const X*>(hidden), static_cast<const X*>(weight), p.V, (int)p.D, (int)p.Dp, st);
+  const dim3 packs((unsigned)std::min<int64_t>(8192, most), p.copy_w ? 2 : 1);
+  const X* h_in = static_cast<const X*>(hidden);
+  const X* w_in = static_cast<const X*>(weight);
+  State in = st;
+  if (reduction == 0 && l.kind != kPreference) in.loss = loss;   // where rows that do not count leave their 0
+  if (l.labels != nullptr && p.T <= kRowsInOne) {
+    rows_pack_kernel<X><<<packs, 256, 0, s>>>(h_in, w_in, l.labels, l.ignore, (int)p.T, (int)p.V, (int)p.D, (int)p.Dp, st, in.loss);
+  } else {
+    if (l.labels != nullptr) rows_kernel<true><<<1, 1024, 0, s>>>(l.labels, l.ignore, p.T, (int)p.V, in);
+    else rows_kernel<false><<<1, 1024, 0, s>>>(nullptr, 0, p.T, (int)p.V, in);
+    pack_kernel<X><<<packs, 256, 0, s>>>(h_in, w_in, p.V, (int)p.D, (int)p.Dp, st);
+  }
   LogitArgs a = logit_args(p, st, weight, K, l.tau);
   a.part = ws.part;
   a.z = p.cuts > 1 ? ws.cut : st.z, a.ldzf = p.Vt, a.ldcut = p.T * p.Vt, a.cuts = (int)p.cuts;
@@ -1346,21 +1526,31 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
     join_kernel<<<dim3((unsigned)p.T, (unsigned)parts), 256, 0, s>>>(st, ws.cut, a.cuts, a.ldcut, a.V, p.Vt, K, a.c, p.Tp,
                                                                     ws.part);
   }
-  const unsigned waves = (unsigned)((p.T + 3) / 4);
+  const unsigned waves = (unsigned)((p.T + 3) / 4), groups = (unsigned)((p.T + kLogpRows - 1) / kLogpRows);
   float* rows = reduction == 0 ? loss : st.loss;
   if (l.kind == kPreference) {
-    row_logp_kernel<false><<<waves, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, st.loss);
-    const int64_t pairs = p.T / (2 * l.L);
-    float* each = reduction == 0 ? loss : reinterpret_cast<float*>(ws.part);   // a float2 a row is there and done with
-    int* counted = reduction == 0 ? nullptr : reinterpret_cast<int*>(each + pairs);
-    pair_kernel<<<(unsigned)pairs, 256, 0, s>>>(st, l.ref, l.L, l.beta, l.eps, each, counted);
-    if (reduction != 0) sum_pairs_kernel<<<1, 1024, 0, s>>>(each, counted, pairs, st.hdr, reduction == 1, loss);
+    row_logp_kernel<false><<<groups, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, st.loss);
+    const int64_t pairs = p.T / (2 * l.pairs.L);
+    const bool all = reduction != 0;
+    if (p.T <= kTokensInOne) {
+      int waves = 16;
+      while (waves > 1 && waves * pairs > 16) waves /= 2;
+      pairs_kernel<<<1, 1024, 0, s>>>(st, l.pairs, pairs, waves, reduction == 1, all ? nullptr : loss, all ? loss : nullptr);
+    } else {
+      float* each = all ? reinterpret_cast<float*>(ws.part) : loss;   // two floats a row are there and done with
+      int* counted = all ? reinterpret_cast<int*>(each + pairs) : nullptr;
+      float* bys = all ? each + 2 * pairs : nullptr;
+      pair_kernel<<<(unsigned)pairs, 256, 0, s>>>(st, l.pairs, each, counted, bys);
+      if (all) sum_pairs_kernel<<<1, 1024, 0, s>>>(each, counted, bys, pairs, st.hdr, reduction == 1, loss);
+    }
     return rr::check_launch("rr_linear_preference");
   }
   if (l.kind == kPolicy) {
-    row_logp_kernel<true><<<waves, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, l.policy, rows);
+    row_logp_kernel<true><<<groups, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, l.policy, rows);
+    if (reduction != 0) sum_policy_kernel<<<1, 1024, 0, s>>>(st, (int)p.T, reduction == 1, loss);
+    return rr::check_launch("rr_linear_policy");
   } else if (l.kind == kLogp) {
-    row_logp_kernel<false><<<waves, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, rows);
+    row_logp_kernel<false><<<groups, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, rows);
   } else {
     row_loss_kernel<<<waves, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, K, l.kind == kLabels, l.zl, l.tau, rows);
   }
@@ -1373,26 +1563,31 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
 struct LossGrad {
   float tau, factor, zl;
   int group;
-  bool weighted;
+  bool weighted, logp;
 };
 
 template <typename X, typename Op, int PZ>
 int backward(const Plan& p, const float* dloss, const void* weight, const State& st, const BwdWs& ws, int K, const LossGrad& l,
              int reduction, void* dh, void* dw, hipStream_t s) {
   const bool each = __is_same(Op, OpF16) && (reduction == 0 || l.weighted);   // a power of two for each row's dz
-  coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, l.group, l.weighted ? st.z2 : nullptr, reduction == 1, l.factor,
-                                 l.zl, __is_same(Op, OpF16), ws.coef, ws.unscale, ws.scale);
+  const bool itself = l.logp && !__is_same(Op, OpF16);   // dz_kernel and logits_kernel find the factors
+  const float2* coef = itself ? nullptr : ws.coef;
+  const Upstream us{dloss, l.factor, l.group, reduction == 0, reduction == 1, l.weighted, ws.scale};
+  if (!itself) {
+    coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, l.group, l.weighted ? st.z2 : nullptr, reduction == 1, l.factor,
+                                   l.zl, __is_same(Op, OpF16), ws.coef, ws.unscale, ws.scale);
+  }
   if (each && dw != nullptr) {
     scale_h_kernel<<<(unsigned)p.T, 256, 0, s>>>(st, ws.unscale, ws.scale, (int)p.Dp, reinterpret_cast<f16*>(ws.h));
   }
   for (int64_t v = 0; v < p.Vt; v += p.Vp) {
     const int64_t cols = std::min(p.Vp, p.Vt - v);   // whole tiles
     LogitArgs a = logit_args(p, st, weight, K, l.tau);
-    a.coef = ws.coef, a.dz = ws.dz, a.ldz = p.Vp * p.eb, a.plane_z = p.Tp * a.ldz, a.v_first = (int)v;
+    a.coef = coef, a.up = us, a.dz = ws.dz, a.ldz = p.Vp * p.eb, a.plane_z = p.Tp * a.ldz, a.v_first = (int)v;
     constexpr bool kFp32 = __is_same(Op, OpF32), kFew = PZ == 2;   // up to kFewRows
     if (kFew || st.z != nullptr) {
       dz_kernel<Op, PZ><<<dim3((unsigned)p.T, (unsigned)(up(cols, kSeg) / kSeg)), 256, 0, s>>>(
-          st, ws.coef, a.V, p.Vt, K, a.v_first, (int)cols, ws.dz, a.ldz, a.plane_z);
+          st, coef, us, a.V, p.Vt, K, a.v_first, (int)cols, ws.dz, a.ldz, a.plane_z);
     } else if constexpr (!kFew) {
       launch_logits<typename std::conditional<kFp32, Tile64, Tile256>::type, Op, kGrad, PZ>(a, p.T, cols, s);
     }
@@ -1498,10 +1693,7 @@ extern "C" int rr_linear_ce_fwd(const void* hidden, const void* weight, int dtyp
   if (int rc = check_buffers(who, rows, D, V, 1, dtype, 0, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
   State st;
   lay_out_state(rows, D, V, 1, dtype, state, state_bytes, &st);
-  State in = st;
-  if (reduction == 0) in.loss = loss;   // where rows that do not count leave their 0
-  rows_kernel<true><<<1, 1024, 0, s>>>(labels, ignore_index, rows, (int)V, in);
-  Loss l{kLabels, 1.f, z_loss};
+  const Loss l{kLabels, 1.f, z_loss, labels, ignore_index};
   return run_forward(hidden, weight, dtype, rows, D, V, 1, l, reduction, loss, st, workspace, s);
 }
 
@@ -1534,10 +1726,7 @@ extern "C" int rr_linear_kd_fwd(const void* hidden, const void* weight, int dtyp
     entries_kernel<InT><<<(unsigned)rows, 64, (size_t)KP * 8, s>>>(static_cast<const InT*>(teacher_logits), teacher_ids, (int)K,
                                                                   KP, (int)V, temperature, st.ids, st.p, st.pos);
   });
-  State in = st;
-  if (reduction == 0) in.loss = loss;
-  rows_kernel<false><<<1, 1024, 0, s>>>(nullptr, 0, rows, (int)V, in);
-  Loss l{kTeacher, temperature, 0.f};
+  const Loss l{kTeacher, temperature, 0.f, nullptr, 0};
   return run_forward(hidden, weight, dtype, rows, D, V, K, l, reduction, loss, st, workspace, s);
 }
 
@@ -1547,7 +1736,7 @@ bool bad_temperature(float t) { return !(t > 0.f) || !(t < 1e30f); }
 
 // The forward of the losses on the labels' log-probabilities, `losses` of them where none are added up.
 int forward_logp(const char* who, const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
-                 const int64_t* labels, int64_t ignore_index, const Loss& l, int reduction, float* loss, int64_t losses,
+                 const Loss& l, int reduction, float* loss, int64_t losses,
                  void* state, size_t state_bytes, void* workspace, size_t workspace_bytes, hipStream_t s) {
   if (int rc = check_dims(who, rows, D, V, 1, dtype, reduction)) return rc;
   const std::string w(who);
@@ -1559,16 +1748,13 @@ int forward_logp(const char* who, const void* hidden, const void* weight, int dt
     zero(loss, reduction != 0 ? 4 : losses * 4, s);
     return rr::check_launch(who);
   }
-  if (labels == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
+  if (l.labels == nullptr) return rr::fail(RR_EINVAL, w + ": null pointer");
   if (l.kind == kPolicy && (l.policy.advantages == nullptr || (l.policy.kl != 0.f && l.policy.ref == nullptr))) {
     return rr::fail(RR_EINVAL, w + ": null pointer");
   }
   if (int rc = check_buffers(who, rows, D, V, 1, dtype, 0, hidden, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
   State st;
   lay_out_state(rows, D, V, 1, dtype, state, state_bytes, &st);
-  State in = st;
-  if (reduction == 0 && l.kind != kPreference) in.loss = loss;   // where rows that do not count leave their 0
-  rows_kernel<true><<<1, 1024, 0, s>>>(labels, ignore_index, rows, (int)V, in);
   return run_forward(hidden, weight, dtype, rows, D, V, 1, l, reduction, loss, st, workspace, s);
 }
 
@@ -1604,7 +1790,7 @@ extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dt
                                   int64_t V, int64_t K, float z_loss, float temperature, int reduction,
                                   const void* state, size_t state_bytes, void* dhidden, void* dweight, void* workspace,
                                   size_t workspace_bytes, void* stream) {
-  const LossGrad l{temperature, temperature, z_loss, 1, false};
+  const LossGrad l{temperature, temperature, z_loss, 1, false, false};
   return run_backward("rr_linear_loss_bwd", dloss, weight, dtype, rows, D, V, K, l, reduction, state, state_bytes, dhidden,
                       dweight, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
@@ -1612,8 +1798,8 @@ extern "C" int rr_linear_loss_bwd(const float* dloss, const void* weight, int dt
 extern "C" int rr_linear_logp_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
                                   const int64_t* labels, int64_t ignore_index, float temperature, float* log_probs,
                                   void* state, size_t state_bytes, void* workspace, size_t workspace_bytes, void* stream) {
-  const Loss l{kLogp, temperature, 0.f};
-  return forward_logp("rr_linear_logp_fwd", hidden, weight, dtype, rows, D, V, labels, ignore_index, l, 0, log_probs, rows,
+  const Loss l{kLogp, temperature, 0.f, labels, ignore_index};
+  return forward_logp("rr_linear_logp_fwd", hidden, weight, dtype, rows, D, V, l, 0, log_probs, rows,
                       state, state_bytes, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
@@ -1627,9 +1813,9 @@ extern "C" int rr_linear_policy_fwd(const void* hidden, const void* weight, int 
   if (!(clip_low >= 0.f) || !(clip_high >= 0.f)) return rr::fail(RR_EINVAL, w + ": the clipping's widths must not be negative");
   if (!(kl_weight >= 0.f) || !(kl_weight < INFINITY)) return rr::fail(RR_EINVAL, w + ": kl_weight must be finite and not negative");
   if (rows_per_advantage <= 0) return rr::fail(RR_EINVAL, w + ": an advantage is for one row or more");
-  Loss l{kPolicy, temperature, 0.f};
+  Loss l{kPolicy, temperature, 0.f, labels, ignore_index};
   l.policy = {advantages, rows_per_advantage, old_log_probs, ref_log_probs, 1.f - clip_low, 1.f + clip_high, kl_weight};
-  return forward_logp(w.c_str(), hidden, weight, dtype, rows, D, V, labels, ignore_index, l, reduction, loss, rows, state,
+  return forward_logp(w.c_str(), hidden, weight, dtype, rows, D, V, l, reduction, loss, rows, state,
                       state_bytes, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
@@ -1643,9 +1829,9 @@ extern "C" int rr_linear_preference_fwd(const void* hidden, const void* weight, 
   if (pairs >= ((int64_t)1 << 23) || L >= ((int64_t)1 << 23)) return rr::fail(RR_EUNSUPPORTED, w + ": too many rows");
   if (!(beta > 0.f) || !(beta < INFINITY)) return rr::fail(RR_EINVAL, w + ": beta must be positive and finite");
   if (!(label_smoothing >= 0.f) || !(label_smoothing <= 0.5f)) return rr::fail(RR_EINVAL, w + ": label_smoothing must be in [0, 0.5]");
-  Loss l{kPreference, 1.f, 0.f};
-  l.ref = ref_log_probs, l.L = L, l.beta = beta, l.eps = label_smoothing;
-  return forward_logp(w.c_str(), hidden, weight, dtype, pairs * 2 * L, D, V, labels, ignore_index, l, reduction, loss, pairs,
+  Loss l{kPreference, 1.f, 0.f, labels, ignore_index};
+  l.pairs = {ref_log_probs, L, beta, label_smoothing};
+  return forward_logp(w.c_str(), hidden, weight, dtype, pairs * 2 * L, D, V, l, reduction, loss, pairs,
                       state, state_bytes, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
@@ -1660,7 +1846,7 @@ extern "C" int rr_linear_logp_bwd(const float* dloss, const void* weight, int dt
     return rr::fail(RR_EINVAL, w + ": log-probabilities have a gradient a row");
   }
   // (the log-probabilities' own derivative by -logp is -1)
-  const LossGrad l{temperature, (itself ? -1.f : 1.f) / temperature, 0.f, (int)rows_per_loss, !itself};
+  const LossGrad l{temperature, (itself ? -1.f : 1.f) / temperature, 0.f, (int)rows_per_loss, !itself, true};
   return run_backward(w.c_str(), dloss, weight, dtype, rows, D, V, 1, l, reduction, state, state_bytes, dhidden, dweight,
                       workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }

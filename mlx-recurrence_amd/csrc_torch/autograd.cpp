@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <deque>
 #include <string>
 #include <utility>
 #include <vector>
@@ -527,7 +528,7 @@ Tensor linear_logp(const Tensor& hidden, const Tensor& weight, const Tensor& lab
 // The tensors are taken from Python's lists as they are: converting a list of 300 takes longer than its
 // kernels.
 Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::list>& out_list, bool clip, double max_norm) {
-  std::vector<Tensor> grads, outs;
+  std::vector<const Tensor*> grads, outs;   // (the lists hold them)
   const Py_ssize_t all = PyList_GET_SIZE(grad_list.ptr());
   grads.reserve(all);
   if (out_list.has_value()) outs.reserve(all);
@@ -535,21 +536,21 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
     PyObject* g = PyList_GET_ITEM(grad_list.ptr(), i);
     if (g == Py_None) continue;
     if (!THPVariable_Check(g)) throw pybind11::type_error("gradients must be tensors or None");
-    grads.push_back(THPVariable_Unpack(g));
+    grads.push_back(&THPVariable_Unpack(g));
     if (!out_list.has_value()) continue;
     PyObject* o = PyList_GET_ITEM(out_list->ptr(), i);
     if (!THPVariable_Check(o)) throw pybind11::value_error("out must have a tensor of each gradient's shape and type");
-    outs.push_back(THPVariable_Unpack(o));
+    outs.push_back(&THPVariable_Unpack(o));
   }
   if (grads.empty()) throw pybind11::value_error("no gradients to take a norm of");
-  const at::Device dev = grads[0].device();
+  const at::Device dev = grads[0]->device();
   const size_t n = grads.size();
   const bool recording = at::GradMode::is_enabled();
-  require_device({&grads[0]});
+  require_device({grads[0]});
   for (size_t i = 0; i < n; ++i) {
-    const Tensor& g = grads[i];
+    const Tensor& g = *grads[i];
     if (g.layout() != at::kStrided) throw pybind11::type_error("gradients must be dense tensors");
-    if (g.device() != dev) require_device({&grads[0], &g});
+    if (g.device() != dev) require_device({grads[0], &g});
     if (recording && g.requires_grad()) {
       throw pybind11::value_error("the norm of gradients is not differentiable; call it under torch.no_grad()");
     }
@@ -558,7 +559,7 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
       throw pybind11::type_error("gradients must be float32, bfloat16 or float16");
     }
     if (outs.empty()) continue;
-    const Tensor& o = outs[i];
+    const Tensor& o = *outs[i];
     if (o.layout() != at::kStrided || o.sizes() != g.sizes() || o.scalar_type() != t) {
       throw pybind11::value_error("out must have a tensor of each gradient's shape and type");
     }
@@ -569,18 +570,20 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
   std::vector<void*> to(n);
   std::vector<int64_t> numel(n);
   std::vector<int> types(n);
-  std::vector<Tensor> held;                                // what lives until the launches are made
+  std::deque<Tensor> held;                                 // what lives until the launches are made
   std::vector<std::pair<Tensor, Tensor>> back;             // copies to go back to tensors with gaps
   std::vector<const void*> gaps;
   for (size_t i = 0; i < n; ++i) {
-    const Tensor& g = grads[i];
-    const bool dense = g.is_non_overlapping_and_dense();
-    Tensor src = g;
-    if (!dense) held.push_back(src = g.contiguous());
-    in[i] = src.data_ptr(), numel[i] = src.numel(), types[i] = dtype_code(src.scalar_type());
+    const Tensor* g = grads[i];
+    if (!g->is_non_overlapping_and_dense()) {
+      held.push_back(g->contiguous());
+      g = &held.back();
+    }
+    const Tensor& src = *g;
+    in[i] = src.const_data_ptr(), numel[i] = src.numel(), types[i] = dtype_code(src.scalar_type());
     if (!clip) continue;
-    const Tensor& o = outs.empty() ? g : outs[i];
-    if (o.is_non_overlapping_and_dense() && o.strides() == src.strides()) {
+    const Tensor& o = outs.empty() ? *grads[i] : *outs[i];
+    if (&o == g || (o.is_non_overlapping_and_dense() && o.strides() == src.strides())) {
       to[i] = o.data_ptr();
       continue;
     }
@@ -596,7 +599,7 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
   if (std::adjacent_find(gaps.begin(), gaps.end()) != gaps.end()) {
     throw pybind11::value_error("two of the tensors to write share memory");
   }
-  Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
+  Tensor norm = at::empty({}, grads[0]->options().dtype(at::kFloat).requires_grad(false));
   const size_t wsb = rr_grad_norm_workspace_bytes((int64_t)n);
   const Tensor ws = workspace(wsb, norm.options());
   if (!clip) {
@@ -609,7 +612,7 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
   const at::NoGradGuard no_grad;
   for (const auto& [o, tmp] : back) o.copy_(tmp);
   // (copy_ has counted its own)
-  for (size_t i = 0; i < n; ++i) (outs.empty() ? grads[i] : outs[i]).unsafeGetTensorImpl()->bump_version();
+  for (const Tensor* t : outs.empty() ? grads : outs) t->unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 
