@@ -13,6 +13,7 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/utils.h>
 
@@ -557,6 +558,10 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
     const at::ScalarType t = g.scalar_type();
     if (t != at::kFloat && t != at::kBFloat16 && t != at::kHalf) {
       throw pybind11::type_error("gradients must be float32, bfloat16 or float16");
+    }
+    const Tensor& to = outs.empty() ? g : *outs[i];
+    if (clip && to.is_inference() && !c10::InferenceMode::is_enabled()) {
+      throw pybind11::value_error("a tensor to write was made in inference mode; call it there");
     }
     if (outs.empty()) continue;
     const Tensor& o = *outs[i];

@@ -47,6 +47,8 @@ def _run(grads, outs, clip, max_norm):
             raise ValueError("the norm of gradients is not differentiable; call it under torch.no_grad()")
         if g.dtype not in _lib.DTYPE_CODE:
             raise TypeError("gradients must be float32, bfloat16 or float16")
+        if clip and (outs[i] if outs else g).is_inference() and not torch.is_inference_mode_enabled():
+            raise ValueError("a tensor to write was made in inference mode; call it there")
         if outs and (outs[i].layout != torch.strided or outs[i].shape != g.shape or outs[i].dtype != g.dtype):
             raise ValueError("out must have a tensor of each gradient's shape and type")
     dev = _lib.require_device(*grads, *(outs or ()))
@@ -71,7 +73,7 @@ def _run(grads, outs, clip, max_norm):
         _lib.grad_norm(src, to, max_norm, norm)
         for o, t in back:
             o.copy_(t)
-        torch.autograd.graph.increment_version(written)
+        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
     return norm
 
 

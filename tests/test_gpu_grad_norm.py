@@ -264,3 +264,61 @@ def test_a_step_of_the_policy_and_the_pairs():
     assert abs(float(norm) / n - 1) < 1e-4
     for got, want in ((h.grad, dh), (w.grad, dw)):
         assert float((got.double() - 0.5 * want).norm() / (0.5 * want).norm()) < 2e-4
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_inference_mode(python, monkeypatch):
+    if python:
+        monkeypatch.setattr(_lib, "_autograd_mod", None)
+    with torch.inference_mode():
+        t = torch.full((100,), 3.0, device="cuda")
+        assert float(mr.clip_grad_norm([t], 15.0)) == 30.0 and t.tolist() == [1.5] * 100
+    assert float(mr.global_grad_norm([t])) == 15.0
+    with pytest.raises(ValueError, match="inference mode"):
+        mr.clip_grad_norm([t], 1.0)
+    assert t.tolist() == [1.5] * 100
+    a = torch.full((100,), 3.0, device="cuda")
+    assert float(mr.clip_grad_norm([t], 1.0, out=[a])) == 15.0 and abs(float(a.norm()) - 1) < 1e-6
+
+
+def test_python_binding_gives_the_same(monkeypatch):
+    grads = tensors([(1000,), (64, 65), (7,)] + [(30,)] * 200, None, seed=12)
+    first, second = ([g.clone() for g in grads] for _ in range(2))
+    a = mr.clip_grad_norm(first, 1.0)
+    monkeypatch.setattr(_lib, "_autograd_mod", None)
+    assert torch.equal(a, mr.clip_grad_norm(second, 1.0)) and all(torch.equal(x, y) for x, y in zip(first, second))
+    assert torch.equal(a, mr.global_grad_norm(grads))
+
+
+def test_workspace_is_written_inside(monkeypatch):
+    buffers = []
+
+    def guarded(n, device):
+        whole = torch.full((n + 8192,), 0xA5, dtype=torch.uint8, device=device)
+        whole[4096:4096 + n] = 0xFF
+        buffers.append((whole, n))
+        return whole[4096:4096 + n]
+
+    monkeypatch.setattr(_lib, "_autograd_mod", None)
+    monkeypatch.setattr(_lib, "_alloc_ws", guarded)
+    for shapes in ([(1,)], [(i * 91 % 3001 + 1,) for i in range(700)], [(20_000_000,), (5,), (3_000_001,)]):
+        grads = tensors(shapes, BF16, seed=13)
+        before = [g.clone() for g in grads]
+        check(mr.clip_grad_norm(grads, 0.5 * norm64(before)), grads, before, 0.5 * norm64(before))
+    for whole, n in buffers:
+        assert (whole[:4096] == 0xA5).all() and (whole[4096 + n:] == 0xA5).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_than_the_cache(dtype):
+    """Sizes whose first part is read past the cache, and whose second reading is."""
+    n = 90_000_001 if dtype == F32 else 180_000_001
+    g = gen(14)
+    grads = [torch.randn(n, generator=g, device="cuda").to(dtype), torch.randn(777, generator=g, device="cuda").to(BF16)]
+    out = [torch.empty_like(t) for t in grads]
+    n64 = norm64(grads)
+    norm = mr.clip_grad_norm(grads, 0.25 * n64, out=out)
+    assert abs(float(norm) / n64 - 1) <= 2.0 ** -23
+    for a, t in zip(out, grads):
+        off = (a.double() - t.double() * 0.25).abs()
+        assert bool((off <= t.double().abs() * 0.25 * (U[a.dtype] + 2.0 ** -23) + LEAST[a.dtype]).all())

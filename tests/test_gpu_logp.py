@@ -429,3 +429,93 @@ def test_other_streams_and_replays():
         graph.replay()
         got = [t.clone() for t in static]
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("pairs,L", [(1, 1), (3, 40), (17, 9), (64, 16), (40, 30), (7, 200)])
+def test_pairs_in_one_launch_and_in_two(pairs, L, dtype, reduction):
+    """Up to 2048 tokens and more; pairs that count for nothing among them; factors shared by a sequence."""
+    g, h, w, labels, logp = head((pairs, 2, L), 72, 300, dtype, 3 * pairs + L, ignored=0.2)
+    labels[1::5] = -100
+    ref = (torch.where(labels != -100, logp, 0).sum(-1) + 4 * randn(g, pairs, 2)).float()
+    up = rand(g, pairs) + 0.1 if reduction == "none" else torch.tensor(0.7, device="cuda")
+    got = run(mr.linear_preference_loss, h, w, up, labels, ref, label_smoothing=0.05, reduction=reduction)
+    want = orc.preference(h, w, labels, ref, up, eps=0.05, reduction=reduction)
+    check_all(got, want, 1 + 0.1 * math.sqrt(2 * L) * orc.size_of(h, w, labels))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("rows", [2047, 2048, 2049, 3000])
+def test_rows_found_in_one_launch_and_in_two(rows, dtype, reduction):
+    g, h, w, labels, logp = head((rows,), 130, 640, dtype, rows, ignored=0.4)
+    labels[-1] = -100 if rows % 2 else 3
+    A = randn(g, rows) + 1
+    old = (logp - away(0.3 * randn(g, rows), (0.2, 0.2))).float()
+    up = rand(g, rows) + 0.1 if reduction == "none" else torch.tensor(0.7, device="cuda")
+    got = run(mr.linear_policy_loss, h, w, up, labels, A, old, reduction=reduction)
+    check_all(got, orc.policy(h, w, labels, A, old, None, up, reduction=reduction), 1 + orc.size_of(h, w, labels))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("pairs,L,D,V", [(1, 1, 8, 2), (2, 5, 200, 257), (1, 25, 3000, 300), (4, 25, 100, 513), (3, 50, 1000, 5003),
+                                         (5, 70, 320, 4096), (25, 60, 200, 641)])
+def test_kernels_write_inside_their_buffers(pairs, L, D, V, dtype, monkeypatch):
+    """State and workspaces of exactly the stated sizes between guards: nothing is written outside them, and
+    what they held before does not matter."""
+    buffers = []
+
+    def guarded(n, device):
+        whole = torch.full((n + 8192,), 0xA5, dtype=torch.uint8, device=device)
+        whole[4096:4096 + n] = 0xFF   # NaN as a float
+        buffers.append((whole, n))
+        return whole[4096:4096 + n]
+
+    g, h, w, labels, logp = head((pairs, 2, L), D, V, dtype, pairs + D + V, ignored=0.3)
+    A, old = randn(g, pairs, 2, 1), logp.float()
+    one = torch.ones((), device="cuda")
+    each = rand(g, pairs, 2, L)
+
+    def calls():
+        return (run(mr.linear_policy_loss, h, w, one, labels, A, old, old, kl_weight=0.1),
+                run(mr.linear_policy_loss, h, w, each, labels, A, reduction="none"),
+                run(mr.linear_preference_loss, h, w, one, labels),
+                run(mr.linear_preference_loss, h, w, each[:, 0, 0], labels, reduction="none"),
+                run(mr.linear_log_probs, h, w, each, labels))
+
+    want = calls()
+    monkeypatch.setattr(_lib, "autograd_ext", lambda: None)
+    monkeypatch.setattr(_lib, "_alloc_ws", guarded)
+    for a, b in zip(calls(), want):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+    assert len(buffers) == 15
+    for whole, n in buffers:
+        assert (whole[:4096] == 0xA5).all() and (whole[4096 + n:] == 0xA5).all()
+
+
+def test_backward_twice_and_two_calls_at_once():
+    """A graph kept for a second backward gives the same; calls on two streams share nothing."""
+    g, h, w, labels, logp = head((6, 2, 32), 256, 1000, BF16, 21)
+    A, old = randn(g, 6, 2, 1), (logp - 0.1).float()
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    loss = mr.linear_policy_loss(h, w, labels, A, old)
+    first = torch.autograd.grad(loss, (h, w), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(loss, (h, w))))
+    want = mr.linear_preference_loss(h, w, labels)
+    want = (want.detach(), *torch.autograd.grad(want, (h, w)))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                loss = mr.linear_policy_loss(h, w, labels, A, old) if i == 0 else mr.linear_preference_loss(h, w, labels)
+                got[i] = (loss.detach(), *torch.autograd.grad(loss, (h, w)))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got[0][1:], first))
+    assert all(torch.equal(a, b) for a, b in zip(got[1], want))
