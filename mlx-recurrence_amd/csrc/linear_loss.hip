@@ -608,21 +608,22 @@ logits_kernel(LogitArgs a) {
   using P = Product<Op, BM, BN, C::WM, C::WN, false, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int n = a.st.hdr->n;
-  int vt, tt;
-  int k0 = 0, k1 = a.Dp, cut = 0;
-  if constexpr (MODE == kCut) {
-    const int tiles = gridDim.x / a.cuts, steps = a.Dp / P::BK;
-    cut = blockIdx.x / tiles;
-    k0 = steps * cut / a.cuts * P::BK, k1 = steps * (cut + 1) / a.cuts * P::BK;
-    tile_of(blockIdx.x - cut * tiles, a.nvt, tiles / a.nvt, vt, tt);
-  } else {
-    tile_of(blockIdx.x, a.nvt, gridDim.x / a.nvt, vt, tt);
-  }
-  const int t0 = tt * BN, v0 = a.v_first + vt * BM;
   if constexpr (GRAD) {
     if (a.coef == nullptr && blockIdx.x == 0 && threadIdx.x == 0) leave_scale(a.up, a.st);
   }
-  if (t0 >= n) return;
+  int vt, tt, id = blockIdx.x;
+  int k0 = 0, k1 = a.Dp, cut = 0;
+  if constexpr (MODE == kCut) {
+    const int tiles = gridDim.x / a.cuts, steps = a.Dp / P::BK;
+    cut = id / tiles, id -= cut * tiles;
+    k0 = steps * cut / a.cuts * P::BK, k1 = steps * (cut + 1) / a.cuts * P::BK;
+  }
+  // The tiles of the rows that count are dealt out, not of all rows: an XCD takes neighbours,
+  // and those of the last rows would leave it without work.
+  const int row_tiles = (n + BN - 1) / BN;
+  if (id >= a.nvt * row_tiles) return;
+  tile_of(id, a.nvt, row_tiles, vt, tt);
+  const int t0 = tt * BN, v0 = a.v_first + vt * BM;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN, wn = wave % P::WN;
   const int quarter = lane >> 4;
@@ -1300,10 +1301,11 @@ dh_kernel(DhArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int n = a.st.hdr->n;
   int dt, tt;
-  const int tiles = gridDim.x / a.splits, sp = blockIdx.x / tiles;
-  tile_of(blockIdx.x - sp * tiles, a.ndt, tiles / a.ndt, dt, tt);
+  const int tiles = gridDim.x / a.splits, sp = blockIdx.x / tiles, id = blockIdx.x - sp * tiles;
+  const int row_tiles = (n + BN - 1) / BN;   // of the rows that count, as in logits_kernel
+  if (id >= a.ndt * row_tiles) return;
+  tile_of(id, a.ndt, row_tiles, dt, tt);
   const int t0 = tt * BN, d0 = dt * BM;
-  if (t0 >= n) return;
   const int steps = a.cols / P::BK;
   const int k0 = (int)((int64_t)steps * sp / a.splits) * P::BK, k1 = (int)((int64_t)steps * (sp + 1) / a.splits) * P::BK;
   typename P::Acc acc;
