@@ -405,13 +405,13 @@ int rr_layer_norm_bwd(const void* dy, int y_dtype, const void* x, int x_dtype, c
  * labels.  V <= 2^24, D <= 65536. */
 size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t V, int64_t K, int dtype, int grad);
 
-/* Workspace of the forward (pass = 0) or backward (pass = 1); 0 for invalid
- * arguments.  The forward's holds two floats a row and 256 words and, where tiles are
+/* Workspace of the forward (pass = 0) or backward (pass = 1; 2 that of
+ * rr_linear_logp_bwd); 0 for invalid arguments.  The forward's holds two floats a row and 256 words and, where tiles are
  * few and their sums are made in parts, at most 256 MiB of those parts of the logits.
  * The backward's holds a piece of the logits' gradient (512 MiB, or 2048 columns of the
  * vocabulary where those are more), dhidden's sums in fp32 (once, or in parts of at most
- * 256 MiB), at most 256 MiB of parts of dweight's, and for fp16 a copy of the hidden
- * states that count. */
+ * 256 MiB; pass = 2: once and at most 128 MiB of parts), at most 256 MiB of parts of
+ * dweight's, and for fp16 a copy of the hidden states that count. */
 size_t rr_linear_loss_workspace_bytes(int64_t rows, int64_t D, int64_t V, int dtype, int pass);
 
 /* Cross entropy: with z = hidden weight^T and lse = log sum exp z of a row,
@@ -478,7 +478,8 @@ int rr_linear_preference_fwd(const void* hidden, const void* weight, int dtype, 
 
 /* Gradients of the three: dloss fp32 ([rows / rows_per_loss] for reduction 0, else [1]) with
  * rows_per_loss 1, or 2 L for the preference loss (whose temperature is 1); of_log_probs is 1 for
- * rr_linear_logp_fwd (reduction 0), else 0.  The rest as for rr_linear_loss_bwd. */
+ * rr_linear_logp_fwd (reduction 0), else 0.  The workspace is that of pass = 2, the rest as for
+ * rr_linear_loss_bwd. */
 int rr_linear_logp_bwd(const float* dloss, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
                        float temperature, int64_t rows_per_loss, int of_log_probs, int reduction, const void* state,
                        size_t state_bytes, void* dhidden, void* dweight, void* workspace, size_t workspace_bytes,

@@ -124,6 +124,7 @@ struct Header {
   int n;                 // rows that count
   int count;             // what the mean is over: those rows, or the pairs that count
   float top;             // the largest of the rows' derivatives that the forward left (State.z2)
+  int whole, parts;      // the losses on log-probabilities: DhShare
 };
 struct State {
   Header* hdr;
@@ -228,6 +229,10 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   return p;
 }
 
+// Whether the logits that are kept are more than the 256 MB cache holds: they are then written and read
+// past it (6.6 x 10^3 and 7.4 x 10^3 rows of 65536 bf16: the forward's product 2035 and 2290 us, 1920 and 2157 so).
+bool keeps_past(const Plan& p) { return p.T * p.Vt * 4 > (int64_t)256 << 20; }
+
 // grad: 0 no backward, 1 logits where they are kept, 2 only those that always are.
 size_t state_layout(const Plan& p, int64_t K, int grad, char* base, State* s) {
   Carve take{base};
@@ -268,10 +273,55 @@ struct BwdWs {
   float* unscale;  // [Tp] the inverse of a row's power of two (fp16)
   char* h;         // [T][Dp] the hidden states times that (fp16)
   char* dz;        // [planes_z][Tp][Vp]
-  float* dh;       // [splits][Tp][Dt]
+  float* dh;       // [splits][Tp][Dt]; log-probabilities: [Tp][Dt], then the shared tiles' parts (DhShare)
   float* dw;       // [cuts_w][Vp][Dt], where there are two or more
 };
-size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
+// dh's tiles in the losses on log-probabilities.  How many rows count is known on the device
+// alone, and with it how many tiles there are: as many as fill whole rounds of the GPU are done by a
+// workgroup each, the others are shared by `parts` workgroups each, along the vocabulary.  Cut in
+// as many equal parts as suit all rows (best_parts), 26 x 10 tiles of 32 x 10 took four rounds of a third
+// each: 1117 us where they take 900 (8192 rows, a fifth ignored, 2560 channels, 32768 words bf16).
+struct DhShare {
+  int whole, parts;
+};
+struct DhShape {
+  int ndt, bn;       // tiles of channels, rows of a tile
+  int slots;         // workgroups at one time
+  int room;          // parts that there is room for
+  int steps;         // of k in a piece
+  float cost;        // of a part's writing and reading, in steps
+};
+// (by a wave: a lane tries a number of parts)
+__device__ __forceinline__ DhShare dh_share(const DhShape& a, int n, int lane) {
+  const int tiles = a.ndt * ((n + a.bn - 1) / a.bn), rest = tiles % a.slots;
+  int s = lane + 1;
+  float c = (float)((rest * s + a.slots - 1) / a.slots * a.steps) / (float)s + (float)(s * rest) * a.cost;
+  if (s > 1 && (rest * s > a.room || 4 * s > a.steps)) c = INFINITY;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float c2 = __shfl_xor(c, o, 64);
+    const int s2 = __shfl_xor(s, o, 64);
+    if (c2 < c || (c2 == c && s2 < s)) c = c2, s = s2;
+  }
+  return {tiles - rest, s};
+}
+DhShape dh_shape(const Plan& p) {
+  const bool big = p.rows == kTile256;
+  DhShape a;
+  a.bn = big ? Tile256::BN : p.rows == kTile64 ? Tile64::BN : Tile32::BN;
+  a.ndt = (int)(p.Dt / kEdge), a.slots = (int)(big ? kCus : 2 * kCus);
+  const int64_t tiles = up(p.T, a.bn) / a.bn * a.ndt;
+  a.room = (int)std::min<int64_t>(2 * a.slots, 64 * tiles);
+  a.steps = (int)(p.Vp * p.eb / 128) * p.planes_z;
+  a.cost = (float)((double)(kEdge * a.bn * 8) / 4e12 / (p.fp32 ? kStepF32 : kStep));
+  return a;
+}
+size_t dh_bytes(const Plan& p, bool logp) {
+  if (!logp) return (size_t)p.splits * p.Tp * p.Dt * 4;
+  const DhShape a = dh_shape(p);
+  return (size_t)(p.Tp * p.Dt + (int64_t)a.room * kEdge * a.bn) * 4;
+}
+size_t bwd_layout(const Plan& p, bool logp, char* base, BwdWs* s) {
   Carve take{base};
   BwdWs t;
   t.scale = reinterpret_cast<float*>(take(256));
@@ -279,7 +329,7 @@ size_t bwd_layout(const Plan& p, char* base, BwdWs* s) {
   t.unscale = reinterpret_cast<float*>(take(p.dtype == RR_F16 ? (size_t)p.Tp * 4 : 0));
   t.h = take(p.dtype == RR_F16 ? (size_t)p.T * p.Dp * p.eb : 0);
   t.dz = take((size_t)p.planes_z * p.Tp * p.Vp * p.eb);
-  t.dh = reinterpret_cast<float*>(take((size_t)p.splits * p.Tp * p.Dt * 4));
+  t.dh = reinterpret_cast<float*>(take(dh_bytes(p, logp)));
   t.dw = reinterpret_cast<float*>(take(p.cuts_w > 1 ? (size_t)p.cuts_w * p.Vp * p.Dt * 4 : 0));
   if (s != nullptr) *s = t;
   return take.off;
@@ -538,6 +588,7 @@ struct LogitArgs {
   float2* part;           // forward
   float* z;               // forward: [n][ldzf] logits that are kept, or [cuts][ldcut] parts of them
   int64_t ldzf, ldcut;
+  bool past;              // the logits are written past the cache, which would not hold them
   int cuts;
   const float2* coef;     // backward: of coef_kernel, or null
   Upstream up;
@@ -660,7 +711,10 @@ logits_kernel(LogitArgs a) {
     const int t = t0 + wn * P::NW + 16 * j;
     float* o = a.z + cut * a.ldcut + (int64_t)t * a.ldzf + vw;
     store_block<P::MI>(fstage, lane, [&](int i) { return acc[i][j]; }, [&](int r, int v, f32x4_t x) {
-      if (t + r < n) *reinterpret_cast<f32x4_t*>(o + (int64_t)r * a.ldzf + v) = x;
+      if (t + r >= n) return;
+      f32x4_t* at = reinterpret_cast<f32x4_t*>(o + (int64_t)r * a.ldzf + v);
+      if (MODE == kStats && a.past) __builtin_nontemporal_store(x, at);
+      else *at = x;
     });
   };
   if constexpr (MODE == kCut) {
@@ -845,7 +899,7 @@ join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, in
 // in join_kernel).  A word's entries are taken off in their order by the thread of the first.
 template <typename Op, int PZ>
 __global__ void __launch_bounds__(256)
-dz_kernel(State st, const float2* __restrict__ coef, Upstream up, int V, int64_t Vt, int K, int v_first, int cols,
+dz_kernel(State st, const float2* __restrict__ coef, Upstream up, bool past, int V, int64_t Vt, int K, int v_first, int cols,
           char* __restrict__ dz, int64_t ldz, int64_t plane_z) {
   const int t = blockIdx.x;
   if (coef == nullptr && t == 0 && blockIdx.y == 0 && threadIdx.x == 0) leave_scale(up, st);
@@ -859,7 +913,7 @@ dz_kernel(State st, const float2* __restrict__ coef, Upstream up, int V, int64_t
     const f32x4_t* i = reinterpret_cast<const f32x4_t*>(st.z + (int64_t)t * Vt + v);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const f32x4_t x = i[q];
+      const f32x4_t x = past ? __builtin_nontemporal_load(i + q) : i[q];
       seg[2 * tid + q] = f32x4_t{exp2_fast(x[0] - l2), exp2_fast(x[1] - l2), exp2_fast(x[2] - l2), exp2_fast(x[3] - l2)};
     }
   }
@@ -969,9 +1023,13 @@ __device__ __forceinline__ float exp_rest(float d) {
 constexpr int kLogpRows = 16;
 template <bool POLICY>
 __global__ void __launch_bounds__(256)
-row_logp_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, Policy a, float* __restrict__ out) {
+row_logp_kernel(State st, const float2* __restrict__ part, int nvt, int64_t Tp, Policy a, DhShape shape, float* __restrict__ out) {
   __shared__ float2 buf[4][kLogpRows];
   const int n = st.hdr->n, t0 = (int)blockIdx.x * kLogpRows;
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x >= 192) {   // for the backward
+    const DhShare sh = dh_share(shape, n, threadIdx.x & 63);
+    if (threadIdx.x == 192) st.hdr->whole = sh.whole, st.hdr->parts = sh.parts;
+  }
   if (t0 >= n) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, mine = threadIdx.x & (kLogpRows - 1);
   const int t = t0 + mine;
@@ -1283,6 +1341,20 @@ scale_h_kernel(State st, const float* __restrict__ unscale, const float* scale, 
 }
 
 // dh^T tiles of one part of the piece: m = channels, n = rows, k = the piece's columns.
+
+// The workgroup's tile (its number in the order of tile_of's bands) and part: those that are whole
+// first, then the parts, one part of all tiles after another; both in contiguous pieces for
+// each XCD.  False: it has none.
+__device__ __forceinline__ bool dh_work(const DhShare& sh, int tiles, int b, int& id, int& part) {
+  const int rest = tiles - sh.whole, all = b < sh.whole ? sh.whole : rest * sh.parts;
+  const int i = b < sh.whole ? b : b - sh.whole;
+  if (i >= all) return false;
+  const int each = all / kXcds, more = all % kXcds, x = i % kXcds;
+  const int at = x * each + min(x, more) + i / kXcds;
+  id = b < sh.whole ? at : sh.whole + at % rest, part = b < sh.whole ? 0 : at / rest;
+  return true;
+}
+
 struct DhArgs {
   const char* w;         // at the piece's first row
   const char* dz;
@@ -1291,6 +1363,7 @@ struct DhArgs {
   float* out;            // [splits][Tp][Dt]
   int Dt;
   bool first;
+  bool share;            // tiles are shared by the state's DhShare, `out` is as BwdWs.dh is then
   State st;
 };
 template <typename C, typename Op, int PZ>
@@ -1300,24 +1373,38 @@ dh_kernel(DhArgs a) {
   using P = Product<Op, BM, BN, C::WM, C::WN, true, false>;
   __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
   const int n = a.st.hdr->n;
-  int dt, tt;
-  const int tiles = gridDim.x / a.splits, sp = blockIdx.x / tiles, id = blockIdx.x - sp * tiles;
+  int dt, tt, sp, parts, slot = -1;
   const int row_tiles = (n + BN - 1) / BN;   // of the rows that count, as in logits_kernel
-  if (id >= a.ndt * row_tiles) return;
-  tile_of(id, a.ndt, row_tiles, dt, tt);
+  if (a.share) {
+    int id;
+    const DhShare sh{a.st.hdr->whole, a.st.hdr->parts};
+    if (!dh_work(sh, a.ndt * row_tiles, blockIdx.x, id, sp)) return;
+    band_tile(id, a.ndt, row_tiles, dt, tt);
+    parts = id < sh.whole ? 1 : sh.parts;
+    if (id >= sh.whole) slot = (id - sh.whole) * parts + sp;
+  } else {
+    const int tiles = gridDim.x / a.splits;
+    sp = blockIdx.x / tiles, parts = a.splits;
+    const int id = blockIdx.x - sp * tiles;
+    if (id >= a.ndt * row_tiles) return;
+    tile_of(id, a.ndt, row_tiles, dt, tt);
+  }
   const int t0 = tt * BN, d0 = dt * BM;
   const int steps = a.cols / P::BK;
-  const int k0 = (int)((int64_t)steps * sp / a.splits) * P::BK, k1 = (int)((int64_t)steps * (sp + 1) / a.splits) * P::BK;
+  const int k0 = (int)((int64_t)steps * sp / parts) * P::BK, k1 = (int)((int64_t)steps * (sp + 1) / parts) * P::BK;
   typename P::Acc acc;
   const Operand A{a.w + d0 * P::EB, a.ldw, 0, a.V, (int)a.ldw - d0 * P::EB};
   const Operand B{a.dz + (int64_t)t0 * a.ldz, a.ldz, a.plane_z, a.Tp - t0, a.cols * P::EB};
   P::template run<PZ>(acc, A, B, k0, k1, lds);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN, wn = wave % P::WN;
+  // the tile's corner: in dh itself, in its own copy of it, or in a buffer of the tile's size
+  float* corner = slot >= 0 ? a.out + ((int64_t)a.Tp * a.Dt + (int64_t)slot * BM * BN)
+                            : a.out + ((int64_t)(a.share ? 0 : sp) * a.Tp + t0) * a.Dt + d0;
+  const int ld = slot >= 0 ? BM : a.Dt;
 #pragma unroll
   for (int j = 0; j < P::NI; ++j) {
-    const int t = t0 + wn * P::NW + 16 * j + (lane & 15);
-    float* o = a.out + ((int64_t)sp * a.Tp + t) * a.Dt + d0 + wm * P::MW + 4 * (lane >> 4);
+    float* o = corner + (int64_t)(wn * P::NW + 16 * j + (lane & 15)) * ld + wm * P::MW + 4 * (lane >> 4);
 #pragma unroll
     for (int i = 0; i < P::MI; ++i) {
       float4* at = reinterpret_cast<float4*>(o + 16 * i);
@@ -1329,6 +1416,41 @@ dh_kernel(DhArgs a) {
       *at = v;
     }
   }
+}
+
+// dh of every row from what dh_kernel shared out, in the inputs' type (0 for rows that do not count).
+// A workgroup per row and 1024 channels, four a thread.
+template <typename X>
+__global__ void __launch_bounds__(256)
+share_out_kernel(State st, const float* __restrict__ dh, int D, int Dt, int Tp, int bn, const float* scale,
+                 const float* unscale, X* __restrict__ out) {
+  const int64_t row = blockIdx.x;
+  const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (c >= D) return;
+  const int t = st.pos[row];
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (t >= 0) {
+    const float f = scale[0] * (unscale != nullptr ? unscale[t] : 1.f);
+    const int row_tiles = (st.hdr->n + bn - 1) / bn, tt = t / bn;
+    const DhShare sh{st.hdr->whole, st.hdr->parts};
+    const int id = band_id(c / kEdge, tt, Dt / kEdge, row_tiles);
+    const bool whole = id < sh.whole;
+    const float* at = whole ? dh + (int64_t)t * Dt + c
+                            : dh + (int64_t)Tp * Dt + (int64_t)(id - sh.whole) * sh.parts * kEdge * bn +
+                                  (int64_t)(t - tt * bn) * kEdge + c % kEdge;
+    const int parts = whole ? 1 : sh.parts;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(at + (int64_t)i * kEdge * bn);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    s.x *= f, s.y *= f, s.z *= f, s.w *= f;
+  }
+  X* o = out + row * D + c;
+  const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < D) o[e] = rr::from_f32<X>(v[e]);
 }
 
 // A gradient from its parts, in the inputs' type: dh of every row (0 for rows that do not
@@ -1473,9 +1595,11 @@ void launch_forward(const LogitArgs& a, const Plan& p, hipStream_t s) {
   else launch_logits<C, Op, kStats, 1>(a, p.T, p.Vt, s);
 }
 template <typename C, typename Op, int PZ>
-void launch_dh(DhArgs a, const Plan& p, hipStream_t s) {
+void launch_dh(DhArgs a, const Plan& p, int room, hipStream_t s) {
   a.ndt = (int)(up(p.D, C::BM) / C::BM);
-  dh_kernel<C, Op, PZ><<<(unsigned)(a.ndt * (up(p.T, C::BN) / C::BN) * p.splits), C::THREADS, 0, s>>>(a);
+  const int64_t tiles = a.ndt * (up(p.T, C::BN) / C::BN);
+  // (whole tiles and parts: some workgroups have nothing to do, whatever rows count)
+  dh_kernel<C, Op, PZ><<<(unsigned)(a.share ? tiles + room : tiles * p.splits), C::THREADS, 0, s>>>(a);
 }
 template <typename C, typename Op, typename X, int PZ, bool CUT>
 void launch_dw(DwArgs a, const Plan& p, int64_t cols, hipStream_t s) {
@@ -1518,6 +1642,7 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
   }
   LogitArgs a = logit_args(p, st, weight, K, l.tau);
   a.part = ws.part;
+  a.past = keeps_past(p);
   a.z = p.cuts > 1 ? ws.cut : st.z, a.ldzf = p.Vt, a.ldcut = p.T * p.Vt, a.cuts = (int)p.cuts;
   if (p.rows == kTile32) launch_forward<Tile32, Op>(a, p, s);
   else if (p.rows == kTile64) launch_forward<Tile64, Op>(a, p, s);
@@ -1530,8 +1655,9 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
   }
   const unsigned waves = (unsigned)((p.T + 3) / 4), groups = (unsigned)((p.T + kLogpRows - 1) / kLogpRows);
   float* rows = reduction == 0 ? loss : st.loss;
+  const DhShape shape = dh_shape(p);
   if (l.kind == kPreference) {
-    row_logp_kernel<false><<<groups, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, st.loss);
+    row_logp_kernel<false><<<groups, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, shape, st.loss);
     const int64_t pairs = p.T / (2 * l.pairs.L);
     const bool all = reduction != 0;
     if (p.T <= kTokensInOne) {
@@ -1548,11 +1674,11 @@ int forward(const Plan& p, const void* hidden, const void* weight, const State& 
     return rr::check_launch("rr_linear_preference");
   }
   if (l.kind == kPolicy) {
-    row_logp_kernel<true><<<groups, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, l.policy, rows);
+    row_logp_kernel<true><<<groups, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, l.policy, shape, rows);
     if (reduction != 0) sum_policy_kernel<<<1, 1024, 0, s>>>(st, (int)p.T, reduction == 1, loss);
     return rr::check_launch("rr_linear_policy");
   } else if (l.kind == kLogp) {
-    row_logp_kernel<false><<<groups, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, rows);
+    row_logp_kernel<false><<<groups, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, {}, shape, rows);
   } else {
     row_loss_kernel<<<waves, 256, 0, s>>>(st, ws.part, (int)parts, p.Tp, K, l.kind == kLabels, l.zl, l.tau, rows);
   }
@@ -1574,6 +1700,7 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
   const bool each = __is_same(Op, OpF16) && (reduction == 0 || l.weighted);   // a power of two for each row's dz
   const bool itself = l.logp && !__is_same(Op, OpF16);   // dz_kernel and logits_kernel find the factors
   const float2* coef = itself ? nullptr : ws.coef;
+  const DhShape shape = l.logp ? dh_shape(p) : DhShape{};
   const Upstream us{dloss, l.factor, l.group, reduction == 0, reduction == 1, l.weighted, ws.scale};
   if (!itself) {
     coef_kernel<<<1, 1024, 0, s>>>(st, dloss, reduction == 0, l.group, l.weighted ? st.z2 : nullptr, reduction == 1, l.factor,
@@ -1589,7 +1716,7 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
     constexpr bool kFp32 = __is_same(Op, OpF32), kFew = PZ == 2;   // up to kFewRows
     if (kFew || st.z != nullptr) {
       dz_kernel<Op, PZ><<<dim3((unsigned)p.T, (unsigned)(up(cols, kSeg) / kSeg)), 256, 0, s>>>(
-          st, coef, us, a.V, p.Vt, K, a.v_first, (int)cols, ws.dz, a.ldz, a.plane_z);
+          st, coef, us, keeps_past(p), a.V, p.Vt, K, a.v_first, (int)cols, ws.dz, a.ldz, a.plane_z);
     } else if constexpr (!kFew) {
       launch_logits<typename std::conditional<kFp32, Tile64, Tile256>::type, Op, kGrad, PZ>(a, p.T, cols, s);
     }
@@ -1598,11 +1725,12 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
       b.w = a.w + v * a.ldw, b.dz = ws.dz, b.ldw = a.ldw, b.ldz = a.ldz, b.plane_z = a.plane_z;
       b.V = (int)(p.V - v), b.Tp = a.Tp, b.splits = (int)p.splits, b.cols = (int)cols;
       b.out = ws.dh, b.Dt = (int)p.Dt, b.first = v == 0, b.st = st;
+      b.share = l.logp;
       if constexpr (kFew || kFp32) {
-        if (p.rows == kTile32) launch_dh<Tile32, Op, PZ>(b, p, s);
-        else launch_dh<Tile64, Op, PZ>(b, p, s);
+        if (p.rows == kTile32) launch_dh<Tile32, Op, PZ>(b, p, shape.room, s);
+        else launch_dh<Tile64, Op, PZ>(b, p, shape.room, s);
       } else {
-        launch_dh<Tile256, Op, PZ>(b, p, s);
+        launch_dh<Tile256, Op, PZ>(b, p, shape.room, s);
       }
     }
     if (dw != nullptr) {
@@ -1618,7 +1746,10 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
       }
     }
   }
-  if (dh != nullptr) {
+  if (dh != nullptr && l.logp) {
+    share_out_kernel<X><<<dim3((unsigned)p.T, (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
+        st, ws.dh, (int)p.D, (int)p.Dt, (int)p.Tp, shape.bn, ws.scale + 1, each ? ws.unscale : nullptr, static_cast<X*>(dh));
+  } else if (dh != nullptr) {
     sum_out_kernel<X, true><<<dim3((unsigned)p.T, (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
         st, ws.dh, (int)p.D, p.Dt, p.Tp * p.Dt, (int)p.splits, ws.scale + 1, each ? ws.unscale : nullptr, static_cast<X*>(dh));
   }
@@ -1675,7 +1806,7 @@ extern "C" size_t rr_linear_loss_state_bytes(int64_t rows, int64_t D, int64_t V,
 extern "C" size_t rr_linear_loss_workspace_bytes(int64_t rows, int64_t D, int64_t V, int dtype, int pass) {
   if (rows <= 0 || check_dims("rr_linear_loss_workspace_bytes", rows, D, V, 1, dtype, 0) != RR_OK) return 0;
   const Plan p = plan_of(rows, D, V, dtype);
-  return pass == 0 ? fwd_layout(p, nullptr, nullptr) : bwd_layout(p, nullptr, nullptr);
+  return pass == 0 ? fwd_layout(p, nullptr, nullptr) : bwd_layout(p, pass == 2, nullptr, nullptr);
 }
 
 extern "C" int rr_linear_ce_fwd(const void* hidden, const void* weight, int dtype, int64_t rows, int64_t D, int64_t V,
@@ -1772,13 +1903,14 @@ int run_backward(const char* who, const float* dloss, const void* weight, int dt
     return rr::check_launch(who);
   }
   if (dloss == nullptr) return rr::fail(RR_EINVAL, std::string(who) + ": null pointer");
-  if (int rc = check_buffers(who, rows, D, V, K, dtype, 1, nullptr, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
+  const int pass = l.logp ? 2 : 1;
+  if (int rc = check_buffers(who, rows, D, V, K, dtype, pass, nullptr, weight, state, state_bytes, workspace, workspace_bytes)) return rc;
   if (dhidden == nullptr && dweight == nullptr) return RR_OK;
   const Plan p = plan_of(rows, D, V, dtype);
   State st;
   lay_out_state(rows, D, V, K, dtype, const_cast<void*>(state), state_bytes, &st);
   BwdWs ws;
-  bwd_layout(p, static_cast<char*>(workspace), &ws);
+  bwd_layout(p, l.logp, static_cast<char*>(workspace), &ws);
 #define LL_BACKWARD(X, OP, PZ) backward<X, OP, PZ>(p, dloss, weight, st, ws, (int)K, l, reduction, dhidden, dweight, s)
   if (dtype == RR_BF16) return p.planes_z == 2 ? LL_BACKWARD(bf16, OpBf16, 2) : LL_BACKWARD(bf16, OpBf16, 1);
   if (dtype == RR_F16) return p.planes_z == 2 ? LL_BACKWARD(f16, OpF16, 2) : LL_BACKWARD(f16, OpF16, 1);

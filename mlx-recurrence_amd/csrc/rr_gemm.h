@@ -199,14 +199,21 @@ struct Loader {
 // along m walked along n, so that the tiles it multiplies at one time share rows of
 // both operands.
 constexpr int kXcds = 8, kBand = 8;
-__device__ __forceinline__ void tile_of(int b, int nm, int nn, int& m, int& n) {
-  const int all = nm * nn, each = all / kXcds, more = all % kXcds;
-  const int x = b % kXcds;
-  const int id = x * each + min(x, more) + b / kXcds;
+// The tile with this number in the bands' order, and the number of a tile.
+__device__ __forceinline__ void band_tile(int id, int nm, int nn, int& m, int& n) {
   const int band = id / (kBand * nn), in = id - band * kBand * nn;
   const int wide = min(kBand, nm - band * kBand);
   m = band * kBand + in % wide;
   n = in / wide;
+}
+__device__ __forceinline__ int band_id(int m, int n, int nm, int nn) {
+  const int band = m / kBand, wide = min(kBand, nm - band * kBand);
+  return band * kBand * nn + n * wide + m % kBand;
+}
+__device__ __forceinline__ void tile_of(int b, int nm, int nn, int& m, int& n) {
+  const int all = nm * nn, each = all / kXcds, more = all % kXcds;
+  const int x = b % kXcds;
+  band_tile(x * each + min(x, more) + b / kXcds, nm, nn, m, n);
 }
 
 // WM x WN waves, each with MI x NI blocks of 16 x 16: element e of a lane's block (i, j)

@@ -504,7 +504,7 @@ struct LinearLogpFn : public torch::autograd::Function<LinearLogpFn> {
     const Tensor dloss = prep(grads[0], at::kFloat);
     Tensor dh = ctx->needs_input_grad(0) ? at::empty({rows, D}, w_.options()) : Tensor();
     Tensor dw = ctx->needs_input_grad(1) ? at::empty_like(w_) : Tensor();
-    const size_t wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 1);
+    const size_t wsb = rr_linear_loss_workspace_bytes(rows, D, V, dtc, 2);
     const Tensor ws = workspace(wsb, w_.options());
     check(rr_linear_logp_bwd(dloss.data_ptr<float>(), P(w_), dtc, rows, D, V, (float)ctx->saved_data["tau"].toDouble(),
                              ctx->saved_data["group"].toInt(), ctx->saved_data["kind"].toInt() == 0 ? 1 : 0,

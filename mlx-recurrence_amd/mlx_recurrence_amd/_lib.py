@@ -611,7 +611,7 @@ def linear_preference_fwd(hidden, weight, labels, ignore_index, pairs, L, ref, b
 
 def linear_logp_bwd(dloss, weight, rows, temperature, rows_per_loss, of_log_probs, reduction, state, dhidden, dweight):
     V, D = weight.shape
-    ws = _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[weight.dtype], 1)), weight.device)
+    ws = _alloc_ws(_ws_bytes("rr_linear_loss_workspace_bytes", (rows, D, V, DTYPE_CODE[weight.dtype], 2)), weight.device)
     _check(load().rr_linear_logp_bwd(ptr(dloss), ptr(weight), DTYPE_CODE[weight.dtype], rows, D, V, temperature,
                                      rows_per_loss, of_log_probs, reduction, *_sized(state), ptr(dhidden), ptr(dweight),
                                      *_sized(ws), stream_of(weight)), "rr_linear_logp_bwd")

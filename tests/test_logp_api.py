@@ -200,7 +200,7 @@ def test_c_abi_refusals():
     for bad in (dict(dl=None), dict(w=None), dict(st=None), dict(tau=-1.0), dict(red=-1), dict(group=0), dict(group=1 << 40),
                 dict(itself=1), dict(itself=1, red=0, group=2)):
         assert bw(**bad) == _lib.RR_EINVAL, bad
-    assert bw(wn=lib.rr_linear_loss_workspace_bytes(8, 8, 10, 1, 1) - 1) == _lib.RR_EWORKSPACE
+    assert bw(wn=lib.rr_linear_loss_workspace_bytes(8, 8, 10, 1, 2) - 1) == _lib.RR_EWORKSPACE
     assert bw(sn=state) == _lib.RR_EWORKSPACE   # that of a forward without a backward
     assert bw(dh=None, dw=None) == _lib.RR_OK
 
