@@ -217,3 +217,18 @@ def test_host_code_under_asan_and_ubsan():
     assert res.returncode == 0, tail
     assert "AddressSanitizer" not in tail and "runtime error" not in tail, tail
     assert " passed" in tail
+
+
+@pytest.mark.parametrize("rows,D,V,dtype", [(8192, 2560, 65536, 1), (32768, 2560, 131072, 1), (1536, 768, 32000, 0),
+                                            (1, 5120, 131072, 1), (100_000, 64, 32000, 2), (512, 65536, 2048, 1), (40, 64, 500, 2)])
+def test_backward_workspace_holds_a_piece_of_the_gradient(rows, D, V, dtype):
+    """A piece of the logits' gradient (512 MiB, or 2048 words of every row where those are more), dhidden's sums once and
+    at most 128 MiB of parts, at most 256 MiB of dweight's, fp16: a copy of the hidden states."""
+    lib, mib = _lib.load(), 1 << 20
+    size, planes = (4, 1) if dtype == 0 else (2, 2 if rows <= 64 else 1)
+    up = lambda a, b: (a + b - 1) // b * b  # noqa: E731
+    rows_up = 32 if rows <= 32 else up(rows, 256)
+    piece = max(512 * mib, 2048 * rows_up * size * planes)
+    sums = rows_up * up(D, 256) * 4 + (128 + 256) * mib
+    copy = rows * up(D, 64) * 2 if dtype == 2 else 0
+    assert 0 < lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 2) <= piece + sums + copy + rows_up * 16 + 4096
