@@ -109,7 +109,8 @@ def clip_grad_norm(grads, max_norm, *, out=None):
     that is infinite or NaN leaves them as they are: the caller sees it in what is returned.
 
     Args:
-        grads:     as for global_grad_norm; tensors that share memory are refused.
+        grads:     as for global_grad_norm.  No two may share memory: those without gaps
+                   between their values are checked.
         max_norm:  the largest norm, 0 or more (math.inf: take the norm alone).
         out:       tensors of the same shapes and types to write to, in place of `grads` (each
                    a tensor of its own, or the gradient itself).
