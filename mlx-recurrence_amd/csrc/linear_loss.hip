@@ -103,6 +103,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, THREADS = 512; };
 struct Tile64 { static constexpr int BM = 256, BN = 64, WM = 4, WN = 1, THREADS = 256; };
 struct Tile32 { static constexpr int BM = 256, BN = 32, WM = 4, WN = 1, THREADS = 256; };
+// Half of a Tile256, for the last round of tiles where that leaves half of the CUs or more without
+// work: then two workgroups take a tile's halves (half_work), in about 0.8 of a round where it has 12 or 18 steps
+// (1152 rows of 768 channels and 32000 words: logits 76.5 and 72.8 us, dw 64.0 and 60.9).
+struct Half256 { static constexpr int BM = 256, BN = 128, WM = 2, WN = 4, THREADS = 512; };
 enum Tiles { kTile256, kTile64, kTile32 };
 constexpr int kEdge = 256;       // BM of all; buffers hold whole tiles
 
@@ -648,34 +652,35 @@ __device__ __forceinline__ void store_block(T* lds, int lane, F value, S store) 
   rr::wave_lds_sync();
 }
 
+// The workgroup's tile of `tiles` (its number in the order of tile_of's bands) and half: -1 for a
+// whole one, 0 or 1 in a last round of halves.  False: it has none.  (kHalfMore workgroups more than tiles.)
+constexpr int kHalfMore = (int)kCus / 2;
+__device__ __forceinline__ bool half_work(int tiles, int b, int& id, int& half) {
+  const int rest = tiles % (int)kCus, whole = tiles - rest;
+  half = -1;
+  if (2 * rest > (int)kCus) {
+    if (b >= tiles) return false;
+    id = xcd_order(b, tiles);
+  } else if (b < whole) {
+    id = xcd_order(b, whole);
+  } else {
+    if (b - whole >= 2 * rest) return false;
+    const int at = xcd_order(b - whole, 2 * rest);
+    id = whole + at / 2, half = at & 1;
+  }
+  return true;
+}
+
 // z^T tiles: m = vocabulary, n = rows, so that a lane holds 4 MI logits of a row.
 // kStats: the forward's maxima and sums, and the logits where they are kept; kCut: one part of
 // the sums, as it is; kGrad: the backward's dz.
 enum Mode { kStats, kCut, kGrad };
 template <typename C, typename Op, Mode MODE, int PZ>
-__global__ void __launch_bounds__(C::THREADS, 2)
-logits_kernel(LogitArgs a) {
+__device__ __forceinline__ void logits_tile(const LogitArgs& a, char* lds, int n, int vt, int t0, int cut, int k0, int k1) {
   constexpr bool GRAD = MODE == kGrad;
   constexpr int BM = C::BM, BN = C::BN;
   using P = Product<Op, BM, BN, C::WM, C::WN, false, false>;
-  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  const int n = a.st.hdr->n;
-  if constexpr (GRAD) {
-    if (a.coef == nullptr && blockIdx.x == 0 && threadIdx.x == 0) leave_scale(a.up, a.st);
-  }
-  int vt, tt, id = blockIdx.x;
-  int k0 = 0, k1 = a.Dp, cut = 0;
-  if constexpr (MODE == kCut) {
-    const int tiles = gridDim.x / a.cuts, steps = a.Dp / P::BK;
-    cut = id / tiles, id -= cut * tiles;
-    k0 = steps * cut / a.cuts * P::BK, k1 = steps * (cut + 1) / a.cuts * P::BK;
-  }
-  // The tiles of the rows that count are dealt out, not of all rows: an XCD takes neighbours,
-  // and those of the last rows would leave it without work.
-  const int row_tiles = (n + BN - 1) / BN;
-  if (id >= a.nvt * row_tiles) return;
-  tile_of(id, a.nvt, row_tiles, vt, tt);
-  const int t0 = tt * BN, v0 = a.v_first + vt * BM;
+  const int v0 = a.v_first + vt * BM;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / P::WN, wn = wave % P::WN;
   const int quarter = lane >> 4;
@@ -834,6 +839,44 @@ logits_kernel(LogitArgs a) {
       a.part[(int64_t)vt * a.Tp + t0 + tl] = make_float2(m, s);
     }
   }
+}
+
+template <typename C, typename Op, Mode MODE, int PZ>
+__global__ void __launch_bounds__(C::THREADS, 2)
+logits_kernel(LogitArgs a) {
+  constexpr int BN = C::BN;
+  constexpr bool kHalves = __is_same(C, Tile256) && MODE != kCut;
+  using P = Product<Op, C::BM, BN, C::WM, C::WN, false, false>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+  const int n = a.st.hdr->n;
+  if constexpr (MODE == kGrad) {
+    if (a.coef == nullptr && blockIdx.x == 0 && threadIdx.x == 0) leave_scale(a.up, a.st);
+  }
+  int vt, tt, id = blockIdx.x, half = -1;
+  int k0 = 0, k1 = a.Dp, cut = 0;
+  if constexpr (MODE == kCut) {
+    const int tiles = gridDim.x / a.cuts, steps = a.Dp / P::BK;
+    cut = id / tiles, id -= cut * tiles;
+    k0 = steps * cut / a.cuts * P::BK, k1 = steps * (cut + 1) / a.cuts * P::BK;
+  }
+  // The tiles of the rows that count are dealt out, not of all rows: an XCD takes neighbours,
+  // and those of the last rows would leave it without work.
+  const int row_tiles = (n + BN - 1) / BN, tiles = a.nvt * row_tiles;
+  if constexpr (kHalves) {
+    if (!half_work(tiles, blockIdx.x, id, half)) return;
+    band_tile(id, a.nvt, row_tiles, vt, tt);
+  } else {
+    if (id >= tiles) return;
+    tile_of(id, a.nvt, row_tiles, vt, tt);
+  }
+  if constexpr (kHalves) {
+    if (half >= 0) {
+      const int t0 = tt * BN + half * Half256::BN;
+      if (t0 < n) logits_tile<Half256, Op, MODE, PZ>(a, lds, n, vt, t0, cut, k0, k1);
+      return;
+    }
+  }
+  logits_tile<C, Op, MODE, PZ>(a, lds, n, vt, tt * BN, cut, k0, k1);
 }
 
 constexpr int kSeg = 2048;   // words of a row that a workgroup of the two kernels below takes, eight a thread
@@ -1350,8 +1393,7 @@ __device__ __forceinline__ bool dh_work(const DhShare& sh, int tiles, int b, int
   const int rest = tiles - sh.whole, all = b < sh.whole ? sh.whole : rest * sh.parts;
   const int i = b < sh.whole ? b : b - sh.whole;
   if (i >= all) return false;
-  const int each = all / kXcds, more = all % kXcds, x = i % kXcds;
-  const int at = x * each + min(x, more) + i / kXcds;
+  const int at = xcd_order(i, all);
   id = b < sh.whole ? at : sh.whole + at % rest, part = b < sh.whole ? 0 : at / rest;
   return true;
 }
@@ -1487,7 +1529,7 @@ struct DwArgs {
   const char* h;
   const char* dz;
   int64_t ldh, ldz, plane_z;
-  int V, D, ndt;         // V: rows of dw from the piece on
+  int V, D, ndt, nvt;    // V: rows of dw from the piece on; nvt: tiles of the piece's columns
   const float* scale;
   void* out;             // dw at the piece's first row
   float* part;           // CUT: [cuts][Vp][Dt]
@@ -1496,16 +1538,10 @@ struct DwArgs {
   State st;
 };
 template <typename C, typename Op, typename X, int PZ, bool CUT>
-__global__ void __launch_bounds__(C::THREADS, 2)
-dw_kernel(DwArgs a) {
+__device__ __forceinline__ void dw_tile(const DwArgs& a, char* lds, int dt, int v0, int cut) {
   constexpr int BM = C::BM, BN = C::BN;
   using P = Product<Op, BM, BN, C::WM, C::WN, true, true>;
-  __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-  const int n = a.st.hdr->n;
-  int dt, vt;
-  const int tiles = CUT ? gridDim.x / a.cuts : gridDim.x, cut = CUT ? blockIdx.x / tiles : 0;
-  tile_of(blockIdx.x - cut * tiles, a.ndt, tiles / a.ndt, dt, vt);
-  const int d0 = dt * BM, v0 = vt * BN;
+  const int n = a.st.hdr->n, d0 = dt * BM;
   typename P::Acc acc;
   const Operand A{a.h + d0 * P::EB, a.ldh, 0, n, (int)a.ldh - d0 * P::EB};
   const Operand B{a.dz + (int64_t)v0 * P::EB, a.ldz, a.plane_z, n, BN * P::EB};
@@ -1552,6 +1588,24 @@ dw_kernel(DwArgs a) {
   }
 }
 
+template <typename C, typename Op, typename X, int PZ, bool CUT>
+__global__ void __launch_bounds__(C::THREADS, 2)
+dw_kernel(DwArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[Product<Op, C::BM, C::BN, C::WM, C::WN, true, true>::LDS_BYTES];
+  int dt, vt;
+  if constexpr (CUT) {
+    const int tiles = gridDim.x / a.cuts, cut = blockIdx.x / tiles;
+    tile_of(blockIdx.x - cut * tiles, a.ndt, tiles / a.ndt, dt, vt);
+    dw_tile<C, Op, X, PZ, true>(a, lds, dt, vt * C::BN, cut);
+  } else {
+    int id, half;
+    if (!half_work(a.ndt * a.nvt, blockIdx.x, id, half)) return;
+    band_tile(id, a.ndt, a.nvt, dt, vt);
+    if (half >= 0) dw_tile<Half256, Op, X, PZ, false>(a, lds, dt, vt * C::BN + half * Half256::BN, 0);
+    else dw_tile<C, Op, X, PZ, false>(a, lds, dt, vt * C::BN, 0);
+  }
+}
+
 // ------------------------------------------------------------------ host
 int check_dims(const char* who, int64_t T, int64_t D, int64_t V, int64_t K, int dtype, int reduction) {
   const std::string w(who);
@@ -1587,7 +1641,9 @@ LogitArgs logit_args(const Plan& p, const State& st, const void* weight, int K, 
 template <typename C, typename Op, Mode MODE, int PZ>
 void launch_logits(LogitArgs a, int64_t T, int64_t cols, hipStream_t s) {
   a.nvt = (int)(cols / C::BM);
-  logits_kernel<C, Op, MODE, PZ><<<(unsigned)(a.nvt * (up(T, C::BN) / C::BN) * (MODE == kCut ? a.cuts : 1)), C::THREADS, 0, s>>>(a);
+  const int64_t tiles = a.nvt * (up(T, C::BN) / C::BN);
+  const int64_t groups = MODE == kCut ? tiles * a.cuts : __is_same(C, Tile256) ? tiles + kHalfMore : tiles;
+  logits_kernel<C, Op, MODE, PZ><<<(unsigned)groups, C::THREADS, 0, s>>>(a);
 }
 // The forward's, whole or in parts.
 template <typename C, typename Op>
@@ -1605,8 +1661,9 @@ void launch_dh(DhArgs a, const Plan& p, int room, hipStream_t s) {
 template <typename C, typename Op, typename X, int PZ, bool CUT>
 void launch_dw(DwArgs a, const Plan& p, int64_t cols, hipStream_t s) {
   a.ndt = (int)(up(p.D, C::BM) / C::BM);
-  const unsigned tiles = (unsigned)(a.ndt * (cols / C::BN));
-  dw_kernel<C, Op, X, PZ, CUT><<<CUT ? tiles * (unsigned)a.cuts : tiles, C::THREADS, 0, s>>>(a);
+  a.nvt = (int)(cols / C::BN);
+  const unsigned tiles = (unsigned)(a.ndt * a.nvt);
+  dw_kernel<C, Op, X, PZ, CUT><<<CUT ? tiles * (unsigned)a.cuts : tiles + kHalfMore, C::THREADS, 0, s>>>(a);
   if constexpr (CUT) {
     sum_out_kernel<X, false><<<dim3((unsigned)std::min<int64_t>(cols, a.V), (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
         a.st, a.part, a.D, a.ldp, a.ldcut, a.cuts, a.scale, nullptr, static_cast<X*>(a.out));

@@ -210,10 +210,13 @@ __device__ __forceinline__ int band_id(int m, int n, int nm, int nn) {
   const int band = m / kBand, wide = min(kBand, nm - band * kBand);
   return band * kBand * nn + n * wide + m % kBand;
 }
+// The b-th of `all` pieces of work in the order in which each XCD has a contiguous part.
+__device__ __forceinline__ int xcd_order(int b, int all) {
+  const int each = all / kXcds, more = all % kXcds, x = b % kXcds;
+  return x * each + min(x, more) + b / kXcds;
+}
 __device__ __forceinline__ void tile_of(int b, int nm, int nn, int& m, int& n) {
-  const int all = nm * nn, each = all / kXcds, more = all % kXcds;
-  const int x = b % kXcds;
-  band_tile(x * each + min(x, more) + b / kXcds, nm, nn, m, n);
+  band_tile(xcd_order(b, nm * nn), nm, nn, m, n);
 }
 
 // WM x WN waves, each with MI x NI blocks of 16 x 16: element e of a lane's block (i, j)
