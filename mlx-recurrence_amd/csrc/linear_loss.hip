@@ -1167,8 +1167,8 @@ __device__ __forceinline__ Close close_up(Close c) {
   for (int w = 0; w < WAVES; ++w) all.sum += buf[w].sum, all.top = fmaxf(all.top, buf[w].top), all.count += buf[w].count;
   return all;
 }
-// (a top whose inverse is no normal value: 1)
-__device__ __forceinline__ float usable(float top) { return top > 0x1p-100f ? top : 1.f; }
+// (1 in place of a top whose inverse is no normal value, or before which the other rows' factors would vanish)
+__device__ __forceinline__ float usable(float top) { return top > 0x1p-100f && top < 0x1p60f ? top : 1.f; }
 __device__ __forceinline__ float finite_abs(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.f; }
 
 // The losses of the pairs from their tokens' log-probabilities in st.loss, and their derivative

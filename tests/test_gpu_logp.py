@@ -519,3 +519,20 @@ def test_backward_twice_and_two_calls_at_once():
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got[0][1:], first))
     assert all(torch.equal(a, b) for a, b in zip(got[1], want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("moved", [30.0, 80.0, 87.0])
+def test_a_row_far_from_its_old_policy_leaves_the_others(dtype, moved):
+    """A ratio of up to e^87 (a negative advantage does not clip it): the other rows' gradients keep their bits."""
+    g, h, w, labels, logp = head((64,), 64, 500, dtype, 23, ignored=0.0)
+    old = logp.clone()
+    old[5] -= moved
+    A = torch.full((64,), -1.0, device="cuda")
+    up = torch.ones((), device="cuda")
+    loss, dh, _ = run(mr.linear_policy_loss, h, w, up, labels, A, old.float(), reduction="sum")
+    want = orc.policy(h, w, labels, A, old.float(), None, up, reduction="sum")
+    rest = [i for i in range(64) if i != 5]
+    check("dhidden", dh[rest], want[1][rest], (1 + orc.size_of(h, w, labels)) * want[3])
+    rel = float((dh[5].double() - want[1][5]).norm() / want[1][5].norm())
+    assert rel <= (2 * U[dtype] if dtype in U else 1e-3)
