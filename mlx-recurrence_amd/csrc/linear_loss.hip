@@ -165,6 +165,7 @@ struct Plan {
   int64_t Vp;          // columns of a piece (whole tiles)
   int64_t splits;      // parts of a piece's columns that dh is added up in
   int64_t cuts_w;      // parts of the rows that dw is added up in
+  bool small_w;        // fp32 losses on log-probabilities: dw whole on Tile64 in place of parts on Tile256
 };
 constexpr int64_t kCus = 256;
 // Seconds of a k step of a round of tiles, against which the parts' bytes (at 4 TB/s, written and read)
@@ -230,6 +231,13 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
     const double step_w = p.fp32 ? kStepF32Dw : kStep;
     p.cuts_w = best_parts(p.Dt / kEdge * (p.Vp / kEdge), kCus, (double)steps, (double)(p.Vp * D * 8) / 4e12 / step_w,
                           kLaunch / step_w, steps, p.Vp * p.Dt * 4);
+    // fp32: small tiles, which are half a Tile256's k step for a quarter of its work, fill the GPU without parts
+    // (dw of 460 rows, 512 channels, 16001 words: 95 us in two parts, 71 so).
+    const int64_t tiles = p.Dt / kEdge * (p.Vp / kEdge);
+    const double whole = (double)((4 * tiles + 2 * kCus - 1) / (2 * kCus)) * (double)steps * kStepF32;
+    const double parts = (double)((tiles * p.cuts_w + kCus - 1) / kCus) * (double)steps / (double)p.cuts_w * kStepF32Dw +
+                         (p.cuts_w > 1 ? (double)(p.cuts_w * p.Vp * D * 8) / 4e12 + kLaunch : 0.);
+    p.small_w = p.fp32 && whole < parts;
   }
   return p;
 }
@@ -1597,12 +1605,15 @@ dw_kernel(DwArgs a) {
     const int tiles = gridDim.x / a.cuts, cut = blockIdx.x / tiles;
     tile_of(blockIdx.x - cut * tiles, a.ndt, tiles / a.ndt, dt, vt);
     dw_tile<C, Op, X, PZ, true>(a, lds, dt, vt * C::BN, cut);
-  } else {
+  } else if constexpr (__is_same(C, Tile256)) {
     int id, half;
     if (!half_work(a.ndt * a.nvt, blockIdx.x, id, half)) return;
     band_tile(id, a.ndt, a.nvt, dt, vt);
     if (half >= 0) dw_tile<Half256, Op, X, PZ, false>(a, lds, dt, vt * C::BN + half * Half256::BN, 0);
     else dw_tile<C, Op, X, PZ, false>(a, lds, dt, vt * C::BN, 0);
+  } else {
+    tile_of(blockIdx.x, a.ndt, a.nvt, dt, vt);
+    dw_tile<C, Op, X, PZ, false>(a, lds, dt, vt * C::BN, 0);
   }
 }
 
@@ -1663,7 +1674,8 @@ void launch_dw(DwArgs a, const Plan& p, int64_t cols, hipStream_t s) {
   a.ndt = (int)(up(p.D, C::BM) / C::BM);
   a.nvt = (int)(cols / C::BN);
   const unsigned tiles = (unsigned)(a.ndt * a.nvt);
-  dw_kernel<C, Op, X, PZ, CUT><<<CUT ? tiles * (unsigned)a.cuts : tiles + kHalfMore, C::THREADS, 0, s>>>(a);
+  dw_kernel<C, Op, X, PZ, CUT><<<CUT ? tiles * (unsigned)a.cuts : tiles + (__is_same(C, Tile256) ? kHalfMore : 0), C::THREADS, 0,
+                                s>>>(a);
   if constexpr (CUT) {
     sum_out_kernel<X, false><<<dim3((unsigned)std::min<int64_t>(cols, a.V), (unsigned)((p.D + 1023) / 1024)), 256, 0, s>>>(
         a.st, a.part, a.D, a.ldp, a.ldcut, a.cuts, a.scale, nullptr, static_cast<X*>(a.out));
@@ -1797,7 +1809,9 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
       c.V = (int)(p.V - v), c.D = (int)p.D, c.scale = ws.scale;
       c.out = static_cast<X*>(dw) + v * p.D, c.st = st;
       c.part = ws.dw, c.ldp = p.Dt, c.ldcut = p.Vp * p.Dt, c.cuts = (int)p.cuts_w;
-      if (kFew || p.cuts_w == 1) {
+      if (kFp32 && l.logp && p.small_w) {
+        if constexpr (kFp32) launch_dw<Tile64, Op, X, PZ, false>(c, p, cols, s);
+      } else if (kFew || p.cuts_w == 1) {
         launch_dw<Tile256, Op, X, PZ, false>(c, p, cols, s);
       } else if constexpr (!kFew) {
         launch_dw<Tile256, Op, X, PZ, true>(c, p, cols, s);
