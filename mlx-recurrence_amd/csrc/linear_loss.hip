@@ -242,8 +242,8 @@ Plan plan_of(int64_t T, int64_t D, int64_t V, int dtype) {
   return p;
 }
 
-// Whether the logits that are kept are more than the 256 MB cache holds: they are then written and read
-// past it (6.6 x 10^3 and 7.4 x 10^3 rows of 65536 bf16: the forward's product 2035 and 2290 us, 1920 and 2157 so).
+// Whether the logits that are kept are more than the 256 MB cache holds: they are then written past it
+// (6.6 x 10^3 and 7.4 x 10^3 rows of 65536 bf16: the forward's product 2030 and 2272 us, 1840 and 2055 so).
 bool keeps_past(const Plan& p) { return p.T * p.Vt * 4 > (int64_t)256 << 20; }
 
 // grad: 0 no backward, 1 logits where they are kept, 2 only those that always are.
@@ -616,6 +616,8 @@ __device__ __forceinline__ float rounded(float x) {
   asm("" : "+v"(x));
   return x;
 }
+// Keeps a store past the cache apart from the ordinary one of the other branch: made one, they are ordinary.
+__device__ __forceinline__ void apart() { asm volatile(""); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // First of a row's K entries at column v0 or behind.
@@ -727,8 +729,13 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& a, char* lds, int n
     store_block<P::MI>(fstage, lane, [&](int i) { return acc[i][j]; }, [&](int r, int v, f32x4_t x) {
       if (t + r >= n) return;
       f32x4_t* at = reinterpret_cast<f32x4_t*>(o + (int64_t)r * a.ldzf + v);
-      if (MODE == kStats && a.past) __builtin_nontemporal_store(x, at);
-      else *at = x;
+      if (MODE == kStats && a.past) {
+        apart();
+        __builtin_nontemporal_store(x, at);
+        apart();
+      } else {
+        *at = x;
+      }
     });
   };
   if constexpr (MODE == kCut) {
@@ -951,7 +958,7 @@ join_kernel(State st, const float* __restrict__ cut, int cuts, int64_t ldcut, in
 // in join_kernel).  A word's entries are taken off in their order by the thread of the first.
 template <typename Op, int PZ>
 __global__ void __launch_bounds__(256)
-dz_kernel(State st, const float2* __restrict__ coef, Upstream up, bool past, int V, int64_t Vt, int K, int v_first, int cols,
+dz_kernel(State st, const float2* __restrict__ coef, Upstream up, int V, int64_t Vt, int K, int v_first, int cols,
           char* __restrict__ dz, int64_t ldz, int64_t plane_z) {
   const int t = blockIdx.x;
   if (coef == nullptr && t == 0 && blockIdx.y == 0 && threadIdx.x == 0) leave_scale(up, st);
@@ -965,7 +972,7 @@ dz_kernel(State st, const float2* __restrict__ coef, Upstream up, bool past, int
     const f32x4_t* i = reinterpret_cast<const f32x4_t*>(st.z + (int64_t)t * Vt + v);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const f32x4_t x = past ? __builtin_nontemporal_load(i + q) : i[q];
+      const f32x4_t x = i[q];
       seg[2 * tid + q] = f32x4_t{exp2_fast(x[0] - l2), exp2_fast(x[1] - l2), exp2_fast(x[2] - l2), exp2_fast(x[3] - l2)};
     }
   }
@@ -1786,7 +1793,7 @@ int backward(const Plan& p, const float* dloss, const void* weight, const State&
     constexpr bool kFp32 = __is_same(Op, OpF32), kFew = PZ == 2;   // up to kFewRows
     if (kFew || st.z != nullptr) {
       dz_kernel<Op, PZ><<<dim3((unsigned)p.T, (unsigned)(up(cols, kSeg) / kSeg)), 256, 0, s>>>(
-          st, coef, us, keeps_past(p), a.V, p.Vt, K, a.v_first, (int)cols, ws.dz, a.ldz, a.plane_z);
+          st, coef, us, a.V, p.Vt, K, a.v_first, (int)cols, ws.dz, a.ldz, a.plane_z);
     } else if constexpr (!kFew) {
       launch_logits<typename std::conditional<kFp32, Tile64, Tile256>::type, Op, kGrad, PZ>(a, p.T, cols, s);
     }
