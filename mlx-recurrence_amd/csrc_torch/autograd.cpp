@@ -569,6 +569,9 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
       throw pybind11::value_error("out must have a tensor of each gradient's shape and type");
     }
     if (o.device() != dev) require_device({&g, &o});
+    if (recording && o.requires_grad()) {
+      throw pybind11::value_error("out must not need a gradient; call it under torch.no_grad()");
+    }
   }
   const at::DeviceGuard guard(dev);
   std::vector<const void*> in(n);

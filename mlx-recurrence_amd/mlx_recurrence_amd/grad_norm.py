@@ -51,6 +51,8 @@ def _run(grads, outs, clip, max_norm):
             raise ValueError("a tensor to write was made in inference mode; call it there")
         if outs and (outs[i].layout != torch.strided or outs[i].shape != g.shape or outs[i].dtype != g.dtype):
             raise ValueError("out must have a tensor of each gradient's shape and type")
+        if outs and torch.is_grad_enabled() and outs[i].requires_grad:
+            raise ValueError("out must not need a gradient; call it under torch.no_grad()")
     dev = _lib.require_device(*grads, *(outs or ()))
     with _lib.device_guard(dev), torch.no_grad():
         src = [g if _dense(g) else g.contiguous() for g in grads]

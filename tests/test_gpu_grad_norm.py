@@ -267,6 +267,21 @@ def test_a_step_of_the_policy_and_the_pairs():
 
 
 @pytest.mark.parametrize("python", [False, True])
+def test_out_that_needs_a_gradient(python, monkeypatch):
+    """What is written has no place in a graph: its gradient would be that of the values before."""
+    if python:
+        monkeypatch.setattr(_lib, "_autograd_mod", None)
+    g, leaf = torch.full((5,), 3.0, device="cuda"), torch.zeros(5, device="cuda", requires_grad=True)
+    for o in (leaf, leaf * 2, (leaf * 2)[:]):
+        with pytest.raises(ValueError, match="out must not need a gradient"):
+            mr.clip_grad_norm([g], 1.0, out=[o])
+    assert not leaf.detach().any()
+    with torch.no_grad():
+        mr.clip_grad_norm([g], math.inf, out=[leaf])
+    assert torch.equal(leaf.detach(), g)
+
+
+@pytest.mark.parametrize("python", [False, True])
 def test_inference_mode(python, monkeypatch):
     if python:
         monkeypatch.setattr(_lib, "_autograd_mod", None)
