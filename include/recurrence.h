@@ -492,8 +492,8 @@ int rr_linear_logp_bwd(const float* dloss, const void* weight, int dtype, int64_
  * memory, of numel[i] contiguous values of dtypes[i] each, at any multiple of an element's size;
  * out[i] may be grads[i], and nothing else of what is written may share memory with another
  * tensor.  The arrays are not read after the call returns.  norm: one fp32 on the device.
- * Sums and products are in 64 bits, added in a fixed order.  A norm that is not finite leaves the
- * values as they are.  max_norm >= 0, infinity: nothing is scaled. */
+ * Sums and products are in 64 bits, added in a fixed order.  One value that is not finite leaves all
+ * as they are (norms beyond fp32's range are infinite only as *norm).  max_norm >= 0, infinity: nothing is scaled. */
 size_t rr_grad_norm_workspace_bytes(int64_t count);
 int rr_grad_norm(int64_t count, const void* const* grads, const int64_t* numel, const int* dtypes, float* norm,
                  void* workspace, size_t workspace_bytes, void* stream);

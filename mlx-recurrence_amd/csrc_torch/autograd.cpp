@@ -591,7 +591,7 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
     in[i] = src.const_data_ptr(), numel[i] = src.numel(), types[i] = dtype_code(src.scalar_type());
     if (!clip) continue;
     const Tensor& o = outs.empty() ? *grads[i] : *outs[i];
-    if (&o == g || (o.is_non_overlapping_and_dense() && o.strides() == src.strides())) {
+    if (&o == g || numel[i] == 0 || (o.is_non_overlapping_and_dense() && o.strides() == src.strides())) {
       to[i] = o.data_ptr();
       continue;
     }

@@ -63,7 +63,7 @@ def _run(grads, outs, clip, max_norm):
         written = outs or grads
         to, back = [], []
         for o, s in zip(written, src):
-            if _dense(o) and o.stride() == s.stride():
+            if s.numel() == 0 or (_dense(o) and o.stride() == s.stride()):
                 to.append(o)
                 continue
             if any(st == 0 and sz > 1 for st, sz in zip(o.stride(), o.shape)):
@@ -107,8 +107,8 @@ def global_grad_norm(grads):
 def clip_grad_norm(grads, max_norm, *, out=None):
     """Scale `grads` in place so that their norm, taken together, is at most `max_norm`, on the GPU.
 
-    ``g *= max_norm / norm`` where ``norm > max_norm``; otherwise they are not touched.  A norm
-    that is infinite or NaN leaves them as they are: the caller sees it in what is returned.
+    ``g *= max_norm / norm`` where ``norm > max_norm``; otherwise they are not touched.  One value
+    that is infinite or NaN leaves them all as they are: the caller sees it in what is returned.
 
     Args:
         grads:     as for global_grad_norm.  No two may share memory: those without gaps

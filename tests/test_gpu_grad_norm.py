@@ -267,6 +267,19 @@ def test_a_step_of_the_policy_and_the_pairs():
 
 
 @pytest.mark.parametrize("python", [False, True])
+def test_empty_tensors_of_another_layout(python, monkeypatch):
+    """They have no memory to share, and no values to be there twice."""
+    if python:
+        monkeypatch.setattr(_lib, "_autograd_mod", None)
+    def zeros(*shape):
+        return torch.zeros(shape, device="cuda")
+    grads = [zeros(0, 3), zeros(0, 3), torch.full((4,), 2.0, device="cuda"), zeros(0, 3)]
+    out = [zeros(3, 0).T, zeros(3, 0).T, zeros(4), zeros(0, 1).expand(0, 3)]
+    assert float(mr.clip_grad_norm(grads, 1.0, out=out)) == 4.0 and torch.equal(out[2], torch.full((4,), 0.5, device="cuda"))
+    assert float(mr.clip_grad_norm([zeros(0, 1).expand(0, 3), zeros(3, 0).T], 1.0)) == 0.0
+
+
+@pytest.mark.parametrize("python", [False, True])
 def test_out_that_needs_a_gradient(python, monkeypatch):
     """What is written has no place in a graph: its gradient would be that of the values before."""
     if python:
