@@ -524,6 +524,24 @@ Tensor linear_logp(const Tensor& hidden, const Tensor& weight, const Tensor& lab
 }
 
 // ------------------------------------------------------------------ norm of gradients
+// What is written to must not be another's.  The library sees the copies in place of tensors that are copied
+// to, so all are looked at here: the whole of a tensor without gaps, the first value of one with gaps.
+void check_written(const std::vector<const Tensor*>& written) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> ranges;   // first byte and end
+  ranges.reserve(written.size());
+  for (const Tensor* t : written) {
+    if (t->numel() == 0) continue;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t->const_data_ptr());
+    ranges.emplace_back(at, at + t->element_size() * (t->is_non_overlapping_and_dense() ? t->numel() : 1));
+  }
+  std::sort(ranges.begin(), ranges.end());
+  uintptr_t end = 0;
+  for (const auto& r : ranges) {
+    if (r.first < end) throw pybind11::value_error("two of the tensors to write share memory");
+    end = r.second;   // (behind those in front, which it does not reach into)
+  }
+}
+
 // The norm of all of `grads` together; with `clip` they leave scaled to max_norm at most, in place or,
 // where `outs` is a list of as many, there (mlx_recurrence_amd.grad_norm._run, which checks the same).
 // The tensors are taken from Python's lists as they are: converting a list of 300 takes longer than its
@@ -579,8 +597,7 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
   std::vector<int64_t> numel(n);
   std::vector<int> types(n);
   std::deque<Tensor> held;                                 // what lives until the launches are made
-  std::vector<std::pair<Tensor, Tensor>> back;             // copies to go back to tensors with gaps
-  std::vector<const void*> gaps;
+  std::vector<std::pair<Tensor, Tensor>> back;             // copies to go back to tensors with gaps or laid out in another way
   for (size_t i = 0; i < n; ++i) {
     const Tensor* g = grads[i];
     if (!g->is_non_overlapping_and_dense()) {
@@ -598,15 +615,11 @@ Tensor grad_norm(const pybind11::list& grad_list, const c10::optional<pybind11::
     for (int64_t d = 0; d < o.dim(); ++d) {
       if (o.stride(d) == 0 && o.size(d) > 1) throw pybind11::value_error("a tensor to write has its values more than once");
     }
-    gaps.push_back(o.data_ptr());
     const Tensor tmp = outs.empty() ? src : at::empty_like(src);
     to[i] = tmp.data_ptr();
     back.emplace_back(o, tmp);
   }
-  std::sort(gaps.begin(), gaps.end());
-  if (std::adjacent_find(gaps.begin(), gaps.end()) != gaps.end()) {
-    throw pybind11::value_error("two of the tensors to write share memory");
-  }
+  if (!back.empty()) check_written(outs.empty() ? grads : outs);
   Tensor norm = at::empty({}, grads[0]->options().dtype(at::kFloat).requires_grad(false));
   const size_t wsb = rr_grad_norm_workspace_bytes((int64_t)n);
   const Tensor ws = workspace(wsb, norm.options());

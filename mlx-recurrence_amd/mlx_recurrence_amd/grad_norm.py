@@ -29,6 +29,15 @@ def _dense(t):
     return True
 
 
+def _check_written(written):
+    """What is written to must not be another's.  The library sees the copies in place of tensors that are copied
+    to, so all are looked at here: the whole of a tensor without gaps, the first value of one with gaps."""
+    ranges = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (t.numel() if _dense(t) else 1))
+                    for t in written if t.numel())
+    if any(b[0] < a[1] for a, b in zip(ranges, ranges[1:])):
+        raise ValueError("two of the tensors to write share memory")
+
+
 def _run(grads, outs, clip, max_norm):
     """The C++ module's grad_norm for where it is not built."""
     if outs is not None:
@@ -70,8 +79,8 @@ def _run(grads, outs, clip, max_norm):
                 raise ValueError("a tensor to write has its values more than once")
             to.append(torch.empty_like(s) if outs else s)
             back.append((o, to[-1]))
-        if len({o.data_ptr() for o, _ in back}) < len(back):
-            raise ValueError("two of the tensors to write share memory")
+        if back:
+            _check_written(written)
         _lib.grad_norm(src, to, max_norm, norm)
         for o, t in back:
             o.copy_(t)
@@ -111,8 +120,8 @@ def clip_grad_norm(grads, max_norm, *, out=None):
     that is infinite or NaN leaves them all as they are: the caller sees it in what is returned.
 
     Args:
-        grads:     as for global_grad_norm.  No two may share memory: those without gaps
-                   between their values are checked.
+        grads:     as for global_grad_norm.  No two may share memory, which is checked (of those
+                   with gaps between their values, the first value's place).
         max_norm:  the largest norm, 0 or more (math.inf: take the norm alone).
         out:       tensors of the same shapes and types to write to, in place of `grads` (each
                    a tensor of its own, or the gradient itself).

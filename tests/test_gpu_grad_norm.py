@@ -350,3 +350,24 @@ def test_more_than_the_cache(dtype):
     for a, t in zip(out, grads):
         off = (a.double() - t.double() * 0.25).abs()
         assert bool((off <= t.double().abs() * 0.25 * (U[a.dtype] + 2.0 ** -23) + LEAST[a.dtype]).all())
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_outputs_of_another_layout_share_no_memory(python, monkeypatch):
+    """Outputs that are copied to are checked too, together with those written directly."""
+    if python:
+        monkeypatch.setattr(_lib, "_autograd_mod", None)
+        monkeypatch.setattr(_lib, "autograd_ext", lambda: None)
+    a, b, o = (torch.zeros(s, device="cuda") for s in ((4, 4), (4, 4), (8, 4)))
+    a, b = a + 1, (b + 2).T
+    for grads, out in (([a, b], [o[:4], o[:4]]), ([a, b], [o[:4], o[1:5]]), ([b, a], [o[1:5], o[:4]]), ([b, b], [o[:4], o[2:6]]),
+                       ([a, b], [o[:4], o[1:5].T]), ([a, b[:2]], [o[:4], o[:4:2]]), ([b[:2], b[:2]], [o[:4:2], o[:4:2]])):
+        with pytest.raises(ValueError, match="share memory"):
+            mr.clip_grad_norm(grads, 1.0, out=out)
+    assert not o.any()
+    keep = [a.clone(), b.clone()]
+    check(mr.clip_grad_norm([a, b], 1.0, out=[o[:4], o[4:]]), [o[:4], o[4:]], keep, 1.0)   # one behind the other
+    o = torch.zeros(4, 8, device="cuda")
+    check(mr.clip_grad_norm([a, b], 1.0, out=[o[:, :4], o[:, 4:]]), [o[:, :4], o[:, 4:]], keep, 1.0)   # in the other's gaps
+    m = torch.ones(4, 8, device="cuda")
+    check(mr.clip_grad_norm([m[:, :4], m[:, 4:]], 1.0), [m[:, :4], m[:, 4:]], [torch.ones(4, 4, device="cuda")] * 2, 1.0)

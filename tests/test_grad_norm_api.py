@@ -1,5 +1,6 @@
 """The norm of gradients and their clipping on the CPU: the plain forms, the refusals of the public
 functions, and the C ABI's argument checks (no kernel runs)."""
+import contextlib
 import ctypes
 import math
 import os
@@ -57,6 +58,37 @@ def test_refusals(python, monkeypatch):
         mr.clip_grad_norm([t], 1.0, out=[t, t])
     with pytest.raises(ValueError, match="out must have a tensor of each gradient's shape"):
         mr.clip_grad_norm([t], 1.0, out=[None])
+
+
+def test_outputs_of_another_layout_share_no_memory(monkeypatch):
+    """Outputs that are copied to are checked too, together with those written directly (the library replaced
+    by the plain form)."""
+    monkeypatch.setattr(_lib, "_autograd_mod", None)
+    monkeypatch.setattr(_lib, "autograd_ext", lambda: None)
+    monkeypatch.setattr(_lib, "require_device", lambda *t: t[0].device)
+    monkeypatch.setattr(_lib, "device_guard", lambda dev: contextlib.nullcontext())
+
+    def plain(grads, out, max_norm, norm):
+        n, scaled = mr.clip_grad_norm_reference(grads, max_norm)
+        norm.copy_(n)
+        for o, v in zip(out, scaled):
+            o.copy_(v)
+
+    monkeypatch.setattr(_lib, "grad_norm", plain)
+    a, b, o = torch.ones(4, 4), torch.full((4, 4), 2.0).T, torch.zeros(8, 4)
+    assert a.stride() != b.stride()
+    for grads, out in (([a, b], [o[:4], o[:4]]), ([a, b], [o[:4], o[1:5]]), ([b, a], [o[1:5], o[:4]]), ([b, b], [o[:4], o[2:6]]),
+                       ([a, b[:2]], [o[:4], o[:4:2]]), ([b[:2], b[:2]], [o[:4:2], o[:4:2]])):
+        with pytest.raises(ValueError, match="share memory"):
+            mr.clip_grad_norm(grads, 1.0, out=out)
+    assert not o.any()
+    mr.clip_grad_norm([a, b, b[:1]], 1.0, out=[o[:4], o[4:], torch.zeros(1, 4)])   # one behind the other
+    f = 1 / math.sqrt(16 + 4 * 16 + 16)
+    assert torch.allclose(o[:4], a * f) and torch.allclose(o[4:], b * f)
+    o = torch.zeros(4, 8)
+    mr.clip_grad_norm([a, b], 1.0, out=[o[:, :4], o[:, 4:]])   # one in the other's gaps
+    f = 1 / math.sqrt(16 + 4 * 16)
+    assert torch.allclose(o[:, :4], a * f) and torch.allclose(o[:, 4:], b * f)
 
 
 def _arrays(tensors):
