@@ -188,7 +188,8 @@ def linear_preference_loss(hidden, weight, labels, ref_log_probs=None, *, beta=0
         labels:           [..., 2, L] integers in [0, V), or `ignore_index` (prompts, padding):
                           such a token counts for nothing.  Any other label makes the pair's
                           loss (and every gradient) NaN.
-        ref_log_probs:    [..., 2] the reference's sums, or None (0).
+        ref_log_probs:    [..., 2] the reference's sums, or None (0).  Sums of long sequences are best
+                          given in float64: what they differ by is not rounded with them.
         beta:             how far the policy may move from the reference: the smaller, the farther.
         label_smoothing:  share of pairs whose order is taken to be wrong, 0 to 0.5.
         reduction:        "mean" over the pairs with a token that counts (0 where there is
@@ -208,6 +209,11 @@ def linear_preference_loss(hidden, weight, labels, ref_log_probs=None, *, beta=0
         raise ValueError(f"beta must be positive and finite, got {beta}")
     if not 0 <= float(label_smoothing) <= 0.5:
         raise ValueError(f"label_smoothing must be in [0, 0.5], got {label_smoothing}")
+    if ref_log_probs is not None and ref_log_probs.dtype == torch.float64:
+        # The loss takes their difference alone.  The sums are in the thousands, and rounded to fp32 each would be
+        # off by up to 2.4e-4.
+        ref = ref_log_probs.detach()
+        ref_log_probs = torch.stack([ref[..., 0] - ref[..., 1], torch.zeros_like(ref[..., 0])], -1)
     out = _apply(hidden, weight, labels, keep_logits, None, None, ref_log_probs, _PREFERENCE, math.prod(lead), labels.shape[-1],
                  ignore_index, (1.0, beta, label_smoothing), _REDUCTIONS[reduction])
     return out.reshape(lead) if reduction == "none" and len(lead) != 1 else out

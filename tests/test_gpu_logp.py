@@ -536,3 +536,19 @@ def test_a_row_far_from_its_old_policy_leaves_the_others(dtype, moved):
     check("dhidden", dh[rest], want[1][rest], (1 + orc.size_of(h, w, labels)) * want[3])
     rel = float((dh[5].double() - want[1][5]).norm() / want[1][5].norm())
     assert rel <= (2 * U[dtype] if dtype in U else 1e-3)
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_reference_sums_in_64_bits(reduction, python, monkeypatch):
+    """Sums of 2^17, which differ by what fp32 cannot hold beside them."""
+    if python:
+        monkeypatch.setattr(_lib, "_autograd_mod", None)
+        monkeypatch.setattr(_lib, "autograd_ext", lambda: None)
+    g, h, w, labels, logp = head((5, 2, 12), 64, 300, F32, 25)
+    ref = torch.where(labels != -100, logp, 0).sum(-1) + 2 * randn(g, 5, 2) - 2.0 ** 17
+    assert ref.dtype == torch.float64
+    up = rand(g, 5) + 0.1 if reduction == "none" else torch.ones((), device="cuda")
+    got = run(mr.linear_preference_loss, h, w, up, labels, ref, beta=0.5, reduction=reduction)
+    want = orc.preference(h, w, labels, ref, up, beta=0.5, reduction=reduction)
+    check_all(got, want, 1 + 0.5 * math.sqrt(24) * orc.size_of(h, w, labels))

@@ -164,6 +164,25 @@ def test_preference_refusals():
             mr.linear_preference_loss(h, w, l, label_smoothing=eps)
 
 
+def test_preference_keeps_what_sums_in_64_bits_differ_by(monkeypatch):
+    """Rounded to fp32, sums of 2^17 and more are off by up to 2^-7 each."""
+    h, w, l = _zeros(3, 2, 4, 8), _zeros(10, 8), torch.zeros(3, 2, 4, dtype=torch.int64)
+    given = []
+    monkeypatch.setattr(mr.linear_logp, "_apply", lambda *a: given.append(a[6]) or _zeros(3))
+    ref = 3 * _rand(3, 2, seed=1)
+    want = ref[:, 0] - ref[:, 1]
+    for offset in (0.0, -3000.0, -200_000.0):
+        sums = ref + offset   # exact but for 2^-36
+        mr.linear_preference_loss(h, w, l, sums)
+        got = given[-1].float().double()   # as the kernel takes it: rounded, then subtracted in 64 bits
+        assert ((got[:, 0] - got[:, 1] - want).abs() <= 2.0 ** -24 * want.abs() + 2.0 ** -34).all()
+    for sums in (ref.float(), ref.bfloat16()):
+        mr.linear_preference_loss(h, w, l, sums)
+        assert given[-1] is sums
+    mr.linear_preference_loss(h, w, l)
+    assert given[-1] is None
+
+
 def test_c_abi_refusals():
     """Argument errors are found before any work is enqueued (the pointers are never read)."""
     lib, p, odd = _lib.load(), ctypes.c_void_p(16), ctypes.c_void_p(24)
