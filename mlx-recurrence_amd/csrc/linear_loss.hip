@@ -287,7 +287,7 @@ struct BwdWs {
   char* h;         // [T][Dp] the hidden states times that (fp16)
   char* dz;        // [planes_z][Tp][Vp]
   float* dh;       // [splits][Tp][Dt]; log-probabilities: [Tp][Dt], then the shared tiles' parts (DhShare)
-  float* dw;       // [cuts_w][Vp][Dt], where there are two or more
+  float* dw;       // [cuts_w][Vp][Dt], where there are two or more and they are used
 };
 // dh's tiles in the losses on log-probabilities.  How many rows count is known on the device
 // alone, and with it how many tiles there are: as many as fill whole rounds of the GPU are done by a
@@ -343,7 +343,7 @@ size_t bwd_layout(const Plan& p, bool logp, char* base, BwdWs* s) {
   t.h = take(p.dtype == RR_F16 ? (size_t)p.T * p.Dp * p.eb : 0);
   t.dz = take((size_t)p.planes_z * p.Tp * p.Vp * p.eb);
   t.dh = reinterpret_cast<float*>(take(dh_bytes(p, logp)));
-  t.dw = reinterpret_cast<float*>(take(p.cuts_w > 1 ? (size_t)p.cuts_w * p.Vp * p.Dt * 4 : 0));
+  t.dw = reinterpret_cast<float*>(take(p.cuts_w > 1 && !(logp && p.small_w) ? (size_t)p.cuts_w * p.Vp * p.Dt * 4 : 0));
   if (s != nullptr) *s = t;
   return take.off;
 }

@@ -495,6 +495,27 @@ def test_kernels_write_inside_their_buffers(pairs, L, D, V, dtype, monkeypatch):
         assert (whole[:4096] == 0xA5).all() and (whole[4096 + n:] == 0xA5).all()
 
 
+def test_dweight_made_whole_in_fp32_writes_inside_its_buffers(monkeypatch):
+    """460 rows of 512 channels: the workspace holds no parts of dweight, which is made whole on small tiles."""
+    buffers = []
+
+    def guarded(n, device):
+        whole = torch.full((n + 8192,), 0xA5, dtype=torch.uint8, device=device)
+        whole[4096:4096 + n] = 0xFF
+        buffers.append((whole, n))
+        return whole[4096:4096 + n]
+
+    g, h, w, labels, logp = head((4, 115), 512, 16001, F32, 26, ignored=0.1)
+    A, up = randn(g, 4, 1), torch.ones((), device="cuda")
+    monkeypatch.setattr(_lib, "autograd_ext", lambda: None)
+    monkeypatch.setattr(_lib, "_alloc_ws", guarded)
+    got = run(mr.linear_policy_loss, h, w, up, labels, A, logp.float())
+    check_all(got, orc.policy(h, w, labels, A, logp.float(), None, up), 1 + orc.size_of(h, w, labels))
+    assert len(buffers) == 3
+    for whole, n in buffers:
+        assert (whole[:4096] == 0xA5).all() and (whole[4096 + n:] == 0xA5).all()
+
+
 def test_backward_twice_and_two_calls_at_once():
     """A graph kept for a second backward gives the same; calls on two streams share nothing."""
     g, h, w, labels, logp = head((6, 2, 32), 256, 1000, BF16, 21)

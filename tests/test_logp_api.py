@@ -251,3 +251,12 @@ def test_backward_workspace_holds_a_piece_of_the_gradient(rows, D, V, dtype):
     sums = rows_up * up(D, 256) * 4 + (128 + 256) * mib
     copy = rows * up(D, 64) * 2 if dtype == 2 else 0
     assert 0 < lib.rr_linear_loss_workspace_bytes(rows, D, V, dtype, 2) <= piece + sums + copy + rows_up * 16 + 4096
+
+
+@pytest.mark.parametrize("rows,D,V", [(512, 512, 16001), (460, 512, 16001), (700, 768, 8000)])
+def test_backward_workspace_of_fp32_has_no_parts_of_dweight_where_it_is_made_whole(rows, D, V):
+    """The gradient of all logits, dhidden's sums, two tiles of 256 x 64 a slot of its 512, and two floats a row."""
+    up = lambda a, b: (a + b - 1) // b * b  # noqa: E731
+    rows_up = up(rows, 256)
+    most = rows_up * up(V, 256) * 4 + rows_up * up(D, 256) * 4 + 1024 * 256 * 64 * 4 + rows_up * 8 + 4096
+    assert 0 < _lib.load().rr_linear_loss_workspace_bytes(rows, D, V, 0, 2) <= most
