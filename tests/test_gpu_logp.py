@@ -573,3 +573,79 @@ def test_reference_sums_in_64_bits(reduction, python, monkeypatch):
     got = run(mr.linear_preference_loss, h, w, up, labels, ref, beta=0.5, reduction=reduction)
     want = orc.preference(h, w, labels, ref, up, beta=0.5, reduction=reduction)
     check_all(got, want, 1 + 0.5 * math.sqrt(24) * orc.size_of(h, w, labels))
+
+
+# Rows (a fifth ignored), channels, words.  dhidden has 17 x 18 tiles of 256 x 256 for 4400 rows of 4200 channels, 5 x 105 of
+# 256 x 64 for 6720 of 1100 in fp32: more than the 256 (512) that run at one time, so that some tiles are made whole and
+# the others in parts.  The last of each type keeps more than 256 MiB of logits, in two pieces of the vocabulary or three.
+LARGE = [(BF16, 5500, 4200, 1001), (F16, 5500, 4200, 1001), (F32, 8400, 1100, 301),
+         (BF16, 5500, 4200, 60000), (F16, 5500, 4200, 60000), (F32, 8400, 1100, 40000)]
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("dtype,rows,D,V", LARGE)
+def test_more_tiles_than_run_at_one_time(dtype, rows, D, V, reduction):
+    g, h, w, labels, logp = head((rows,), D, V, dtype, rows + V, ignored=0.2)
+    A = 1 + 0.5 * randn(g, rows)
+    old = (logp - away(0.15 * randn(g, rows), (0.2, 0.2))).float()
+    # (a mean's gradients are a few thousandths of a token's: above fp16's least steps by this)
+    up = rand(g, rows) + 0.1 if reduction == "none" else torch.tensor(700.0, device="cuda")
+    want = orc.policy(h, w, labels, A, old, None, up, reduction=reduction)
+    size = 1 + orc.size_of(h, w, labels)
+    for keep in (True, False):
+        got = run(mr.linear_policy_loss, h, w, up, labels, A, old, reduction=reduction, keep_logits=keep)
+        check_all(got, want, size)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,D,V", [(300, 200, 5003), (1500, 768, 16001)])
+def test_gradients_of_16_bits_are_rounded_twice_and_no_more(rows, D, V, dtype):
+    """Factors spread over many values: the logits' gradient and the output are each off by up to u, half a step at the
+    least value of a binade, evenly between -u and u: u / sqrt(3) in the 2-norm at most.  With fp32's errors, sqrt(2 / 3) u."""
+    g, h, w, labels, logp = head((rows,), D, V, dtype, rows + D)
+    A = torch.exp(0.5 * randn(g, rows))
+    old = (logp - away(0.05 * randn(g, rows), (0.2, 0.2))).float()
+    up = torch.ones((), device="cuda")
+    # (the upstream gradient keeps fp16's least steps far below what is compared)
+    got = run(mr.linear_policy_loss, h, w, up * 64, labels, A, old)
+    want = orc.policy(h, w, labels, A, old, None, up * 64)
+    for name, a, e in zip(("dhidden", "dweight"), got[1:], want[1:3]):
+        rel = float((a.double() - e).norm() / e.norm())
+        assert rel <= math.sqrt(2 / 3) * U[dtype] * 1.01, f"{name}: {rel:.2e}"
+
+
+def two_sure_words(T, dtype, seed):
+    """Row 5's softmax is on words 7 and 8 alone (the others' probabilities are 0 in fp32), which no other row has as its
+    label: what row 5 gives dweight is in those two rows.  (hidden, weight, labels)"""
+    g, h, w, labels, _ = head((T,), 64, 500, dtype, seed, ignored=0.0)
+    labels = torch.where((labels == 7) | (labels == 8), 9, labels)
+    w[:, 0] = 0.0
+    w[7:9, 0] = 32.0
+    h[:, 0] = 0.0
+    h[5] = 0.0
+    h[5, 0] = 4.0
+    labels[5] = 7
+    return g, h, w, labels
+
+
+@pytest.mark.parametrize("T", [48, 300])
+@pytest.mark.parametrize("dtype,moved", [(F32, 30.0), (F32, 80.0), (BF16, 30.0), (BF16, 80.0), (F16, 7.0), (F16, 14.0)])
+def test_a_row_far_from_its_old_policy_leaves_the_others_words(dtype, moved, T):
+    """A ratio of e^moved in row 5: dhidden's other rows, and the rows of dweight that only the other tokens give
+    anything.  In fp16 the upstream gradient keeps row 5's own in the type's range."""
+    g, h, w, labels = two_sure_words(T, dtype, 23)
+    logp = orc.log_probs(h, w, labels, torch.zeros(T, device="cuda"))[0]
+    assert abs(float(logp[5]) + math.log(2)) < 0.01
+    old = logp.clone()
+    old[5] -= moved
+    A = torch.full((T,), -1.0, device="cuda")
+    up = torch.tensor(2.0 ** -8 if moved == 14.0 else 1.0, device="cuda")
+    loss, dh, dw = run(mr.linear_policy_loss, h, w, up, labels, A, old.float(), reduction="sum")
+    want = orc.policy(h, w, labels, A, old.float(), None, up, reduction="sum")
+    rows = [i for i in range(T) if i != 5]
+    words = [i for i in range(500) if i not in (7, 8)]
+    times = (1 + orc.size_of(h, w, labels)) * want[3]
+    check("dhidden", dh[rows], want[1][rows], times)
+    check("dweight", dw[words], want[2][words], times)
+    for a, e in ((dh[5], want[1][5]), (dw[7:9], want[2][7:9])):
+        assert float((a.double() - e).norm() / e.norm()) <= (2 * U[dtype] if dtype in U else 1e-3)
