@@ -30,13 +30,13 @@
 // up over the pieces in fp32).
 //
 // What bounds it: with many rows the products, two to four of 2 rows V D flops (8192 x
-// 65536 x 2560 bf16 forward and backward 7.45 ms, 1.1 PFLOP/s of the three it cannot do
+// 65536 x 2560 bf16 forward and backward 7.3 to 7.5 ms, 1.1 PFLOP/s of the three it cannot do
 // without; a large product alone runs at 1.4); with few rows the weight's bytes, read
-// once forward and once backward and dw's written (16 x 65536 x 5120 bf16 forward 131 us, 5.1
-// TB/s, with the backward 545 us, 3.7 TB/s); below about 200 us the launches, 10 to 15.
+// once forward and once backward and dw's written (16 x 65536 x 5120 bf16 forward 137 us, 4.9
+// TB/s, with the backward 540 us, 3.7 TB/s); below about 200 us the launches, 10 to 15.
 // Where a product has fewer tiles than CUs its sum is cut in parts that are joined by a
 // launch more (best_parts): the logits' over the channels, dh's over the words, dw's over the
-// rows (fp32, 209 rows of 3456 channels, 832 words, forward and backward: 543 us whole, 151 cut).
+// rows (fp32, 209 rows of 3456 channels, 832 words, forward and backward: 117 us, 3.6 times that whole).
 //
 // Rows that count for nothing (an ignored label, no teacher entry) are left out
 // before the products: the rows that remain are gathered, in order, and their
@@ -51,7 +51,13 @@
 // fp16 dz carries a power of two that brings the largest |dz| just below 2^14, so that
 // small probabilities keep their bits; bf16 and fp32 need none.  Where each row has an
 // upstream gradient of its own the power is the row's own too: dh's rows are divided by it
-// at the end, and dw reads the hidden states divided by it (a copy, for dw sums over rows).
+// at the end, and dw reads the hidden states divided by it (a copy, for dw sums over rows), where a
+// row whose |factor hidden| is below 2^-29 of the largest loses bits, and all of them below 2^-40.
+//
+// dz of 16-bit inputs is in 16 bits, as they are: with more than kFewRows rows in one plane, which is
+// the second rounding of a gradient whose output is the first.  A second plane would undo it at the
+// price of twice the products of dw and dh: gradients 2.3e-3 and 1.66e-3 off in the 2-norm, 6.8 and
+// 10.9 ms (policy loss, 8192 x 65536 x 2560 bf16), 133 and 179 us (preference loss, 512 x 32000 x 768).
 //
 // Everything is added up in a fixed order, without atomics.
 #include "rr_common.h"
@@ -82,7 +88,7 @@ constexpr int64_t kKeepRows = 256;         // rows whose logits are always kept
 // Logits are kept where they take no more than 4 GiB (of 288) and, with many rows, writing and
 // reading one costs less than its product: forward and backward of 1024 x 32000 in bf16 with 768,
 // 1024 and 2560 channels 267, 293 and 568 us kept, 266, 298 and 633 formed again; 8192 x 65536
-// x 2560 7.6 and 8.9 ms.  fp32 products cost more, so theirs are kept from a twelfth of the
+// x 2560 7.5 and 9.0 ms.  fp32 products cost more, so theirs are kept from a twelfth of the
 // channels on: 1536 x 32000 with 64, 96 and 192 channels 588, 634 and 680 us kept, 583, 671 and
 // 762 formed again.  Few rows' are always kept: their product is a whole reading of the weight.
 constexpr int64_t kKeepBytes = (int64_t)4 << 30;
@@ -98,8 +104,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // 294 us, 301 to 307 with them).  Tile64 and Tile32 are for a few rows, whose products are
 // bound by the weight's bytes (two workgroups a CU): 16 x 65536 x 5120 forward 137 us, 156
 // with Tile256.  fp32 has no tile above Tile64 but for dw: its products are slow enough to hide
-// the loads, and small tiles fill the last round (300 x 5003 x 1000 forward and backward 212
-// us, 274 with Tile256; 2048 x 32000 x 2048 5.86 and 5.77 ms).
+// the loads, and small tiles fill the last round (with Tile256 300 x 5003 x 1000 forward and
+// backward took 29 % longer, 2048 x 32000 x 2048 1.5 % less).
 struct Tile256 { static constexpr int BM = 256, BN = 256, WM = 2, WN = 4, THREADS = 512; };
 struct Tile64 { static constexpr int BM = 256, BN = 64, WM = 4, WN = 1, THREADS = 256; };
 struct Tile32 { static constexpr int BM = 256, BN = 32, WM = 4, WN = 1, THREADS = 256; };
@@ -169,8 +175,8 @@ struct Plan {
 };
 constexpr int64_t kCus = 256;
 // Seconds of a k step of a round of tiles, against which the parts' bytes (at 4 TB/s, written and read)
-// and a launch are weighed: fp32's at 1.4 us too took 210 us at 300 x 5003 x 1000 forward and backward, 185
-// now, 5.4 and 4.9 ms at 4678 x 30720 x 535 (but 694 and 719 us at 512 x 32000 x 768).
+// and a launch are weighed: with fp32's at 1.4 us too 300 x 5003 x 1000 forward and backward took 14 %
+// longer, 4678 x 30720 x 535 10 % (but 512 x 32000 x 768 3.5 % less).
 constexpr double kStep = 1.4e-6;        // Tile256 of 16 bits (smaller tiles: the weight's bytes)
 constexpr double kStepF32 = 3.5e-6;     // Tile64, two a CU
 constexpr double kStepF32Dw = 7e-6;     // Tile256
@@ -572,6 +578,13 @@ pack_kernel(const X* __restrict__ hidden, const X* __restrict__ weight, int64_t 
 // What multiplies a row of dz where nothing has to be known of the other rows (the losses on
 // log-probabilities in bf16 and fp32): found where dz is made, coef_kernel's launch saved (2.4 us of 146
 // for 512 rows of 768 channels and 32000 words, 8 of 6300 for 8192).
+//
+// All tokens of a sequence may share one factor c, and -c at their words is off by the same rounding in
+// all of them, up to half a step of dz's 16 bits: bf16 gradients are 1.9e-3 to 2.4e-3 off in the 2-norm
+// where the mean cross entropy's, whose rows have the factor 1, are 1.9e-3, 4.3e-3 at worst.  (c kept out
+// of dz, on dh's rows and on a copy of the hidden states for dw: dh 1.9e-3 and dw 2.6e-3, and 0.5 to 2 %
+// more time.)  The largest |c| goes into the factors on dw and dh, so that it is 1 in dz: a single
+// pair, or advantages of one size, are off by no more than cross entropy.
 struct Upstream {
   const float* dloss;   // [losses], or one for all
   float factor;
@@ -1328,12 +1341,7 @@ sum_pairs_kernel(const float* __restrict__ loss, const int* __restrict__ counted
 // (scale_h_kernel), which brings the largest of those below 2^15.
 //
 // The loss of a pair is that of `group` rows; weights: null, or each row's derivative by -logp,
-// which c carries.  Then all tokens of a sequence may share one c, and -c at their words is off by
-// the same rounding in all of them, up to half a step of dz's 16 bits: the gradients are 2.4e-3 off
-// in the 2-norm in bf16 where cross entropy's are 1.9e-3, 4.3e-3 at worst.  (c kept out of dz, on dh's
-// rows and on a copy of the hidden states for dw: 1.9e-3 and 2.6e-3, and 0.5 to 2 % more time.)  The
-// largest |c| goes into the factors too, so that it is 1 in dz: a single pair, or advantages of one size,
-// are off by nothing.  One workgroup.
+// which c carries, but for the largest of them (row_factor).  One workgroup.
 __global__ void __launch_bounds__(1024)
 coef_kernel(State st, const float* __restrict__ dloss, bool per_row, int group, const float* __restrict__ weights, bool mean,
             float factor, float zl, bool scaled, float2* __restrict__ coef, float* __restrict__ unscale, float* scale) {
