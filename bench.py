@@ -867,10 +867,10 @@ def cpu_baseline(w, seconds):
     med = t_cpu[len(t_cpu) // 2]
     ctok = w["cpu_tokens"]
     return dict(value=ctok / med, unit="tokens/s", cores=n, kind="port",
-                sample=f"fp32 torch per-step *_scan_reference forward + autograd backward on the host, "
-                       f"{w['cpu_desc']} ({ctok} tokens), {n} threads (of {n_aff} cores in the affinity mask; "
-                       f"{platform.processor() or platform.machine()}), median of {len(t_cpu)} runs "
-                       f"({med:.3f} s each, {sum(t_cpu):.1f} s in all)")
+                sample=f"{w['cpu_desc']} ({ctok} tokens), median of {len(t_cpu)} runs "
+                       f"({med:.3f} s each, {sum(t_cpu):.1f} s in all)",
+                method=f"fp32 torch per-step *_scan_reference forward + autograd backward on the host, {n} threads "
+                       f"(of {n_aff} cores in the affinity mask; {platform.processor() or platform.machine()})")
 
 
 # ------------------------------------------------------------------ counters
@@ -1260,6 +1260,38 @@ def mfma_of(name, dom):
                        "cycles / (GRBM_GUI_ACTIVE / 8 XCDs x 1024 SIMDs)"}
 
 
+def compact(line):
+    """The line as it is printed, short enough for a log that holds the last 16 KB (the whole of it is 24).  Numbers but the
+    headline's to six digits; what the workloads of `also` have in common once, under `notes`; their kernels'
+    times by pass, in order; their counted instructions not at all (profiles/pmc_traffic.json has them)."""
+    def rounded(x):
+        if isinstance(x, float):
+            return float(f"{x:.6g}")
+        if isinstance(x, dict):
+            return {k: rounded(v) for k, v in x.items()}
+        return [rounded(v) for v in x] if isinstance(x, list) else x
+
+    out = rounded(line)
+    out.update(value=line["value"], ms_per_step=line["ms_per_step"])
+    notes = out["notes"] = {}
+    for name, e in (("", out), *out["also"].items()):
+        if e.get("mfma"):
+            notes[f"mfma_{e['mfma']['dtype']}"] = e["mfma"].pop("formula")
+        if e.get("cpu_baseline"):
+            notes["cpu_baseline"] = e["cpu_baseline"].pop("method")
+        if not name:
+            continue
+        for k in ("flops_per_launch", "mops_per_mfma_inst", "valu_insts", "mfma_insts") if e.get("mfma") else ():
+            del e["mfma"][k]
+        if "arithmetic" in e["config"]:
+            notes["arithmetic_also_f32_or_dense"] = e["config"].pop("arithmetic")
+        times = {}
+        for k in e["kernels"]:
+            times.setdefault(k["pass"], []).append(k["us"])
+        e["kernels"] = times
+    return out
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--gpus", type=int, default=1)
@@ -1372,7 +1404,8 @@ def main():
         "also": extras,
         "decode": decode,
     }
-    print(json.dumps(line), flush=True)
+    print(f"[bench] in full: {json.dumps(line)}", file=sys.stderr, flush=True)
+    print(json.dumps(compact(line), separators=(",", ":")), flush=True)
 
 
 if __name__ == "__main__":
