@@ -11,7 +11,9 @@ They run on the kernels of linear_loss.py: the logits are formed tile by tile, r
 ignored cost nothing, and `keep_logits` is as there.  The losses are taken in the launch that
 closes a row's softmax, which leaves the backward one value a row.  The products run in the
 inputs' type with fp32 accumulation; log-probabilities and losses are fp32, sums over a
-sequence and what follows from them 64 bits.
+sequence and what follows from them 64 bits.  With 16-bit inputs and more than 64 rows the
+gradient of the logits is rounded to their type, half a step at most: give fp32 inputs where
+that is too much.
 """
 from __future__ import annotations
 
